@@ -117,6 +117,15 @@ SIGNATURES = {
     "bn_gqa_step_splits": (_i, [_i, _i, _i, _i, _i, _i, _i]),
     "bn_gqa_step": (_i, [_p, _p, _p, _p, _i64, _p, _i64, _f, _p, _p, _i, _i, _i, _p, _p, _p, _p, _i, _p, _i64, _i, _i, _i, _i, _i,
                          _i, _f, _f, _p, _i, _p]),
+    "bn_gemm_bf16_nn_workspace_bytes": (_sz, [_i, _i, _i]),
+    "bn_gemm_bf16_nn": (_i, [_p, _p, _p, _i, _i, _i, _p, _sz, _p, _p]),
+    "bn_gemm_bf16_tn": (_i, [_p, _p, _p, _i, _i, _i, _p, _p]),
+    "bn_linear_cross_entropy_bf16_workspace_bytes": (_sz, [_i, _i, _i]),
+    "bn_linear_cross_entropy_bf16": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _p, _sz, _p, _p, _p]),
+    "bn_linear_cross_entropy_backward_bf16_workspace_bytes": (_sz, [_i, _i, _i]),
+    "bn_linear_cross_entropy_backward_bf16": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _sz, _p, _p]),
+    "bn_gated_ff_backward_bf16_workspace_bytes": (_sz, [_i, _i, _i]),
+    "bn_gated_ff_backward_bf16": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _sz, _p, _p]),
     "bn_gated_group_norm": (_i, [_p, _i64, _i, _p, _i64, _p, _p, _i64, _i, _i, _i, _f, _i, _p]),
 }
 

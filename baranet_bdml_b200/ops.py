@@ -752,3 +752,117 @@ def status_word(device) -> torch.Tensor:
     """The int32 per device that launches report a bounded wait that ran out into (read by `gemm_status`)."""
     _gemm_error_ptr(device, None)
     return _gemm_err[torch.device(device).index if torch.device(device).index is not None else torch.cuda.current_device()]
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Training: the loss over a vocabulary and gradients.  Nothing here is recorded by torch's autograd: a caller keeps what a
+# backward call asks for and passes it on.
+# ---------------------------------------------------------------------------------------------------------------------
+def _operands(what: str, *tensors: torch.Tensor) -> torch.device:
+    """All of them contiguous bf16 on the current device (whose current stream the launches go to)"""
+    for t in tensors:
+        _need(t, torch.bfloat16, what)
+    return _here(what, *tensors)
+
+
+def _here(what: str, *tensors: torch.Tensor) -> torch.device:
+    dev = tensors[0].device
+    if any(t.device != dev for t in tensors) or dev.index != torch.cuda.current_device():
+        raise RuntimeError(f"{what}: all tensors must lie on the current device")
+    return dev
+
+
+def _scratch(nbytes: int, device) -> torch.Tensor:
+    return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+def gemm_bf16_nn(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """a (M,K) bf16 @ b (K,N) bf16 -> (M,N) bf16, fp32 accumulation: the gradient dy @ W of a product x @ W^T by its rows."""
+    dev = _operands("gemm_bf16_nn", a, b)
+    if a.dim() != 2 or b.dim() != 2 or a.shape[1] != b.shape[0]:
+        raise RuntimeError(f"MatMul: inner dimensions mismatch {tuple(a.shape)} x {tuple(b.shape)}")
+    (M, K), N, lib = a.shape, b.shape[1], _lib.load()
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    ws = _scratch(lib.bn_gemm_bf16_nn_workspace_bytes(M, N, K), dev)
+    _lib.check(lib.bn_gemm_bf16_nn(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, ws.data_ptr(), ws.numel(), _gemm_error_ptr(dev, None),
+                                   _stream()))
+    return out
+
+
+def gemm_bf16_tn(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """a (K,M)^T bf16 @ b (K,N) bf16 -> (M,N) bf16, fp32 accumulation: the gradient dy^T @ x of a product x @ W^T by its weight."""
+    dev = _operands("gemm_bf16_tn", a, b)
+    if a.dim() != 2 or b.dim() != 2 or a.shape[0] != b.shape[0]:
+        raise RuntimeError(f"MatMul: inner dimensions mismatch {tuple(a.shape)}^T x {tuple(b.shape)}")
+    (K, M), N = a.shape, b.shape[1]
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    _lib.check(_lib.load().bn_gemm_bf16_tn(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, _gemm_error_ptr(dev, None), _stream()))
+    return out
+
+
+def _loss_shapes(what: str, x: torch.Tensor, weight_t: torch.Tensor, *per_row: torch.Tensor) -> torch.device:
+    dev = _operands(what, x, weight_t)
+    if x.dim() != 2 or weight_t.dim() != 2 or x.shape[1] != weight_t.shape[1]:
+        raise RuntimeError(f"MatMul: inner dimensions mismatch {tuple(x.shape)} x {tuple(weight_t.shape)}^T")
+    for t, dtype in zip(per_row, (torch.int32, torch.float32, torch.float32)):
+        _need(t, dtype, what)
+        if t.shape != (x.shape[0],):
+            raise RuntimeError(f"{what}: targets, log-sum-exp and gradient must have one value for each of {x.shape[0]} rows")
+    _here(what, x, *per_row)
+    return dev
+
+
+def linear_cross_entropy(x: torch.Tensor, weight_t: torch.Tensor, targets: torch.Tensor, *,
+                         id_error: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Softmax cross entropy of the logits x (rows, hidden) @ weight_t (vocab, hidden)^T, bf16, without the logits: (loss, the log of the
+    sum of exponentials), fp32 for each row.  `targets` (rows) int32; a row with a negative one has loss 0.  A target of vocab or more
+    is treated likewise and raises `id_error` (int32), where one is given."""
+    what = "linear_cross_entropy"
+    dev = _loss_shapes(what, x, weight_t, targets)
+    if id_error is not None:
+        _need(id_error, torch.int32, what)
+        _here(what, x, id_error)
+    (rows, hidden), vocab, lib = x.shape, weight_t.shape[0], _lib.load()
+    loss, lse = (torch.empty((rows,), dtype=torch.float32, device=dev) for _ in range(2))
+    ws = _scratch(lib.bn_linear_cross_entropy_bf16_workspace_bytes(rows, vocab, hidden), dev)
+    _lib.check(lib.bn_linear_cross_entropy_bf16(x.data_ptr(), weight_t.data_ptr(), targets.data_ptr(), loss.data_ptr(), lse.data_ptr(), rows, vocab,
+                                                hidden, ws.data_ptr(), ws.numel(), _ptr(id_error), _gemm_error_ptr(dev, None), _stream()))
+    return loss, lse
+
+
+def linear_cross_entropy_backward(x: torch.Tensor, weight_t: torch.Tensor, targets: torch.Tensor, lse: torch.Tensor, grad_loss: torch.Tensor, *,
+                                  want_dx: bool = True, want_dweight: bool = True) -> Tuple[Optional[torch.Tensor], Optional[torch.Tensor]]:
+    """Gradients of sum(grad_loss * loss) by x and weight_t, bf16: `lse` from linear_cross_entropy on the same inputs, `grad_loss` (rows)
+    fp32 (1 / rows for a mean).  The logits' gradients exist for a piece of the vocabulary at a time, as bf16."""
+    what = "linear_cross_entropy_backward"
+    dev = _loss_shapes(what, x, weight_t, targets, lse, grad_loss)
+    if not want_dx and not want_dweight:
+        raise RuntimeError(f"{what}: neither gradient is wanted")
+    (rows, hidden), vocab, lib = x.shape, weight_t.shape[0], _lib.load()
+    dx = torch.empty_like(x) if want_dx else None
+    dw = torch.empty_like(weight_t) if want_dweight else None
+    ws = _scratch(lib.bn_linear_cross_entropy_backward_bf16_workspace_bytes(rows, vocab, hidden), dev)
+    _lib.check(lib.bn_linear_cross_entropy_backward_bf16(
+        x.data_ptr(), weight_t.data_ptr(), targets.data_ptr(), lse.data_ptr(), grad_loss.data_ptr(), _ptr(dx), _ptr(dw), rows, vocab, hidden,
+        ws.data_ptr(), ws.numel(), _gemm_error_ptr(dev, None), _stream()))
+    return dx, dw
+
+
+def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, gate_t: torch.Tensor, up_t: torch.Tensor, down_t: torch.Tensor, *,
+                      act: str = "silu") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of (act(x @ gate_t^T) * (x @ up_t^T)) @ down_t^T by x, gate_t, up_t and down_t, bf16, given dy (rows, hidden) and the input
+    x: gate_t and up_t (inter, hidden), down_t (hidden, inter), as they are stored, `act` "silu" or "gelu_tanh"."""
+    what = "gated_ff_backward"
+    dev = _operands(what, dy, x, gate_t, up_t, down_t)
+    if x.dim() != 2 or gate_t.dim() != 2 or dy.shape != x.shape or gate_t.shape[1] != x.shape[1] or up_t.shape != gate_t.shape or \
+            down_t.shape != (gate_t.shape[1], gate_t.shape[0]):
+        raise RuntimeError(f"{what}: dy and x must be (rows, hidden), gate and up (inter, hidden), down (hidden, inter)")
+    if act not in ("silu", "gelu_tanh"):
+        raise RuntimeError(f"{what}: activation {act!r} (silu or gelu_tanh)")
+    (rows, hidden), inter, lib = x.shape, gate_t.shape[0], _lib.load()
+    grads = tuple(torch.empty_like(t) for t in (x, gate_t, up_t, down_t))
+    ws = _scratch(lib.bn_gated_ff_backward_bf16_workspace_bytes(rows, hidden, inter), dev)
+    _lib.check(lib.bn_gated_ff_backward_bf16(
+        dy.data_ptr(), x.data_ptr(), gate_t.data_ptr(), up_t.data_ptr(), down_t.data_ptr(), *(g.data_ptr() for g in grads), rows, hidden, inter,
+        ACTIVATIONS[act], ws.data_ptr(), ws.numel(), _gemm_error_ptr(dev, None), _stream()))
+    return grads

@@ -600,6 +600,44 @@ BN_API int bn_gqa_step(const void* q, const void* k, const void* v, const void* 
                        void* out, int64_t out_ld, int B, int H, int kv_heads, int dim_ld, int vdim_ld, int rms_dim,
                        float eps, float scale, int* error_word, int dtype, bn_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * training: products of a backward pass, the loss over a vocabulary, gradients of the gated feed-forward block and of attention
+ * (bf16, fp32 accumulation; sums in a fixed order, so two runs give the same bits)
+ * ------------------------------------------------------------------------ */
+
+/* c (M, N) = a (M, K) @ b (K, N): dx = dy @ W for a weight W stored (out, in).  K and N multiples of 8, pointers 16-byte aligned.
+ * Few output tiles share K between CTAs; their fp32 sums lie in the workspace (256-byte aligned; 0 bytes where none is needed). */
+BN_API size_t bn_gemm_bf16_nn_workspace_bytes(int M, int N, int K);
+BN_API int bn_gemm_bf16_nn(const void* a, const void* b, void* c, int M, int N, int K, void* workspace, size_t workspace_bytes, int* error_word,
+                           bn_stream_t stream);
+/* c (M, N) = a (K, M)^T @ b (K, N): dW = dy^T @ x.  M and N multiples of 8, pointers 16-byte aligned. */
+BN_API int bn_gemm_bf16_tn(const void* a, const void* b, void* c, int M, int N, int K, int* error_word, bn_stream_t stream);
+
+/* Softmax cross entropy of the logits x @ weight_t^T, which are kept nowhere: x (rows, hidden), weight_t (vocab, hidden) bf16;
+ *   lse[r] = log sum_v exp z[r][v] (may be NULL),  loss[r] = lse[r] - z[r][targets[r]], both fp32.
+ * A row whose target is negative has loss 0 and no gradient; one whose target is vocab or more likewise, and raises id_error (an
+ * int32 that may be NULL), as the reference's loss over logits (op_cross_entropy, src/ops/op_cross_entropy.cuh:5-45) cannot.
+ * hidden a multiple of 8; x and weight_t 16-byte aligned; workspace 256-byte aligned. */
+BN_API size_t bn_linear_cross_entropy_bf16_workspace_bytes(int rows, int vocab, int hidden);
+BN_API int bn_linear_cross_entropy_bf16(const void* x, const void* weight_t, const int32_t* targets, float* loss, float* lse, int rows, int vocab,
+                                        int hidden, void* workspace, size_t workspace_bytes, int* id_error, int* error_word,
+                                        bn_stream_t stream);
+/* Its gradients: dz[r][v] = grad_loss[r] (exp(z[r][v] - lse[r]) - [v = targets[r]]) rounded to bf16, a piece of the vocabulary at a
+ * time; dx (rows, hidden) = dz @ weight_t, dweight_t (vocab, hidden) = dz^T @ x, bf16.  Either may be NULL.  lse from the call above. */
+BN_API size_t bn_linear_cross_entropy_backward_bf16_workspace_bytes(int rows, int vocab, int hidden);
+BN_API int bn_linear_cross_entropy_backward_bf16(const void* x, const void* weight_t, const int32_t* targets, const float* lse,
+                                                 const float* grad_loss, void* dx, void* dweight_t, int rows, int vocab, int hidden,
+                                                 void* workspace, size_t workspace_bytes, int* error_word, bn_stream_t stream);
+
+/* Gradients of y = (act(x @ gate_t^T) * (x @ up_t^T)) @ down_t^T, what bn_gemm_glu_bf16_nt and the product behind it compute
+ * (MLP.__call__, mygrad/llama/llama_layers.py:194-235): dy, x, dx (rows, hidden); gate_t, up_t, dgate_t, dup_t (inter, hidden);
+ * down_t, ddown_t (hidden, inter).  gate and up are computed again from x.  act BN_ACT_SILU or BN_ACT_GELU_TANH; hidden and inter
+ * multiples of 8; operands 16-byte, workspace 256-byte aligned.  rows = 0 gives zero weight gradients. */
+BN_API size_t bn_gated_ff_backward_bf16_workspace_bytes(int rows, int hidden, int inter);
+BN_API int bn_gated_ff_backward_bf16(const void* dy, const void* x, const void* gate_t, const void* up_t, const void* down_t, void* dx,
+                                     void* dgate_t, void* dup_t, void* ddown_t, int rows, int hidden, int inter, int act, void* workspace,
+                                     size_t workspace_bytes, int* error_word, bn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
