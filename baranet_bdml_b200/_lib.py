@@ -126,6 +126,8 @@ SIGNATURES = {
     "bn_linear_cross_entropy_backward_bf16": (_i, [_p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _p, _sz, _p, _p]),
     "bn_gated_ff_backward_bf16_workspace_bytes": (_sz, [_i, _i, _i]),
     "bn_gated_ff_backward_bf16": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _sz, _p, _p]),
+    "bn_attn_prefill_bf16_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "bn_attn_prefill_bf16_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _f, _i, _i, _p, _sz, _p, _p]),
     "bn_gated_group_norm": (_i, [_p, _i64, _i, _p, _i64, _p, _p, _i64, _i, _i, _i, _f, _i, _p]),
 }
 

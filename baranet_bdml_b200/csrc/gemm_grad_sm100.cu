@@ -195,13 +195,13 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_const
         bool ok = rank == 0;
         for (int t = first; ok && t < items; t += stride, ++local) {
             const uint32_t acc = local & 1u;
-            ok = mbar_wait(smem_u32(&bar_acc_empty[acc]), ((local >> 1) & 1u) ^ 1u, &s_abort);    // drained two tiles ago
+            ok = mbar_wait_warp(smem_u32(&bar_acc_empty[acc]), ((local >> 1) & 1u) ^ 1u, &s_abort);    // drained two tiles ago
             if (!ok) break;
             tc::fence_after_sync();
             const Item w = item(t);
             for (int ks = w.ks0; ks < w.ks1; ++ks, ++it) {
                 const int stage = it % NSTAGE;
-                ok = mbar_wait(smem_u32(&bar_full[stage]), (it / NSTAGE) & 1u, &s_abort);
+                ok = mbar_wait_warp(smem_u32(&bar_full[stage]), (it / NSTAGE) & 1u, &s_abort);
                 if (!ok) break;
                 if (elect_one()) {
                     tc::fence_after_sync();
@@ -248,7 +248,7 @@ gemm_grad_kernel(const __grid_constant__ CUtensorMap tmap_a0, const __grid_const
                     target = INT32_MIN;                                    // no loss, no gradient
                 }
             }
-            ok = mbar_wait(smem_u32(&bar_acc_full[acc]), (local >> 1) & 1u, &s_abort);
+            ok = mbar_wait_warp(smem_u32(&bar_acc_full[acc]), (local >> 1) & 1u, &s_abort);
             if (!ok) break;
             tc::fence_after_sync();
             const uint32_t tacc = tmem + lane_base + acc * GG_BN;

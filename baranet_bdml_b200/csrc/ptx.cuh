@@ -115,6 +115,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
+// The same for a whole warp whose next step is collective: all lanes leave with one answer, also where the wait runs out
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
 // Named barrier `id` over `n_threads` threads (a multiple of 32) that also ORs a predicate across them
 __device__ __forceinline__ bool named_bar_or(int id, int n_threads, bool pred) {
     uint32_t out;
@@ -220,6 +225,12 @@ __device__ __forceinline__ void prefetch_l2(const void* p) {
 // asks for a 2-D tile in L2 (the point of coherence: a tile that is written later is not stale)
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* m, int x, int y) {
     asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(m)), "r"(x), "r"(y) : "memory");
+}
+
+// `bytes` (a multiple of 16, both addresses too) global -> shared, completion counted on an mbarrier
+__device__ __forceinline__ void bulk_load(uint32_t smem_dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* m, int c0, int c1, int c2, uint32_t bar) {

@@ -866,3 +866,26 @@ def gated_ff_backward(dy: torch.Tensor, x: torch.Tensor, gate_t: torch.Tensor, u
         dy.data_ptr(), x.data_ptr(), gate_t.data_ptr(), up_t.data_ptr(), down_t.data_ptr(), *(g.data_ptr() for g in grads), rows, hidden, inter,
         ACTIVATIONS[act], ws.data_ptr(), ws.numel(), _gemm_error_ptr(dev, None), _stream()))
     return grads
+
+
+def attn_prefill_bf16_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, lse: torch.Tensor, *,
+                               scale: Optional[float] = None, theta: float = 10000.0, position_offset: int = 0,
+                               causal: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients of attn_prefill_bf16 by q, k and v (pre-RoPE, as that call takes them), bf16: `out` (B,S,Hq,D) and `lse` (B,Hq,S) fp32 are
+    what that call gave for the same arguments, `dout` the gradient of `out`.  k and v have the sums over their group's query heads."""
+    what = "attn_prefill_bf16_backward"
+    dev = _operands(what, dout, q, k, v, out)
+    _need(lse, torch.float32, what)
+    _here(what, q, lse)
+    if q.dim() != 4 or v.dim() != 4:
+        raise RuntimeError(f"{what}: q must be (B, S, Hq, D), k and v (B, S, Hkv, D)")
+    (B, S, Hq, D), Hkv, lib = q.shape, v.shape[2], _lib.load()
+    if v.shape != (B, S, Hkv, D) or k.shape != v.shape or out.shape != q.shape or dout.shape != q.shape or lse.shape != (B, Hq, S):
+        raise RuntimeError("Attention: hidden size mismatch")
+    dq, dk, dv = (torch.empty_like(t) for t in (q, k, v))
+    ws = _scratch(lib.bn_attn_prefill_bf16_backward_workspace_bytes(B, S, Hq, Hkv, D, int(bool(causal))), dev)
+    _lib.check(lib.bn_attn_prefill_bf16_backward(
+        dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, S,
+        Hq, Hkv, D, 1.0 / (D ** 0.5) if scale is None else float(scale), float(theta), int(position_offset), int(bool(causal)), ws.data_ptr(),
+        ws.numel(), _gemm_error_ptr(dev, None), _stream()))
+    return dq, dk, dv

@@ -638,6 +638,16 @@ BN_API int bn_gated_ff_backward_bf16(const void* dy, const void* x, const void* 
                                      void* dgate_t, void* dup_t, void* ddown_t, int rows, int hidden, int inter, int act, void* workspace,
                                      size_t workspace_bytes, int* error_word, bn_stream_t stream);
 
+/* Gradients of bn_attn_prefill_bf16 by q, k and v as that call takes them (pre-RoPE), given its output, its lse and the output's gradient:
+ *   q, out, dout, dq (B, S, Hq, D) bf16;  k, v, dk, dv (B, S, Hkv, D) bf16;  lse (B, Hq, S) fp32, natural log.
+ * k and v have the sums over the query heads of their group.  Arguments as there; operands must be finite: a masked score has no
+ * gradient, but its key and query are factors of its tile's products.  Tensors 16-byte, workspace 256-byte aligned. */
+BN_API size_t bn_attn_prefill_bf16_backward_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int causal);
+BN_API int bn_attn_prefill_bf16_backward(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, void* dq,
+                                         void* dk, void* dv, int B, int S, int Hq, int Hkv, int D, float scale, float theta,
+                                         int position_offset, int causal, void* workspace, size_t workspace_bytes, int* error_word,
+                                         bn_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -97,3 +97,58 @@ def test_gated_block_gradients(lib, rows, hidden, inter, act):
     want = torch.autograd.grad((a * (leaves[0] @ leaves[2].T)) @ leaves[3].T, leaves, dy.double())
     for name, a, b in zip(("dx", "dgate", "dup", "ddown"), got, want):
         assert off(a, b) <= 3 * HALF, name
+
+
+# ------------------------------------------------------------------------------------------------------------- attention
+def turned(x, offset, theta=10000.0):
+    """(B, S, heads, D) in 64 bits, pairs turned by their position's angle"""
+    D = x.shape[-1]
+    freq = theta ** (-torch.arange(0, D, 2, dtype=torch.float64, device=x.device) / D)
+    angle = (torch.arange(x.shape[1], dtype=torch.float64, device=x.device) + offset)[:, None] * freq
+    z = torch.view_as_complex(x.unflatten(-1, (D // 2, 2)).contiguous()) * torch.polar(torch.ones_like(angle), angle)[:, None]
+    return torch.view_as_real(z).flatten(-2)
+
+
+def attention_oracle(q, k, v, offset, causal, scale):
+    """out, lse of (B, S, heads, D) operands in 64 bits, differentiable"""
+    S, rep = q.shape[1], q.shape[2] // k.shape[2]
+    s = torch.einsum("bqhd,bkhd->bhqk", turned(q, offset), turned(k, offset).repeat_interleave(rep, 2)) * scale
+    if causal:
+        at = torch.arange(S, device=q.device)
+        s = s.masked_fill(at[None, :] > at[:, None] + offset, -float("inf"))
+    return torch.einsum("bhqk,bkhd->bqhd", torch.softmax(s, -1), v.repeat_interleave(rep, 2)), torch.logsumexp(s, -1)
+
+
+def attention_grads(B, S, Hq, Hkv, offset, causal, seed, scale=0.125, std=1.0):
+    from baranet_bdml_b200 import ops
+    rng = np.random.default_rng(seed)
+    q, k, v, dout = (bf16(rng, B, S, h, 64, std=std) for h in (Hq, Hkv, Hkv, Hq))
+    lse = torch.empty((B, Hq, S), dtype=torch.float32, device="cuda")
+    out = ops.attn_prefill_bf16(q, k, v, scale=scale, position_offset=offset, causal=causal, lse=lse)
+    got = ops.attn_prefill_bf16_backward(dout, q, k, v, out, lse, scale=scale, position_offset=offset, causal=causal)
+    ops.gemm_status()
+    leaves = [t.double().requires_grad_(True) for t in (q, k, v)]
+    return got, torch.autograd.grad(attention_oracle(*leaves, offset, causal, scale)[0], leaves, dout.double())
+
+
+# Rounded on the way: the rotated q and k (their product moves a score s by at most 2 * 2^-8 |q||k| scale, and P by that factor), P or dS,
+# the other operand, the output that d comes from, and the result.
+WITHIN = 6 * HALF
+
+
+@pytest.mark.parametrize("S", [1, 2, 63, 64, 65, 127, 128, 129, 200, 333, 513])
+@pytest.mark.parametrize("offset,causal", [(0, True), (5, True), (1000, True), (0, False), (3, False)])
+def test_attention_gradients_of_lengths(lib, S, offset, causal):
+    got, want = attention_grads(2, S, 8, 2, offset, causal, S + offset)
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        if S == 1 and name != "dv":          # one key has all the weight: dP = d but for the order of 64 fp32 products of size < 20,
+            assert a.double().abs().max().item() <= 8 * 64 * 20 * 2.0 ** -23 * 5       # which at most 8 heads have, times a factor < 5
+            continue
+        assert off(a, b) <= WITHIN, name
+
+
+@pytest.mark.parametrize("B,S,Hq,Hkv", [(1, 300, 1, 1), (3, 130, 6, 2), (1, 257, 7, 1), (5, 70, 12, 12), (1, 1500, 32, 4), (8, 700, 16, 2)])
+def test_attention_gradients_of_heads(lib, B, S, Hq, Hkv):
+    got, want = attention_grads(B, S, Hq, Hkv, 0, True, B + S)
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        assert off(a, b) <= WITHIN, name
