@@ -35,7 +35,7 @@ constexpr int AG_SMEM_BYTES = 1024 + 2 * AG_F_BYTES + AG_STAGES * (AG_STAGE_BYTE
 constexpr uint32_t AG_TMEM = 256, AG_S = 0, AG_DP = 64, AG_ACC1 = 128, AG_ACC2 = 192;
 
 struct AttnGradParams {
-    const float2* stats;                 // [B][Hq][padded S]: lse * log2(e), d; rows behind S: +inf, 0
+    const float* stats;                  // [B][Hq][-lse * log2(e), -d][padded S]; rows behind S: -inf, 0
     const float2* table;                 // [S][32] cos, sin
     __nv_bfloat16 *dq, *dk, *dv;
     float* partial;                      // [part][dv, dk][B][S][Hkv][64]
@@ -68,7 +68,7 @@ __device__ __forceinline__ void store_gradient(__nv_bfloat16* row, const float2*
 constexpr int AP_POS = 16, AP_THREADS = 256;
 __global__ void __launch_bounds__(AP_THREADS)
 attn_grad_prepare_kernel(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* out, const __nv_bfloat16* dout, const float* lse, __nv_bfloat16* qrot,
-                         __nv_bfloat16* krot, float2* table, float2* stats, int S, int padded, int Hq, int Hkv, float theta, int offset) {
+                         __nv_bfloat16* krot, float2* table, float* stats, int S, int padded, int Hq, int Hkv, float theta, int offset) {
     __shared__ float2 cs[AP_POS][AG_D / 2];
     grid_dependency_wait();
     const int s0 = blockIdx.x * AP_POS, b = blockIdx.y, share = blockIdx.z, shares = gridDim.z;
@@ -106,8 +106,11 @@ attn_grad_prepare_kernel(const __nv_bfloat16* q, const __nv_bfloat16* k, const _
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        if (c == 0 && pos < padded)
-            stats[((size_t)b * Hq + h) * padded + pos] = pos < S ? make_float2(lse[((size_t)b * Hq + h) * S + pos] * 1.4426950408889634f, sum) : make_float2(INFINITY, 0.f);
+        if (c == 0 && pos < padded) {
+            float* to = stats + ((size_t)b * Hq + h) * 2 * padded + pos;
+            to[0] = pos < S ? lse[((size_t)b * Hq + h) * S + pos] * -1.4426950408889634f : -INFINITY;
+            to[padded] = pos < S ? -sum : 0.f;
+        }
     }
     const int g0 = (int)((long long)Hkv * share / shares), groups = (int)((long long)Hkv * (share + 1) / shares) - g0;
     for (int e = threadIdx.x; e < AP_POS * groups * 8; e += AP_THREADS) {
@@ -168,7 +171,11 @@ __device__ __forceinline__ void attn_grad_block(const CUtensorMap* map_f1, const
                 mbar_arrive_expect_tx(full, AG_STAGE_BYTES + (KEYS ? AG_STAT_BYTES : 0));
                 tma_load_4d(dst, map_x1, 0, h, x * AG_BX, b, full);
                 tma_load_4d(dst + AG_X_BYTES, map_x2, 0, h, x * AG_BX, b, full);
-                if (KEYS) bulk_load(sStat + st * AG_STAT_BYTES, p.stats + ((size_t)b * p.Hq + h) * p.padded + x * AG_BX, AG_STAT_BYTES, full);
+                if (KEYS) {
+                    const float* from = p.stats + ((size_t)b * p.Hq + h) * 2 * p.padded + x * AG_BX;
+                    bulk_load(sStat + st * AG_STAT_BYTES, from, AG_STAT_BYTES / 2, full);
+                    bulk_load(sStat + st * AG_STAT_BYTES + AG_STAT_BYTES / 2, from + p.padded, AG_STAT_BYTES / 2, full);
+                }
                 if (++x == x_hi) { x = x_lo; ++h; }
             }
         }
@@ -223,12 +230,13 @@ __device__ __forceinline__ void attn_grad_block(const CUtensorMap* map_f1, const
         // ------------------------------------------------ softmax warps: thread = (row = TMEM lane, half of the tile's 64 columns)
         const int half = warp / 4, row = tid % 128, f = f0 + row;
         const uint32_t mine = tmem + ((uint32_t)(warp % 4 * 32) << 16) + half * 32;
-        float lse2 = 0.f, d = 0.f;
+        uint64_t lse2 = 0, d2 = 0;                                                 // -lse * log2(e) and -d of the row, twice
         if (!KEYS) {
-            const float2 v = p.stats[((size_t)b * p.Hq + hf) * p.padded + f];      // (rows behind S are padded)
-            lse2 = v.x;
-            d = v.y;
+            const float* of = p.stats + ((size_t)b * p.Hq + hf) * 2 * p.padded + f;    // (rows behind S are padded)
+            lse2 = pack_f32x2(of[0], of[0]);
+            d2 = pack_f32x2(of[p.padded], of[p.padded]);
         }
+        const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
         // which columns of a tile a row sees: keys from x >= first on, queries up to x <= last
         const int first = KEYS && p.causal ? f - p.offset : 0, last = KEYS ? INT32_MAX : (p.causal ? (int)min((long long)p.S - 1, (long long)f + p.offset) : p.S - 1);
         const int all_first = KEYS && p.causal ? f0 + AG_BF - 1 - p.offset : 0, all_last = KEYS ? INT32_MAX : (p.causal ? (int)min((long long)p.S - 1, (long long)f0 + p.offset) : p.S - 1);
@@ -238,34 +246,51 @@ __device__ __forceinline__ void attn_grad_block(const CUtensorMap* map_f1, const
             const int st = i % AG_STAGES, x0 = x * AG_BX;
             if (++x == x_hi) x = x_lo;
             const bool masked = x0 < all_first || x0 + AG_BX - 1 > all_last;       // (the same for the whole block)
-            const uint32_t stat = sStat + st * AG_STAT_BYTES + half * 256;
-            ok = (!KEYS || mbar_wait_warp(smem_u32(&sh.bar_full[st]), (i / AG_STAGES) & 1u, &sh.abort)) && mbar_wait_warp(smem_u32(&sh.bar_s), i & 1, &sh.abort);
+            const uint32_t stat = sStat + st * AG_STAT_BYTES + half * (AG_STAT_BYTES / 4);      // of the half's 32 columns
+            // four columns' values of one kind; for a row of queries the row's own
+            auto of_columns = [&](uint32_t from, int e, uint64_t own, uint64_t& lo, uint64_t& hi) {
+                if (KEYS) asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(from + e * 4));
+                else lo = hi = own;
+            };
+            ok = mbar_wait_warp(smem_u32(&sh.bar_s), i & 1, &sh.abort);          // (the tile and its statistics came before)
+            if (KEYS && ok) ok = mbar_wait_warp(smem_u32(&sh.bar_full[st]), (i / AG_STAGES) & 1u, &sh.abort);
             if (!ok) break;
             tc::fence_after_sync();
             uint32_t s[32];
             tc::ld32(mine + AG_S, s);
             tc::wait_ld(s);
-            float pr[32];
-            auto stat_of = [&](int e, float (&v)[4]) {
-                asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(stat + e * 8));
-            };
+            uint64_t pr[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                float v[4] = {lse2, d, lse2, d};
-                if (KEYS) stat_of(e, v);
-                pr[e] = ex2(fmaf(__uint_as_float(s[e]), p.scale_log2, -v[0]));
-                pr[e + 1] = ex2(fmaf(__uint_as_float(s[e + 1]), p.scale_log2, -v[2]));
+            for (int e = 0; e < 32; e += 4) {
+                uint64_t l[2];
+                of_columns(stat, e, lse2, l[0], l[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float a, c;
+                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), scale2, l[j]), a, c);
+                    pr[e / 2 + j] = pack_f32x2(ex2(a), ex2(c));
+                }
             }
-            if (masked) {
+            if (masked) {                                // (dS has the factor P, so one mask is enough)
                 const int c0 = x0 + half * 32;
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    if (c0 + e < first || c0 + e > last) pr[e] = 0.f;
+                for (int e = 0; e < 16; ++e) {
+                    float a, c;
+                    unpack_f32x2(pr[e], a, c);
+                    if (c0 + 2 * e < first || c0 + 2 * e > last) a = 0.f;
+                    if (c0 + 2 * e + 1 < first || c0 + 2 * e + 1 > last) c = 0.f;
+                    pr[e] = pack_f32x2(a, c);
+                }
             }
+            auto packed = [](uint64_t v) {
+                float a, c;
+                unpack_f32x2(v, a, c);
+                return pack_bf16(a, c);
+            };
+            uint32_t pk[16];
             if (KEYS) {
-                uint32_t pk[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) pk[e] = pack_bf16(pr[2 * e], pr[2 * e + 1]);
+                for (int e = 0; e < 16; ++e) pk[e] = packed(pr[e]);
                 tc::st16(mine + AG_S, pk);
                 tc::wait_st();
             }
@@ -277,18 +302,13 @@ __device__ __forceinline__ void attn_grad_block(const CUtensorMap* map_f1, const
             tc::fence_after_sync();
             tc::ld32(mine + AG_DP, s);
             tc::wait_ld(s);
-            uint32_t pk[16];
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-                float v[4] = {lse2, d, lse2, d};
-                if (KEYS) stat_of(e, v);
-                float a = pr[e] * (__uint_as_float(s[e]) - v[1]), c = pr[e + 1] * (__uint_as_float(s[e + 1]) - v[3]);
-                if (masked) {                            // (what is masked may be infinite)
-                    const int c0 = x0 + half * 32 + e;
-                    if (c0 < first || c0 > last) a = 0.f;
-                    if (c0 + 1 < first || c0 + 1 > last) c = 0.f;
-                }
-                pk[e / 2] = pack_bf16(a, c);
+            for (int e = 0; e < 32; e += 4) {
+                uint64_t l[2];
+                of_columns(stat + AG_STAT_BYTES / 2, e, d2, l[0], l[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    pk[e / 2 + j] = packed(mul_f32x2(pr[e / 2 + j], add_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), l[j])));
             }
             tc::st16(mine + AG_DP, pk);
             tc::wait_st();
@@ -412,7 +432,7 @@ AttnGradLayout attn_grad_layout(int B, int S, int Hq, int Hkv, int causal) {
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     L.table = 0;
     L.stats = up((size_t)S * (AG_D / 2) * sizeof(float2));
-    L.qrot = L.stats + up((size_t)B * Hq * L.padded * sizeof(float2));
+    L.qrot = L.stats + up((size_t)B * Hq * 2 * L.padded * sizeof(float));
     L.krot = L.qrot + up((size_t)B * S * Hq * AG_D * 2);
     L.partial = L.krot + up((size_t)B * S * Hkv * AG_D * 2);
     L.total = L.partial + (parts > 1 ? up((size_t)parts * 2 * B * S * Hkv * AG_D * sizeof(float)) : 0);
@@ -450,7 +470,7 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     cudaStream_t st = as_stream(stream);
     AttnGradParams p{};
-    p.stats = reinterpret_cast<const float2*>(ws + L.stats);
+    p.stats = reinterpret_cast<const float*>(ws + L.stats);
     p.table = reinterpret_cast<const float2*>(ws + L.table);
     p.dq = static_cast<__nv_bfloat16*>(dq);
     p.dk = static_cast<__nv_bfloat16*>(dk);
@@ -481,7 +501,7 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     shares = shares < 1 ? 1 : shares > Hq ? Hq : shares;
     launch_dependent(attn_grad_prepare_kernel, dim3(pos_blocks, (unsigned)B, (unsigned)shares), AP_THREADS, 0, st, static_cast<const __nv_bfloat16*>(q),
                      static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), lse, qrot, krot,
-                     reinterpret_cast<float2*>(ws + L.table), reinterpret_cast<float2*>(ws + L.stats), S, L.padded, Hq, Hkv, theta, position_offset);
+                     reinterpret_cast<float2*>(ws + L.table), reinterpret_cast<float*>(ws + L.stats), S, L.padded, Hq, Hkv, theta, position_offset);
     if (int rc = launch_status(what)) return rc;
     if (int rc = allow_smem(attn_grad_kernel, AG_SMEM_BYTES, what, AG_SMEM_BYTES)) return rc;
     launch_dependent(attn_grad_kernel, dim3((unsigned)blocks), AG_THREADS, AG_SMEM_BYTES, st, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6],
