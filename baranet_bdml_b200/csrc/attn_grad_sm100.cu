@@ -13,12 +13,19 @@
 // Both kinds are one program: F1, F2 are held and X1, X2 come in tiles of 64 rows,
 //     S = F1 X1^T,  dP = F2 X2^T,  acc2 += dS X1,  and for keys acc1 += P X2        (keys: F = K, V, X = Q, dO; queries: F = Q, dO, X = K, V)
 // P and dS are written as bf16 over the scores they came from and are the A operands of the second products (from tensor memory); X1 and X2
-// are B operands twice, along both of their dimensions.  256 columns of tensor memory and 101 KB of shared memory: two blocks to an SM,
-// so one block's softmax runs beside the other's products.
-// Ten warps: 0-7 softmax (two threads a row, 32 columns each), 8 issues the MMAs, 9 loads by TMA.  S of the next tile is computed while
-// dS of this one is.
+// are B operands twice, along both of their dimensions.
+// One CTA per SM takes blocks from a counter, the longest first, and goes on to the next without a pause: three F are kept, tiles of X
+// come through a ring.  Tensor memory: three slots of S and dP (128 columns) and 128 columns of gradients, so three tiles are under way:
+// warps 0-11 are three groups that take tiles in turn (thread = row, 64 columns); warp 13 loads by TMA; warps 12, 14 and 15 have a thread
+// each that issues the products of S, of the gradients and of dP.  (One thread for all took 1950 cycles a tile for its waits and commits of
+// 100 to 200 cycles each, where the products take 530 to 690.)  A slot's S is free for the next tile as soon as P X2 has been computed, or
+// a query block's group has read it, so S of a tile is there before its group is.
+// A block's gradients are stored by all groups, 16 columns at a time, each behind its first tile of the next block: a group that waited for
+// the block's last products and stored all of them held the others up (a pause of 10000 cycles a block, 165 -> X us at 3 x 1371).
 // Launch 3, where the heads of a group are shared by several blocks: their fp32 sums of dK and dV are added in order.
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
+#include <type_traits>
+
 #include "common.cuh"
 #include "ptx.cuh"
 #include "tcgen05.cuh"
@@ -28,49 +35,34 @@ namespace bn {
 
 using namespace ptx;
 
-constexpr int AG_D = 64, AG_BF = 128, AG_BX = 64, AG_STAGES = 4, AG_THREADS = 320;
+constexpr int AG_D = 64, AG_BF = 128, AG_BX = 64, AG_STAGES = 6, AG_SLOTS = 3, AG_F = 3, AG_THREADS = 512, AG_UNITS = 8;
 constexpr int AG_F_BYTES = AG_BF * AG_D * 2, AG_X_BYTES = AG_BX * AG_D * 2, AG_STAT_BYTES = AG_BX * 8;
 constexpr int AG_STAGE_BYTES = 2 * AG_X_BYTES;
-constexpr int AG_SMEM_BYTES = 1024 + 2 * AG_F_BYTES + AG_STAGES * (AG_STAGE_BYTES + AG_STAT_BYTES);
-constexpr uint32_t AG_TMEM = 256, AG_S = 0, AG_DP = 64, AG_ACC1 = 128, AG_ACC2 = 192;
+constexpr int AG_SMEM_BYTES = 1024 + AG_F * 2 * AG_F_BYTES + AG_STAGES * (AG_STAGE_BYTES + AG_STAT_BYTES);
+constexpr uint32_t AG_TMEM = 512, AG_DP = 64, AG_ACC = 384;               // slot: S, then dP; behind the slots two gradients of 64 columns
 
 struct AttnGradParams {
     const float* stats;                  // [B][Hq][-lse * log2(e), -d][padded S]; rows behind S: -inf, 0
     const float2* table;                 // [S][32] cos, sin
     __nv_bfloat16 *dq, *dk, *dv;
     float* partial;                      // [part][dv, dk][B][S][Hkv][64]
-    int* error_word;
-    int B, S, padded, Hq, Hkv, rep, tiles, parts, key_blocks, offset, causal;
+    int *error_word, *counter;           // the next block that nobody has
+    int blocks, B, S, padded, Hq, Hkv, rep, tiles, parts, key_blocks, offset, causal;
     float scale, scale_log2;
 };
 
-// 32 columns of a gradient row, `col` on: scaled, turned back by the row's angles where `table` is given, stored as bf16
-__device__ __forceinline__ void store_gradient(__nv_bfloat16* row, const float2* table, int col, float scale, const float (&v)[32]) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const float a = v[q * 8 + 2 * e] * scale, b = v[q * 8 + 2 * e + 1] * scale;
-            if (table) {
-                const float2 t = table[col / 2 + q * 4 + e];
-                w[e] = pack_bf16(a * t.x + b * t.y, b * t.x - a * t.y);
-            } else {
-                w[e] = pack_bf16(a, b);
-            }
-        }
-        *reinterpret_cast<uint4*>(row + col + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-}
+// a pair of a gradient by a rotated row, by the row itself
+__device__ __forceinline__ uint32_t turned_back(float a, float b, float cos, float sin) { return pack_bf16(a * cos + b * sin, b * cos - a * sin); }
 
 // Rotated copies of q and k, the table of cos and sin, and a query's lse and d side by side.  A block has 16 positions and a share of the
 // heads; 8 neighbouring lanes have a head's 64 values.
 constexpr int AP_POS = 16, AP_THREADS = 256;
 __global__ void __launch_bounds__(AP_THREADS)
 attn_grad_prepare_kernel(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* out, const __nv_bfloat16* dout, const float* lse, __nv_bfloat16* qrot,
-                         __nv_bfloat16* krot, float2* table, float* stats, int S, int padded, int Hq, int Hkv, float theta, int offset) {
+                         __nv_bfloat16* krot, float2* table, float* stats, int* counter, int taken, int S, int padded, int Hq, int Hkv, float theta, int offset) {
     __shared__ float2 cs[AP_POS][AG_D / 2];
     grid_dependency_wait();
+    if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) *counter = taken;
     const int s0 = blockIdx.x * AP_POS, b = blockIdx.y, share = blockIdx.z, shares = gridDim.z;
     for (int e = threadIdx.x; e < AP_POS * (AG_D / 2); e += AP_THREADS) {
         const int s = e / (AG_D / 2), i = e % (AG_D / 2);
@@ -121,294 +113,437 @@ attn_grad_prepare_kernel(const __nv_bfloat16* q, const __nv_bfloat16* k, const _
     }
 }
 
+// A block: rows f0 .. f0 + 127 of head hf of sequence b, and `steps` tiles: x_lo .. x_hi - 1 of heads hx, hx + 1, ..  (steps 0: there is none)
+struct AttnGradUnit { int keys, b, hf, f0, hx, x_lo, x_hi, part, steps; };
+
 struct AttnGradShared {
-    uint64_t bar_full[AG_STAGES], bar_empty[AG_STAGES], bar_fixed, bar_s, bar_dp, bar_p, bar_ds, bar_done;
+    uint64_t full[AG_STAGES], tile_done[AG_STAGES], f_full[AG_F], f_empty[AG_F], s[AG_SLOTS], dp[AG_SLOTS], p[AG_SLOTS], ds[AG_SLOTS], s_free[AG_SLOTS], done[2], acc_free[2], unit[AG_UNITS];
+    AttnGradUnit units[AG_UNITS];        // (decoded once: the divisions take 1400 cycles)
     uint32_t tmem_base;
     int abort;
 };
 
-template <bool KEYS>
-__device__ __forceinline__ void attn_grad_block(const CUtensorMap* map_f1, const CUtensorMap* map_f2, const CUtensorMap* map_x1, const CUtensorMap* map_x2,
-                                                const AttnGradParams& p, AttnGradShared& sh, uint32_t smem0, int unit) {
-    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-    const uint32_t sF1 = smem0, sF2 = smem0 + AG_F_BYTES, sX = smem0 + 2 * AG_F_BYTES, sStat = sX + AG_STAGES * AG_STAGE_BYTES;
-    const uint32_t tmem = sh.tmem_base;
-    // the block's rows f0 .. f0 + 127 of head hf of sequence b; its tiles of 64 rows: x tile x_lo .. x_hi - 1 of heads hx .. hx + heads - 1
-    int b, hf, f0, hx, heads, x_lo, x_hi, part = 0;
-    if (KEYS) {                                          // the first key tiles, which most queries see, come first
-        part = unit % p.parts;
-        const int bg = unit / p.parts % (p.B * p.Hkv), tile = unit / p.parts / (p.B * p.Hkv);
-        b = bg / p.Hkv;
-        hf = bg % p.Hkv;
-        f0 = tile * AG_BF;
-        hx = hf * p.rep + p.rep * part / p.parts;
-        heads = hf * p.rep + p.rep * (part + 1) / p.parts - hx;
-        x_lo = p.causal ? max(0, f0 - p.offset) / AG_BX : 0;
-        x_hi = (p.S + AG_BX - 1) / AG_BX;
+__device__ __forceinline__ AttnGradUnit attn_grad_unit(const AttnGradParams& p, int unit) {
+    AttnGradUnit w;
+    w.keys = unit < p.key_blocks;
+    w.part = w.x_lo = 0;
+    int heads = 1;
+    if (unit >= p.blocks) {
+        heads = w.b = w.hf = w.f0 = w.hx = w.x_hi = 0;
+    } else if (w.keys) {                                 // the first key tiles, which most queries see, come first
+        w.part = unit % p.parts;
+        const int bg = unit / p.parts % (p.B * p.Hkv);
+        w.b = bg / p.Hkv;
+        w.hf = bg % p.Hkv;
+        w.f0 = unit / p.parts / (p.B * p.Hkv) * AG_BF;
+        w.hx = w.hf * p.rep + p.rep * w.part / p.parts;
+        heads = w.hf * p.rep + p.rep * (w.part + 1) / p.parts - w.hx;
+        w.x_lo = p.causal ? max(0, w.f0 - p.offset) / AG_BX : 0;
+        w.x_hi = (p.S + AG_BX - 1) / AG_BX;
     } else {                                             // the last query tiles, which see most keys, come first
-        const int bh = unit % (p.B * p.Hq), tile = p.tiles - 1 - unit / (p.B * p.Hq);
-        b = bh / p.Hq;
-        hf = bh % p.Hq;
-        f0 = tile * AG_BF;
-        hx = hf / p.rep;
-        heads = 1;
-        x_lo = 0;
-        x_hi = (p.causal ? (int)min((long long)p.S - 1, (long long)f0 + AG_BF - 1 + p.offset) : p.S - 1) / AG_BX + 1;
+        unit -= p.key_blocks;
+        const int bh = unit % (p.B * p.Hq);
+        w.b = bh / p.Hq;
+        w.hf = bh % p.Hq;
+        w.f0 = (p.tiles - 1 - unit / (p.B * p.Hq)) * AG_BF;
+        w.hx = w.hf / p.rep;
+        w.x_hi = (p.causal ? (int)min((long long)p.S - 1, (long long)w.f0 + AG_BF - 1 + p.offset) : p.S - 1) / AG_BX + 1;
     }
-    const int per_head = x_hi - x_lo, steps = heads * per_head;
-
-    if (warp == 9) {
-        // ---------------------------------------------------------- TMA producer
-        if (lane == 0) {
-            mbar_arrive_expect_tx(smem_u32(&sh.bar_fixed), 2 * AG_F_BYTES);
-            tma_load_4d(sF1, map_f1, 0, hf, f0, b, smem_u32(&sh.bar_fixed));
-            tma_load_4d(sF2, map_f2, 0, hf, f0, b, smem_u32(&sh.bar_fixed));
-            int h = hx, x = x_lo;
-            for (int i = 0; i < steps; ++i) {
-                const int st = i % AG_STAGES;
-                if (!mbar_wait(smem_u32(&sh.bar_empty[st]), ((i / AG_STAGES) & 1u) ^ 1u, &sh.abort)) break;
-                const uint32_t full = smem_u32(&sh.bar_full[st]), dst = sX + st * AG_STAGE_BYTES;
-                mbar_arrive_expect_tx(full, AG_STAGE_BYTES + (KEYS ? AG_STAT_BYTES : 0));
-                tma_load_4d(dst, map_x1, 0, h, x * AG_BX, b, full);
-                tma_load_4d(dst + AG_X_BYTES, map_x2, 0, h, x * AG_BX, b, full);
-                if (KEYS) {
-                    const float* from = p.stats + ((size_t)b * p.Hq + h) * 2 * p.padded + x * AG_BX;
-                    bulk_load(sStat + st * AG_STAT_BYTES, from, AG_STAT_BYTES / 2, full);
-                    bulk_load(sStat + st * AG_STAT_BYTES + AG_STAT_BYTES / 2, from + p.padded, AG_STAT_BYTES / 2, full);
-                }
-                if (++x == x_hi) { x = x_lo; ++h; }
-            }
-        }
-    } else if (warp == 8) {
-        // ------------------------------------------------------------ MMA issuer
-        constexpr uint32_t I_SCORE = tc::idesc_bf16(AG_BF, AG_BX, 0), I_GRAD = tc::idesc_bf16(AG_BF, AG_D, 1);
-        const uint64_t d0 = tc::smem_desc_sw128(0);
-        auto at = [&](uint32_t addr) { return d0 + (uint64_t)(addr >> 4); };
-        auto score = [&](uint32_t column, uint32_t sF, uint32_t sXi, uint32_t bar) {          // F X^T
-#pragma unroll
-            for (int kk = 0; kk < AG_D / 16; ++kk) tc::mma_ss(tmem + column, at(sF + kk * 32), at(sXi + kk * 32), I_SCORE, kk > 0);
-            tc::commit(bar);
-        };
-        auto grad = [&](uint32_t column, uint32_t from, uint32_t sXi, bool first) {           // (P or dS) X; the halves of a row lie 32 columns apart
-#pragma unroll
-            for (int kk = 0; kk < AG_BX / 16; ++kk)
-                tc::mma_ts(tmem + column, tmem + from + kk / 2 * 32 + kk % 2 * 8, at(sXi + kk * 2048), I_GRAD, !first || kk > 0);
-        };
-        bool ok = mbar_wait_warp(smem_u32(&sh.bar_fixed), 0, &sh.abort) && mbar_wait_warp(smem_u32(&sh.bar_full[0]), 0, &sh.abort);
-        if (ok && elect_one()) {
-            tc::fence_after_sync();
-            score(AG_S, sF1, sX, smem_u32(&sh.bar_s));
-            score(AG_DP, sF2, sX + AG_X_BYTES, smem_u32(&sh.bar_dp));
-        }
-        __syncwarp();
-        for (int i = 0; ok && i < steps; ++i) {
-            const int st = i % AG_STAGES, nx = (i + 1) % AG_STAGES;
-            const uint32_t here = sX + st * AG_STAGE_BYTES, next = sX + nx * AG_STAGE_BYTES;
-            const bool more = i + 1 < steps;
-            // the scores have been read (and P lies over them): P X2, then the next tile's scores into their place (MMAs run in order)
-            ok = mbar_wait_warp(smem_u32(&sh.bar_p), i & 1, &sh.abort);
-            if (ok && more) ok = mbar_wait_warp(smem_u32(&sh.bar_full[nx]), ((i + 1) / AG_STAGES) & 1u, &sh.abort);
-            if (!ok) break;
-            if (elect_one()) {
-                tc::fence_after_sync();
-                if (KEYS) grad(AG_ACC1, AG_S, here + AG_X_BYTES, i == 0);
-                if (more) score(AG_S, sF1, next, smem_u32(&sh.bar_s));
-            }
-            __syncwarp();
-            ok = mbar_wait_warp(smem_u32(&sh.bar_ds), i & 1, &sh.abort);
-            if (!ok) break;
-            if (elect_one()) {
-                tc::fence_after_sync();
-                grad(AG_ACC2, AG_DP, here, i == 0);
-                tc::commit(smem_u32(&sh.bar_empty[st]));
-                if (more) score(AG_DP, sF2, next + AG_X_BYTES, smem_u32(&sh.bar_dp));
-                else tc::commit(smem_u32(&sh.bar_done));
-            }
-            __syncwarp();
-        }
-    } else {
-        // ------------------------------------------------ softmax warps: thread = (row = TMEM lane, half of the tile's 64 columns)
-        const int half = warp / 4, row = tid % 128, f = f0 + row;
-        const uint32_t mine = tmem + ((uint32_t)(warp % 4 * 32) << 16) + half * 32;
-        uint64_t lse2 = 0, d2 = 0;                                                 // -lse * log2(e) and -d of the row, twice
-        if (!KEYS) {
-            const float* of = p.stats + ((size_t)b * p.Hq + hf) * 2 * p.padded + f;    // (rows behind S are padded)
-            lse2 = pack_f32x2(of[0], of[0]);
-            d2 = pack_f32x2(of[p.padded], of[p.padded]);
-        }
-        const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
-        // which columns of a tile a row sees: keys from x >= first on, queries up to x <= last
-        const int first = KEYS && p.causal ? f - p.offset : 0, last = KEYS ? INT32_MAX : (p.causal ? (int)min((long long)p.S - 1, (long long)f + p.offset) : p.S - 1);
-        const int all_first = KEYS && p.causal ? f0 + AG_BF - 1 - p.offset : 0, all_last = KEYS ? INT32_MAX : (p.causal ? (int)min((long long)p.S - 1, (long long)f0 + p.offset) : p.S - 1);
-        int x = x_lo;
-        bool ok = true;
-        for (int i = 0; i < steps; ++i) {
-            const int st = i % AG_STAGES, x0 = x * AG_BX;
-            if (++x == x_hi) x = x_lo;
-            const bool masked = x0 < all_first || x0 + AG_BX - 1 > all_last;       // (the same for the whole block)
-            const uint32_t stat = sStat + st * AG_STAT_BYTES + half * (AG_STAT_BYTES / 4);      // of the half's 32 columns
-            // four columns' values of one kind; for a row of queries the row's own
-            auto of_columns = [&](uint32_t from, int e, uint64_t own, uint64_t& lo, uint64_t& hi) {
-                if (KEYS) asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(from + e * 4));
-                else lo = hi = own;
-            };
-            ok = mbar_wait_warp(smem_u32(&sh.bar_s), i & 1, &sh.abort);          // (the tile and its statistics came before)
-            if (KEYS && ok) ok = mbar_wait_warp(smem_u32(&sh.bar_full[st]), (i / AG_STAGES) & 1u, &sh.abort);
-            if (!ok) break;
-            tc::fence_after_sync();
-            uint32_t s[32];
-            tc::ld32(mine + AG_S, s);
-            tc::wait_ld(s);
-            uint64_t pr[16];
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                uint64_t l[2];
-                of_columns(stat, e, lse2, l[0], l[1]);
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float a, c;
-                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), scale2, l[j]), a, c);
-                    pr[e / 2 + j] = pack_f32x2(ex2(a), ex2(c));
-                }
-            }
-            if (masked) {                                // (dS has the factor P, so one mask is enough)
-                const int c0 = x0 + half * 32;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float a, c;
-                    unpack_f32x2(pr[e], a, c);
-                    if (c0 + 2 * e < first || c0 + 2 * e > last) a = 0.f;
-                    if (c0 + 2 * e + 1 < first || c0 + 2 * e + 1 > last) c = 0.f;
-                    pr[e] = pack_f32x2(a, c);
-                }
-            }
-            auto packed = [](uint64_t v) {
-                float a, c;
-                unpack_f32x2(v, a, c);
-                return pack_bf16(a, c);
-            };
-            uint32_t pk[16];
-            if (KEYS) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) pk[e] = packed(pr[e]);
-                tc::st16(mine + AG_S, pk);
-                tc::wait_st();
-            }
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sh.bar_p));
-            ok = mbar_wait_warp(smem_u32(&sh.bar_dp), i & 1, &sh.abort);
-            if (!ok) break;
-            tc::fence_after_sync();
-            tc::ld32(mine + AG_DP, s);
-            tc::wait_ld(s);
-#pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-                uint64_t l[2];
-                of_columns(stat + AG_STAT_BYTES / 2, e, d2, l[0], l[1]);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    pk[e / 2 + j] = packed(mul_f32x2(pr[e / 2 + j], add_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), l[j])));
-            }
-            tc::st16(mine + AG_DP, pk);
-            tc::wait_st();
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&sh.bar_ds));
-        }
-        // ------------------------------------------------ the block's gradients
-        if (ok) ok = mbar_wait_warp(smem_u32(&sh.bar_done), 0, &sh.abort);
-        if (ok) {
-            tc::fence_after_sync();
-            // keys: the first four warps have dV, the others dK; queries: each half of dQ's columns
-            const int n = KEYS ? 2 : 1;
-#pragma unroll
-            for (int c = 0; c < n; ++c) {
-                const int col = KEYS ? c * 32 : half * 32;
-                uint32_t r[32];
-                tc::ld32(tmem + ((uint32_t)(warp % 4 * 32) << 16) + (KEYS && half == 0 ? AG_ACC1 : AG_ACC2) + col, r);
-                tc::wait_ld(r);
-                if (f < p.S) {
-                    float v[32];
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(r[e]);
-                    const float2* table = p.table + (size_t)f * (AG_D / 2);
-                    if (!KEYS) {
-                        store_gradient(p.dq + (((size_t)b * p.S + f) * p.Hq + hf) * AG_D, table, col, p.scale, v);
-                    } else if (p.parts == 1) {
-                        const size_t at = (((size_t)b * p.S + f) * p.Hkv + hf) * AG_D;
-                        store_gradient((half ? p.dk : p.dv) + at, half ? table : nullptr, col, half ? p.scale : 1.f, v);
-                    } else {
-                        float* to = p.partial + ((((size_t)(part * 2 + half) * p.B + b) * p.S + f) * p.Hkv + hf) * AG_D + col;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) reinterpret_cast<float4*>(to)[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                    }
-                }
-            }
-        }
-    }
+    w.steps = heads * (w.x_hi - w.x_lo);
+    return w;
 }
 
-__global__ void __launch_bounds__(AG_THREADS, 2)
+__device__ __forceinline__ uint32_t packed_bf16(uint64_t v) {
+    float a, c;
+    unpack_f32x2(v, a, c);
+    return pack_bf16(a, c);
+}
+
+// A group's share of a tile, `edge`: the first column (of queries) or the last (of keys) that the thread's row sees: scores -> P (bf16, over them) -> with dP, dS (bf16, over that).  `mine`: the slot's columns in the warp's lanes.
+template <bool KEYS>
+__device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uint32_t parity, uint32_t mine, uint32_t stat, int stage, uint32_t stage_parity,
+                                               uint64_t lse2, uint64_t d2, uint64_t scale2, bool masked, int edge, int lane) {
+    // four columns' values of one kind; for a row of queries the row's own
+    auto of_columns = [&](uint32_t from, int e, uint64_t own, uint64_t& lo, uint64_t& hi) {
+        if (KEYS) asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(from + e * 4));
+        else lo = hi = own;
+    };
+    if (!mbar_wait_warp(smem_u32(&sh.s[slot]), parity, &sh.abort)) return false;
+    if (KEYS && !mbar_wait_warp(smem_u32(&sh.full[stage]), stage_parity, &sh.abort)) return false;      // (the statistics; they came before)
+    tc::fence_after_sync();
+    uint64_t pr[32];
+    {
+        uint32_t s[2][32];
+        tc::ld32(mine, s[0]);
+        tc::ld32(mine + 32, s[1]);
+        tc::wait_ld(s[0]);
+        tc::wait_ld(s[1]);
+        if (!KEYS) {
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&sh.p[slot]));
+        }
+#pragma unroll
+        for (int e = 0; e < 64; e += 4) {
+            uint64_t l[2];
+            of_columns(stat, e, lse2, l[0], l[1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float a, c;
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e / 32][e % 32 + 2 * j]), __uint_as_float(s[e / 32][e % 32 + 2 * j + 1])), scale2, l[j]), a, c);
+                pr[e / 2 + j] = pack_f32x2(ex2(a), ex2(c));
+            }
+        }
+    }
+    if (masked) {                                        // (dS has the factor P, so one mask is enough)
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            float a, c;
+            unpack_f32x2(pr[e], a, c);
+            if (KEYS ? 2 * e < edge : 2 * e > edge) a = 0.f;
+            if (KEYS ? 2 * e + 1 < edge : 2 * e + 1 > edge) c = 0.f;
+            pr[e] = pack_f32x2(a, c);
+        }
+    }
+    if (KEYS) {
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) pk[e] = packed_bf16(pr[hf * 16 + e]);
+            tc::st16(mine + hf * 16, pk);
+        }
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p[slot]));
+    }
+    if (!mbar_wait_warp(smem_u32(&sh.dp[slot]), parity, &sh.abort)) return false;
+    tc::fence_after_sync();
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {                     // (the second half's columns are read before any are written: 32 bf16 columns lie in 16)
+        uint32_t s[2][16], pk[16];
+        tc::ld16(mine + AG_DP + hf * 32, s[0]);
+        tc::ld16(mine + AG_DP + hf * 32 + 16, s[1]);
+        tc::wait_ld(s[0]);
+        tc::wait_ld(s[1]);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+            uint64_t l[2];
+            of_columns(stat + AG_STAT_BYTES / 2, hf * 32 + e, d2, l[0], l[1]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                pk[e / 2 + j] = packed_bf16(mul_f32x2(
+                    pr[hf * 16 + e / 2 + j],
+                    add_f32x2(pack_f32x2(__uint_as_float(s[e / 16][e % 16 + 2 * j]), __uint_as_float(s[e / 16][e % 16 + 2 * j + 1])), l[j])));
+        }
+        tc::st16(mine + AG_DP + hf * 16, pk);
+    }
+    tc::wait_st();
+    tc::fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.ds[slot]));
+    return true;
+}
+
+__global__ void __launch_bounds__(AG_THREADS, 1)
 attn_grad_kernel(const __grid_constant__ CUtensorMap q_tile, const __grid_constant__ CUtensorMap do_tile, const __grid_constant__ CUtensorMap k_tile,
                  const __grid_constant__ CUtensorMap v_tile, const __grid_constant__ CUtensorMap q_rows, const __grid_constant__ CUtensorMap do_rows,
                  const __grid_constant__ CUtensorMap k_rows, const __grid_constant__ CUtensorMap v_rows, const AttnGradParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) AttnGradShared sh;
-    const int warp = threadIdx.x / 32;
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < AG_STAGES; ++s) {
-            mbar_init(smem_u32(&sh.bar_full[s]), 1);
-            mbar_init(smem_u32(&sh.bar_empty[s]), 1);
+    const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sF = smem0, sX = smem0 + AG_F * 2 * AG_F_BYTES, sStat = sX + AG_STAGES * AG_STAGE_BYTES;
+    if (tid == 0) {
+        for (int i = 0; i < AG_STAGES; ++i) {
+            mbar_init(smem_u32(&sh.full[i]), 1);
+            mbar_init(smem_u32(&sh.tile_done[i]), 1);
         }
-        mbar_init(smem_u32(&sh.bar_fixed), 1);
-        mbar_init(smem_u32(&sh.bar_s), 1);
-        mbar_init(smem_u32(&sh.bar_dp), 1);
-        mbar_init(smem_u32(&sh.bar_p), 8);                // one arrive per softmax warp
-        mbar_init(smem_u32(&sh.bar_ds), 8);
-        mbar_init(smem_u32(&sh.bar_done), 1);
+        for (int i = 0; i < AG_F; ++i) {
+            mbar_init(smem_u32(&sh.f_full[i]), 1);
+            mbar_init(smem_u32(&sh.f_empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&sh.done[i]), 1);
+            mbar_init(smem_u32(&sh.acc_free[i]), 12);     // one arrive per softmax warp
+        }
+        for (int i = 0; i < AG_SLOTS; ++i) {
+            mbar_init(smem_u32(&sh.s[i]), 1);
+            mbar_init(smem_u32(&sh.dp[i]), 1);
+            mbar_init(smem_u32(&sh.p[i]), 4);
+            mbar_init(smem_u32(&sh.ds[i]), 4);
+            mbar_init(smem_u32(&sh.s_free[i]), 1);
+        }
+        for (int i = 0; i < AG_UNITS; ++i) mbar_init(smem_u32(&sh.unit[i]), 1);
         sh.abort = 0;
         fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == 12) {
         tc::tmem_alloc(smem_u32(&sh.tmem_base), AG_TMEM);
         tc::tmem_relinquish();
     }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
+    const uint32_t tmem = sh.tmem_base;
     grid_dependency_wait();
-    const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    if ((int)blockIdx.x < p.key_blocks) attn_grad_block<true>(&k_tile, &v_tile, &q_rows, &do_rows, p, sh, smem0, blockIdx.x);
-    else attn_grad_block<false>(&q_tile, &do_tile, &k_rows, &v_rows, p, sh, smem0, blockIdx.x - p.key_blocks);
+
+    // number `u` of this CTA's blocks.  The ring is long enough: the loader is at most AG_F blocks ahead of the MMAs, of any three tiles that
+    // follow one another each group has had one, and a group comes back to the block before its own at most.  (Three tiles may belong to
+    // three blocks: so many F are kept.)
+    auto unit_at = [&](uint32_t u, bool& ok) -> const AttnGradUnit& {
+        ok = mbar_wait(smem_u32(&sh.unit[u % AG_UNITS]), u / AG_UNITS & 1u, &sh.abort);
+        return sh.units[u % AG_UNITS];
+    };
+
+    if (warp == 13) {
+        // ---------------------------------------------------------- blocks, TMA producer
+        if (elect_one()) {
+            int unit = blockIdx.x;
+            uint32_t n = 0;
+            bool ok = true;
+            for (uint32_t u = 0; ok; ++u) {
+                const AttnGradUnit w = attn_grad_unit(p, unit);
+                sh.units[u % AG_UNITS] = w;
+                mbar_arrive(smem_u32(&sh.unit[u % AG_UNITS]));
+                if (w.steps == 0) break;
+                unit = atomicAdd(p.counter, 1);           // (asked for ahead of the loads)
+                const CUtensorMap *f1 = w.keys ? &k_tile : &q_tile, *f2 = w.keys ? &v_tile : &do_tile, *x1 = w.keys ? &q_rows : &k_rows, *x2 = w.keys ? &do_rows : &v_rows;
+                ok = mbar_wait(smem_u32(&sh.f_empty[u % AG_F]), (u / AG_F & 1u) ^ 1u, &sh.abort);
+                if (!ok) break;
+                const uint32_t f_full = smem_u32(&sh.f_full[u % AG_F]), f_dst = sF + u % AG_F * 2 * AG_F_BYTES;
+                mbar_arrive_expect_tx(f_full, 2 * AG_F_BYTES);
+                tma_load_4d(f_dst, f1, 0, w.hf, w.f0, w.b, f_full);
+                tma_load_4d(f_dst + AG_F_BYTES, f2, 0, w.hf, w.f0, w.b, f_full);
+                int h = w.hx, x = w.x_lo;
+                for (int i = 0; i < w.steps; ++i, ++n) {
+                    const uint32_t st = n % AG_STAGES;
+                    ok = mbar_wait(smem_u32(&sh.tile_done[st]), (n / AG_STAGES & 1u) ^ 1u, &sh.abort);
+                    if (!ok) break;
+                    const uint32_t full = smem_u32(&sh.full[st]), dst = sX + st * AG_STAGE_BYTES;
+                    mbar_arrive_expect_tx(full, AG_STAGE_BYTES + (w.keys ? AG_STAT_BYTES : 0));
+                    tma_load_4d(dst, x1, 0, h, x * AG_BX, w.b, full);
+                    tma_load_4d(dst + AG_X_BYTES, x2, 0, h, x * AG_BX, w.b, full);
+                    if (w.keys) {
+                        const float* from = p.stats + ((size_t)w.b * p.Hq + h) * 2 * p.padded + x * AG_BX;
+                        bulk_load(sStat + st * AG_STAT_BYTES, from, AG_STAT_BYTES / 2, full);
+                        bulk_load(sStat + st * AG_STAT_BYTES + AG_STAT_BYTES / 2, from + p.padded, AG_STAT_BYTES / 2, full);
+                    }
+                    if (++x == w.x_hi) { x = w.x_lo; ++h; }
+                }
+            }
+        }
+    } else if (warp == 12 || warp == 15) {
+        // ------------------------------------------------------------ products of the scores: S (warp 12), dP (warp 15)
+        constexpr uint32_t I_SCORE = tc::idesc_bf16(AG_BF, AG_BX, 0);
+        const uint64_t d0 = tc::smem_desc_sw128(0);
+        auto at = [&](uint32_t addr) { return d0 + (uint64_t)(addr >> 4); };
+        const uint32_t second = warp == 15;
+        if (elect_one()) {
+            uint32_t n = 0, was_keys = 0, freed = 0;      // per slot: whether its last tile was one of keys; the parity of s_free
+            bool ok = true;
+            for (uint32_t u = 0; ok; ++u) {
+                const AttnGradUnit& w = unit_at(u, ok);
+                if (!ok || w.steps == 0) break;
+                const int steps = w.steps, keys = w.keys;
+                ok = mbar_wait(smem_u32(&sh.f_full[u % AG_F]), u / AG_F & 1u, &sh.abort);
+                const uint32_t f = sF + (u % AG_F * 2 + second) * AG_F_BYTES;
+                for (int i = 0; ok && i < steps; ++i, ++n) {
+                    const uint32_t st = n % AG_STAGES, slot = n % AG_SLOTS, x = sX + st * AG_STAGE_BYTES + second * AG_X_BYTES;
+                    const uint32_t col = tmem + slot * 128 + second * AG_DP;
+                    if (n >= AG_SLOTS) {                  // what the tile before in this slot had here has been used
+                        const uint32_t before = n - AG_SLOTS;
+                        if (second) {
+                            ok = mbar_wait(smem_u32(&sh.tile_done[before % AG_STAGES]), before / AG_STAGES & 1u, &sh.abort);
+                        } else if (was_keys >> slot & 1u) {
+                            ok = mbar_wait(smem_u32(&sh.s_free[slot]), freed >> slot & 1u, &sh.abort);
+                            freed ^= 1u << slot;
+                        } else {
+                            ok = mbar_wait(smem_u32(&sh.p[slot]), before / AG_SLOTS & 1u, &sh.abort);
+                        }
+                    }
+                    was_keys = (was_keys & ~(1u << slot)) | (uint32_t)keys << slot;
+                    ok = ok && mbar_wait(smem_u32(&sh.full[st]), n / AG_STAGES & 1u, &sh.abort);
+                    if (!ok) break;
+                    tc::fence_after_sync();
+#pragma unroll
+                    for (int kk = 0; kk < AG_D / 16; ++kk) tc::mma_ss(col, at(f + kk * 32), at(x + kk * 32), I_SCORE, kk > 0);
+                    tc::commit(second ? smem_u32(&sh.dp[slot]) : smem_u32(&sh.s[slot]));
+                }
+            }
+        }
+    } else if (warp == 14) {
+        // ------------------------------------------------------------ products of the gradients
+        constexpr uint32_t I_GRAD = tc::idesc_bf16(AG_BF, AG_D, 1);
+        const uint64_t d0 = tc::smem_desc_sw128(0);
+        auto grad = [&](uint32_t column, uint32_t from, uint32_t sXi, bool first) {           // (P or dS) X
+#pragma unroll
+            for (int kk = 0; kk < AG_BX / 16; ++kk) tc::mma_ts(tmem + column, tmem + from + kk * 8, d0 + (uint64_t)((sXi + kk * 2048) >> 4), I_GRAD, !first || kk > 0);
+        };
+        if (elect_one()) {
+            uint32_t n = 0, uses0 = 0, uses1 = 0;
+            bool ok = true;
+            for (uint32_t u = 0; ok; ++u) {
+                const AttnGradUnit& w = unit_at(u, ok);
+                if (!ok || w.steps == 0) break;
+                const int steps = w.steps, keys = w.keys;
+                // keys: dV and dK in both gradients; queries: dQ in one of them
+                const uint32_t acc2 = keys ? 1u : u & 1u;
+                if (keys || acc2 == 0) ok = mbar_wait(smem_u32(&sh.acc_free[0]), (uses0++ & 1u) ^ 1u, &sh.abort);
+                if (ok && (keys || acc2 == 1)) ok = mbar_wait(smem_u32(&sh.acc_free[1]), (uses1++ & 1u) ^ 1u, &sh.abort);
+                for (int i = 0; ok && i < steps; ++i, ++n) {
+                    const uint32_t st = n % AG_STAGES, slot = n % AG_SLOTS, here = sX + st * AG_STAGE_BYTES;
+                    if (keys) {
+                        ok = mbar_wait(smem_u32(&sh.p[slot]), n / AG_SLOTS & 1u, &sh.abort);
+                        if (!ok) break;
+                        tc::fence_after_sync();
+                        grad(AG_ACC, slot * 128, here + AG_X_BYTES, i == 0);
+                        tc::commit(smem_u32(&sh.s_free[slot]));
+                    }
+                    ok = mbar_wait(smem_u32(&sh.ds[slot]), n / AG_SLOTS & 1u, &sh.abort);     // (behind p)
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                    grad(AG_ACC + acc2 * 64, slot * 128 + AG_DP, here, i == 0);
+                    tc::commit(smem_u32(&sh.tile_done[st]));
+                    if (i == steps - 1) {
+                        tc::commit(smem_u32(&sh.done[u & 1]));
+                        tc::commit(smem_u32(&sh.f_empty[u % AG_F]));
+                    }
+                }
+            }
+        }
+    } else {
+        // ------------------------------------------------ softmax groups
+        const int group = warp / 4, row = tid % 128;
+        const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), mine = lanes + group * 128;
+        const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
+        uint32_t n0 = 0;                                  // the block's first tile among all of this CTA's
+        bool ok = true;
+        // 16 columns of a block's gradients: dV and dK (keys) or dQ, of which a group has every third
+        auto gradients = [&](uint32_t u) {
+            if (!mbar_wait_warp(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) return false;
+            tc::fence_after_sync();
+            const AttnGradUnit& w = sh.units[u % AG_UNITS];
+            const bool keys = w.keys;
+            const int f = w.f0 + row, heads = keys ? p.Hkv : p.Hq;
+            const size_t at = (((size_t)w.b * p.S + f) * heads + w.hf) * AG_D, all = (size_t)p.B * p.S * p.Hkv * AG_D;
+            const float4* table = reinterpret_cast<const float4*>(p.table + (size_t)min(f, p.S - 1) * (AG_D / 2));
+#pragma unroll 1
+            for (int c = keys ? group : 4 + group; c < 8; c += AG_SLOTS) {
+                const int col = c % 4 * 16;
+                const bool dv = c < 4;
+                float4 angle[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) angle[e] = dv ? make_float4(1.f, 0.f, 1.f, 0.f) : __ldcg(table + col / 4 + e);
+                uint32_t r[16];
+                tc::ld16(lanes + AG_ACC + (keys ? c / 4 : u & 1u) * 64 + col, r);
+                tc::wait_ld(r);
+                if (f < p.S) {
+                    if (keys && p.parts > 1) {
+                        float4* to = reinterpret_cast<float4*>(p.partial + (w.part * 2 + (dv ? 0 : 1)) * all + at + col);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            to[e] = make_float4(__uint_as_float(r[4 * e]), __uint_as_float(r[4 * e + 1]), __uint_as_float(r[4 * e + 2]), __uint_as_float(r[4 * e + 3]));
+                    } else {
+                        const float scale = dv ? 1.f : p.scale;
+                        uint32_t o[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const float4 t = angle[e / 2];
+                            o[e] = turned_back(__uint_as_float(r[2 * e]) * scale, __uint_as_float(r[2 * e + 1]) * scale, e % 2 ? t.z : t.x, e % 2 ? t.w : t.y);
+                        }
+                        uint4* to = reinterpret_cast<uint4*>((keys ? dv ? p.dv : p.dk : p.dq) + at + col);
+                        to[0] = make_uint4(o[0], o[1], o[2], o[3]);
+                        to[1] = make_uint4(o[4], o[5], o[6], o[7]);
+                    }
+                }
+                __syncwarp();
+            }
+            tc::fence_before_sync();
+            __syncwarp();
+            if (lane == 0) {
+                if (keys || (u & 1u) == 0) mbar_arrive(smem_u32(&sh.acc_free[0]));
+                if (keys || (u & 1u) == 1) mbar_arrive(smem_u32(&sh.acc_free[1]));
+            }
+            return true;
+        };
+        for (uint32_t u = 0; ok; ++u) {
+            const AttnGradUnit& w = unit_at(u, ok);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int steps = w.steps, f0 = w.f0, f = f0 + row, x_lo = w.x_lo, width = w.x_hi - x_lo;
+            const int i0 = (int)((group + AG_SLOTS - n0 % AG_SLOTS) % AG_SLOTS);
+            bool owed = u > 0;                            // the gradients of the block before
+            // the group's tiles; from which column on (queries) or up to which (keys) its rows see everything
+            auto tiles = [&](auto keys, uint64_t lse2, uint64_t d2, int mine_sees, int all_see) {
+                constexpr bool KEYS = decltype(keys)::value;
+                uint32_t n = n0 + i0;
+                int x0 = (x_lo + i0 % width) * AG_BX;
+                const int behind = (x_lo + width) * AG_BX;
+                for (int i = i0; i < steps; i += AG_SLOTS, n += AG_SLOTS) {
+                    const uint32_t st = n % AG_STAGES;
+                    const bool masked = KEYS ? x0 < all_see : x0 + AG_BX - 1 > all_see;
+                    if (!attn_grad_tile<KEYS>(sh, group, n / AG_SLOTS & 1u, mine, sStat + st * AG_STAT_BYTES, st, n / AG_STAGES & 1u, lse2, d2, scale2, masked,
+                                              mine_sees - x0, lane))
+                        return false;
+                    x0 += AG_SLOTS * AG_BX;
+                    while (x0 >= behind) x0 -= width * AG_BX;
+                    if (owed) {
+                        owed = false;
+                        if (!gradients(u - 1)) return false;
+                    }
+                }
+                return true;
+            };
+            if (i0 >= steps) {
+            } else if (w.keys) {
+                ok = tiles(std::true_type{}, 0, 0, p.causal ? f - p.offset : 0, p.causal ? f0 + AG_BF - 1 - p.offset : 0);
+            } else {                                      // -lse * log2(e) and -d of the row, twice (rows behind S are padded)
+                const float* of = p.stats + ((size_t)w.b * p.Hq + w.hf) * 2 * p.padded + f;
+                const float lse = of[0], d = of[p.padded];
+                const long long sees = p.causal ? p.offset : p.S;
+                ok = tiles(std::false_type{}, pack_f32x2(lse, lse), pack_f32x2(d, d), (int)min((long long)p.S - 1, f + sees), (int)min((long long)p.S - 1, f0 + sees));
+            }
+            if (ok && owed) ok = gradients(u - 1);
+            if (steps == 0) break;
+            n0 += steps;
+        }
+    }
     // common exit: everybody arrives here (bounded waits), then TMEM is freed
     tc::fence_before_sync();
     __syncthreads();
-    if (threadIdx.x == 0 && sh.abort && p.error_word) atomicExch(p.error_word, BN_ERR_TIMEOUT);
-    if (warp == 8) {
+    if (tid == 0 && sh.abort && p.error_word) atomicExch(p.error_word, BN_ERR_TIMEOUT);
+    if (warp == 12) {
         tc::fence_after_sync();
-        tc::tmem_dealloc(sh.tmem_base, AG_TMEM);
+        tc::tmem_dealloc(tmem, AG_TMEM);
     }
 }
 
-// dV and dK of the blocks that share a group's heads, added in their order; a thread has 32 columns of a row
-__global__ void __launch_bounds__(128) attn_grad_sum_kernel(const AttnGradParams p) {
+// dV and dK of the blocks that share a group's heads, added in their order; a thread has 8 columns of a row
+__global__ void __launch_bounds__(256) attn_grad_sum_kernel(const AttnGradParams p) {
     grid_dependency_wait();
-    const long long rows = (long long)p.B * p.S * p.Hkv, e = (long long)blockIdx.x * 128 + threadIdx.x, row = e / 2;
+    const long long rows = (long long)p.B * p.S * p.Hkv, e = (long long)blockIdx.x * 256 + threadIdx.x, row = e / 8;
     if (row >= rows) return;
-    const int col = (int)(e % 2) * 32, which = blockIdx.y;
-    float v[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = 0.f;
+    const int col = (int)(e % 8) * 8, which = blockIdx.y;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    const float4* from = reinterpret_cast<const float4*>(p.partial + ((size_t)which * rows + row) * AG_D + col);
     for (int part = 0; part < p.parts; ++part) {
-        const float4* from = reinterpret_cast<const float4*>(p.partial + ((size_t)(part * 2 + which) * rows + row) * AG_D + col);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 t = __ldcg(from + i);
+        for (int i = 0; i < 2; ++i) {
+            const float4 t = __ldcg(from + (size_t)part * 2 * rows * (AG_D / 4) + i);
             v[4 * i] += t.x; v[4 * i + 1] += t.y; v[4 * i + 2] += t.z; v[4 * i + 3] += t.w;
         }
     }
-    store_gradient((which ? p.dk : p.dv) + (size_t)row * AG_D, which ? p.table + (size_t)(row / p.Hkv % p.S) * (AG_D / 2) : nullptr, col, which ? p.scale : 1.f, v);
+    const float2* table = p.table + (size_t)(row / p.Hkv % p.S) * (AG_D / 2) + col / 2;
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 t = which ? table[i] : make_float2(1.f, 0.f);
+        const float scale = which ? p.scale : 1.f;
+        o[i] = turned_back(v[2 * i] * scale, v[2 * i + 1] * scale, t.x, t.y);
+    }
+    reinterpret_cast<uint4*>((which ? p.dk : p.dv) + (size_t)row * AG_D)[col / 8] = make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 }  // namespace bn
@@ -417,21 +552,22 @@ using namespace bn;
 
 namespace {
 
-struct AttnGradLayout { size_t table, stats, qrot, krot, partial, total; int parts, padded; };
+struct AttnGradLayout { size_t counter, table, stats, qrot, krot, partial, total; int parts, padded; };
 
-// How many blocks share the heads of a group: the longest block should not take longer than all blocks' work spread over the GPU
-// (two blocks to an SM), or it is what the launch waits for; each further part is written and read again in fp32.
+// How many blocks share the heads of a group: the longest block should not take longer than all blocks' work spread over the GPU, or it
+// is what the launch waits for; each further part is written and read again in fp32.
 AttnGradLayout attn_grad_layout(int B, int S, int Hq, int Hkv, int causal) {
     AttnGradLayout L;
     const long long tiles = (S + AG_BF - 1) / AG_BF, n = (S + AG_BX - 1) / AG_BX, rep = Hq / Hkv;
-    const long long all = 2 * (long long)B * Hq * tiles * n / (causal ? 2 : 1), slots = 2 * sm_count();
+    const long long all = 2 * (long long)B * Hq * tiles * n / (causal ? 2 : 1), slots = sm_count();
     int parts = 1;
     while (parts < rep && (rep + parts - 1) / parts * n * slots > all) ++parts;
     L.parts = parts;
     L.padded = (int)(tiles * AG_BF);
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    L.table = 0;
-    L.stats = up((size_t)S * (AG_D / 2) * sizeof(float2));
+    L.counter = 0;
+    L.table = 256;
+    L.stats = L.table + up((size_t)S * (AG_D / 2) * sizeof(float2));
     L.qrot = L.stats + up((size_t)B * Hq * 2 * L.padded * sizeof(float));
     L.krot = L.qrot + up((size_t)B * S * Hq * AG_D * 2);
     L.partial = L.krot + up((size_t)B * S * Hkv * AG_D * 2);
@@ -463,8 +599,8 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     if (!workspace || workspace_bytes < L.total) return fail(BN_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", what, workspace_bytes, L.total);
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(BN_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", what);
     const long long tiles = (S + AG_BF - 1) / AG_BF, key_blocks = tiles * B * Hkv * L.parts, blocks = key_blocks + tiles * B * Hq;
-    const long long sum_blocks = ((long long)B * S * Hkv * 2 + 127) / 128;
-    if (blocks > INT32_MAX || sum_blocks > INT32_MAX || B > 65535 || S > INT32_MAX - 256 || position_offset > INT32_MAX - S - 256)
+    const long long sum_blocks = ((long long)B * S * Hkv * 8 + 255) / 256;
+    if (blocks > INT32_MAX / 2 || sum_blocks > INT32_MAX || B > 65535 || S > INT32_MAX - 256 || position_offset > INT32_MAX - S - 256)
         return fail(BN_ERR_UNSUPPORTED, "%s: problem too large for one launch", what);
 
     uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -477,6 +613,9 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     p.dv = static_cast<__nv_bfloat16*>(dv);
     p.partial = reinterpret_cast<float*>(ws + L.partial);
     p.error_word = error_word;
+    p.counter = reinterpret_cast<int*>(ws + L.counter);
+    p.blocks = (int)blocks;
+    const unsigned grid = (unsigned)(blocks < sm_count() ? blocks : sm_count());
     p.B = B; p.S = S; p.padded = L.padded; p.Hq = Hq; p.Hkv = Hkv; p.rep = Hq / Hkv; p.tiles = (int)tiles; p.parts = L.parts;
     p.key_blocks = (int)key_blocks;
     p.offset = position_offset;
@@ -501,14 +640,14 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     shares = shares < 1 ? 1 : shares > Hq ? Hq : shares;
     launch_dependent(attn_grad_prepare_kernel, dim3(pos_blocks, (unsigned)B, (unsigned)shares), AP_THREADS, 0, st, static_cast<const __nv_bfloat16*>(q),
                      static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), lse, qrot, krot,
-                     reinterpret_cast<float2*>(ws + L.table), reinterpret_cast<float*>(ws + L.stats), S, L.padded, Hq, Hkv, theta, position_offset);
+                     reinterpret_cast<float2*>(ws + L.table), reinterpret_cast<float*>(ws + L.stats), p.counter, (int)grid, S, L.padded, Hq, Hkv, theta, position_offset);
     if (int rc = launch_status(what)) return rc;
     if (int rc = allow_smem(attn_grad_kernel, AG_SMEM_BYTES, what, AG_SMEM_BYTES)) return rc;
-    launch_dependent(attn_grad_kernel, dim3((unsigned)blocks), AG_THREADS, AG_SMEM_BYTES, st, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6],
+    launch_dependent(attn_grad_kernel, dim3(grid), AG_THREADS, AG_SMEM_BYTES, st, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6],
                      maps[7], p);
     if (int rc = launch_status(what)) return rc;
     if (L.parts > 1) {
-        launch_dependent(attn_grad_sum_kernel, dim3((unsigned)sum_blocks, 2), 128, 0, st, p);
+        launch_dependent(attn_grad_sum_kernel, dim3((unsigned)sum_blocks, 2), 256, 0, st, p);
         return launch_status(what);
     }
     return BN_OK;
