@@ -422,22 +422,29 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_tile, const __grid_consta
         bool ok = true;
         // 16 columns of a block's gradients: dV and dK (keys) or dQ, of which a group has every third
         auto gradients = [&](uint32_t u) {
-            if (!mbar_wait_warp(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) return false;
-            tc::fence_after_sync();
             const AttnGradUnit& w = sh.units[u % AG_UNITS];
             const bool keys = w.keys;
             const int f = w.f0 + row, heads = keys ? p.Hkv : p.Hq;
             const size_t at = (((size_t)w.b * p.S + f) * heads + w.hf) * AG_D, all = (size_t)p.B * p.S * p.Hkv * AG_D;
             const float4* table = reinterpret_cast<const float4*>(p.table + (size_t)min(f, p.S - 1) * (AG_D / 2));
+            const int c0 = keys ? group : 4 + group;
+            float4 angle[4], next[4];
+            auto ask = [&](int c, float4 (&to)[4]) {      // (dV is not turned; 64 bytes of a line that the next columns share)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[e] = c >= 4 && c < 8 ? table[c % 4 * 4 + e] : make_float4(1.f, 0.f, 1.f, 0.f);
+            };
+            ask(c0, next);
+            if (!mbar_wait_warp(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) return false;
+            tc::fence_after_sync();
 #pragma unroll 1
-            for (int c = keys ? group : 4 + group; c < 8; c += AG_SLOTS) {
+            for (int c = c0; c < 8; c += AG_SLOTS) {
                 const int col = c % 4 * 16;
                 const bool dv = c < 4;
-                float4 angle[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) angle[e] = dv ? make_float4(1.f, 0.f, 1.f, 0.f) : __ldcg(table + col / 4 + e);
                 uint32_t r[16];
                 tc::ld16(lanes + AG_ACC + (keys ? c / 4 : u & 1u) * 64 + col, r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) angle[e] = next[e];
+                ask(c + AG_SLOTS, next);
                 tc::wait_ld(r);
                 if (f < p.S) {
                     if (keys && p.parts > 1) {
