@@ -56,11 +56,12 @@ __device__ __forceinline__ uint32_t turned_back(float a, float b, float cos, flo
 
 // Rotated copies of q and k, the table of cos and sin, and a query's lse and d side by side.  A block has 16 positions and a share of the
 // heads; 8 neighbouring lanes have a head's 64 values.
-constexpr int AP_POS = 16, AP_THREADS = 256;
+constexpr int AP_POS = 16, AP_HEADS = 32, AP_THREADS = 256;
 __global__ void __launch_bounds__(AP_THREADS)
 attn_grad_prepare_kernel(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* out, const __nv_bfloat16* dout, const float* lse, __nv_bfloat16* qrot,
                          __nv_bfloat16* krot, float2* table, float* stats, int* counter, int taken, int S, int padded, int Hq, int Hkv, float theta, int offset) {
     __shared__ float2 cs[AP_POS][AG_D / 2];
+    __shared__ float sums[AP_HEADS][AP_POS + 1];
     grid_dependency_wait();
     if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) *counter = taken;
     const int s0 = blockIdx.x * AP_POS, b = blockIdx.y, share = blockIdx.z, shares = gridDim.z;
@@ -82,27 +83,34 @@ attn_grad_prepare_kernel(const __nv_bfloat16* q, const __nv_bfloat16* k, const _
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
-    const int h0 = (int)((long long)Hq * share / shares), heads = (int)((long long)Hq * (share + 1) / shares) - h0;
+    const int h0 = (int)((long long)Hq * share / shares), h1 = (int)((long long)Hq * (share + 1) / shares);
+    for (int hc = h0; hc < h1; hc += AP_HEADS) {
+        const int heads = min(AP_HEADS, h1 - hc);
 #pragma unroll 2
-    for (int e = threadIdx.x; e < AP_POS * heads * 8; e += AP_THREADS) {              // (a multiple of 32: whole warps)
-        const int c = e % 8, h = h0 + e / 8 % heads, s = e / 8 / heads, pos = s0 + s;
-        float sum = 0.f;
-        if (pos < S) {
-            const size_t at = (((size_t)b * S + pos) * Hq + h) * 8 + c;
-            const uint4 x = reinterpret_cast<const uint4*>(q)[at], o = reinterpret_cast<const uint4*>(out)[at], d = reinterpret_cast<const uint4*>(dout)[at];
-            reinterpret_cast<uint4*>(qrot)[at] = rotate(x, s, c);
-            const uint32_t ow[4] = {o.x, o.y, o.z, o.w}, dw[4] = {d.x, d.y, d.z, d.w};
+        for (int e = threadIdx.x; e < AP_POS * heads * 8; e += AP_THREADS) {          // (a multiple of 32: whole warps)
+            const int c = e % 8, h = e / 8 % heads, s = e / 8 / heads, pos = s0 + s;
+            float sum = 0.f;
+            if (pos < S) {
+                const size_t at = (((size_t)b * S + pos) * Hq + hc + h) * 8 + c;
+                const uint4 x = reinterpret_cast<const uint4*>(q)[at], o = reinterpret_cast<const uint4*>(out)[at], d = reinterpret_cast<const uint4*>(dout)[at];
+                reinterpret_cast<uint4*>(qrot)[at] = rotate(x, s, c);
+                const uint32_t ow[4] = {o.x, o.y, o.z, o.w}, dw[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
-            for (int t = 0; t < 4; ++t) sum = fmaf(bf16_lo(ow[t]), bf16_lo(dw[t]), fmaf(bf16_hi(ow[t]), bf16_hi(dw[t]), sum));
+                for (int t = 0; t < 4; ++t) sum = fmaf(bf16_lo(ow[t]), bf16_lo(dw[t]), fmaf(bf16_hi(ow[t]), bf16_hi(dw[t]), sum));
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+            if (c == 0) sums[h][s] = sum;
         }
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-        if (c == 0 && pos < padded) {
-            float* to = stats + ((size_t)b * Hq + h) * 2 * padded + pos;
-            to[0] = pos < S ? lse[((size_t)b * Hq + h) * S + pos] * -1.4426950408889634f : -INFINITY;
-            to[padded] = pos < S ? -sum : 0.f;
+        __syncthreads();
+        for (int e = threadIdx.x; e < AP_POS * heads; e += AP_THREADS) {              // positions side by side, as lse and stats have them
+            const int s = e % AP_POS, h = e / AP_POS, pos = s0 + s;
+            float* to = stats + ((size_t)b * Hq + hc + h) * 2 * padded + pos;
+            to[0] = pos < S ? lse[((size_t)b * Hq + hc + h) * S + pos] * -1.4426950408889634f : -INFINITY;
+            to[padded] = pos < S ? -sums[h][s] : 0.f;
         }
+        __syncthreads();
     }
     const int g0 = (int)((long long)Hkv * share / shares), groups = (int)((long long)Hkv * (share + 1) / shares) - g0;
     for (int e = threadIdx.x; e < AP_POS * groups * 8; e += AP_THREADS) {
@@ -153,6 +161,12 @@ __device__ __forceinline__ AttnGradUnit attn_grad_unit(const AttnGradParams& p, 
     return w;
 }
 
+// The waits of the softmax warps: mostly over before they begin, so the loop is kept out of the tiles' code (3 x 1371 tokens 147 -> 142 us)
+__device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag) { return mbar_wait_warp(bar, parity, abort_flag); }
+__device__ __forceinline__ bool wait_quick(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || wait_on(bar, parity, abort_flag);
+}
+
 __device__ __forceinline__ uint32_t packed_bf16(uint64_t v) {
     float a, c;
     unpack_f32x2(v, a, c);
@@ -168,8 +182,8 @@ __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uin
         if (KEYS) asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(from + e * 4));
         else lo = hi = own;
     };
-    if (!mbar_wait_warp(smem_u32(&sh.s[slot]), parity, &sh.abort)) return false;
-    if (KEYS && !mbar_wait_warp(smem_u32(&sh.full[stage]), stage_parity, &sh.abort)) return false;      // (the statistics; they came before)
+    if (!wait_quick(smem_u32(&sh.s[slot]), parity, &sh.abort)) return false;
+    if (KEYS && !wait_quick(smem_u32(&sh.full[stage]), stage_parity, &sh.abort)) return false;      // (the statistics; they came before)
     tc::fence_after_sync();
     uint64_t pr[32];
     {
@@ -218,7 +232,7 @@ __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uin
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.p[slot]));
     }
-    if (!mbar_wait_warp(smem_u32(&sh.dp[slot]), parity, &sh.abort)) return false;
+    if (!wait_quick(smem_u32(&sh.dp[slot]), parity, &sh.abort)) return false;
     tc::fence_after_sync();
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {                     // (the second half's columns are read before any are written: 32 bf16 columns lie in 16)
@@ -434,7 +448,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_tile, const __grid_consta
                 for (int e = 0; e < 4; ++e) to[e] = c >= 4 && c < 8 ? table[c % 4 * 4 + e] : make_float4(1.f, 0.f, 1.f, 0.f);
             };
             ask(c0, next);
-            if (!mbar_wait_warp(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) return false;
+            if (!wait_quick(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) return false;
             tc::fence_after_sync();
 #pragma unroll 1
             for (int c = c0; c < 8; c += AG_SLOTS) {
