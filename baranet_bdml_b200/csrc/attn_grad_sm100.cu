@@ -21,7 +21,7 @@
 // 100 to 200 cycles each, where the products take 530 to 690.)  A slot's S is free for the next tile as soon as P X2 has been computed, or
 // a query block's group has read it, so S of a tile is there before its group is.
 // A block's gradients are stored by all groups, 16 columns at a time, each behind its first tile of the next block: a group that waited for
-// the block's last products and stored all of them held the others up (a pause of 10000 cycles a block, 165 -> X us at 3 x 1371).
+// the block's last products and stored all of them held the others up (a pause of 10000 cycles a block; 3 x 1371 tokens 165 -> 156 us).
 // Launch 3, where the heads of a group are shared by several blocks: their fp32 sums of dK and dV are added in order.
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
 #include <type_traits>

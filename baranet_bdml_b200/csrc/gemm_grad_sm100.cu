@@ -8,8 +8,8 @@
 // 64 contiguous m or n), so nothing is transposed in memory.
 // Persistent kernel, 192 threads: warps 0-3 epilogue, warp 4 issues the MMAs, warp 5 loads by TMA.  Output tile 128 x 256, or (PAIR) 256 x
 // 256 shared by a cluster of two CTAs (tcgen05.mma.cta_group::2); fp32 accumulators double buffered in tensor memory, so that the
-// epilogue of a tile runs under the products of the next.  Tiles go in bands of 16 tile rows, n outside, so that what runs at one time
-// shares both operands in L2.
+// epilogue of a tile runs under the products of the next.  Tiles may have 128 columns, where there are few
+// (tile_columns).  They go in bands of 16 tile rows, n outside, so that what runs at one time shares both operands in L2.
 //
 // Results leave through shared memory: a warp writes 32 rows of 128 bytes and one thread has TMA store them (a thread that stores its own
 // row takes 32 places in memory for every 16 bytes: 32000 x 2048 of K = 200 71 -> 46 us; eight epilogue warps instead of four 46, and 2 - 5 %
@@ -19,7 +19,7 @@
 //   STORE     the result as bf16
 //   PARTIAL   fp32 sums of a range of K, kept or added to what an earlier launch left: few tiles share K, pieces of the vocabulary follow
 //             one another.  An element gets one sum from a launch, and grad_sum_kernel adds the ranges in order: the same bits in every run
-//   LOSS      logits: of every row's 256 columns the maximum and the sum of exponentials, and the target's logit: the logits stay in
+//   LOSS      logits: of every row's columns in a tile the maximum and the sum of exponentials, and the target's logit: the logits stay in
 //             tensor memory
 //   DLOGITS   logits again -> g (exp(z - lse) - [v = target]) as bf16
 //   GLU       columns [0,128) gate, [128,256) up of the same indices, and dh, fp32 -> dgate, dup and the product that the forward pass had
@@ -37,13 +37,13 @@ using namespace ptx;
 constexpr int GG_BM = 128, GG_BN = 256, GG_BK = 64, GG_THREADS = 192, GG_BAND = 16;
 constexpr int GG_A_BYTES = GG_BM * GG_BK * 2;
 constexpr int GG_OUT_BYTES = 32 * 128;                                     // what a warp stores at a time
-template <bool PAIR, bool GLU> struct GradShape {
-    static constexpr int NSTAGE = PAIR ? 5 : GLU ? 3 : 4;
-    static constexpr int B_BYTES = (PAIR ? GG_BN / 2 : GG_BN) * GG_BK * 2;
-    static constexpr int STAGE_BYTES = GG_A_BYTES + B_BYTES;
-    static constexpr int OUT = GLU ? 3 : 2;                                // buffers of a warp: three results, or two in turn
-    static constexpr int SMEM_BYTES = 1024 + NSTAGE * STAGE_BYTES + 4 * OUT * GG_OUT_BYTES;
-};
+// Shared memory: as many stages of operands as fit beside each epilogue warp's buffers (GLU: one for each of three results, else two in turn)
+constexpr int GG_MAX_STAGES = 6;
+struct GradRing { int stage_bytes, stages; };
+constexpr GradRing grad_ring(bool pair, bool glu, int bn) {
+    const int stage = GG_A_BYTES + (pair ? bn / 2 : bn) * GG_BK * 2, room = 225 * 1024 - 4 * (glu ? 3 : 2) * GG_OUT_BYTES;
+    return {stage, room / stage < GG_MAX_STAGES ? room / stage : GG_MAX_STAGES};
+}
 
 constexpr int GE_STORE = 0, GE_PARTIAL = 1, GE_LOSS = 2, GE_DLOGITS = 3, GE_GLU = 4;
 // what the second pair of operands is: none, the second half of K (NN), further rows of the result (TN), the upper 128 columns of every
@@ -53,12 +53,14 @@ constexpr int SECOND_NONE = 0, SECOND_K = 1, SECOND_M = 2;
 struct GradParams {
     int M, N, K;                       // of one pair of operands
     int second;
+    int bn;                            // columns of a tile (GLU: of gate and up together)
+    GradRing ring;
     int splits, k_per_split;           // PARTIAL: ranges of K steps
     int* error_word;
     int add;                           // PARTIAL: added to what is there
     const int32_t* targets;            // LOSS, DLOGITS: (M), minus first_column is the column here
     int first_column;
-    float2* stats;                     // LOSS: [tile of 256 columns][M] maximum, sum of exponentials of the distances to it
+    float2* stats;                     // LOSS: [tile][M] maximum, sum of exponentials of the distances to it
     float* picked;                     // LOSS: (M) the target's logit
     const float *lse, *grad;           // DLOGITS: (M)
     const float* dh;                   // GLU: [dh_parts][M][N], to be added up
@@ -84,13 +86,13 @@ template <int ACT> __device__ __forceinline__ void act_and_slope(float z, float&
 template <bool A_MN, bool B_MN, int EPI, int ACT, bool PAIR>
 __global__ void __launch_bounds__(GG_THREADS, 1)
 gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
-    using Shape = GradShape<PAIR, EPI == GE_GLU>;
-    constexpr int NSTAGE = Shape::NSTAGE, STAGE_BYTES = Shape::STAGE_BYTES, TILE_M = PAIR ? 2 * GG_BM : GG_BM;
-    constexpr int N_HERE = PAIR ? GG_BN / 2 : GG_BN;                       // columns of the tile that this CTA loads
-    constexpr int COLUMNS = EPI == GE_GLU ? GG_BN / 2 : GG_BN;             // columns of the result that a tile covers
+    constexpr int TILE_M = PAIR ? 2 * GG_BM : GG_BM, OUT = EPI == GE_GLU ? 3 : 2;
+    const int n_stages = p.ring.stages;
+    const int n_here = PAIR ? p.bn / 2 : p.bn;                             // columns of the tile that this CTA loads
+    const int columns = EPI == GE_GLU ? p.bn / 2 : p.bn;                   // columns of the result that a tile covers
     constexpr uint32_t TMEM_COLS = 2 * GG_BN;
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bar_full[NSTAGE], bar_empty[NSTAGE], bar_acc_full[2], bar_acc_empty[2];
+    __shared__ __align__(8) uint64_t bar_full[GG_MAX_STAGES], bar_empty[GG_MAX_STAGES], bar_acc_full[2], bar_acc_empty[2];
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort;
 
@@ -99,7 +101,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     const uint32_t rank = PAIR ? cluster_rank() : 0;
     const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
     const int tiles_m0 = (p.M + TILE_M - 1) / TILE_M, tiles_m = p.second == SECOND_M ? 2 * tiles_m0 : tiles_m0;
-    const int tiles_n = (p.N + COLUMNS - 1) / COLUMNS, tiles = tiles_m * tiles_n;
+    const int tiles_n = (p.N + columns - 1) / columns, tiles = tiles_m * tiles_n;
     const int steps0 = (p.K + GG_BK - 1) / GG_BK, steps = p.second == SECOND_K ? 2 * steps0 : steps0;
     const int items = tiles * (EPI == GE_PARTIAL ? p.splits : 1);
     struct Item { int m, n, part, ks0, ks1; };                             // tile row and column; which operands; K steps
@@ -119,7 +121,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     };
 
     if (tid == 0) {
-        for (int s = 0; s < NSTAGE; ++s) {
+        for (int s = 0; s < n_stages; ++s) {
             mbar_init(smem_u32(&bar_full[s]), 1);
             mbar_init(smem_u32(&bar_empty[s]), 1);
         }
@@ -149,22 +151,23 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     if (warp == 5) {
         // ---------------------------------------------------------- TMA producer
         if (lane == 0) {
-            uint32_t it = 0;
+            int stage = 0;
+            uint32_t phase = 0;
             bool ok = true;
             for (int t = first; ok && t < items; t += stride) {
                 const Item w = item(t);
-                const int m0 = w.m * TILE_M + rank * GG_BM, n0 = w.n * COLUMNS + (EPI == GE_GLU ? 0 : rank * N_HERE);
-                for (int ks = w.ks0; ks < w.ks1; ++ks, ++it) {
-                    const int stage = it % NSTAGE;
-                    ok = mbar_wait(smem_u32(&bar_empty[stage]), ((it / NSTAGE) & 1u) ^ 1u, &s_abort);
+                const int m0 = w.m * TILE_M + rank * GG_BM, n0 = w.n * columns + (EPI == GE_GLU ? 0 : rank * n_here);
+                const uint32_t bytes = (PAIR ? 2 : 1) * (GG_A_BYTES + n_here * GG_BK * 2);
+                for (int ks = w.ks0; ks < w.ks1; ++ks) {
+                    ok = mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &s_abort);
                     if (!ok) break;
                     const bool half2 = p.second == SECOND_K && ks >= steps0;
                     const int k0 = (half2 ? ks - steps0 : ks) * GG_BK;
                     const CUtensorMap* ma = half2 || w.part ? &maps.a1 : &maps.a0;
                     const CUtensorMap* mb = half2 ? &maps.b1 : &maps.b0;
-                    const uint32_t sA = smem0 + stage * STAGE_BYTES, sB = sA + GG_A_BYTES;
+                    const uint32_t sA = smem0 + stage * p.ring.stage_bytes, sB = sA + GG_A_BYTES;
                     const uint32_t full = PAIR ? in_rank(smem_u32(&bar_full[stage]), 0) : smem_u32(&bar_full[stage]);
-                    if (rank == 0) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), (PAIR ? 2 : 1) * STAGE_BYTES);
+                    if (rank == 0) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), bytes);
                     auto load = [&](uint32_t dst, const CUtensorMap* m, int x, int y) {
                         if (PAIR) tma_load_2d_pair(dst, m, x, y, full);
                         else tma_load_2d(dst, m, x, y, full);
@@ -180,24 +183,25 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                             load(sB, rank ? &maps.b1 : &maps.b0, k0, n0);
                         } else {
                             load(sB, &maps.b0, k0, n0);
-                            load(sB + 128 * GG_BK * 2, &maps.b1, k0, n0);
+                            load(sB + p.bn / 2 * GG_BK * 2, &maps.b1, k0, n0);
                         }
                     } else if (B_MN) {
-#pragma unroll
-                        for (int j = 0; j < N_HERE / 64; ++j) load(sB + j * 8192, mb, n0 + j * 64, k0);
+                        for (int j = 0; j < n_here / 64; ++j) load(sB + j * 8192, mb, n0 + j * 64, k0);
                     } else {
                         load(sB, mb, k0, n0);
                     }
+                    if (++stage == n_stages) stage = 0, phase ^= 1u;
                 }
             }
         }
     } else if (warp == 4) {
         // ------------------------------------------------------------ MMA issuer
-        constexpr uint32_t IDESC = tc::idesc_bf16(TILE_M, GG_BN, B_MN ? 1 : 0) | (A_MN ? 1u << 15 : 0u);
+        const uint32_t IDESC = tc::idesc_bf16(TILE_M, p.bn, B_MN ? 1 : 0) | (A_MN ? 1u << 15 : 0u);
         const uint64_t dK = tc::smem_desc_sw128(0);                        // descriptor = this + (address >> 4)
         const uint64_t dMN = (dK & ~((uint64_t)0x3fff << 16)) | (uint64_t)(8192 >> 4) << 16;      // the next 64 m or n lie 8 KB on
         constexpr uint32_t A_STEP = A_MN ? 128 : 2, B_STEP = B_MN ? 128 : 2;                      // 16 k further, in 16 bytes
-        uint32_t it = 0, local = 0;
+        uint32_t local = 0, phase = 0;
+        int stage = 0;
         bool ok = rank == 0;
         for (int t = first; ok && t < items; t += stride, ++local) {
             const uint32_t acc = local & 1u;
@@ -205,13 +209,12 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
             if (!ok) break;
             tc::fence_after_sync();
             const Item w = item(t);
-            for (int ks = w.ks0; ks < w.ks1; ++ks, ++it) {
-                const int stage = it % NSTAGE;
-                ok = mbar_wait_warp(smem_u32(&bar_full[stage]), (it / NSTAGE) & 1u, &s_abort);
+            for (int ks = w.ks0; ks < w.ks1; ++ks) {
+                ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &s_abort);
                 if (!ok) break;
                 if (elect_one()) {
                     tc::fence_after_sync();
-                    const uint32_t sA = smem0 + stage * STAGE_BYTES, sB = sA + GG_A_BYTES;
+                    const uint32_t sA = smem0 + stage * p.ring.stage_bytes, sB = sA + GG_A_BYTES;
 #pragma unroll
                     for (int kk = 0; kk < GG_BK / 16; ++kk) {
                         const uint64_t da = (A_MN ? dMN : dK) + (uint64_t)((sA >> 4) + kk * A_STEP);
@@ -229,12 +232,13 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                     }
                 }
                 __syncwarp();
+                if (++stage == n_stages) stage = 0, phase ^= 1u;
             }
         }
     } else {
         // ------------------------------------------------------ epilogue: thread = row of the tile = TMEM lane
         const uint32_t lane_base = ((uint32_t)(warp * 32)) << 16;
-        const uint32_t out0 = smem0 + NSTAGE * STAGE_BYTES + warp * Shape::OUT * GG_OUT_BYTES;
+        const uint32_t out0 = smem0 + n_stages * p.ring.stage_bytes + warp * OUT * GG_OUT_BYTES;
         int out_turn = 0;
         // the warp's next buffer, when what was sent from it before has been read
         auto out_buffer = [&] {
@@ -266,7 +270,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
         for (int t = first; ok && t < items; t += stride, ++local) {
             const uint32_t acc = local & 1u;
             const Item w = item(t);
-            const int gm = w.m * TILE_M + rank * GG_BM + tid, n0 = w.n * COLUMNS;
+            const int gm = w.m * TILE_M + rank * GG_BM + tid, n0 = w.n * columns;
             const bool live = gm < p.M;
             // what a row needs beside its products, fetched while those run
             int target = -1;
@@ -281,6 +285,26 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                     target = INT32_MIN;                                    // no loss, no gradient
                 }
             }
+            float d[EPI == GE_GLU ? 32 : 1];                               // 32 columns of dh
+            auto load_dh = [&](int col0) {
+                if (EPI != GE_GLU || col0 >= p.N) return;
+                const float4* from = reinterpret_cast<const float4*>(p.dh + (size_t)(live ? gm : 0) * p.N + col0);
+                const size_t part = (size_t)p.M * p.N / 4;
+#pragma unroll
+                for (int v = 0; v < 8; ++v) {                              // (columns are a multiple of 8)
+                    const float4 f = col0 + v * 4 < p.N ? __ldcg(from + v) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    d[v * 4] = f.x; d[v * 4 + 1] = f.y; d[v * 4 + 2] = f.z; d[v * 4 + 3] = f.w;
+                }
+#pragma unroll 2
+                for (int k = 1; k < p.dh_parts; ++k) {                     // (eight loads under way, or sixteen)
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) {
+                        const float4 f = col0 + v * 4 < p.N ? __ldcg(from + k * part + v) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        d[v * 4] += f.x; d[v * 4 + 1] += f.y; d[v * 4 + 2] += f.z; d[v * 4 + 3] += f.w;
+                    }
+                }
+            };
+            load_dh(n0);
             ok = mbar_wait_warp(smem_u32(&bar_acc_full[acc]), (local >> 1) & 1u, &s_abort);
             if (!ok) break;
             tc::fence_after_sync();
@@ -288,7 +312,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
             const int y = w.m * TILE_M + rank * GG_BM + warp * 32;          // the warp's first row
             if (EPI == GE_STORE || EPI == GE_DLOGITS) {
 #pragma unroll 1
-                for (int c = 0; c < GG_BN / 64; ++c) {
+                for (int c = 0; c < p.bn / 64; ++c) {
                     if (n0 + c * 64 >= p.N) break;                         // (uniform)
                     const uint32_t buf = out_buffer();
 #pragma unroll
@@ -310,7 +334,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                 }
             } else if (EPI == GE_PARTIAL) {
 #pragma unroll 1
-                for (int c = 0; c < GG_BN / 32; ++c) {
+                for (int c = 0; c < p.bn / 32; ++c) {
                     if (n0 + c * 32 >= p.N) break;
                     const uint32_t buf = out_buffer();
                     uint32_t r[32];
@@ -328,7 +352,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                 // one pass: the sum is kept relative to the largest logit so far
                 float top = -INFINITY, sum = 0.f;
 #pragma unroll 1
-                for (int c = 0; c < GG_BN / 32; ++c) {
+                for (int c = 0; c < p.bn / 32; ++c) {
                     uint32_t r[32];
                     tc::ld32(tacc + c * 32, r);
                     tc::wait_ld(r);
@@ -361,28 +385,12 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
             } else {
                 const uint32_t h_buf = out0, g_buf = out0 + GG_OUT_BYTES, u_buf = out0 + 2 * GG_OUT_BYTES;
 #pragma unroll 1
-                for (int c = 0; c < GG_BN / 64; ++c) {                     // 32 columns: half of what is stored at a time
+                for (int c = 0; c < p.bn / 64; ++c) {                      // 32 columns: half of what is stored at a time
                     const int col0 = n0 + c * 32;
                     if (col0 >= p.N) break;
-                    float d[32];
-                    const float4* from = reinterpret_cast<const float4*>(p.dh + (size_t)(live ? gm : 0) * p.N + col0);
-                    const size_t part = (size_t)p.M * p.N / 4;
-#pragma unroll
-                    for (int v = 0; v < 8; ++v) {                          // (columns are a multiple of 8)
-                        const float4 f = col0 + v * 4 < p.N ? __ldcg(from + v) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        d[v * 4] = f.x; d[v * 4 + 1] = f.y; d[v * 4 + 2] = f.z; d[v * 4 + 3] = f.w;
-                    }
-#pragma unroll 1
-                    for (int k = 1; k < p.dh_parts; ++k) {                 // (eight loads under way, not one)
-#pragma unroll
-                        for (int v = 0; v < 8; ++v) {
-                            const float4 f = col0 + v * 4 < p.N ? __ldcg(from + k * part + v) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            d[v * 4] += f.x; d[v * 4 + 1] += f.y; d[v * 4 + 2] += f.z; d[v * 4 + 3] += f.w;
-                        }
-                    }
                     uint32_t g[32], u[32];
                     tc::ld32(tacc + c * 32, g);
-                    tc::ld32(tacc + GG_BN / 2 + c * 32, u);
+                    tc::ld32(tacc + p.bn / 2 + c * 32, u);
                     tc::wait_ld(g);
                     tc::wait_ld(u);
                     if (c % 2 == 0) {                                      // the buffers have been read
@@ -414,6 +422,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                         put16(g_buf, chunk, g4[0], g4[1], g4[2], g4[3]);
                         put16(u_buf, chunk, u4[0], u4[1], u4[2], u4[3]);
                     }
+                    if (c + 1 < p.bn / 64) load_dh(col0 + 32);             // (the next tile's: before its products are waited for)
                     if ((c % 2 == 1 || col0 + 32 >= p.N) && y < p.M) {     // (what a last half does not fill lies behind the columns)
                         const int x = n0 + c / 2 * 64;
                         send([&] {
@@ -447,12 +456,13 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
 }
 
 // the ranges' sums, added in their order, rounded once
-__global__ void __launch_bounds__(256) grad_sum_kernel(const float* partial, __nv_bfloat16* c, long long groups, int splits) {
+__global__ void __launch_bounds__(128) grad_sum_kernel(const float* partial, __nv_bfloat16* c, long long groups, int splits) {
     grid_dependency_wait();
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;  // of 4 elements
+    const long long i = (long long)blockIdx.x * 128 + threadIdx.x;         // of 4 elements
     if (i >= groups) return;
     const float4* p4 = reinterpret_cast<const float4*>(partial);
     float4 s = __ldcg(p4 + i);
+#pragma unroll 8
     for (int k = 1; k < splits; ++k) {
         const float4 v = __ldcg(p4 + (long long)k * groups + i);
         s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
@@ -510,20 +520,23 @@ struct Result {
     long long ld;
 };
 
-// Whether two CTAs share a tile: not where one wave of single tiles is all there is, nor where tiles of twice the rows make a wave more
-// than they save (an eighth).
-bool grad_pairs(int M, int columns, int second) {
-    const long long sms = sm_count(), twice = second == SECOND_M ? 2 : 1, single = twice * ((M + GG_BM - 1) / GG_BM) * columns,
-                    pairs = twice * ((M + 2 * GG_BM - 1) / (2 * GG_BM)) * columns;
+// How a product is cut.  Two CTAs share a tile of 256 x 256, but not where one wave of single tiles is all there is, nor where tiles of twice
+// the rows make a wave more than they save (an eighth).  Single tiles that would leave half of the SMs without one have 128 columns: what
+// few rows wait for is the weight, and more SMs ask for it (gradients of a gated block of 64 rows, 2048 x 5632: 84 us with 44 tiles for gate
+// and up, 79 with 88, 75 with the stages that the narrower tiles leave room for).
+struct Cut { bool pair; int bn; };
+Cut tile_columns(int M, int N, int second, bool glu) {
+    const long long sms = sm_count(), twice = second == SECOND_M ? 2 : 1, columns = (N + (glu ? GG_BN / 2 : GG_BN) - 1) / (glu ? GG_BN / 2 : GG_BN);
+    const long long single = twice * ((M + GG_BM - 1) / GG_BM) * columns, pairs = twice * ((M + 2 * GG_BM - 1) / (2 * GG_BM)) * columns;
     const long long waves = (single + sms - 1) / sms, waves_of_pairs = (pairs + sms / 2 - 1) / (sms / 2);
-    return waves > 1 && waves_of_pairs * 7 <= waves * 8;
+    return {waves > 1 && waves_of_pairs * 7 <= waves * 8, 2 * single <= sms ? GG_BN / 2 : GG_BN};
 }
 
 template <bool A_MN, bool B_MN, int EPI, int ACT, bool PAIR>
 int grad_run(const GradMaps& m, const GradParams& p, unsigned grid, cudaStream_t st, const char* what) {
-    constexpr size_t smem = GradShape<PAIR, EPI == GE_GLU>::SMEM_BYTES;
+    const size_t smem = 1024 + (size_t)p.ring.stages * p.ring.stage_bytes + 4 * (EPI == GE_GLU ? 3 : 2) * GG_OUT_BYTES;
     auto kernel = gemm_grad_kernel<A_MN, B_MN, EPI, ACT, PAIR>;
-    if (int rc = allow_smem(kernel, smem, what, smem)) return rc;
+    if (int rc = allow_smem(kernel, smem, what, 226 * 1024)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(GG_THREADS);
@@ -553,9 +566,13 @@ int grad_run(const GradMaps& m, const GradParams& p, unsigned grid, cudaStream_t
 // M, N, K > 0; all sizes and addresses are ones that a tensor map takes
 template <bool A_MN, bool B_MN, int EPI, int ACT = 0>
 int grad_gemm(const Operand& a, const Operand& b, const Result& c, GradParams p, cudaStream_t st, const char* what) {
-    const int columns = EPI == GE_GLU ? GG_BN / 2 : GG_BN, tiles_n = (p.N + columns - 1) / columns, sms = sm_count();
-    const bool pair = p.splits <= 1 && grad_pairs(p.M, tiles_n, p.second);
-    const uint32_t n_box = EPI == GE_GLU ? 128 : pair ? GG_BN / 2 : GG_BN;
+    const int sms = sm_count();
+    const Cut cut = p.splits > 1 ? Cut{false, GG_BN} : tile_columns(p.M, p.N, p.second, EPI == GE_GLU);
+    const bool pair = cut.pair;
+    p.bn = cut.bn;
+    p.ring = grad_ring(pair, EPI == GE_GLU, p.bn);
+    const int columns = EPI == GE_GLU ? p.bn / 2 : p.bn, tiles_n = (p.N + columns - 1) / columns;
+    const uint32_t n_box = EPI == GE_GLU || pair ? p.bn / 2 : p.bn;
     GradMaps m;
     auto map = [&](CUtensorMap* out, const void* base, long long ld, bool mn, int extent, uint32_t box_rows) {
         const uint64_t dims[2] = {(uint64_t)(mn ? extent : p.K), (uint64_t)(mn ? p.K : extent)}, strides[1] = {(uint64_t)ld * 2};
@@ -589,11 +606,11 @@ int grad_gemm(const Operand& a, const Operand& b, const Result& c, GradParams p,
     return pair ? grad_run<A_MN, B_MN, EPI, ACT, true>(m, p, grid, st, what) : grad_run<A_MN, B_MN, EPI, ACT, false>(m, p, grid, st, what);
 }
 
-// Ranges of K for a product of few tiles: about one work item for every SM, none shorter than 8 steps of 64
+// Ranges of K for a product of few tiles: about one work item for every SM, none shorter than 4 steps of 64
 void grad_splits(int M, int N, int K_steps, int* splits, int* per) {
     const long long tiles = (long long)((M + GG_BM - 1) / GG_BM) * ((N + GG_BN - 1) / GG_BN), sms = sm_count();
     long long want = tiles * 2 > sms ? 1 : sms / tiles;
-    if (want > K_steps / 8) want = K_steps / 8 > 0 ? K_steps / 8 : 1;
+    if (want > K_steps / 4) want = K_steps / 4 > 0 ? K_steps / 4 : 1;
     *per = (int)((K_steps + want - 1) / want);
     *splits = (K_steps + *per - 1) / *per;
 }
@@ -609,7 +626,7 @@ size_t nn_bytes(int M, int N, int K_steps, bool pieces) {
 }
 int nn_sum(const float* partial, void* c, int M, int N, int splits, cudaStream_t st, const char* what) {
     const long long groups = (long long)M * N / 4;
-    launch_dependent(grad_sum_kernel, (unsigned)((groups + 255) / 256), 256, 0, st, partial, static_cast<__nv_bfloat16*>(c), groups, splits);
+    launch_dependent(grad_sum_kernel, (unsigned)((groups + 127) / 128), 128, 0, st, partial, static_cast<__nv_bfloat16*>(c), groups, splits);
     return launch_status(what);
 }
 int nn_product(const Operand& a, const Operand& b, void* c, int M, int N, int K, int second, float* partial, int* error_word, cudaStream_t st, const char* what) {
@@ -701,7 +718,8 @@ extern "C" int bn_gemm_bf16_tn(const void* a, const void* b, void* c, int M, int
 // ------------------------------------------------------------------------------------------------- loss over the vocabulary
 extern "C" size_t bn_linear_cross_entropy_bf16_workspace_bytes(int rows, int vocab, int hidden) {
     if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
-    const size_t tiles = ((size_t)vocab + GG_BN - 1) / GG_BN;
+    const int columns = tile_columns(rows, vocab, SECOND_NONE, false).bn;
+    const size_t tiles = ((size_t)vocab + columns - 1) / columns;
     return up256(tiles * rows * sizeof(float2)) + up256((size_t)rows * sizeof(float));
 }
 
@@ -713,7 +731,7 @@ extern "C" int bn_linear_cross_entropy_bf16(const void* x, const void* weight_t,
     if (int rc = require_sm100()) return rc;
     if (rows == 0) return BN_OK;
     if (int rc = check_ws(what, workspace, workspace_bytes, bn_linear_cross_entropy_bf16_workspace_bytes(rows, vocab, hidden))) return rc;
-    const int tiles = (vocab + GG_BN - 1) / GG_BN;
+    const int columns = tile_columns(rows, vocab, SECOND_NONE, false).bn, tiles = (vocab + columns - 1) / columns;
     GradParams p{};
     p.M = rows; p.N = vocab; p.K = hidden; p.error_word = error_word;
     p.targets = targets;
