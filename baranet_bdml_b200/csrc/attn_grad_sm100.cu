@@ -607,7 +607,7 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
                                              void* dk, void* dv, int B, int S, int Hq, int Hkv, int D, float scale, float theta, int position_offset,
                                              int causal, void* workspace, size_t workspace_bytes, int* error_word, bn_stream_t stream) {
     const char* what = "bn_attn_prefill_bf16_backward";
-    if (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (B > 0 && S > 0 && (!dout || !q || !k || !v || !out || !lse || !dq || !dk || !dv)) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape B=%d S=%d Hq=%d Hkv=%d", what, B, S, Hq, Hkv);
     if (Hq % Hkv) return fail(BN_ERR_INVALID_ARG, "%s: Hq=%d not a multiple of Hkv=%d", what, Hq, Hkv);
     if (D != AG_D) return fail(BN_ERR_UNSUPPORTED, "%s: head_dim=%d (64 supported)", what, D);

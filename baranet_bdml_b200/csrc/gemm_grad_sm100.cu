@@ -21,7 +21,7 @@
 //             one another.  An element gets one sum from a launch, and grad_sum_kernel adds the ranges in order: the same bits in every run
 //   LOSS      logits: of every row's columns in a tile the maximum and the sum of exponentials, and the target's logit: the logits stay in
 //             tensor memory
-//   DLOGITS   logits again -> g (exp(z - lse) - [v = target]) as bf16
+//   DLOGITS   logits again -> g (exp(z - lse) - [v = target]) over the first row's g, as bf16
 //   GLU       columns [0,128) gate, [128,256) up of the same indices, and dh, fp32 -> dgate, dup and the product that the forward pass had
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
 #include "common.cuh"
@@ -59,10 +59,11 @@ struct GradParams {
     int* error_word;
     int add;                           // PARTIAL: added to what is there
     const int32_t* targets;            // LOSS, DLOGITS: (M), minus first_column is the column here
-    int first_column;
+    int first_column, vocab;
     float2* stats;                     // LOSS: [tile][M] maximum, sum of exponentials of the distances to it
     float* picked;                     // LOSS: (M) the target's logit
     const float *lse, *grad;           // DLOGITS: (M)
+    const float* factor;               // STORE: what common_factor makes of it is a factor of the result
     const float* dh;                   // GLU: [dh_parts][M][N], to be added up
     int dh_parts;
 };
@@ -70,6 +71,13 @@ struct GradParams {
 // Tensor maps of the operands and of what is stored: STORE c0 and (of the second rows) c1, bf16; PARTIAL c0, fp32 (N, M, split); DLOGITS c0;
 // GLU c0 = h, c1 = dgate, c2 = dup
 struct GradMaps { CUtensorMap a0, a1, b0, b1, c0, c1, c2; };
+
+// What the logits' gradients are divided by before they are rounded, and their products multiplied by: the first row's gradient, so that a
+// mean's 1 / rows, which all rows have, is not rounded to bf16 in every one of them alike (errors of 2.9e-3 instead of 2.4e-3)
+__device__ __forceinline__ float common_factor(const float* grad) {
+    const float g = grad ? *grad : 1.f, size = fabsf(g);
+    return size >= 0x1p-40f && size <= 0x1p40f ? g : 1.f;
+}
 
 __device__ __forceinline__ float log2e() { return 1.4426950408889634f; }
 
@@ -278,9 +286,9 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
             if ((EPI == GE_LOSS || EPI == GE_DLOGITS) && live) {
                 const int v = p.targets[gm];
                 target = v < 0 ? -1 : v - p.first_column;
-                if (EPI == GE_DLOGITS && v >= 0) {
+                if (EPI == GE_DLOGITS && v >= 0 && v < p.vocab) {
                     lse2 = p.lse[gm] * log2e();
-                    grad = p.grad[gm];
+                    grad = p.grad[gm] / common_factor(p.grad);
                 } else if (EPI == GE_DLOGITS) {
                     target = INT32_MIN;                                    // no loss, no gradient
                 }
@@ -320,6 +328,11 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                         uint32_t r[32];
                         tc::ld32(tacc + c * 64 + hf * 32, r);
                         tc::wait_ld(r);
+                        if (EPI == GE_STORE && p.factor) {
+                            const float factor = common_factor(p.factor);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
+                        }
                         if (EPI == GE_DLOGITS) {
                             const int at = target - (n0 + c * 64 + hf * 32);
 #pragma unroll
@@ -456,7 +469,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
 }
 
 // the ranges' sums, added in their order, rounded once
-__global__ void __launch_bounds__(128) grad_sum_kernel(const float* partial, __nv_bfloat16* c, long long groups, int splits) {
+__global__ void __launch_bounds__(128) grad_sum_kernel(const float* partial, __nv_bfloat16* c, long long groups, int splits, const float* factor) {
     grid_dependency_wait();
     const long long i = (long long)blockIdx.x * 128 + threadIdx.x;         // of 4 elements
     if (i >= groups) return;
@@ -467,7 +480,8 @@ __global__ void __launch_bounds__(128) grad_sum_kernel(const float* partial, __n
         const float4 v = __ldcg(p4 + (long long)k * groups + i);
         s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
-    reinterpret_cast<uint2*>(c)[i] = make_uint2(pack_bf16(s.x, s.y), pack_bf16(s.z, s.w));
+    const float f = common_factor(factor);
+    reinterpret_cast<uint2*>(c)[i] = make_uint2(pack_bf16(s.x * f, s.y * f), pack_bf16(s.z * f, s.w * f));
 }
 
 // the tiles' maxima and sums of 32 rows: 32 warps take the tiles in turn, the first warp joins theirs
@@ -624,9 +638,9 @@ size_t nn_bytes(int M, int N, int K_steps, bool pieces) {
     grad_splits(M, N, K_steps, &splits, &per);
     return splits > 1 || pieces ? up256((size_t)splits * M * N * 4) : 0;
 }
-int nn_sum(const float* partial, void* c, int M, int N, int splits, cudaStream_t st, const char* what) {
+int nn_sum(const float* partial, void* c, int M, int N, int splits, const float* factor, cudaStream_t st, const char* what) {
     const long long groups = (long long)M * N / 4;
-    launch_dependent(grad_sum_kernel, (unsigned)((groups + 127) / 128), 128, 0, st, partial, static_cast<__nv_bfloat16*>(c), groups, splits);
+    launch_dependent(grad_sum_kernel, (unsigned)((groups + 127) / 128), 128, 0, st, partial, static_cast<__nv_bfloat16*>(c), groups, splits, factor);
     return launch_status(what);
 }
 int nn_product(const Operand& a, const Operand& b, void* c, int M, int N, int K, int second, float* partial, int* error_word, cudaStream_t st, const char* what) {
@@ -635,12 +649,13 @@ int nn_product(const Operand& a, const Operand& b, void* c, int M, int N, int K,
     grad_splits(M, N, steps_of(K) * (second == SECOND_K ? 2 : 1), &p.splits, &p.k_per_split);
     if (p.splits == 1) return grad_gemm<false, true, GE_STORE>(a, b, {c, nullptr, nullptr, N}, p, st, what);
     if (int rc = grad_gemm<false, true, GE_PARTIAL>(a, b, {partial, nullptr, nullptr, N}, p, st, what)) return rc;
-    return nn_sum(partial, c, M, N, p.splits, st, what);
+    return nn_sum(partial, c, M, N, p.splits, nullptr, st, what);
 }
 
-int tn_product(const Operand& a, const Operand& b, void* c0, void* c1, int M, int N, int K, int* error_word, cudaStream_t st, const char* what) {
+int tn_product(const Operand& a, const Operand& b, void* c0, void* c1, int M, int N, int K, int* error_word, cudaStream_t st, const char* what,
+               const float* factor = nullptr) {
     GradParams p{};
-    p.M = M; p.N = N; p.K = K; p.second = c1 ? SECOND_M : SECOND_NONE; p.error_word = error_word;
+    p.M = M; p.N = N; p.K = K; p.second = c1 ? SECOND_M : SECOND_NONE; p.error_word = error_word; p.factor = factor;
     return grad_gemm<true, true, GE_STORE>(a, b, {c0, c1, nullptr, N}, p, st, what);
 }
 
@@ -669,7 +684,7 @@ int piece_columns(int rows, int vocab) {
 }
 
 int check_loss(const char* what, const void* x, const void* w, const void* targets, int rows, int vocab, int hidden) {
-    if (!x || !w || !targets) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (!w || (rows > 0 && (!x || !targets))) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (rows < 0 || vocab <= 0 || hidden <= 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape rows=%d vocab=%d hidden=%d", what, rows, vocab, hidden);
     if (hidden % 8) return fail(BN_ERR_UNSUPPORTED, "%s: hidden=%d must be a multiple of 8 (16-byte rows)", what, hidden);
     if (vocab > INT32_MAX - 256) return fail(BN_ERR_UNSUPPORTED, "%s: vocab=%d", what, vocab);
@@ -689,7 +704,7 @@ int check_ws(const char* what, const void* ws, size_t given, size_t needed) {
 extern "C" size_t bn_gemm_bf16_nn_workspace_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? nn_bytes(M, N, steps_of(K), false) : 0; }
 
 static int check_product(const char* what, const void* a, const void* b, const void* c, int M, int N, int K, int inner_a) {
-    if (!a || !b || !c) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if ((M > 0 && N > 0 && !c) || (M > 0 && K > 0 && !a) || (N > 0 && K > 0 && !b)) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (M < 0 || N < 0 || K < 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape M=%d N=%d K=%d", what, M, N, K);
     if (N % 8 || inner_a % 8) return fail(BN_ERR_UNSUPPORTED, "%s: rows of %d and %d elements must be multiples of 8 (16 bytes)", what, inner_a, N);
     if (misaligned({a, b, c})) return fail(BN_ERR_INVALID_ARG, "%s: a/b/c must be 16-byte aligned", what);
@@ -727,7 +742,7 @@ extern "C" int bn_linear_cross_entropy_bf16(const void* x, const void* weight_t,
                                             int hidden, void* workspace, size_t workspace_bytes, int* id_error, int* error_word, bn_stream_t stream) {
     const char* what = "bn_linear_cross_entropy_bf16";
     if (int rc = check_loss(what, x, weight_t, targets, rows, vocab, hidden)) return rc;
-    if (!loss) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (rows > 0 && !loss) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (int rc = require_sm100()) return rc;
     if (rows == 0) return BN_OK;
     if (int rc = check_ws(what, workspace, workspace_bytes, bn_linear_cross_entropy_bf16_workspace_bytes(rows, vocab, hidden))) return rc;
@@ -755,7 +770,7 @@ extern "C" int bn_linear_cross_entropy_backward_bf16(const void* x, const void* 
                                                      int* error_word, bn_stream_t stream) {
     const char* what = "bn_linear_cross_entropy_backward_bf16";
     if (int rc = check_loss(what, x, weight_t, targets, rows, vocab, hidden)) return rc;
-    if (!lse || !grad_loss || (!dx && !dweight_t)) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (rows > 0 && (!lse || !grad_loss || (!dx && !dweight_t))) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (misaligned({dx, dweight_t})) return fail(BN_ERR_INVALID_ARG, "%s: gradients must be 16-byte aligned", what);
     if (int rc = require_sm100()) return rc;
     cudaStream_t st = as_stream(stream);
@@ -772,11 +787,11 @@ extern "C" int bn_linear_cross_entropy_backward_bf16(const void* x, const void* 
         const void* w = static_cast<const __nv_bfloat16*>(weight_t) + (size_t)v0 * hidden;
         GradParams p{};
         p.M = rows; p.N = n; p.K = hidden; p.error_word = error_word;
-        p.targets = targets; p.first_column = v0; p.lse = lse; p.grad = grad_loss;
+        p.targets = targets; p.first_column = v0; p.vocab = vocab; p.lse = lse; p.grad = grad_loss;
         if (int rc = grad_gemm<false, false, GE_DLOGITS>({x, nullptr, hidden}, {w, nullptr, hidden}, {ws, nullptr, nullptr, columns}, p, st, what)) return rc;
         if (dx) {
             GradParams q{};
-            q.M = rows; q.N = hidden; q.K = n; q.error_word = error_word;
+            q.M = rows; q.N = hidden; q.K = n; q.error_word = error_word; q.factor = grad_loss;
             const Operand dz{ws, nullptr, columns}, wt{w, nullptr, hidden};
             if (sums) {
                 // a last, shorter piece leaves ranges without a step: they are not launched, and what they have so far stays
@@ -790,10 +805,10 @@ extern "C" int bn_linear_cross_entropy_backward_bf16(const void* x, const void* 
         }
         if (dweight_t)
             if (int rc = tn_product({ws, nullptr, columns}, {x, nullptr, hidden}, static_cast<__nv_bfloat16*>(dweight_t) + (size_t)v0 * hidden, nullptr, n,
-                                    hidden, rows, error_word, st, what))
+                                    hidden, rows, error_word, st, what, grad_loss))
                 return rc;
     }
-    return dx && sums ? nn_sum(partial, dx, rows, hidden, splits, st, what) : BN_OK;
+    return dx && sums ? nn_sum(partial, dx, rows, hidden, splits, grad_loss, st, what) : BN_OK;
 }
 
 // --------------------------------------------------------------------------------------------- gated feed-forward block
@@ -809,7 +824,7 @@ extern "C" int bn_gated_ff_backward_bf16(const void* dy, const void* x, const vo
                                          void* dup_t, void* ddown_t, int rows, int hidden, int inter, int act, void* workspace, size_t workspace_bytes,
                                          int* error_word, bn_stream_t stream) {
     const char* what = "bn_gated_ff_backward_bf16";
-    if (!dy || !x || !gate_t || !up_t || !down_t || !dx || !dgate_t || !dup_t || !ddown_t) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (!gate_t || !up_t || !down_t || !dgate_t || !dup_t || !ddown_t || (rows > 0 && (!dy || !x || !dx))) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (rows < 0 || hidden <= 0 || inter <= 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape rows=%d hidden=%d inter=%d", what, rows, hidden, inter);
     if (hidden % 8 || inter % 8)
         return fail(BN_ERR_UNSUPPORTED, "%s: hidden=%d and inter=%d must be multiples of 8 (16-byte rows)", what, hidden, inter);

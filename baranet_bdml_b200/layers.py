@@ -179,7 +179,8 @@ class GroupedQueryAttentionBF16:
     bf16; RoPE(K) in its epilogue), the core is `bn_attn_prefill_bf16` (RoPE(Q), causal softmax, P V fused), o_proj
     is `bn_gemm_bf16_nt`: three kernel launches.  Same constructor arguments, attribute names and
     `__call__(hidden_states, position_offset, use_causal_mask)` as mygrad/llama/llama_layers.py:46-191;
-    hidden_states is a torch bf16 tensor (B, S, hidden) or (S, hidden) on the GPU.  Inference only."""
+    hidden_states is a torch bf16 tensor (B, S, hidden) or (S, hidden) on the GPU.  A call keeps nothing for a backward
+    pass: `backward` takes the input again."""
 
     def __init__(self, config, is_cuda: bool = True):
         import torch
@@ -245,6 +246,28 @@ class GroupedQueryAttentionBF16:
         out = ops.gemm_bf16_nt(attn, self.o_proj).view(B, S, H)
         return out if hidden_states.dim() == 3 else out[0]
 
+    def backward(self, grad_output, hidden_states, position_offset: int = 0, use_causal_mask: bool = True):
+        """Gradients of `__call__` by its input and by parameters(), in their order, given the gradient of its output and its
+        input: (grad_input, [grad_q, grad_k, grad_v, grad_o]).  q, k, v and the attention rows are computed again."""
+        import torch
+        from . import ops
+        x = hidden_states if hidden_states.dim() == 3 else hidden_states[None]
+        B, S, H = x.shape
+        if H != self.hidden_size or grad_output.shape != hidden_states.shape:
+            raise RuntimeError("Attention: hidden size mismatch")
+        n, nq, nkv, D = B * S, self.num_heads, self.num_kv_heads, self.head_dim
+        x2, dy = x.reshape(n, H), grad_output.reshape(n, H)
+        q = ops.gemm_bf16_nt(x2, self.q_proj).view(B, S, nq, D)
+        k, v = (ops.gemm_bf16_nt(x2, w).view(B, S, nkv, D) for w in (self.k_proj, self.v_proj))
+        lse = torch.empty((B, nq, S), dtype=torch.float32, device=x.device)
+        how = dict(scale=float(self.scale), theta=self.rotary_emb.base, position_offset=position_offset, causal=use_causal_mask)
+        attn = ops.attn_prefill_bf16(q, k, v, lse=lse, **how)
+        dattn = ops.gemm_bf16_nn(dy, self.o_proj).view(B, S, nq, D)
+        do = ops.gemm_bf16_tn(dy, attn.view(n, nq * D))
+        dqkv = torch.cat([g.view(n, -1) for g in ops.attn_prefill_bf16_backward(dattn, q, k, v, attn, lse, **how)], dim=1)
+        dx = ops.gemm_bf16_nn(dqkv, self.packed_qkv()).view(hidden_states.shape)
+        return dx, [*ops.gemm_bf16_tn(dqkv, x2).split([nq * D, nkv * D, nkv * D]), do]
+
     def parameters(self):
         return [self.q_proj, self.k_proj, self.v_proj, self.o_proj]
 
@@ -253,7 +276,7 @@ class MLPBF16:
     """The SwiGLU feed-forward block (mygrad/llama/llama_layers.py:194-235: gate_proj, up_proj, down_proj;
     `(SiLU(x @ gate) * (x @ up)) @ down`) on the tensor-core path: one fused gate/up GEMM with the SiLU * mul epilogue
     and one down GEMM.  Weights are held transposed in bf16; `gate_proj` / `up_proj` / `down_proj` keep the reference's
-    names.  x: torch bf16 (tokens, hidden) on the GPU.  Inference only."""
+    names.  x: torch bf16 (tokens, hidden) on the GPU.  A call keeps nothing for a backward pass: `backward` takes x again."""
 
     def __init__(self, config, is_cuda: bool = True):
         import torch
@@ -279,6 +302,13 @@ class MLPBF16:
         # the down projection has few output tiles: with few rows (a decode step) the split-K form streams its weight
         # with all SMs
         return ops.linear_bf16(h, self.down_proj) if few_rows else ops.gemm_bf16_nt(h, self.down_proj)
+
+    def backward(self, grad_output, x):
+        """Gradients of `__call__` by x and by parameters(), in their order, given the gradient of its output and x:
+        (grad_x, [grad_gate, grad_up, grad_down])."""
+        from . import ops
+        dx, *grads = ops.gated_ff_backward(grad_output, x, self.gate_proj, self.up_proj, self.down_proj, act="silu")
+        return dx, grads
 
     def parameters(self):
         return [self.gate_proj, self.up_proj, self.down_proj]

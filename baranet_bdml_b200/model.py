@@ -284,6 +284,24 @@ class LLaMAModelBF16(CausalLM):
         H = self.config.hidden_size
         return self._logits(h.reshape(B * S, H), pending.reshape(B * S, H)).view(B, S, -1)
 
+    def score(self, input_ids: torch.Tensor) -> torch.Tensor:
+        """The log-probability that the model gives each id behind the first: (B, S) ids -> (B, S - 1) fp32.  The logits, which
+        `__call__` returns as B * S * vocab numbers, are kept nowhere."""
+        B, S = input_ids.shape
+        H, ids = self.config.hidden_size, input_ids.to(torch.int32)
+        if S < 2:
+            raise RuntimeError(f"score: {S} ids in a sequence; the first has no probability, so at least two are needed")
+        h = self.embed(ids.reshape(-1)).view(B, S, H)
+        pending = None
+        for layer in self.layers:
+            h, pending = layer.forward_parts(h, 0, True, pending=pending)
+        _, normed = ops.add_rmsnorm_bf16(h.reshape(B * S, H), pending.reshape(B * S, H), self.norm_weight, self.config.rms_norm_eps,
+                                         want_sum=False)
+        targets = torch.full((B, S), -1, dtype=torch.int32, device="cuda")       # the last position has none
+        targets[:, :-1] = ids[:, 1:]
+        loss, _ = ops.linear_cross_entropy(normed, self.lm_head, targets.view(-1))
+        return -loss.view(B, S)[:, :-1]
+
     def _alloc_caches(self, B: int, max_len: int):
         cfg = self.config
         pages_per_seq = (max_len + PAGE_TOKENS - 1) // PAGE_TOKENS

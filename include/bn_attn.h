@@ -616,14 +616,16 @@ BN_API int bn_gemm_bf16_tn(const void* a, const void* b, void* c, int M, int N, 
 /* Softmax cross entropy of the logits x @ weight_t^T, which are kept nowhere: x (rows, hidden), weight_t (vocab, hidden) bf16;
  *   lse[r] = log sum_v exp z[r][v] (may be NULL),  loss[r] = lse[r] - z[r][targets[r]], both fp32.
  * A row whose target is negative has loss 0 and no gradient; one whose target is vocab or more likewise, and raises id_error (an
- * int32 that may be NULL), as the reference's loss over logits (op_cross_entropy, src/ops/op_cross_entropy.cuh:5-45) cannot.
+ * int32 that may be NULL).  (The reference's loss, op_cross_entropy, src/ops/op_cross_entropy.cuh:5-45, takes the logits.)
  * hidden a multiple of 8; x and weight_t 16-byte aligned; workspace 256-byte aligned. */
 BN_API size_t bn_linear_cross_entropy_bf16_workspace_bytes(int rows, int vocab, int hidden);
 BN_API int bn_linear_cross_entropy_bf16(const void* x, const void* weight_t, const int32_t* targets, float* loss, float* lse, int rows, int vocab,
                                         int hidden, void* workspace, size_t workspace_bytes, int* id_error, int* error_word,
                                         bn_stream_t stream);
-/* Its gradients: dz[r][v] = grad_loss[r] (exp(z[r][v] - lse[r]) - [v = targets[r]]) rounded to bf16, a piece of the vocabulary at a
- * time; dx (rows, hidden) = dz @ weight_t, dweight_t (vocab, hidden) = dz^T @ x, bf16.  Either may be NULL.  lse from the call above. */
+/* Its gradients: dz[r][v] = grad_loss[r] (exp(z[r][v] - lse[r]) - [v = targets[r]]), a piece of the vocabulary at a time and as bf16
+ * multiples of grad_loss[0]; dx (rows, hidden) = dz @ weight_t, dweight_t (vocab, hidden) = dz^T @ x, bf16.  Either may be NULL.
+ * lse from the call above.  Every row of x has to be finite, for one without a target is a factor of 0 in dweight_t's sums.  rows = 0
+ * gives a zero dweight_t. */
 BN_API size_t bn_linear_cross_entropy_backward_bf16_workspace_bytes(int rows, int vocab, int hidden);
 BN_API int bn_linear_cross_entropy_backward_bf16(const void* x, const void* weight_t, const int32_t* targets, const float* lse,
                                                  const float* grad_loss, void* dx, void* dweight_t, int rows, int vocab, int hidden,

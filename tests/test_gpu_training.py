@@ -160,3 +160,225 @@ def test_attention_gradients_of_a_single_key(lib):
     assert ((got[0].double().abs() <= left * k.double().abs().max()).all())
     assert (got[1].double().abs() <= left.unflatten(2, (2, 4)).sum(3) * q.double().abs().max()).all()
     assert off(got[2], want[2]) <= WITHIN
+
+
+# ----------------------------------------------------------------------------------- where these operators go wrong, if they do
+def test_rows_without_a_target(lib):
+    """No loss and no gradient for negative targets; targets behind the vocabulary likewise, and they raise the error word."""
+    from baranet_bdml_b200 import ops
+    x, w, targets, grad = loss_inputs(300, 264, 700, 5)
+    targets[:] = -100
+    error = torch.zeros(1, dtype=torch.int32, device="cuda")
+    loss, lse = ops.linear_cross_entropy(x, w, targets, id_error=error)
+    dx, dw = ops.linear_cross_entropy_backward(x, w, targets, lse, grad)
+    assert not loss.any() and not dx.any() and not dw.any() and int(error) == 0
+    targets[7], targets[8] = 700, 699
+    loss, lse = ops.linear_cross_entropy(x, w, targets, id_error=error)
+    dx, dw = ops.linear_cross_entropy_backward(x, w, targets, lse, grad)
+    assert int(error) == 1 and torch.nonzero(loss).view(-1).tolist() == [8] and torch.nonzero(dx.any(1)).view(-1).tolist() == [8]
+    want = loss_oracle(x, w, torch.where(targets == 700, -1, targets), grad)
+    assert off(dx, want[2]) <= 2 * HALF and off(dw, want[3]) <= 2 * HALF
+
+
+def test_gradients_that_differ_by_row(lib):
+    """Row gradients of many sizes and signs, the first 0, tiny or negative: what the rows are divided by before they are rounded."""
+    from baranet_bdml_b200 import ops
+    x, w, targets, _ = loss_inputs(257, 264, 1000, 6)
+    targets = targets.abs() % 1000
+    for first in (0.0, 1e-30, -3.0, 1e-7):
+        grad = torch.from_numpy((np.random.default_rng(1).standard_normal(257) * 1e-3).astype(np.float32)).cuda()
+        grad[0] = first
+        _, lse = ops.linear_cross_entropy(x, w, targets)
+        dx, dw = ops.linear_cross_entropy_backward(x, w, targets, lse, grad)
+        want = loss_oracle(x, w, targets, grad)
+        assert off(dx, want[2]) <= 2 * HALF and off(dw, want[3]) <= 2 * HALF, first
+        if first == 0.0:
+            assert not dx[0].any()
+
+
+def test_large_logits(lib):
+    """Logits of some hundreds, one of them far ahead: exp(z - lse) neither overflows nor loses the target"""
+    from baranet_bdml_b200 import ops
+    x, w, targets, grad = loss_inputs(130, 256, 1500, 7)
+    x *= 40
+    targets = targets.abs() % 1500
+    loss, lse = ops.linear_cross_entropy(x, w, targets)
+    dx, dw = ops.linear_cross_entropy_backward(x, w, targets, lse, grad)
+    want = loss_oracle(x, w, targets, grad)
+    largest = (x.double() @ w.double().T).abs().max().item()
+    assert largest > 200 and (loss.double() - want[0]).abs().max().item() <= 2 * (256 / 16 + 8) * 2.0 ** -23 * largest
+    # p is exp of a difference of two numbers of that size: off by their roundings, 24 2^-23 of `largest` each
+    assert off(dx, want[2]) <= 2 * HALF + 2 * 24 * 2.0 ** -23 * largest and off(dw, want[3]) <= 2 * HALF + 2 * 24 * 2.0 ** -23 * largest
+
+
+def test_one_of_the_gradients_alone(lib):
+    from baranet_bdml_b200 import ops
+    x, w, targets, grad = loss_inputs(200, 264, 5000, 8)
+    _, lse = ops.linear_cross_entropy(x, w, targets)
+    both = ops.linear_cross_entropy_backward(x, w, targets, lse, grad)
+    dx, none = ops.linear_cross_entropy_backward(x, w, targets, lse, grad, want_dweight=False)
+    assert none is None and torch.equal(dx, both[0])
+    none, dw = ops.linear_cross_entropy_backward(x, w, targets, lse, grad, want_dx=False)
+    assert none is None and torch.equal(dw, both[1])
+
+
+def test_no_rows(lib):
+    from baranet_bdml_b200 import ops
+    x, w = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda"), bf16(np.random.default_rng(1), 104, 64)
+    targets, grad = torch.empty((0,), dtype=torch.int32, device="cuda"), torch.empty((0,), dtype=torch.float32, device="cuda")
+    loss, lse = ops.linear_cross_entropy(x, w, targets)
+    dx, dw = ops.linear_cross_entropy_backward(x, w, targets, lse, grad)
+    assert loss.shape == (0,) and dx.shape == (0, 64) and not dw.any()
+    grads = ops.gated_ff_backward(x, x, w, w, w.T.contiguous())
+    assert grads[0].shape == (0, 64) and not any(g.any() for g in grads[1:])
+    q = torch.empty((2, 0, 8, 64), dtype=torch.bfloat16, device="cuda")
+    assert ops.attn_prefill_bf16_backward(q, q, q, q, q, torch.empty((2, 8, 0), device="cuda"))[0].shape == q.shape
+    assert not ops.gemm_bf16_tn(x, x).any() and ops.gemm_bf16_nn(x, w.T.contiguous()).shape == (0, 104)
+
+
+def test_attention_gradients_against_differences(lib):
+    """The derivative along a direction against two forward passes: in 64 bits the oracle's, so that its own formula is not taken on trust."""
+    rng = np.random.default_rng(3)
+    q, k, v, dout = (torch.from_numpy(rng.standard_normal((1, 70, h, 64))) for h in (4, 2, 2, 4))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    grads = torch.autograd.grad((attention_oracle(*leaves, 3, True, 0.125)[0] * dout).sum(), leaves)
+    for i, g in enumerate(grads):
+        step = torch.from_numpy(rng.standard_normal(g.shape))
+        value = [(attention_oracle(*[t + (s * step if j == i else 0) for j, t in enumerate((q, k, v))], 3, True, 0.125)[0] * dout).sum() for s in (1e-5, -1e-5)]
+        assert abs((value[0] - value[1]).item() / 2e-5 - (g * step).sum().item()) <= 1e-6 * g.norm().item() * step.norm().item()
+
+
+@pytest.mark.parametrize("std,scale", [(4.0, 0.125), (1.0, 1.0), (0.01, 0.125)])
+def test_attention_gradients_of_sharp_and_flat_rows(lib, std, scale):
+    """Scores of about std^2 scale 8: rows that one key has almost alone, and rows that all keys have alike.  A score is off by the roundings
+    of the rotated q and k, 2^-8 of |q||k| scale each at most, sqrt(64) below that for independent ones; P is off by that factor."""
+    got, want, (q, k, _, dout) = attention_grads(1, 200, 8, 2, 0, True, 17, scale=scale, std=std)
+    scores = std * std * 8 * scale
+    for name, a, b in zip(("dq", "dk", "dv"), got, want):
+        assert off(a, b) <= WITHIN + 2 * HALF * scores, name
+
+
+def test_bits_streams_and_graphs(lib):
+    """The same bits in every run, on another stream, beside a second call under way, and from a captured graph on new inputs."""
+    from baranet_bdml_b200 import ops
+    rng = np.random.default_rng(23)
+
+    def inputs():
+        q, k, v, dout = (bf16(rng, 2, 300, h, 64) for h in (8, 2, 2, 8))
+        x, w, targets, grad = loss_inputs(333, 512, 3001, int(rng.integers(1 << 30)))
+        return [q, k, v, dout, x, w, targets, grad, bf16(rng, 640, 512, std=0.05), bf16(rng, 640, 512, std=0.05), bf16(rng, 512, 640, std=0.05)]
+
+    def step(q, k, v, dout, x, w, targets, grad, gate, up, down):
+        lse = torch.empty((2, 8, 300), dtype=torch.float32, device="cuda")
+        out = ops.attn_prefill_bf16(q, k, v, lse=lse)
+        loss, total = ops.linear_cross_entropy(x, w, targets)
+        dx, dw = ops.linear_cross_entropy_backward(x, w, targets, total, grad)
+        return [loss, dx, dw, *ops.gated_ff_backward(dx, x, gate, up, down), *ops.attn_prefill_bf16_backward(dout, q, k, v, out, lse)]
+
+    a, b = inputs(), inputs()
+    first, other = step(*a), step(*b)
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(first, step(*a)))
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in side:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side[0]):
+            got_a = step(*a)
+        with torch.cuda.stream(side[1]):
+            got_b = step(*b)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(first, got_a)) and all(torch.equal(p, q) for p, q in zip(other, got_b))
+    static = [t.clone() for t in a]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(*static)
+    for source, want in ((b, other), (a, first)):
+        for t, s in zip(static, source):
+            t.copy_(s)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(want, captured))
+    ops.gemm_status()
+
+
+def test_a_block_and_its_loss_together(lib):
+    """x + attention(x), + the gated block of that, loss over the vocabulary; then all gradients, by the layers' own backward calls."""
+    from baranet_bdml_b200 import ops
+    from baranet_bdml_b200.layers import GroupedQueryAttentionBF16, LLaMAConfig, MLPBF16
+    np.random.seed(4)
+    cfg = LLaMAConfig(vocab_size=777, hidden_size=512, intermediate_size=1416, num_attention_heads=8, num_key_value_heads=2)
+    attn, mlp = GroupedQueryAttentionBF16(cfg), MLPBF16(cfg)
+    rng = np.random.default_rng(4)
+    B, S, H = 2, 150, 512
+    x, head = bf16(rng, B, S, H), bf16(rng, 777, H, std=2 * H ** -0.5)
+    targets = torch.from_numpy(rng.integers(-50, 777, B * S).astype(np.int32)).cuda()
+    grad = torch.full((B * S,), 1.0 / (B * S), device="cuda")
+    h1 = x + attn(x)
+    h2 = h1 + mlp(h1.view(-1, H)).view(B, S, H)
+    loss, lse = ops.linear_cross_entropy(h2.view(-1, H), head, targets)
+    d2, dhead = ops.linear_cross_entropy_backward(h2.view(-1, H), head, targets, lse, grad)
+    dmlp, gmlp = mlp.backward(d2, h1.view(-1, H))
+    d1 = (d2 + dmlp).view(B, S, H)
+    dattn, gattn = attn.backward(d1, x)
+    dx = d1 + dattn
+    ops.gemm_status()
+
+    leaves = [t.double().requires_grad_(True) for t in (x, *attn.parameters(), *mlp.parameters(), head)]
+    X, wq, wk, wv, wo, wg, wu, wd, whead = leaves
+    o, _ = attention_oracle((X @ wq.T).view(B, S, 8, 64), (X @ wk.T).view(B, S, 2, 64), (X @ wv.T).view(B, S, 2, 64), 0, True, 0.125)
+    H1 = X + o.reshape(B, S, H) @ wo.T
+    H2 = H1 + (torch.nn.functional.silu(H1 @ wg.T) * (H1 @ wu.T)) @ wd.T
+    z = H2.view(B * S, H) @ whead.T
+    picked = z.gather(1, targets.clamp(min=0).long()[:, None])[:, 0]
+    losses = torch.where(targets >= 0, torch.logsumexp(z, 1) - picked, 0.0)
+    want = torch.autograd.grad((losses * grad.double()).sum(), leaves)
+    # roundings on the way, each of at most half a step of what is summed: forward q, k, v, P, rows, o, h1, gate and up, h, y, h2 (11), back dz, d2,
+    # dh .. dmlp, d1 (5), the attention's own (6), and the result's
+    for name, a, b in zip(("x", "q", "k", "v", "o", "gate", "up", "down", "head"), (dx, *gattn, *gmlp, dhead), want):
+        assert off(a, b.view(a.shape)) <= 23 * HALF, name
+    # logits move by the roundings of h2 and what it comes from: 11 half steps of values of size |z|
+    assert (loss.double() - losses).abs().max().item() <= 11 * HALF * z.abs().max().item()
+
+
+def test_scores_of_a_model(lib):
+    """LLaMAModelBF16.score against the log-softmax of the logits that __call__ gives on the same weights"""
+    from baranet_bdml_b200.layers import LLaMAConfig
+    from baranet_bdml_b200.model import LLaMAModelBF16
+    np.random.seed(5)
+    cfg = LLaMAConfig(vocab_size=1008, hidden_size=256, intermediate_size=704, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2)
+    model = LLaMAModelBF16(cfg)
+    ids = torch.from_numpy(np.random.default_rng(6).integers(0, 1008, (3, 37)).astype(np.int32)).cuda()
+    got = model.score(ids)
+    logits = model(ids).double()
+    want = torch.log_softmax(logits[:, :-1], -1).gather(2, ids[:, 1:, None].long())[..., 0]
+    # `__call__` rounds its logits to bf16: half a step of |z| for the picked one, and no more for the mean that lse takes of them
+    assert got.shape == (3, 36) and (got.double() - want).abs().max().item() <= 2 * HALF * logits.abs().max().item()
+    with pytest.raises(IndexError):
+        model.score(torch.full((1, 4), 1008, dtype=torch.int32, device="cuda"))
+    with pytest.raises(RuntimeError, match="at least two"):
+        model.score(ids[:, :1])
+    model.status()
+
+
+def test_refusals(lib):
+    from baranet_bdml_b200 import ops
+    rng = np.random.default_rng(1)
+    x, w, t = bf16(rng, 10, 64), bf16(rng, 100, 64), torch.zeros(10, dtype=torch.int32, device="cuda")
+    one = torch.ones(10, device="cuda")
+    for bad in (lambda: ops.linear_cross_entropy(x.float(), w, t), lambda: ops.linear_cross_entropy(x, w.T, t), lambda: ops.linear_cross_entropy(x, w, t.long()),
+                lambda: ops.linear_cross_entropy(x, w, t[:9]), lambda: ops.linear_cross_entropy(x[:, :60].contiguous(), w[:, :60].contiguous(), t),
+                lambda: ops.linear_cross_entropy(x.cpu(), w, t), lambda: ops.linear_cross_entropy_backward(x, w, t, one, one.double()),
+                lambda: ops.linear_cross_entropy_backward(x, w, t, one, one, want_dx=False, want_dweight=False),
+                lambda: ops.gated_ff_backward(x, x, w, w, w), lambda: ops.gated_ff_backward(x, x, w, w, w.T.contiguous(), act="relu2"),
+                lambda: ops.gated_ff_backward(x[:5], x, w, w, w.T.contiguous()), lambda: ops.gemm_bf16_nn(x, w), lambda: ops.gemm_bf16_tn(x, w),
+                lambda: ops.gemm_bf16_tn(bf16(rng, 10, 60), x)):
+        with pytest.raises(RuntimeError):
+            bad()
+    q, k, lse = bf16(rng, 1, 20, 8, 64), bf16(rng, 1, 20, 2, 64), torch.zeros((1, 8, 20), device="cuda")
+    back = ops.attn_prefill_bf16_backward
+    for bad in (lambda: back(q, q, k, k, q, lse[:, :4]), lambda: back(q, q, k, k[:, :10], q, lse), lambda: back(q[:, ::2], q, k, k, q, lse),
+                lambda: back(q, q, bf16(rng, 1, 20, 3, 64), bf16(rng, 1, 20, 3, 64), q, lse), lambda: back(q, q, k, k, q, lse, position_offset=-1),
+                lambda: back(*(t.reshape(1, 40, -1, 32) for t in (q, q, k, k, q)), lse)):
+        with pytest.raises(RuntimeError):
+            bad()
