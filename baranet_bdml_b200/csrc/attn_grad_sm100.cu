@@ -261,9 +261,8 @@ __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uin
 }
 
 __global__ void __launch_bounds__(AG_THREADS, 1)
-attn_grad_kernel(const __grid_constant__ CUtensorMap q_tile, const __grid_constant__ CUtensorMap do_tile, const __grid_constant__ CUtensorMap k_tile,
-                 const __grid_constant__ CUtensorMap v_tile, const __grid_constant__ CUtensorMap q_rows, const __grid_constant__ CUtensorMap do_rows,
-                 const __grid_constant__ CUtensorMap k_rows, const __grid_constant__ CUtensorMap v_rows, const AttnGradParams p) {
+attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_constant__ CUtensorMap do_rows, const __grid_constant__ CUtensorMap k_rows,
+                 const __grid_constant__ CUtensorMap v_rows, const AttnGradParams p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) AttnGradShared sh;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -323,13 +322,16 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_tile, const __grid_consta
                 mbar_arrive(smem_u32(&sh.unit[u % AG_UNITS]));
                 if (w.steps == 0) break;
                 unit = atomicAdd(p.counter, 1);           // (asked for ahead of the loads)
-                const CUtensorMap *f1 = w.keys ? &k_tile : &q_tile, *f2 = w.keys ? &v_tile : &do_tile, *x1 = w.keys ? &q_rows : &k_rows, *x2 = w.keys ? &do_rows : &v_rows;
+                const CUtensorMap *f1 = w.keys ? &k_rows : &q_rows, *f2 = w.keys ? &v_rows : &do_rows, *x1 = w.keys ? &q_rows : &k_rows, *x2 = w.keys ? &do_rows : &v_rows;
                 ok = mbar_wait(smem_u32(&sh.f_empty[u % AG_F]), (u / AG_F & 1u) ^ 1u, &sh.abort);
                 if (!ok) break;
                 const uint32_t f_full = smem_u32(&sh.f_full[u % AG_F]), f_dst = sF + u % AG_F * 2 * AG_F_BYTES;
                 mbar_arrive_expect_tx(f_full, 2 * AG_F_BYTES);
-                tma_load_4d(f_dst, f1, 0, w.hf, w.f0, w.b, f_full);
-                tma_load_4d(f_dst + AG_F_BYTES, f2, 0, w.hf, w.f0, w.b, f_full);
+#pragma unroll
+                for (int j = 0; j < AG_BF / AG_BX; ++j) {
+                    tma_load_4d(f_dst + j * AG_X_BYTES, f1, 0, w.hf, w.f0 + j * AG_BX, w.b, f_full);
+                    tma_load_4d(f_dst + AG_F_BYTES + j * AG_X_BYTES, f2, 0, w.hf, w.f0 + j * AG_BX, w.b, f_full);
+                }
                 int h = w.hx, x = w.x_lo;
                 for (int i = 0; i < w.steps; ++i, ++n) {
                     const uint32_t st = n % AG_STAGES;
@@ -645,14 +647,14 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     p.scale_log2 = scale * 1.4426950408889634f;
     __nv_bfloat16 *qrot = reinterpret_cast<__nv_bfloat16*>(ws + L.qrot), *krot = reinterpret_cast<__nv_bfloat16*>(ws + L.krot);
 
-    CUtensorMap maps[8];
+    CUtensorMap maps[4];                                                       // one box: 64 rows of a head
     {
         const void* base[4] = {qrot, dout, krot, v};
-        for (int i = 0; i < 8; ++i) {
-            const uint64_t heads = i % 4 < 2 ? Hq : Hkv;
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t heads = i < 2 ? Hq : Hkv;
             const uint64_t dims[4] = {AG_D, heads, (uint64_t)S, (uint64_t)B}, strides[3] = {AG_D * 2, heads * AG_D * 2, (uint64_t)S * heads * AG_D * 2};
-            const uint32_t box[4] = {AG_D, 1, (uint32_t)(i < 4 ? AG_BF : AG_BX), 1};
-            if (int rc = make_tensor_map(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base[i % 4], dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+            const uint32_t box[4] = {AG_D, 1, AG_BX, 1};
+            if (int rc = make_tensor_map(&maps[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base[i], dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
         }
     }
     // enough blocks for the GPU, by positions and, where those are few, by heads too
@@ -663,9 +665,14 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
                      static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), lse, qrot, krot,
                      reinterpret_cast<float2*>(ws + L.table), reinterpret_cast<float*>(ws + L.stats), p.counter, (int)grid, S, L.padded, Hq, Hkv, theta, position_offset);
     if (int rc = launch_status(what)) return rc;
-    if (int rc = allow_smem(attn_grad_kernel, AG_SMEM_BYTES, what, AG_SMEM_BYTES)) return rc;
-    launch_dependent(attn_grad_kernel, dim3(grid), AG_THREADS, AG_SMEM_BYTES, st, maps[0], maps[1], maps[2], maps[3], maps[4], maps[5], maps[6],
-                     maps[7], p);
+    static thread_local int configured_dev = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configured_dev != dev) {
+        if (int rc = allow_smem(attn_grad_kernel, AG_SMEM_BYTES, what, AG_SMEM_BYTES)) return rc;
+        configured_dev = dev;
+    }
+    launch_dependent(attn_grad_kernel, dim3(grid), AG_THREADS, AG_SMEM_BYTES, st, maps[0], maps[1], maps[2], maps[3], p);
     if (int rc = launch_status(what)) return rc;
     if (L.parts > 1) {
         launch_dependent(attn_grad_sum_kernel, dim3((unsigned)sum_blocks, 2), 256, 0, st, p);

@@ -550,7 +550,13 @@ template <bool A_MN, bool B_MN, int EPI, int ACT, bool PAIR>
 int grad_run(const GradMaps& m, const GradParams& p, unsigned grid, cudaStream_t st, const char* what) {
     const size_t smem = 1024 + (size_t)p.ring.stages * p.ring.stage_bytes + 4 * (EPI == GE_GLU ? 3 : 2) * GG_OUT_BYTES;
     auto kernel = gemm_grad_kernel<A_MN, B_MN, EPI, ACT, PAIR>;
-    if (int rc = allow_smem(kernel, smem, what, 226 * 1024)) return rc;
+    static thread_local int configured_dev = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (configured_dev != dev) {
+        if (int rc = allow_smem(kernel, smem, what, 226 * 1024)) return rc;
+        configured_dev = dev;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(GG_THREADS);
@@ -594,9 +600,13 @@ int grad_gemm(const Operand& a, const Operand& b, const Result& c, GradParams p,
         return make_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
     if (int rc = map(&m.a0, a.p0, a.ld, A_MN, p.M, GG_BM)) return rc;
-    if (int rc = map(&m.a1, a.p1 ? a.p1 : a.p0, a.ld, A_MN, p.M, GG_BM)) return rc;
     if (int rc = map(&m.b0, b.p0, b.ld, B_MN, p.N, n_box)) return rc;
-    if (int rc = map(&m.b1, b.p1 ? b.p1 : b.p0, b.ld, B_MN, p.N, n_box)) return rc;
+    m.a1 = m.a0;
+    m.b1 = m.b0;
+    if (a.p1)
+        if (int rc = map(&m.a1, a.p1, a.ld, A_MN, p.M, GG_BM)) return rc;
+    if (b.p1)
+        if (int rc = map(&m.b1, b.p1, b.ld, B_MN, p.N, n_box)) return rc;
     if (p.splits < 1) p.splits = 1, p.k_per_split = 1 << 30;
     m.c0 = m.c1 = m.c2 = m.a0;
     if (EPI == GE_PARTIAL) {
