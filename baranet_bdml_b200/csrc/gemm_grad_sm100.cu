@@ -3,10 +3,13 @@
 // lm_head product before it) and the gradients of the gated feed-forward block (MLP.__call__, mygrad/llama/llama_layers.py:194-235;
 // op_silu_backward, src/ops/op_silu.cuh).
 //
-// One kernel, three operand orders.  y = x W^T reads both operands along K (NT).  Its gradients do not: dx = dy W reads W across its
+// One kernel, three operand orders, several products in a launch.  y = x W^T reads both operands along K (NT).  Its gradients do not: dx = dy W reads W across its
 // rows (NN), dW = dy^T x reads both across (TN).  tcgen05 takes either order from shared memory (MN-major operands: tiles of 64 k rows of
 // 64 contiguous m or n), so nothing is transposed in memory.
-// Persistent kernel, 192 threads: warps 0-3 epilogue, warp 4 issues the MMAs, warp 5 loads by TMA.  Output tile 128 x 256, or (PAIR) 256 x
+// Persistent kernel: four epilogue warps (GLU: eight, thread = row and half of the columns, for its arithmetic: 16384 x 5632 x 2048 613 us, 588
+// with eight), one that issues the MMAs, one that loads by TMA (by an elected thread: with lane == 0, for which the
+// compiler keeps a tensor map's address and coordinates in ordinary registers, four loads a step took longer than its MMAs; 1490 -> 1376 us
+// for the gradients of that block).  Output tile 128 x 256, or (PAIR) 256 x
 // 256 shared by a cluster of two CTAs (tcgen05.mma.cta_group::2); fp32 accumulators double buffered in tensor memory, so that the
 // epilogue of a tile runs under the products of the next.  Tiles may have 128 columns, where there are few
 // (tile_columns).  They go in bands of 16 tile rows, n outside, so that what runs at one time shares both operands in L2.
@@ -15,15 +18,20 @@
 // row takes 32 places in memory for every 16 bytes: 32000 x 2048 of K = 200 71 -> 46 us; eight epilogue warps instead of four 46, and 2 - 5 %
 // more for long K).
 //
+// Gradients that wait for the same operand are one launch: the tiles of up to three products (NN and TN) follow one another, those of the
+// longest K first, so that one's last wave is filled by the next.
+//
 // Epilogues
-//   STORE     the result as bf16
-//   PARTIAL   fp32 sums of a range of K, kept or added to what an earlier launch left: few tiles share K, pieces of the vocabulary follow
-//             one another.  An element gets one sum from a launch, and grad_sum_kernel adds the ranges in order: the same bits in every run
+//   PRODUCTS  the result as bf16, or, PARTIAL, fp32 sums of a range of K, kept or added to what an earlier launch left: few tiles share K,
+//             pieces of the vocabulary follow one another.  An element gets one sum from a launch, and grad_sum_kernel adds the ranges in
+//             order: the same bits in every run
 //   LOSS      logits: of every row's columns in a tile the maximum and the sum of exponentials, and the target's logit: the logits stay in
 //             tensor memory
 //   DLOGITS   logits again -> g (exp(z - lse) - [v = target]) over the first row's g, as bf16
 //   GLU       columns [0,128) gate, [128,256) up of the same indices, and dh, fp32 -> dgate, dup and the product that the forward pass had
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
+#include <type_traits>
+
 #include "common.cuh"
 #include "hybrid.cuh"
 #include "ptx.cuh"
@@ -34,43 +42,53 @@ namespace bn {
 
 using namespace ptx;
 
-constexpr int GG_BM = 128, GG_BN = 256, GG_BK = 64, GG_THREADS = 192, GG_BAND = 16;
+constexpr int GG_BM = 128, GG_BN = 256, GG_BK = 64, GG_BAND = 16;
 constexpr int GG_A_BYTES = GG_BM * GG_BK * 2;
-constexpr int GG_OUT_BYTES = 32 * 128;                                     // what a warp stores at a time
-// Shared memory: as many stages of operands as fit beside each epilogue warp's buffers (GLU: one for each of three results, else two in turn)
+constexpr int GG_OUT_BYTES = 32 * 128;                                     // what a warp stores at a time (GLU: half of that, of three results)
+// Shared memory: as many stages of operands as fit beside the epilogue warps' buffers (GLU: one for each of three results, else two in turn)
 constexpr int GG_MAX_STAGES = 6;
 struct GradRing { int stage_bytes, stages; };
+constexpr int grad_out_bytes(bool glu) { return glu ? 8 * 3 * GG_OUT_BYTES / 2 : 4 * 2 * GG_OUT_BYTES; }
 constexpr GradRing grad_ring(bool pair, bool glu, int bn) {
-    const int stage = GG_A_BYTES + (pair ? bn / 2 : bn) * GG_BK * 2, room = 225 * 1024 - 4 * (glu ? 3 : 2) * GG_OUT_BYTES;
+    const int stage = GG_A_BYTES + (pair ? bn / 2 : bn) * GG_BK * 2, room = 225 * 1024 - grad_out_bytes(glu);
     return {stage, room / stage < GG_MAX_STAGES ? room / stage : GG_MAX_STAGES};
 }
 
-constexpr int GE_STORE = 0, GE_PARTIAL = 1, GE_LOSS = 2, GE_DLOGITS = 3, GE_GLU = 4;
-// what the second pair of operands is: none, the second half of K (NN), further rows of the result (TN), the upper 128 columns of every
-// tile (NT, GLU)
+constexpr int GE_PRODUCTS = 0, GE_LOSS = 1, GE_DLOGITS = 2, GE_GLU = 3;
+// what the second pair of operands is: none, the second half of K (NN), further rows of the result (TN), the upper half of every tile's
+// columns (NT, GLU)
 constexpr int SECOND_NONE = 0, SECOND_K = 1, SECOND_M = 2;
 
-struct GradParams {
+struct GradJob {
     int M, N, K;                       // of one pair of operands
     int second;
+    int a_mn;                          // PRODUCTS: A is (K, M)
+    int partial, add;                  // PRODUCTS: fp32 sums of ranges of K, added to what is there
+    int splits, k_per_split;
+    const float* factor;               // PRODUCTS: what common_factor makes of it is a factor of the result
+    int tiles_m0, tiles_m, tiles_n, tiles;      // of one pair of operands' rows, all, columns, rows x columns
+    int first;                         // number of the job's first item: a tile and a range of K
+};
+constexpr int GG_JOBS = 3;
+struct GradParams {
+    GradJob job[GG_JOBS];              // those behind the last begin at `items`
+    int items;
     int bn;                            // columns of a tile (GLU: of gate and up together)
     GradRing ring;
-    int splits, k_per_split;           // PARTIAL: ranges of K steps
     int* error_word;
-    int add;                           // PARTIAL: added to what is there
     const int32_t* targets;            // LOSS, DLOGITS: (M), minus first_column is the column here
     int first_column, vocab;
     float2* stats;                     // LOSS: [tile][M] maximum, sum of exponentials of the distances to it
     float* picked;                     // LOSS: (M) the target's logit
     const float *lse, *grad;           // DLOGITS: (M)
-    const float* factor;               // STORE: what common_factor makes of it is a factor of the result
     const float* dh;                   // GLU: [dh_parts][M][N], to be added up
     int dh_parts;
 };
 
-// Tensor maps of the operands and of what is stored: STORE c0 and (of the second rows) c1, bf16; PARTIAL c0, fp32 (N, M, split); DLOGITS c0;
-// GLU c0 = h, c1 = dgate, c2 = dup
+// Tensor maps of a job's operands and of what is stored: PRODUCTS c0 and (of the second rows) c1, bf16, or c0, fp32 (N, M, range); DLOGITS
+// c0; GLU c0 = h, c1 = dgate, c2 = dup
 struct GradMaps { CUtensorMap a0, a1, b0, b1, c0, c1, c2; };
+struct AllMaps { GradMaps job[GG_JOBS]; };
 
 // What the logits' gradients are divided by before they are rounded, and their products multiplied by: the first row's gradient, so that a
 // mean's 1 / rows, which all rows have, is not rounded to bf16 in every one of them alike (errors of 2.9e-3 instead of 2.4e-3)
@@ -91,10 +109,11 @@ template <int ACT> __device__ __forceinline__ void act_and_slope(float z, float&
     slope = fmaf(a * (1.f - s), dt, s);
 }
 
-template <bool A_MN, bool B_MN, int EPI, int ACT, bool PAIR>
-__global__ void __launch_bounds__(GG_THREADS, 1)
-gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
-    constexpr int TILE_M = PAIR ? 2 * GG_BM : GG_BM, OUT = EPI == GE_GLU ? 3 : 2;
+template <int EPI, int ACT, bool PAIR>
+__global__ void __launch_bounds__(EPI == GE_GLU ? 320 : 192, 1)
+gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ GradParams p) {
+    constexpr bool PRODUCTS = EPI == GE_PRODUCTS;
+    constexpr int TILE_M = PAIR ? 2 * GG_BM : GG_BM, EW = EPI == GE_GLU ? 8 : 4;      // epilogue warps
     const int n_stages = p.ring.stages;
     const int n_here = PAIR ? p.bn / 2 : p.bn;                             // columns of the tile that this CTA loads
     const int columns = EPI == GE_GLU ? p.bn / 2 : p.bn;                   // columns of the result that a tile covers
@@ -108,24 +127,38 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const uint32_t rank = PAIR ? cluster_rank() : 0;
     const int first = PAIR ? blockIdx.x / 2 : blockIdx.x, stride = PAIR ? gridDim.x / 2 : gridDim.x;
-    const int tiles_m0 = (p.M + TILE_M - 1) / TILE_M, tiles_m = p.second == SECOND_M ? 2 * tiles_m0 : tiles_m0;
-    const int tiles_n = (p.N + columns - 1) / columns, tiles = tiles_m * tiles_n;
-    const int steps0 = (p.K + GG_BK - 1) / GG_BK, steps = p.second == SECOND_K ? 2 * steps0 : steps0;
-    const int items = tiles * (EPI == GE_PARTIAL ? p.splits : 1);
-    struct Item { int m, n, part, ks0, ks1; };                             // tile row and column; which operands; K steps
-    auto item = [&](int t) {
+    struct Item { int m, n, part, split, ks0, ks1; };                      // tile row and column; which operands; K steps
+    auto item = [&](const GradJob& q, int t) {
         Item w;
-        const int split = EPI == GE_PARTIAL ? t / tiles : 0;
-        t -= split * tiles;
-        const int band = t / (GG_BAND * tiles_n), in_band = t - band * GG_BAND * tiles_n;
-        const int height = min(GG_BAND, tiles_m - band * GG_BAND);
+        t -= q.first;
+        w.split = PRODUCTS ? t / q.tiles : 0;
+        t -= w.split * q.tiles;
+        const int band = t / (GG_BAND * q.tiles_n), in_band = t - band * GG_BAND * q.tiles_n;
+        const int height = min(GG_BAND, q.tiles_m - band * GG_BAND);
         w.n = in_band / height;
         w.m = band * GG_BAND + in_band - w.n * height;
-        w.part = w.m >= tiles_m0;
-        if (w.part) w.m -= tiles_m0;
-        w.ks0 = EPI == GE_PARTIAL ? split * p.k_per_split : 0;
-        w.ks1 = EPI == GE_PARTIAL ? min(steps, w.ks0 + p.k_per_split) : steps;
+        w.part = w.m >= q.tiles_m0;
+        if (w.part) w.m -= q.tiles_m0;
+        const int steps = (q.K + GG_BK - 1) / GG_BK * (q.second == SECOND_K ? 2 : 1);
+        w.ks0 = PRODUCTS ? w.split * q.k_per_split : 0;
+        w.ks1 = PRODUCTS ? min(steps, w.ks0 + q.k_per_split) : steps;
         return w;
+    };
+    // a CTA's items, job by job; the body is unrolled by jobs, so that what it reads of one is uniform (MMAs take their operands from uniform
+    // registers: with a job's number in a register 16384 x 5632 x 2048 took 323 us instead of 271), and once for each order of A
+    auto each_item = [&](auto&& body) {
+        int t = first;
+#pragma unroll
+        for (int j = 0; j < (PRODUCTS ? GG_JOBS : 1); ++j) {
+            const int end = PRODUCTS && j + 1 < GG_JOBS ? p.job[j + 1].first : p.items;
+            if (PRODUCTS && p.job[j].a_mn) {
+                for (; t < end; t += stride)
+                    if (!body(std::true_type{}, j, t)) return;
+            } else {
+                for (; t < end; t += stride)
+                    if (!body(std::false_type{}, j, t)) return;
+            }
+        }
     };
 
     if (tid == 0) {
@@ -135,12 +168,12 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&bar_acc_full[i]), 1);
-            mbar_init(smem_u32(&bar_acc_empty[i]), PAIR ? 8 : 4);          // one arrive per epilogue warp
+            mbar_init(smem_u32(&bar_acc_empty[i]), PAIR ? 2 * EW : EW);          // one arrive per epilogue warp
         }
         s_abort = 0;
         fence_mbar_init();
     }
-    if (warp == 4) {
+    if (warp == EW) {
         if (PAIR) {
             tc::pair_tmem_alloc(smem_u32(&s_tmem_base), TMEM_COLS);
             tc::pair_tmem_relinquish();
@@ -156,20 +189,23 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     const uint32_t tmem = s_tmem_base;
     grid_dependency_wait();
 
-    if (warp == 5) {
+    if (warp == EW + 1) {
         // ---------------------------------------------------------- TMA producer
-        if (lane == 0) {
+        if (elect_one()) {
             int stage = 0;
             uint32_t phase = 0;
-            bool ok = true;
-            for (int t = first; ok && t < items; t += stride) {
-                const Item w = item(t);
+            each_item([&](auto mn, int job, int t) {
+                constexpr bool a_mn = decltype(mn)::value;
+                const GradJob& q = p.job[job];
+                const GradMaps& maps = all.job[job];
+                const Item w = item(q, t);
+                const bool second_k = q.second == SECOND_K;
+                const int steps0 = (q.K + GG_BK - 1) / GG_BK;
                 const int m0 = w.m * TILE_M + rank * GG_BM, n0 = w.n * columns + (EPI == GE_GLU ? 0 : rank * n_here);
                 const uint32_t bytes = (PAIR ? 2 : 1) * (GG_A_BYTES + n_here * GG_BK * 2);
                 for (int ks = w.ks0; ks < w.ks1; ++ks) {
-                    ok = mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &s_abort);
-                    if (!ok) break;
-                    const bool half2 = p.second == SECOND_K && ks >= steps0;
+                    if (!mbar_wait(smem_u32(&bar_empty[stage]), phase ^ 1u, &s_abort)) return false;
+                    const bool half2 = second_k && ks >= steps0;
                     const int k0 = (half2 ? ks - steps0 : ks) * GG_BK;
                     const CUtensorMap* ma = half2 || w.part ? &maps.a1 : &maps.a0;
                     const CUtensorMap* mb = half2 ? &maps.b1 : &maps.b0;
@@ -180,7 +216,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                         if (PAIR) tma_load_2d_pair(dst, m, x, y, full);
                         else tma_load_2d(dst, m, x, y, full);
                     };
-                    if (A_MN) {
+                    if (a_mn) {
 #pragma unroll
                         for (int j = 0; j < GG_BM / 64; ++j) load(sA + j * 8192, ma, m0 + j * 64, k0);
                     } else {
@@ -193,42 +229,45 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                             load(sB, &maps.b0, k0, n0);
                             load(sB + p.bn / 2 * GG_BK * 2, &maps.b1, k0, n0);
                         }
-                    } else if (B_MN) {
+                    } else if (PRODUCTS) {
                         for (int j = 0; j < n_here / 64; ++j) load(sB + j * 8192, mb, n0 + j * 64, k0);
                     } else {
                         load(sB, mb, k0, n0);
                     }
                     if (++stage == n_stages) stage = 0, phase ^= 1u;
                 }
-            }
+                return true;
+            });
         }
-    } else if (warp == 4) {
+    } else if (warp == EW) {
         // ------------------------------------------------------------ MMA issuer
-        const uint32_t IDESC = tc::idesc_bf16(TILE_M, p.bn, B_MN ? 1 : 0) | (A_MN ? 1u << 15 : 0u);
+        const uint32_t idesc = tc::idesc_bf16(TILE_M, p.bn, PRODUCTS ? 1 : 0);
         const uint64_t dK = tc::smem_desc_sw128(0);                        // descriptor = this + (address >> 4)
         const uint64_t dMN = (dK & ~((uint64_t)0x3fff << 16)) | (uint64_t)(8192 >> 4) << 16;      // the next 64 m or n lie 8 KB on
-        constexpr uint32_t A_STEP = A_MN ? 128 : 2, B_STEP = B_MN ? 128 : 2;                      // 16 k further, in 16 bytes
+        constexpr uint32_t B_STEP = PRODUCTS ? 128 : 2;                                           // 16 k further, in 16 bytes
         uint32_t local = 0, phase = 0;
         int stage = 0;
-        bool ok = rank == 0;
-        for (int t = first; ok && t < items; t += stride, ++local) {
+        if (rank == 0) each_item([&](auto mn, int job, int t) {
+            constexpr bool a_mn = decltype(mn)::value;
             const uint32_t acc = local & 1u;
-            ok = mbar_wait_warp(smem_u32(&bar_acc_empty[acc]), ((local >> 1) & 1u) ^ 1u, &s_abort);    // drained two tiles ago
-            if (!ok) break;
+            if (!mbar_wait_warp(smem_u32(&bar_acc_empty[acc]), ((local >> 1) & 1u) ^ 1u, &s_abort)) return false;       // drained two tiles ago
+            ++local;
             tc::fence_after_sync();
-            const Item w = item(t);
+            const GradJob& q = p.job[job];
+            const Item w = item(q, t);
+            const uint32_t i_desc = idesc | (a_mn ? 1u << 15 : 0u);
+            constexpr uint32_t a_step = a_mn ? 128 : 2;
             for (int ks = w.ks0; ks < w.ks1; ++ks) {
-                ok = mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &s_abort);
-                if (!ok) break;
+                if (!mbar_wait_warp(smem_u32(&bar_full[stage]), phase, &s_abort)) return false;
                 if (elect_one()) {
                     tc::fence_after_sync();
                     const uint32_t sA = smem0 + stage * p.ring.stage_bytes, sB = sA + GG_A_BYTES;
 #pragma unroll
                     for (int kk = 0; kk < GG_BK / 16; ++kk) {
-                        const uint64_t da = (A_MN ? dMN : dK) + (uint64_t)((sA >> 4) + kk * A_STEP);
-                        const uint64_t db = (B_MN ? dMN : dK) + (uint64_t)((sB >> 4) + kk * B_STEP);
-                        if (PAIR) tc::pair_mma_ss(tmem + acc * GG_BN, da, db, IDESC, (ks > w.ks0) || (kk > 0));
-                        else tc::mma_ss(tmem + acc * GG_BN, da, db, IDESC, (ks > w.ks0) || (kk > 0));
+                        const uint64_t da = (a_mn ? dMN : dK) + (uint64_t)((sA >> 4) + kk * a_step);
+                        const uint64_t db = (PRODUCTS ? dMN : dK) + (uint64_t)((sB >> 4) + kk * B_STEP);
+                        if (PAIR) tc::pair_mma_ss(tmem + acc * GG_BN, da, db, i_desc, (ks > w.ks0) || (kk > 0));
+                        else tc::mma_ss(tmem + acc * GG_BN, da, db, i_desc, (ks > w.ks0) || (kk > 0));
                     }
                     const uint32_t empty = smem_u32(&bar_empty[stage]), full = smem_u32(&bar_acc_full[acc]);
                     if (PAIR) {
@@ -242,11 +281,13 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                 __syncwarp();
                 if (++stage == n_stages) stage = 0, phase ^= 1u;
             }
-        }
+            return true;
+        });
     } else {
         // ------------------------------------------------------ epilogue: thread = row of the tile = TMEM lane
-        const uint32_t lane_base = ((uint32_t)(warp * 32)) << 16;
-        const uint32_t out0 = smem0 + n_stages * p.ring.stage_bytes + warp * OUT * GG_OUT_BYTES;
+        const int half = EW == 8 ? warp / 4 : 0, row = tid % GG_BM;
+        const uint32_t lane_base = ((uint32_t)(warp % 4 * 32)) << 16;
+        const uint32_t out0 = smem0 + n_stages * p.ring.stage_bytes + warp * (grad_out_bytes(EPI == GE_GLU) / EW);
         int out_turn = 0;
         // the warp's next buffer, when what was sent from it before has been read
         auto out_buffer = [&] {
@@ -255,8 +296,11 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
             out_turn ^= 1;
             return out0 + out_turn * GG_OUT_BYTES;
         };
-        auto put16 = [&](uint32_t buf, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {      // 16 bytes of the thread's row, swizzled
-            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(buf + lane * 128 + ((chunk ^ (lane & 7)) << 4)), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+        auto put_at = [&](uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+        };
+        auto put16 = [&](uint32_t buf, int chunk, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {      // 16 bytes of the thread's row of 128, swizzled
+            put_at(buf + lane * 128 + ((chunk ^ (lane & 7)) << 4), a, b, c, d);
         };
         auto put_row = [&](uint32_t buf, int hf, const uint32_t (&r)[32]) {
 #pragma unroll
@@ -275,11 +319,15 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
         };
         uint32_t local = 0;
         bool ok = true;
-        for (int t = first; ok && t < items; t += stride, ++local) {
+        for (int t = first; ok && t < p.items; t += stride, ++local) {
             const uint32_t acc = local & 1u;
-            const Item w = item(t);
-            const int gm = w.m * TILE_M + rank * GG_BM + tid, n0 = w.n * columns;
-            const bool live = gm < p.M;
+            const int job = !PRODUCTS ? 0 : t >= p.job[2].first ? 2 : t >= p.job[1].first ? 1 : 0;
+            const GradJob& q = p.job[job];
+            const GradMaps& maps = all.job[job];
+            const Item w = item(q, t);
+            const int M = q.M, N = q.N;
+            const int gm = w.m * TILE_M + rank * GG_BM + row, n0 = w.n * columns + half * (columns / 2);
+            const bool live = gm < M;
             // what a row needs beside its products, fetched while those run
             int target = -1;
             float lse2 = 0.f, grad = 0.f;
@@ -295,19 +343,19 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
             }
             float d[EPI == GE_GLU ? 32 : 1];                               // 32 columns of dh
             auto load_dh = [&](int col0) {
-                if (EPI != GE_GLU || col0 >= p.N) return;
-                const float4* from = reinterpret_cast<const float4*>(p.dh + (size_t)(live ? gm : 0) * p.N + col0);
-                const size_t part = (size_t)p.M * p.N / 4;
+                if (EPI != GE_GLU || col0 >= N) return;
+                const float4* from = reinterpret_cast<const float4*>(p.dh + (size_t)(live ? gm : 0) * N + col0);
+                const size_t part = (size_t)M * N / 4;
 #pragma unroll
                 for (int v = 0; v < 8; ++v) {                              // (columns are a multiple of 8)
-                    const float4 f = col0 + v * 4 < p.N ? __ldcg(from + v) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const float4 f = col0 + v * 4 < N ? __ldcg(from + v) : make_float4(0.f, 0.f, 0.f, 0.f);
                     d[v * 4] = f.x; d[v * 4 + 1] = f.y; d[v * 4 + 2] = f.z; d[v * 4 + 3] = f.w;
                 }
 #pragma unroll 2
                 for (int k = 1; k < p.dh_parts; ++k) {                     // (eight loads under way, or sixteen)
 #pragma unroll
                     for (int v = 0; v < 8; ++v) {
-                        const float4 f = col0 + v * 4 < p.N ? __ldcg(from + k * part + v) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        const float4 f = col0 + v * 4 < N ? __ldcg(from + k * part + v) : make_float4(0.f, 0.f, 0.f, 0.f);
                         d[v * 4] += f.x; d[v * 4 + 1] += f.y; d[v * 4 + 2] += f.z; d[v * 4 + 3] += f.w;
                     }
                 }
@@ -316,20 +364,20 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
             ok = mbar_wait_warp(smem_u32(&bar_acc_full[acc]), (local >> 1) & 1u, &s_abort);
             if (!ok) break;
             tc::fence_after_sync();
-            const uint32_t tacc = tmem + lane_base + acc * GG_BN;
-            const int y = w.m * TILE_M + rank * GG_BM + warp * 32;          // the warp's first row
-            if (EPI == GE_STORE || EPI == GE_DLOGITS) {
+            const uint32_t tacc = tmem + lane_base + acc * GG_BN + half * (columns / 2);
+            const int y = w.m * TILE_M + rank * GG_BM + warp % 4 * 32;          // the warp's first row
+            if (EPI == GE_DLOGITS || (PRODUCTS && !q.partial)) {
+                const float factor = PRODUCTS ? common_factor(q.factor) : 1.f;
 #pragma unroll 1
                 for (int c = 0; c < p.bn / 64; ++c) {
-                    if (n0 + c * 64 >= p.N) break;                         // (uniform)
+                    if (n0 + c * 64 >= N) break;                         // (uniform)
                     const uint32_t buf = out_buffer();
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
                         uint32_t r[32];
                         tc::ld32(tacc + c * 64 + hf * 32, r);
                         tc::wait_ld(r);
-                        if (EPI == GE_STORE && p.factor) {
-                            const float factor = common_factor(p.factor);
+                        if (PRODUCTS) {
 #pragma unroll
                             for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
                         }
@@ -337,28 +385,29 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                             const int at = target - (n0 + c * 64 + hf * 32);
 #pragma unroll
                             for (int e = 0; e < 32; ++e) {
-                                const float q = ex2(fmaf(__uint_as_float(r[e]), log2e(), -lse2)) - (e == at ? 1.f : 0.f);
-                                r[e] = __float_as_uint(target == INT32_MIN ? 0.f : grad * q);
+                                const float dz = ex2(fmaf(__uint_as_float(r[e]), log2e(), -lse2)) - (e == at ? 1.f : 0.f);
+                                r[e] = __float_as_uint(target == INT32_MIN ? 0.f : grad * dz);
                             }
                         }
                         put_row(buf, hf, r);
                     }
-                    if (y < p.M) send([&] { tma_store_2d(w.part ? &maps.c1 : &maps.c0, buf, n0 + c * 64, y); });
+                    if (y < M) send([&] { tma_store_2d(w.part ? &maps.c1 : &maps.c0, buf, n0 + c * 64, y); });
                 }
-            } else if (EPI == GE_PARTIAL) {
+            } else if (PRODUCTS) {
+                const bool add = q.add;
 #pragma unroll 1
                 for (int c = 0; c < p.bn / 32; ++c) {
-                    if (n0 + c * 32 >= p.N) break;
+                    if (n0 + c * 32 >= N) break;
                     const uint32_t buf = out_buffer();
                     uint32_t r[32];
                     tc::ld32(tacc + c * 32, r);
                     tc::wait_ld(r);
 #pragma unroll
                     for (int v = 0; v < 8; ++v) put16(buf, v, r[v * 4], r[v * 4 + 1], r[v * 4 + 2], r[v * 4 + 3]);
-                    if (y < p.M)
+                    if (y < M)
                         send([&] {
-                            if (p.add) tma_add_3d(&maps.c0, buf, n0 + c * 32, y, t / tiles);
-                            else tma_store_3d(&maps.c0, buf, n0 + c * 32, y, t / tiles);
+                            if (add) tma_add_3d(&maps.c0, buf, n0 + c * 32, y, w.split);
+                            else tma_store_3d(&maps.c0, buf, n0 + c * 32, y, w.split);
                         });
                 }
             } else if (EPI == GE_LOSS) {
@@ -370,11 +419,11 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                     tc::ld32(tacc + c * 32, r);
                     tc::wait_ld(r);
                     const int col = n0 + c * 32;
-                    if (col >= p.N) continue;                              // (uniform)
-                    if (col + 32 > p.N) {
+                    if (col >= N) continue;                              // (uniform)
+                    if (col + 32 > N) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (col + e >= p.N) r[e] = __float_as_uint(-INFINITY);
+                            if (col + e >= N) r[e] = __float_as_uint(-INFINITY);
                     }
                     float m = top;
 #pragma unroll
@@ -391,25 +440,23 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                         float z = 0.f;
 #pragma unroll
                         for (int e = 0; e < 32; ++e) z = e == at ? __uint_as_float(r[e]) : z;
-                        if (at >= 0 && at < 32 && target < p.N) p.picked[gm] = z;
+                        if (at >= 0 && at < 32 && target < N) p.picked[gm] = z;
                     }
                 }
-                if (live) p.stats[(size_t)w.n * p.M + gm] = make_float2(top, sum);
+                if (live) p.stats[(size_t)w.n * M + gm] = make_float2(top, sum);
             } else {
-                const uint32_t h_buf = out0, g_buf = out0 + GG_OUT_BYTES, u_buf = out0 + 2 * GG_OUT_BYTES;
+                const uint32_t h_buf = out0, g_buf = out0 + GG_OUT_BYTES / 2, u_buf = out0 + GG_OUT_BYTES;
 #pragma unroll 1
-                for (int c = 0; c < p.bn / 64; ++c) {                      // 32 columns: half of what is stored at a time
+                for (int c = 0; c < p.bn / 128; ++c) {                     // 32 columns of the half
                     const int col0 = n0 + c * 32;
-                    if (col0 >= p.N) break;
+                    if (col0 >= N) break;
                     uint32_t g[32], u[32];
                     tc::ld32(tacc + c * 32, g);
                     tc::ld32(tacc + p.bn / 2 + c * 32, u);
                     tc::wait_ld(g);
                     tc::wait_ld(u);
-                    if (c % 2 == 0) {                                      // the buffers have been read
-                        if (lane == 0) bulk_wait_group_read<0>();
-                        __syncwarp();
-                    }
+                    if (lane == 0) bulk_wait_group_read<0>();              // the buffers have been read
+                    __syncwarp();
 #pragma unroll
                     for (int v = 0; v < 4; ++v) {
                         uint32_t h4[4], g4[4], u4[4];
@@ -430,20 +477,18 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
                             g4[e] = pack_bf16(dgate[0], dgate[1]);
                             u4[e] = pack_bf16(dup[0], dup[1]);
                         }
-                        const int chunk = c % 2 * 4 + v;
-                        put16(h_buf, chunk, h4[0], h4[1], h4[2], h4[3]);
-                        put16(g_buf, chunk, g4[0], g4[1], g4[2], g4[3]);
-                        put16(u_buf, chunk, u4[0], u4[1], u4[2], u4[3]);
+                        const uint32_t at = lane * 64 + ((v ^ (lane >> 1 & 3)) << 4);       // (64-byte swizzle)
+                        put_at(h_buf + at, h4[0], h4[1], h4[2], h4[3]);
+                        put_at(g_buf + at, g4[0], g4[1], g4[2], g4[3]);
+                        put_at(u_buf + at, u4[0], u4[1], u4[2], u4[3]);
                     }
-                    if (c + 1 < p.bn / 64) load_dh(col0 + 32);             // (the next tile's: before its products are waited for)
-                    if ((c % 2 == 1 || col0 + 32 >= p.N) && y < p.M) {     // (what a last half does not fill lies behind the columns)
-                        const int x = n0 + c / 2 * 64;
+                    if (c + 1 < p.bn / 128) load_dh(col0 + 32);            // (the next tile's: before its products are waited for)
+                    if (y < M)
                         send([&] {
-                            tma_store_2d(&maps.c0, h_buf, x, y);
-                            tma_store_2d(&maps.c1, g_buf, x, y);
-                            tma_store_2d(&maps.c2, u_buf, x, y);
+                            tma_store_2d(&maps.c0, h_buf, col0, y);
+                            tma_store_2d(&maps.c1, g_buf, col0, y);
+                            tma_store_2d(&maps.c2, u_buf, col0, y);
                         });
-                    }
                 }
             }
             tc::fence_before_sync();
@@ -461,7 +506,7 @@ gemm_grad_kernel(const __grid_constant__ GradMaps maps, const GradParams p) {
     __syncthreads();
     if (PAIR) cluster_sync();                                              // nothing more is on its way from one CTA to the other
     if (tid == 0 && s_abort && p.error_word) atomicExch(p.error_word, BN_ERR_TIMEOUT);
-    if (warp == 4) {
+    if (warp == EW) {
         tc::fence_after_sync();
         if (PAIR) tc::pair_tmem_dealloc(tmem, TMEM_COLS);
         else tc::tmem_dealloc(tmem, TMEM_COLS);
@@ -528,28 +573,86 @@ struct Operand {
     const void *p0, *p1;
     long long ld;
 };
-// What is stored: bf16 (M, N) with rows of ld elements, up to three of them, or `splits` fp32 (M, N)
-struct Result {
-    void *p0, *p1, *p2;
-    long long ld;
+// A product to be launched: bf16 results (M, N) with rows of ldc elements, up to three of them, or `partial`: fp32, [range][M][N]
+struct Product {
+    int M, N, K, second;
+    bool a_mn;
+    Operand a, b;
+    void *c0, *c1, *c2;
+    long long ldc;
+    bool sums;                                                             // fp32 sums are kept in any case (pieces, or a reader of sums)
+    float* partial;
+    int add;
+    const float* factor;
+    int splits, per;                                                       // from a plan
+    int steps() const { return (K + GG_BK - 1) / GG_BK * (second == SECOND_K ? 2 : 1); }
 };
 
-// How a product is cut.  Two CTAs share a tile of 256 x 256, but not where one wave of single tiles is all there is, nor where tiles of twice
-// the rows make a wave more than they save (an eighth).  Single tiles that would leave half of the SMs without one have 128 columns: what
-// few rows wait for is the weight, and more SMs ask for it (gradients of a gated block of 64 rows, 2048 x 5632: 84 us with 44 tiles for gate
-// and up, 79 with 88, 75 with the stages that the narrower tiles leave room for).
+// Whether two CTAs share a tile of 256 x 256 (NT): not where one wave of single tiles is all there is, nor where tiles of twice the rows
+// make a wave more than they save (an eighth).  Single tiles that would leave half of the SMs without one have 128 columns: what few rows
+// wait for is the weight, and more SMs ask for it (gradients of a gated block of 64 rows, 2048 x 5632: 84 us with 44 tiles for gate and up,
+// 79 with 88, 75 with the stages that the narrower tiles leave room for).
 struct Cut { bool pair; int bn; };
-Cut tile_columns(int M, int N, int second, bool glu) {
-    const long long sms = sm_count(), twice = second == SECOND_M ? 2 : 1, columns = (N + (glu ? GG_BN / 2 : GG_BN) - 1) / (glu ? GG_BN / 2 : GG_BN);
-    const long long single = twice * ((M + GG_BM - 1) / GG_BM) * columns, pairs = twice * ((M + 2 * GG_BM - 1) / (2 * GG_BM)) * columns;
+Cut tile_columns(int M, int N, bool glu) {
+    const long long sms = sm_count(), columns = (N + (glu ? GG_BN / 2 : GG_BN) - 1) / (glu ? GG_BN / 2 : GG_BN);
+    const long long single = ((M + GG_BM - 1) / GG_BM) * columns, pairs = ((M + 2 * GG_BM - 1) / (2 * GG_BM)) * columns;
     const long long waves = (single + sms - 1) / sms, waves_of_pairs = (pairs + sms / 2 - 1) / (sms / 2);
     return {waves > 1 && waves_of_pairs * 7 <= waves * 8, 2 * single <= sms ? GG_BN / 2 : GG_BN};
 }
 
-template <bool A_MN, bool B_MN, int EPI, int ACT, bool PAIR>
-int grad_run(const GradMaps& m, const GradParams& p, unsigned grid, cudaStream_t st, const char* what) {
-    const size_t smem = 1024 + (size_t)p.ring.stages * p.ring.stage_bytes + 4 * (EPI == GE_GLU ? 3 : 2) * GG_OUT_BYTES;
-    auto kernel = gemm_grad_kernel<A_MN, B_MN, EPI, ACT, PAIR>;
+long long tiles_of(const Product& p, bool pair) {
+    const int rows = pair ? 2 * GG_BM : GG_BM;
+    return (long long)((p.M + rows - 1) / rows) * ((p.N + GG_BN - 1) / GG_BN) * (p.second == SECOND_M ? 2 : 1);
+}
+
+// How products that share a launch are cut: all in pairs of CTAs or none, and the first of them (NN) into ranges of K, by the time until the
+// last CTA is done.  Its unit is a pair's step of 64 k, 0.38 us; a single CTA's, of half the rows, half as long again (768
+// cycles for its shared memory instead of 512).  An item takes its steps, or 6 for its epilogue where those are fewer, and 1.  CTAs take items in turn, the longest
+// first.  A range of K is at least 4 steps, and its sums are written and read once more (0.75 MB a unit, and a launch).
+struct Plan { bool pair; };
+Plan plan_products(Product* p, int n) {
+    const int sms = sm_count();
+    double least = 1e30;
+    Plan best{false};
+    int best_splits = 1;
+    const int most = p[0].a_mn ? 1 : p[0].steps() / 4 < 1 ? 1 : p[0].steps() / 4 > 32 ? 32 : p[0].steps() / 4;
+    for (int pair = 0; pair < 2; ++pair)
+        for (int s = 1; s <= most; ++s) {
+            const int places = pair ? sms / 2 : sms, per = (p[0].steps() + s - 1) / s;
+            if ((p[0].steps() + per - 1) / per != s) continue;
+            double cost[GG_JOBS];
+            long long count[GG_JOBS];
+            int order[GG_JOBS];
+            for (int i = 0; i < n; ++i) {
+                const double steps = (i ? p[i].steps() : per) * (pair ? 1. : 1.5);
+                cost[i] = (steps < 6 ? 6 : steps) + 1;
+                count[i] = tiles_of(p[i], pair) * (i ? 1 : s);
+                order[i] = i;
+                for (int j = i; j > 0 && cost[order[j]] > cost[order[j - 1]]; --j) { const int t = order[j]; order[j] = order[j - 1]; order[j - 1] = t; }
+            }
+            // a round of all CTAs takes as long as its first item
+            double time = 0;
+            long long at = 0, end = 0;
+            for (int k = 0; k < n; ++k) {
+                end += count[order[k]];
+                const long long rounds = end > at ? (end - at + places - 1) / places : 0;
+                time += rounds * cost[order[k]];
+                at += rounds * places;
+            }
+            if (s > 1) time += (double)s * p[0].M * p[0].N * 4 / 0.75e6 + (p[0].sums ? 0 : 8);
+            if (time < least) least = time, best.pair = pair, best_splits = s;
+        }
+    for (int i = 0; i < n; ++i) {
+        p[i].splits = i ? 1 : best_splits;
+        p[i].per = i ? p[i].steps() : (p[0].steps() + best_splits - 1) / best_splits;
+    }
+    return best;
+}
+
+template <int EPI, int ACT, bool PAIR>
+int grad_run(const AllMaps& m, const GradParams& p, unsigned grid, cudaStream_t st, const char* what) {
+    const size_t smem = 1024 + (size_t)p.ring.stages * p.ring.stage_bytes + grad_out_bytes(EPI == GE_GLU);
+    auto kernel = gemm_grad_kernel<EPI, ACT, PAIR>;
     static thread_local int configured_dev = -1;
     int dev = 0;
     cudaGetDevice(&dev);
@@ -559,7 +662,7 @@ int grad_run(const GradMaps& m, const GradParams& p, unsigned grid, cudaStream_t
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(GG_THREADS);
+    cfg.blockDim = dim3(EPI == GE_GLU ? 320 : 192);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -583,90 +686,112 @@ int grad_run(const GradMaps& m, const GradParams& p, unsigned grid, cudaStream_t
     return BN_OK;
 }
 
-// M, N, K > 0; all sizes and addresses are ones that a tensor map takes
-template <bool A_MN, bool B_MN, int EPI, int ACT = 0>
-int grad_gemm(const Operand& a, const Operand& b, const Result& c, GradParams p, cudaStream_t st, const char* what) {
+// n products in one launch (EPI other than PRODUCTS: one); sizes > 0, sizes and addresses are ones that a tensor map takes
+template <int EPI, int ACT = 0>
+int grad_gemm(const Product* products, int n, Cut cut, GradParams p, cudaStream_t st, const char* what) {
+    constexpr bool MANY = EPI == GE_PRODUCTS;
     const int sms = sm_count();
-    const Cut cut = p.splits > 1 ? Cut{false, GG_BN} : tile_columns(p.M, p.N, p.second, EPI == GE_GLU);
     const bool pair = cut.pair;
     p.bn = cut.bn;
     p.ring = grad_ring(pair, EPI == GE_GLU, p.bn);
-    const int columns = EPI == GE_GLU ? p.bn / 2 : p.bn, tiles_n = (p.N + columns - 1) / columns;
+    const int columns = EPI == GE_GLU ? p.bn / 2 : p.bn, rows = pair ? 2 * GG_BM : GG_BM, places = pair ? sms / 2 : sms;
     const uint32_t n_box = EPI == GE_GLU || pair ? p.bn / 2 : p.bn;
-    GradMaps m;
-    auto map = [&](CUtensorMap* out, const void* base, long long ld, bool mn, int extent, uint32_t box_rows) {
-        const uint64_t dims[2] = {(uint64_t)(mn ? extent : p.K), (uint64_t)(mn ? p.K : extent)}, strides[1] = {(uint64_t)ld * 2};
-        const uint32_t box[2] = {64, mn ? 64 : box_rows};
-        return make_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    };
-    if (int rc = map(&m.a0, a.p0, a.ld, A_MN, p.M, GG_BM)) return rc;
-    if (int rc = map(&m.b0, b.p0, b.ld, B_MN, p.N, n_box)) return rc;
-    m.a1 = m.a0;
-    m.b1 = m.b0;
-    if (a.p1)
-        if (int rc = map(&m.a1, a.p1, a.ld, A_MN, p.M, GG_BM)) return rc;
-    if (b.p1)
-        if (int rc = map(&m.b1, b.p1, b.ld, B_MN, p.N, n_box)) return rc;
-    if (p.splits < 1) p.splits = 1, p.k_per_split = 1 << 30;
-    m.c0 = m.c1 = m.c2 = m.a0;
-    if (EPI == GE_PARTIAL) {
-        const uint64_t dims[3] = {(uint64_t)p.N, (uint64_t)p.M, (uint64_t)p.splits}, strides[2] = {(uint64_t)p.N * 4, (uint64_t)p.M * p.N * 4};
-        const uint32_t box[3] = {32, 32, 1};
-        if (int rc = make_tensor_map(&m.c0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, c.p0, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
-    } else if (EPI != GE_LOSS) {
+    AllMaps all;
+    long long items = 0;
+    for (int i = 0; i < GG_JOBS; ++i) {
+        GradJob& q = p.job[i];
+        q.first = (int)items;
+        if (i >= n) {
+            all.job[i] = all.job[0];
+            q.tiles = q.tiles_n = 1;
+            continue;
+        }
+        // the longest items first
+        const Product* o = &products[i];
+        if (MANY) {
+            const Product* order[GG_JOBS];
+            for (int k = 0; k < n; ++k) {
+                order[k] = &products[k];
+                for (int j = k; j > 0 && order[j]->per > order[j - 1]->per; --j) { const Product* t = order[j]; order[j] = order[j - 1]; order[j - 1] = t; }
+            }
+            o = order[i];
+        }
+        const bool partial = MANY && (o->sums || o->splits > 1);
+        q.M = o->M; q.N = o->N; q.K = o->K; q.second = o->second; q.a_mn = o->a_mn;
+        q.partial = partial;
+        q.add = o->add;
+        q.splits = MANY ? (o->steps() + o->per - 1) / o->per : 1;
+        q.k_per_split = o->per;
+        q.factor = o->factor;
+        q.tiles_m0 = (o->M + rows - 1) / rows;
+        q.tiles_m = q.tiles_m0 * (o->second == SECOND_M ? 2 : 1);
+        q.tiles_n = (o->N + columns - 1) / columns;
+        const long long tiles = (long long)q.tiles_m * q.tiles_n;
+        items += tiles * q.splits;
+        if (items > INT32_MAX / 2) return fail(BN_ERR_UNSUPPORTED, "%s: more than 2^30 tiles", what);
+        q.tiles = (int)tiles;
+        GradMaps& m = all.job[i];
+        auto map = [&](CUtensorMap* out, const void* base, long long ld, bool mn, int extent, uint32_t box_rows) {
+            const uint64_t dims[2] = {(uint64_t)(mn ? extent : o->K), (uint64_t)(mn ? o->K : extent)}, strides[1] = {(uint64_t)ld * 2};
+            const uint32_t box[2] = {64, mn ? 64 : box_rows};
+            return make_tensor_map(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+        };
+        if (int rc = map(&m.a0, o->a.p0, o->a.ld, o->a_mn, o->M, GG_BM)) return rc;
+        if (int rc = map(&m.b0, o->b.p0, o->b.ld, MANY, o->N, n_box)) return rc;
+        m.a1 = m.c0 = m.c1 = m.c2 = m.a0;
+        m.b1 = m.b0;
+        if (o->a.p1)
+            if (int rc = map(&m.a1, o->a.p1, o->a.ld, o->a_mn, o->M, GG_BM)) return rc;
+        if (o->b.p1)
+            if (int rc = map(&m.b1, o->b.p1, o->b.ld, MANY, o->N, n_box)) return rc;
+        if (partial) {
+            const uint64_t dims[3] = {(uint64_t)o->N, (uint64_t)o->M, (uint64_t)q.splits}, strides[2] = {(uint64_t)o->N * 4, (uint64_t)o->M * o->N * 4};
+            const uint32_t box[3] = {32, 32, 1};
+            if (int rc = make_tensor_map(&m.c0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, o->partial, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+            continue;
+        }
         CUtensorMap* to[3] = {&m.c0, &m.c1, &m.c2};
-        void* const base[3] = {c.p0, c.p1, c.p2};
-        for (int i = 0; i < 3; ++i) {
-            if (!base[i]) continue;
-            const uint64_t dims[2] = {(uint64_t)p.N, (uint64_t)p.M}, strides[1] = {(uint64_t)c.ld * 2};
-            const uint32_t box[2] = {64, 32};
-            if (int rc = make_tensor_map(to[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base[i], dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+        void* const base[3] = {o->c0, o->c1, o->c2};
+        for (int k = 0; k < 3; ++k) {
+            if (!base[k]) continue;
+            const uint64_t dims[2] = {(uint64_t)o->N, (uint64_t)o->M}, strides[1] = {(uint64_t)o->ldc * 2};
+            const uint32_t box[2] = {EPI == GE_GLU ? 32u : 64u, 32};
+            if (int rc = make_tensor_map(to[k], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base[k], dims, strides, box,
+                                         EPI == GE_GLU ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B))
+                return rc;
         }
     }
-    const int tile_m = pair ? 2 * GG_BM : GG_BM, places = pair ? sms / 2 : sms;
-    const long long items = (long long)((p.M + tile_m - 1) / tile_m) * tiles_n * (p.second == SECOND_M ? 2 : 1) * p.splits;
-    if (items > INT32_MAX / 2) return fail(BN_ERR_UNSUPPORTED, "%s: %lld tiles", what, items);
+    p.items = (int)items;
     const unsigned grid = (unsigned)(items < places ? items : places) * (pair ? 2 : 1);
-    return pair ? grad_run<A_MN, B_MN, EPI, ACT, true>(m, p, grid, st, what) : grad_run<A_MN, B_MN, EPI, ACT, false>(m, p, grid, st, what);
+    return pair ? grad_run<EPI, ACT, true>(all, p, grid, st, what) : grad_run<EPI, ACT, false>(all, p, grid, st, what);
 }
 
-// Ranges of K for a product of few tiles: about one work item for every SM, none shorter than 4 steps of 64
-void grad_splits(int M, int N, int K_steps, int* splits, int* per) {
-    const long long tiles = (long long)((M + GG_BM - 1) / GG_BM) * ((N + GG_BN - 1) / GG_BN), sms = sm_count();
-    long long want = tiles * 2 > sms ? 1 : sms / tiles;
-    if (want > K_steps / 4) want = K_steps / 4 > 0 ? K_steps / 4 : 1;
-    *per = (int)((K_steps + want - 1) / want);
-    *splits = (K_steps + *per - 1) / *per;
+int products(const Product* p, int n, Plan plan, int* error_word, cudaStream_t st, const char* what) {
+    GradParams g{};
+    g.error_word = error_word;
+    return grad_gemm<GE_PRODUCTS>(p, n, {plan.pair, GG_BN}, g, st, what);
 }
 
-int steps_of(int K) { return (K + GG_BK - 1) / GG_BK; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// c (M, N) = a0 (M, K) b0 (K, N) [+ a1 b1] in `pieces` launches that this is number `piece` of; partial: room for the ranges' sums
-size_t nn_bytes(int M, int N, int K_steps, bool pieces) {
-    int splits, per;
-    grad_splits(M, N, K_steps, &splits, &per);
-    return splits > 1 || pieces ? up256((size_t)splits * M * N * 4) : 0;
+Product nn(int M, int N, int K, int second, bool sums) {
+    Product p{};
+    p.M = M; p.N = N; p.K = K; p.second = second; p.sums = sums;
+    return p;
 }
-int nn_sum(const float* partial, void* c, int M, int N, int splits, const float* factor, cudaStream_t st, const char* what) {
-    const long long groups = (long long)M * N / 4;
-    launch_dependent(grad_sum_kernel, (unsigned)((groups + 127) / 128), 128, 0, st, partial, static_cast<__nv_bfloat16*>(c), groups, splits, factor);
+Product tn(int M, int N, int K, int second) {
+    Product p{};
+    p.M = M; p.N = N; p.K = K; p.second = second; p.a_mn = true;
+    return p;
+}
+// the fp32 sums that a planned product leaves
+size_t sum_bytes(const Product& p) { return p.sums || p.splits > 1 ? up256((size_t)p.splits * p.M * p.N * 4) : 0; }
+// adds them, where it has left any
+int add_sums(const Product& p, void* c, int splits, cudaStream_t st, const char* what) {
+    if (!p.sums && splits == 1) return BN_OK;
+    const long long groups = (long long)p.M * p.N / 4;
+    launch_dependent(grad_sum_kernel, (unsigned)((groups + 127) / 128), 128, 0, st, (const float*)p.partial, static_cast<__nv_bfloat16*>(c), groups, splits, p.factor);
     return launch_status(what);
-}
-int nn_product(const Operand& a, const Operand& b, void* c, int M, int N, int K, int second, float* partial, int* error_word, cudaStream_t st, const char* what) {
-    GradParams p{};
-    p.M = M; p.N = N; p.K = K; p.second = second; p.error_word = error_word;
-    grad_splits(M, N, steps_of(K) * (second == SECOND_K ? 2 : 1), &p.splits, &p.k_per_split);
-    if (p.splits == 1) return grad_gemm<false, true, GE_STORE>(a, b, {c, nullptr, nullptr, N}, p, st, what);
-    if (int rc = grad_gemm<false, true, GE_PARTIAL>(a, b, {partial, nullptr, nullptr, N}, p, st, what)) return rc;
-    return nn_sum(partial, c, M, N, p.splits, nullptr, st, what);
-}
-
-int tn_product(const Operand& a, const Operand& b, void* c0, void* c1, int M, int N, int K, int* error_word, cudaStream_t st, const char* what,
-               const float* factor = nullptr) {
-    GradParams p{};
-    p.M = M; p.N = N; p.K = K; p.second = c1 ? SECOND_M : SECOND_NONE; p.error_word = error_word; p.factor = factor;
-    return grad_gemm<true, true, GE_STORE>(a, b, {c0, c1, nullptr, N}, p, st, what);
 }
 
 bool misaligned(std::initializer_list<const void*> all) {
@@ -711,7 +836,12 @@ int check_ws(const char* what, const void* ws, size_t given, size_t needed) {
 }  // namespace
 
 // ------------------------------------------------------------------------------------------------------------- products
-extern "C" size_t bn_gemm_bf16_nn_workspace_bytes(int M, int N, int K) { return M > 0 && N > 0 && K > 0 ? nn_bytes(M, N, steps_of(K), false) : 0; }
+extern "C" size_t bn_gemm_bf16_nn_workspace_bytes(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    Product p = nn(M, N, K, SECOND_NONE, false);
+    plan_products(&p, 1);
+    return sum_bytes(p);
+}
 
 static int check_product(const char* what, const void* a, const void* b, const void* c, int M, int N, int K, int inner_a) {
     if ((M > 0 && N > 0 && !c) || (M > 0 && K > 0 && !a) || (N > 0 && K > 0 && !b)) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
@@ -728,8 +858,15 @@ extern "C" int bn_gemm_bf16_nn(const void* a, const void* b, void* c, int M, int
     if (M == 0 || N == 0) return BN_OK;
     if (K == 0) return zero(c, (size_t)M * N * 2, as_stream(stream), what);
     if (int rc = check_ws(what, workspace, workspace_bytes, bn_gemm_bf16_nn_workspace_bytes(M, N, K))) return rc;
-    return nn_product({a, nullptr, K}, {b, nullptr, N}, c, M, N, K, SECOND_NONE, static_cast<float*>(workspace), error_word,
-                      as_stream(stream), what);
+    Product p = nn(M, N, K, SECOND_NONE, false);
+    p.a = {a, nullptr, K};
+    p.b = {b, nullptr, N};
+    p.c0 = c;
+    p.ldc = N;
+    p.partial = static_cast<float*>(workspace);
+    const Plan plan = plan_products(&p, 1);
+    if (int rc = products(&p, 1, plan, error_word, as_stream(stream), what)) return rc;
+    return add_sums(p, c, p.splits, as_stream(stream), what);
 }
 
 extern "C" int bn_gemm_bf16_tn(const void* a, const void* b, void* c, int M, int N, int K, int* error_word, bn_stream_t stream) {
@@ -737,13 +874,19 @@ extern "C" int bn_gemm_bf16_tn(const void* a, const void* b, void* c, int M, int
     if (int rc = check_product(what, a, b, c, M, N, K, M)) return rc;
     if (M == 0 || N == 0) return BN_OK;
     if (K == 0) return zero(c, (size_t)M * N * 2, as_stream(stream), what);
-    return tn_product({a, nullptr, M}, {b, nullptr, N}, c, nullptr, M, N, K, error_word, as_stream(stream), what);
+    Product p = tn(M, N, K, SECOND_NONE);
+    p.a = {a, nullptr, M};
+    p.b = {b, nullptr, N};
+    p.c0 = c;
+    p.ldc = N;
+    const Plan plan = plan_products(&p, 1);
+    return products(&p, 1, plan, error_word, as_stream(stream), what);
 }
 
 // ------------------------------------------------------------------------------------------------- loss over the vocabulary
 extern "C" size_t bn_linear_cross_entropy_bf16_workspace_bytes(int rows, int vocab, int hidden) {
     if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
-    const int columns = tile_columns(rows, vocab, SECOND_NONE, false).bn;
+    const int columns = tile_columns(rows, vocab, false).bn;
     const size_t tiles = ((size_t)vocab + columns - 1) / columns;
     return up256(tiles * rows * sizeof(float2)) + up256((size_t)rows * sizeof(float));
 }
@@ -756,23 +899,37 @@ extern "C" int bn_linear_cross_entropy_bf16(const void* x, const void* weight_t,
     if (int rc = require_sm100()) return rc;
     if (rows == 0) return BN_OK;
     if (int rc = check_ws(what, workspace, workspace_bytes, bn_linear_cross_entropy_bf16_workspace_bytes(rows, vocab, hidden))) return rc;
-    const int columns = tile_columns(rows, vocab, SECOND_NONE, false).bn, tiles = (vocab + columns - 1) / columns;
+    const Cut cut = tile_columns(rows, vocab, false);
+    const int tiles = (vocab + cut.bn - 1) / cut.bn;
+    Product z = nn(rows, vocab, hidden, SECOND_NONE, false);               // (logits: along K on both sides)
+    z.a = {x, nullptr, hidden};
+    z.b = {weight_t, nullptr, hidden};
+    z.per = z.steps();
     GradParams p{};
-    p.M = rows; p.N = vocab; p.K = hidden; p.error_word = error_word;
+    p.error_word = error_word;
     p.targets = targets;
     p.stats = static_cast<float2*>(workspace);
     p.picked = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + up256((size_t)tiles * rows * sizeof(float2)));
     cudaStream_t st = as_stream(stream);
-    if (int rc = grad_gemm<false, false, GE_LOSS>({x, nullptr, hidden}, {weight_t, nullptr, hidden}, {}, p, st, what)) return rc;
+    if (int rc = grad_gemm<GE_LOSS>(&z, 1, cut, p, st, what)) return rc;
     launch_dependent(loss_join_kernel, (unsigned)((rows + 31) / 32), 32 * GG_JOIN, 0, st, (const float2*)p.stats, (const float*)p.picked, targets, loss, lse, id_error,
                      rows, tiles, vocab);
     return launch_status(what);
 }
 
+// a piece's two products
+static Plan plan_piece(Product (&p)[2], int rows, int vocab, int hidden) {
+    const int columns = piece_columns(rows, vocab), n = columns < vocab ? columns : vocab;
+    p[0] = nn(rows, hidden, n, SECOND_NONE, columns < vocab);
+    p[1] = tn(n, hidden, rows, SECOND_NONE);
+    return plan_products(p, 2);
+}
+
 extern "C" size_t bn_linear_cross_entropy_backward_bf16_workspace_bytes(int rows, int vocab, int hidden) {
     if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
-    const int columns = piece_columns(rows, vocab);
-    return up256((size_t)rows * columns * 2) + nn_bytes(rows, hidden, steps_of(columns < vocab ? columns : vocab), columns < vocab);
+    Product p[2];
+    plan_piece(p, rows, vocab, hidden);
+    return up256((size_t)rows * piece_columns(rows, vocab) * 2) + sum_bytes(p[0]);
 }
 
 extern "C" int bn_linear_cross_entropy_backward_bf16(const void* x, const void* weight_t, const int32_t* targets, const float* lse, const float* grad_loss,
@@ -788,45 +945,59 @@ extern "C" int bn_linear_cross_entropy_backward_bf16(const void* x, const void* 
     if (int rc = check_ws(what, workspace, workspace_bytes, bn_linear_cross_entropy_backward_bf16_workspace_bytes(rows, vocab, hidden))) return rc;
     const int columns = piece_columns(rows, vocab);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    float* partial = reinterpret_cast<float*>(ws + up256((size_t)rows * columns * 2));
-    int splits = 1, per = 1 << 30;
-    grad_splits(rows, hidden, steps_of(columns < vocab ? columns : vocab), &splits, &per);
-    const bool sums = splits > 1 || columns < vocab;
+    Product p[2];                                                          // dx and dweight of a piece, in one launch
+    const Plan plan = plan_piece(p, rows, vocab, hidden);
+    const int splits = p[0].splits;
+    p[0].a = p[1].a = {ws, nullptr, columns};
+    p[0].c0 = dx;
+    p[0].ldc = p[1].ldc = hidden;
+    p[0].partial = reinterpret_cast<float*>(ws + up256((size_t)rows * columns * 2));
+    p[0].factor = p[1].factor = grad_loss;
+    p[1].b = {x, nullptr, hidden};
     for (int v0 = 0; v0 < vocab; v0 += columns) {
         const int n = vocab - v0 < columns ? vocab - v0 : columns;
         const void* w = static_cast<const __nv_bfloat16*>(weight_t) + (size_t)v0 * hidden;
-        GradParams p{};
-        p.M = rows; p.N = n; p.K = hidden; p.error_word = error_word;
-        p.targets = targets; p.first_column = v0; p.vocab = vocab; p.lse = lse; p.grad = grad_loss;
-        if (int rc = grad_gemm<false, false, GE_DLOGITS>({x, nullptr, hidden}, {w, nullptr, hidden}, {ws, nullptr, nullptr, columns}, p, st, what)) return rc;
-        if (dx) {
-            GradParams q{};
-            q.M = rows; q.N = hidden; q.K = n; q.error_word = error_word; q.factor = grad_loss;
-            const Operand dz{ws, nullptr, columns}, wt{w, nullptr, hidden};
-            if (sums) {
-                // a last, shorter piece leaves ranges without a step: they are not launched, and what they have so far stays
-                q.k_per_split = per;
-                q.splits = (steps_of(n) + per - 1) / per;
-                q.add = v0 > 0;
-                if (int rc = grad_gemm<false, true, GE_PARTIAL>(dz, wt, {partial, nullptr, nullptr, hidden}, q, st, what)) return rc;
-            } else if (int rc = grad_gemm<false, true, GE_STORE>(dz, wt, {dx, nullptr, nullptr, hidden}, q, st, what)) {
-                return rc;
-            }
-        }
-        if (dweight_t)
-            if (int rc = tn_product({ws, nullptr, columns}, {x, nullptr, hidden}, static_cast<__nv_bfloat16*>(dweight_t) + (size_t)v0 * hidden, nullptr, n,
-                                    hidden, rows, error_word, st, what, grad_loss))
-                return rc;
+        Product z = nn(rows, n, hidden, SECOND_NONE, false);
+        z.a = {x, nullptr, hidden};
+        z.b = {w, nullptr, hidden};
+        z.c0 = ws;
+        z.ldc = columns;
+        z.per = z.steps();
+        GradParams g{};
+        g.error_word = error_word;
+        g.targets = targets; g.first_column = v0; g.vocab = vocab; g.lse = lse; g.grad = grad_loss;
+        if (int rc = grad_gemm<GE_DLOGITS>(&z, 1, tile_columns(rows, n, false), g, st, what)) return rc;
+        // a last, shorter piece leaves ranges of K without a step: they are not launched, and what they have so far stays
+        p[0].K = p[1].M = n;
+        p[0].add = v0 > 0;
+        p[0].b = {w, nullptr, hidden};
+        p[1].c0 = dweight_t ? static_cast<__nv_bfloat16*>(dweight_t) + (size_t)v0 * hidden : nullptr;
+        if (int rc = products(dx ? p : p + 1, (dx != nullptr) + (dweight_t != nullptr), plan, error_word, st, what)) return rc;
     }
-    return dx && sums ? nn_sum(partial, dx, rows, hidden, splits, grad_loss, st, what) : BN_OK;
+    return dx ? add_sums(p[0], dx, splits, st, what) : BN_OK;
 }
 
 // --------------------------------------------------------------------------------------------- gated feed-forward block
+// dh; then dx and the weights' gradients
+static Plan plan_dh(Product& p, int rows, int hidden, int inter) {
+    p = nn(rows, inter, hidden, SECOND_NONE, true);
+    return plan_products(&p, 1);
+}
+static Plan plan_gradients(Product (&p)[3], int rows, int hidden, int inter) {
+    p[0] = nn(rows, hidden, inter, SECOND_K, false);
+    p[1] = tn(inter, hidden, rows, SECOND_M);
+    p[2] = tn(hidden, inter, rows, SECOND_NONE);
+    return plan_products(p, 3);
+}
+
 // h, dgate and dup (bf16); dh and, when that has been used, the sums of dx (fp32): dh rounded to bf16 would add half of the error that the
 // gradients have from their own roundings (2.9e-3 instead of 2.4e-3), and its ranges of K are added where it is read
 extern "C" size_t bn_gated_ff_backward_bf16_workspace_bytes(int rows, int hidden, int inter) {
     if (rows <= 0 || hidden <= 0 || inter <= 0) return 0;
-    const size_t a = nn_bytes(rows, inter, steps_of(hidden), true), b = nn_bytes(rows, hidden, 2 * steps_of(inter), false);
+    Product dh, p[3];
+    plan_dh(dh, rows, hidden, inter);
+    plan_gradients(p, rows, hidden, inter);
+    const size_t a = sum_bytes(dh), b = sum_bytes(p[0]);
     return 3 * up256((size_t)rows * inter * 2) + (a > b ? a : b);
 }
 
@@ -855,22 +1026,43 @@ extern "C" int bn_gated_ff_backward_bf16(const void* dy, const void* x, const vo
     void *h = ws, *dg = ws + each, *du = ws + 2 * each;
     float* partial = reinterpret_cast<float*>(ws + 3 * each);
     // dh = dy Wdown
-    GradParams q{};
-    q.M = rows; q.N = inter; q.K = hidden; q.error_word = error_word;
-    grad_splits(rows, inter, steps_of(hidden), &q.splits, &q.k_per_split);
-    if (int rc = grad_gemm<false, true, GE_PARTIAL>({dy, nullptr, hidden}, {down_t, nullptr, inter}, {partial, nullptr, nullptr, inter}, q, st, what)) return rc;
+    Product d;
+    const Plan first = plan_dh(d, rows, hidden, inter);
+    d.a = {dy, nullptr, hidden};
+    d.b = {down_t, nullptr, inter};
+    d.partial = partial;
+    if (int rc = products(&d, 1, first, error_word, st, what)) return rc;
     // gate and up again; their gradients, and the product of the forward pass
-    GradParams p{};
-    p.M = rows; p.N = inter; p.K = hidden; p.error_word = error_word;
-    p.dh = partial;
-    p.dh_parts = q.splits;
-    const Operand xr{x, nullptr, hidden}, weights{gate_t, up_t, hidden};
-    const Result three{h, dg, du, inter};
-    if (int rc = act == BN_ACT_SILU ? grad_gemm<false, false, GE_GLU, BN_ACT_SILU>(xr, weights, three, p, st, what)
-                                    : grad_gemm<false, false, GE_GLU, BN_ACT_GELU_TANH>(xr, weights, three, p, st, what))
+    Product gu = nn(rows, inter, hidden, SECOND_NONE, false);              // (along K on both sides)
+    gu.a = {x, nullptr, hidden};
+    gu.b = {gate_t, up_t, hidden};
+    gu.c0 = h;
+    gu.c1 = dg;
+    gu.c2 = du;
+    gu.ldc = inter;
+    gu.per = gu.steps();
+    GradParams g{};
+    g.error_word = error_word;
+    g.dh = partial;
+    g.dh_parts = d.splits;
+    const Cut cut = tile_columns(rows, inter, true);
+    if (int rc = act == BN_ACT_SILU ? grad_gemm<GE_GLU, BN_ACT_SILU>(&gu, 1, cut, g, st, what) : grad_gemm<GE_GLU, BN_ACT_GELU_TANH>(&gu, 1, cut, g, st, what))
         return rc;
-    // dx = dgate Wgate + dup Wup, one product of twice the K
-    if (int rc = nn_product({dg, du, inter}, {gate_t, up_t, hidden}, dx, rows, hidden, inter, SECOND_K, partial, error_word, st, what)) return rc;
-    if (int rc = tn_product({dg, du, inter}, {x, nullptr, hidden}, dgate_t, dup_t, inter, hidden, rows, error_word, st, what)) return rc;
-    return tn_product({dy, nullptr, hidden}, {h, nullptr, inter}, ddown_t, nullptr, hidden, inter, rows, error_word, st, what);
+    // dx = dgate Wgate + dup Wup (one product of twice the K), dWgate and dWup = dgate^T x, dup^T x, dWdown = dy^T h
+    Product p[3];
+    const Plan plan = plan_gradients(p, rows, hidden, inter);
+    p[0].a = p[1].a = {dg, du, inter};
+    p[0].b = {gate_t, up_t, hidden};
+    p[0].c0 = dx;
+    p[0].partial = partial;
+    p[1].b = {x, nullptr, hidden};
+    p[1].c0 = dgate_t;
+    p[1].c1 = dup_t;
+    p[2].a = {dy, nullptr, hidden};
+    p[2].b = {h, nullptr, inter};
+    p[2].c0 = ddown_t;
+    p[0].ldc = p[1].ldc = hidden;
+    p[2].ldc = inter;
+    if (int rc = products(p, 3, plan, error_word, st, what)) return rc;
+    return add_sums(p[0], dx, p[0].splits, st, what);
 }
