@@ -3,16 +3,15 @@
 // lm_head product before it) and the gradients of the gated feed-forward block (MLP.__call__, mygrad/llama/llama_layers.py:194-235;
 // op_silu_backward, src/ops/op_silu.cuh).
 //
-// One kernel, three operand orders, several products in a launch.  y = x W^T reads both operands along K (NT).  Its gradients do not: dx = dy W reads W across its
-// rows (NN), dW = dy^T x reads both across (TN).  tcgen05 takes either order from shared memory (MN-major operands: tiles of 64 k rows of
-// 64 contiguous m or n), so nothing is transposed in memory.
-// Persistent kernel: four epilogue warps (GLU: eight, thread = row and half of the columns, for its arithmetic: 16384 x 5632 x 2048 613 us, 588
-// with eight), one that issues the MMAs, one that loads by TMA (by an elected thread: with lane == 0, for which the
-// compiler keeps a tensor map's address and coordinates in ordinary registers, four loads a step took longer than its MMAs; 1490 -> 1376 us
-// for the gradients of that block).  Output tile 128 x 256, or (PAIR) 256 x
-// 256 shared by a cluster of two CTAs (tcgen05.mma.cta_group::2); fp32 accumulators double buffered in tensor memory, so that the
-// epilogue of a tile runs under the products of the next.  Tiles may have 128 columns, where there are few
-// (tile_columns).  They go in bands of 16 tile rows, n outside, so that what runs at one time shares both operands in L2.
+// One kernel, three operand orders, several products in a launch.  y = x W^T reads both operands along K (NT).  Its gradients do not: dx =
+// dy W reads W across its rows (NN), dW = dy^T x reads both across (TN).  tcgen05 takes either order from shared memory (MN-major operands:
+// tiles of 64 k rows of 64 contiguous m or n), so nothing is transposed in memory.
+// Persistent kernel: four epilogue warps (GLU: eight, thread = row and half of the columns, for its arithmetic: 16384 x 5632 x 2048 613 us,
+// 588 with eight), one that issues the MMAs, one that loads by TMA (an elected thread: with lane == 0, for which the compiler keeps a tensor
+// map's address and coordinates in ordinary registers, four loads a step took longer than its MMAs; 1490 -> 1376 us for the gradients of
+// that block).  Output tile 128 x 256, or (PAIR) 256 x 256 shared by a cluster of two CTAs (tcgen05.mma.cta_group::2); fp32 accumulators
+// double buffered in tensor memory, so that the epilogue of a tile runs under the products of the next.  Tiles may have 128 columns, where
+// there are few (tile_columns).  They go in bands of 16 tile rows, n outside, so that what runs at one time shares both operands in L2.
 //
 // Results leave through shared memory: a warp writes 32 rows of 128 bytes and one thread has TMA store them (a thread that stores its own
 // row takes 32 places in memory for every 16 bytes: 32000 x 2048 of K = 200 71 -> 46 us; eight epilogue warps instead of four 46, and 2 - 5 %
@@ -144,23 +143,6 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
         w.ks1 = PRODUCTS ? min(steps, w.ks0 + q.k_per_split) : steps;
         return w;
     };
-    // a CTA's items, job by job; the body is unrolled by jobs, so that what it reads of one is uniform (MMAs take their operands from uniform
-    // registers: with a job's number in a register 16384 x 5632 x 2048 took 323 us instead of 271), and once for each order of A
-    auto each_item = [&](auto&& body) {
-        int t = first;
-#pragma unroll
-        for (int j = 0; j < (PRODUCTS ? GG_JOBS : 1); ++j) {
-            const int end = PRODUCTS && j + 1 < GG_JOBS ? p.job[j + 1].first : p.items;
-            if (PRODUCTS && p.job[j].a_mn) {
-                for (; t < end; t += stride)
-                    if (!body(std::true_type{}, j, t)) return;
-            } else {
-                for (; t < end; t += stride)
-                    if (!body(std::false_type{}, j, t)) return;
-            }
-        }
-    };
-
     if (tid == 0) {
         for (int s = 0; s < n_stages; ++s) {
             mbar_init(smem_u32(&bar_full[s]), 1);
@@ -188,6 +170,23 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
     tc::fence_after_sync();
     const uint32_t tmem = s_tmem_base;
     grid_dependency_wait();
+
+    // a CTA's items, job by job; the body is unrolled by jobs, so that what it reads of one is uniform (MMAs take their operands from uniform
+    // registers: with a job's number in a register 16384 x 5632 x 2048 took 323 us instead of 271), and once for each order of A
+    auto each_item = [&](auto&& body) {
+        int t = first;
+#pragma unroll
+        for (int j = 0; j < (PRODUCTS ? GG_JOBS : 1); ++j) {
+            const int end = PRODUCTS && j + 1 < GG_JOBS ? p.job[j + 1].first : p.items;
+            if (PRODUCTS && p.job[j].a_mn) {
+                for (; t < end; t += stride)
+                    if (!body(std::true_type{}, j, t)) return;
+            } else {
+                for (; t < end; t += stride)
+                    if (!body(std::false_type{}, j, t)) return;
+            }
+        }
+    };
 
     if (warp == EW + 1) {
         // ---------------------------------------------------------- TMA producer
