@@ -265,7 +265,8 @@ class GroupedQueryAttentionBF16:
         dattn = ops.gemm_bf16_nn(dy, self.o_proj).view(B, S, nq, D)
         do = ops.gemm_bf16_tn(dy, attn.view(n, nq * D))
         dqkv = torch.cat([g.view(n, -1) for g in ops.attn_prefill_bf16_backward(dattn, q, k, v, attn, lse, **how)], dim=1)
-        dx = ops.gemm_bf16_nn(dqkv, self.packed_qkv()).view(hidden_states.shape)
+        # (the weights as they are now: the packed copy of the forward pass knows only of tensors that were replaced)
+        dx = ops.gemm_bf16_nn(dqkv, torch.cat([self.q_proj, self.k_proj, self.v_proj])).view(hidden_states.shape)
         return dx, [*ops.gemm_bf16_tn(dqkv, x2).split([nq * D, nkv * D, nkv * D]), do]
 
     def parameters(self):

@@ -602,7 +602,7 @@ BN_API int bn_gqa_step(const void* q, const void* k, const void* v, const void* 
 
 /* ------------------------------------------------------------------------
  * training: products of a backward pass, the loss over a vocabulary, gradients of the gated feed-forward block and of attention
- * (bf16, fp32 accumulation; sums in a fixed order, so two runs give the same bits)
+ * (bf16, fp32 accumulation; sums in a fixed order, so two runs give the same bits; results may not overlap operands)
  * ------------------------------------------------------------------------ */
 
 /* c (M, N) = a (M, K) @ b (K, N): dx = dy @ W for a weight W stored (out, in).  K and N multiples of 8, pointers 16-byte aligned.

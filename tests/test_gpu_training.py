@@ -341,6 +341,25 @@ def test_a_block_and_its_loss_together(lib):
     assert (loss.double() - losses).abs().max().item() <= 11 * HALF * z.abs().max().item()
 
 
+def test_attention_layers_gradients_follow_weights_written_in_place(lib):
+    from baranet_bdml_b200.layers import GroupedQueryAttentionBF16, LLaMAConfig
+    np.random.seed(9)
+    attn = GroupedQueryAttentionBF16(LLaMAConfig(vocab_size=100, hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=2))
+    rng = np.random.default_rng(9)
+    x, dy = bf16(rng, 60, 256), bf16(rng, 60, 256)
+    attn(x)                                               # packs its weights
+    for w in attn.parameters():
+        w.mul_(-0.5)
+    got, grads = attn.backward(dy, x)
+    leaves = [t.double().requires_grad_(True) for t in (x, *attn.parameters())]
+    X, wq, wk, wv, wo = leaves
+    o, _ = attention_oracle((X @ wq.T).view(1, 60, 4, 64), (X @ wk.T).view(1, 60, 2, 64), (X @ wv.T).view(1, 60, 2, 64), 0, True, 0.125)
+    want = torch.autograd.grad(o.reshape(60, 256) @ wo.T, leaves, dy.double())
+    # the attention's own roundings, q, k, v, dattn, the gradients of q, k and v, and the result's
+    for name, a, b in zip(("x", "q", "k", "v", "o"), (got, *grads), want):
+        assert off(a, b) <= 12 * HALF, name
+
+
 def test_scores_of_a_model(lib):
     """LLaMAModelBF16.score against the log-softmax of the logits that __call__ gives on the same weights"""
     from baranet_bdml_b200.layers import LLaMAConfig
