@@ -14,8 +14,8 @@
 // there are few (tile_columns).  They go in bands of 16 tile rows, n outside, so that what runs at one time shares both operands in L2.
 //
 // Results leave through shared memory: a warp writes 32 rows of 128 bytes and one thread has TMA store them (a thread that stores its own
-// row takes 32 places in memory for every 16 bytes: 32000 x 2048 of K = 200 71 -> 46 us; eight epilogue warps instead of four 46, and 2 - 5 %
-// more for long K).
+// row takes 32 places in memory for every 16 bytes: 32000 x 2048 of K = 200 71 -> 46 us, and 39 since the elected thread loads, of which 32
+// without the stores; eight epilogue warps instead of four made no difference there, and 2 - 5 % more for long K).
 //
 // Gradients that wait for the same operand are one launch: the tiles of up to three products (NN and TN) follow one another, those of the
 // longest K first, so that one's last wave is filled by the next.
