@@ -601,7 +601,7 @@ AttnGradLayout attn_grad_layout(int B, int S, int Hq, int Hkv, int causal) {
 }  // namespace
 
 extern "C" size_t bn_attn_prefill_bf16_backward_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int causal) {
-    if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D != AG_D) return 0;
+    if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || D != AG_D || B > 65535 || S > INT32_MAX - 256) return 0;
     return attn_grad_layout(B, S, Hq, Hkv, causal).total;
 }
 
@@ -613,6 +613,7 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     if (B < 0 || S < 0 || Hq <= 0 || Hkv <= 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape B=%d S=%d Hq=%d Hkv=%d", what, B, S, Hq, Hkv);
     if (Hq % Hkv) return fail(BN_ERR_INVALID_ARG, "%s: Hq=%d not a multiple of Hkv=%d", what, Hq, Hkv);
     if (D != AG_D) return fail(BN_ERR_UNSUPPORTED, "%s: head_dim=%d (64 supported)", what, D);
+    if (B > 65535 || S > INT32_MAX - 256 || position_offset > INT32_MAX - S - 256) return fail(BN_ERR_UNSUPPORTED, "%s: B=%d S=%d offset=%d too large", what, B, S, position_offset);
     if (position_offset < 0) return fail(BN_ERR_INVALID_ARG, "%s: position_offset=%d < 0", what, position_offset);
     for (const void* t : {dout, q, k, v, out, static_cast<const void*>(dq), static_cast<const void*>(dk), static_cast<const void*>(dv)})
         if (reinterpret_cast<uintptr_t>(t) & 15) return fail(BN_ERR_INVALID_ARG, "%s: tensors must be 16-byte aligned", what);
@@ -623,7 +624,7 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(BN_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", what);
     const long long tiles = (S + AG_BF - 1) / AG_BF, key_blocks = tiles * B * Hkv * L.parts, blocks = key_blocks + tiles * B * Hq;
     const long long sum_blocks = ((long long)B * S * Hkv * 8 + 255) / 256;
-    if (blocks > INT32_MAX / 2 || sum_blocks > INT32_MAX || B > 65535 || S > INT32_MAX - 256 || position_offset > INT32_MAX - S - 256)
+    if (blocks > INT32_MAX / 2 || sum_blocks > INT32_MAX)
         return fail(BN_ERR_UNSUPPORTED, "%s: problem too large for one launch", what);
 
     uint8_t* ws = static_cast<uint8_t*>(workspace);

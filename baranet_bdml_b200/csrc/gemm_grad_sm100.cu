@@ -771,6 +771,10 @@ int products(const Product* p, int n, Plan plan, int* error_word, cudaStream_t s
     return grad_gemm<GE_PRODUCTS>(p, n, {plan.pair, GG_BN}, g, st, what);
 }
 
+// sizes that stay 32-bit numbers when they are rounded up to tiles
+constexpr int GG_LONGEST = INT32_MAX - 256;
+bool longer(int a, int b, int c) { return a > GG_LONGEST || b > GG_LONGEST || c > GG_LONGEST; }
+
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 Product nn(int M, int N, int K, int second, bool sums) {
@@ -821,7 +825,7 @@ int check_loss(const char* what, const void* x, const void* w, const void* targe
     if (!w || (rows > 0 && (!x || !targets))) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (rows < 0 || vocab <= 0 || hidden <= 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape rows=%d vocab=%d hidden=%d", what, rows, vocab, hidden);
     if (hidden % 8) return fail(BN_ERR_UNSUPPORTED, "%s: hidden=%d must be a multiple of 8 (16-byte rows)", what, hidden);
-    if (vocab > INT32_MAX - 256) return fail(BN_ERR_UNSUPPORTED, "%s: vocab=%d", what, vocab);
+    if (longer(rows, vocab, hidden)) return fail(BN_ERR_UNSUPPORTED, "%s: rows=%d vocab=%d hidden=%d too large", what, rows, vocab, hidden);
     if (misaligned({x, w})) return fail(BN_ERR_INVALID_ARG, "%s: x and the weight must be 16-byte aligned", what);
     return BN_OK;
 }
@@ -836,7 +840,7 @@ int check_ws(const char* what, const void* ws, size_t given, size_t needed) {
 
 // ------------------------------------------------------------------------------------------------------------- products
 extern "C" size_t bn_gemm_bf16_nn_workspace_bytes(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || longer(M, N, K)) return 0;
     Product p = nn(M, N, K, SECOND_NONE, false);
     plan_products(&p, 1);
     return sum_bytes(p);
@@ -845,6 +849,7 @@ extern "C" size_t bn_gemm_bf16_nn_workspace_bytes(int M, int N, int K) {
 static int check_product(const char* what, const void* a, const void* b, const void* c, int M, int N, int K, int inner_a) {
     if ((M > 0 && N > 0 && !c) || (M > 0 && K > 0 && !a) || (N > 0 && K > 0 && !b)) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (M < 0 || N < 0 || K < 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape M=%d N=%d K=%d", what, M, N, K);
+    if (longer(M, N, K)) return fail(BN_ERR_UNSUPPORTED, "%s: M=%d N=%d K=%d too large", what, M, N, K);
     if (N % 8 || inner_a % 8) return fail(BN_ERR_UNSUPPORTED, "%s: rows of %d and %d elements must be multiples of 8 (16 bytes)", what, inner_a, N);
     if (misaligned({a, b, c})) return fail(BN_ERR_INVALID_ARG, "%s: a/b/c must be 16-byte aligned", what);
     return require_sm100();
@@ -884,7 +889,7 @@ extern "C" int bn_gemm_bf16_tn(const void* a, const void* b, void* c, int M, int
 
 // ------------------------------------------------------------------------------------------------- loss over the vocabulary
 extern "C" size_t bn_linear_cross_entropy_bf16_workspace_bytes(int rows, int vocab, int hidden) {
-    if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
+    if (rows <= 0 || vocab <= 0 || hidden <= 0 || longer(rows, vocab, hidden)) return 0;
     const int columns = tile_columns(rows, vocab, false).bn;
     const size_t tiles = ((size_t)vocab + columns - 1) / columns;
     return up256(tiles * rows * sizeof(float2)) + up256((size_t)rows * sizeof(float));
@@ -925,7 +930,7 @@ static Plan plan_piece(Product (&p)[2], int rows, int vocab, int hidden) {
 }
 
 extern "C" size_t bn_linear_cross_entropy_backward_bf16_workspace_bytes(int rows, int vocab, int hidden) {
-    if (rows <= 0 || vocab <= 0 || hidden <= 0) return 0;
+    if (rows <= 0 || vocab <= 0 || hidden <= 0 || longer(rows, vocab, hidden)) return 0;
     Product p[2];
     plan_piece(p, rows, vocab, hidden);
     return up256((size_t)rows * piece_columns(rows, vocab) * 2) + sum_bytes(p[0]);
@@ -992,7 +997,7 @@ static Plan plan_gradients(Product (&p)[3], int rows, int hidden, int inter) {
 // h, dgate and dup (bf16); dh and, when that has been used, the sums of dx (fp32): dh rounded to bf16 would add half of the error that the
 // gradients have from their own roundings (2.9e-3 instead of 2.4e-3), and its ranges of K are added where it is read
 extern "C" size_t bn_gated_ff_backward_bf16_workspace_bytes(int rows, int hidden, int inter) {
-    if (rows <= 0 || hidden <= 0 || inter <= 0) return 0;
+    if (rows <= 0 || hidden <= 0 || inter <= 0 || longer(rows, hidden, inter)) return 0;
     Product dh, p[3];
     plan_dh(dh, rows, hidden, inter);
     plan_gradients(p, rows, hidden, inter);
@@ -1006,6 +1011,7 @@ extern "C" int bn_gated_ff_backward_bf16(const void* dy, const void* x, const vo
     const char* what = "bn_gated_ff_backward_bf16";
     if (!gate_t || !up_t || !down_t || !dgate_t || !dup_t || !ddown_t || (rows > 0 && (!dy || !x || !dx))) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (rows < 0 || hidden <= 0 || inter <= 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape rows=%d hidden=%d inter=%d", what, rows, hidden, inter);
+    if (longer(rows, hidden, inter)) return fail(BN_ERR_UNSUPPORTED, "%s: rows=%d hidden=%d inter=%d too large", what, rows, hidden, inter);
     if (hidden % 8 || inter % 8)
         return fail(BN_ERR_UNSUPPORTED, "%s: hidden=%d and inter=%d must be multiples of 8 (16-byte rows)", what, hidden, inter);
     if (act != BN_ACT_SILU && act != BN_ACT_GELU_TANH) return fail(BN_ERR_UNSUPPORTED, "%s: activation %d", what, act);

@@ -89,3 +89,24 @@ def test_operators_refuse_host_tensors():
                  lambda: ops.attn_prefill_bf16_backward(q, q, q, q, q, torch.zeros((1, 8, 4)))):
         with pytest.raises(RuntimeError, match="only GPU implementation available"):
             call()
+
+
+LONGEST = 2**31 - 1
+
+
+def test_sizes_that_tiles_do_not_number(lib):
+    """Lengths that leave 32 bits when they are rounded up to a tile"""
+    from baranet_bdml_b200 import _lib
+    unsupported = _lib.BN_ERR_UNSUPPORTED
+    refused(lib, unsupported, "too large", "bn_gemm_bf16_nn", P, P, P, LONGEST, 8, 8, P, 1 << 30, None, None)
+    refused(lib, unsupported, "too large", "bn_gemm_bf16_tn", P, P, P, 8, 8, LONGEST, None, None)
+    refused(lib, unsupported, "too large", "bn_linear_cross_entropy_bf16", *[P] * 5, LONGEST, 100, 8, P, 1 << 30, None, None, None)
+    refused(lib, unsupported, "too large", "bn_linear_cross_entropy_backward_bf16", *[P] * 7, 8, LONGEST, 8, P, 1 << 30, None, None)
+    refused(lib, unsupported, "too large", "bn_gated_ff_backward_bf16", *[P] * 9, LONGEST, 8, 8, _lib.BN_ACT_SILU, P, 1 << 30, None, None)
+    attn, tail = "bn_attn_prefill_bf16_backward", (P, 1 << 30, None, None)
+    refused(lib, unsupported, "too large", attn, *[P] * 9, 1, LONGEST, 1, 1, 64, 0.125, 1e4, 0, 1, *tail)
+    refused(lib, unsupported, "too large", attn, *[P] * 9, 65536, 1, 1, 1, 64, 0.125, 1e4, 0, 1, *tail)
+    refused(lib, unsupported, "too large", attn, *[P] * 9, 1, 10, 1, 1, 64, 0.125, 1e4, LONGEST - 100, 1, *tail)
+    assert lib.bn_gemm_bf16_nn_workspace_bytes(LONGEST, 8, 8) == 0
+    assert lib.bn_linear_cross_entropy_bf16_workspace_bytes(LONGEST, 8, 8) == lib.bn_linear_cross_entropy_backward_bf16_workspace_bytes(8, LONGEST, 8) == 0
+    assert lib.bn_gated_ff_backward_bf16_workspace_bytes(8, 8, LONGEST) == lib.bn_attn_prefill_bf16_backward_workspace_bytes(1, LONGEST, 1, 1, 64, 1) == 0
