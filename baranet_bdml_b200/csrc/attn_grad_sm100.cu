@@ -17,11 +17,13 @@
 // One CTA per SM takes blocks from a counter, the longest first, and goes on to the next without a pause: three F are kept, tiles of X
 // come through a ring.  Tensor memory: three slots of S and dP (128 columns) and 128 columns of gradients, so three tiles are under way:
 // warps 0-11 are three groups that take tiles in turn (thread = row, 64 columns); warp 13 loads by TMA; warps 12, 14 and 15 have a thread
-// each that issues the products of S, of the gradients and of dP.  (One thread for all took 1950 cycles a tile for its waits and commits of
-// 100 to 200 cycles each, where the products take 530 to 690.)  A slot's S is free for the next tile as soon as P X2 has been computed, or
-// a query block's group has read it, so S of a tile is there before its group is.
-// A block's gradients are stored by all groups, 16 columns at a time, each behind its first tile of the next block: a group that waited for
-// the block's last products and stored all of them held the others up (a pause of 10000 cycles a block; 3 x 1371 tokens 165 -> 156 us).
+// each that issues the products of S, of the gradients and of dP; warps 16-19 store a block's gradients under the tiles of the next.  (One
+// thread for all products took 1950 cycles a tile for its waits and commits of 100 to 200 cycles each, where the products take 530 to 690.)
+// A slot's S is free for the next tile as soon as P X2 has been computed, or a query block's group has read it, so S of a tile is there
+// before its group is.
+// A block's gradients need warps of their own: groups that stored them, 16 columns at a time behind their first tile of the next block, were
+// late for their tiles by 3000 cycles a block, most of it code that had left the instruction cache (8 x 2048 591 -> 571 us, and 562 with the
+// registers that the warps which issue and store do without: 128 a softmax thread instead of 120, so that nearly nothing is spilled).
 // Launch 3, where the heads of a group are shared by several blocks: their fp32 sums of dK and dV are added in order.
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
 #include <type_traits>
@@ -35,10 +37,10 @@ namespace bn {
 
 using namespace ptx;
 
-constexpr int AG_D = 64, AG_BF = 128, AG_BX = 64, AG_STAGES = 6, AG_SLOTS = 3, AG_F = 3, AG_THREADS = 512, AG_UNITS = 8;
-constexpr int AG_F_BYTES = AG_BF * AG_D * 2, AG_X_BYTES = AG_BX * AG_D * 2, AG_STAT_BYTES = AG_BX * 8;
+constexpr int AG_D = 64, AG_BF = 128, AG_BX = 64, AG_STAGES = 6, AG_SLOTS = 3, AG_F = 3, AG_THREADS = 640, AG_UNITS = 8;
+constexpr int AG_F_BYTES = AG_BF * AG_D * 2, AG_X_BYTES = AG_BX * AG_D * 2, AG_STAT_BYTES = AG_BX * 8, AG_F_STAT_BYTES = AG_BF * 8;
 constexpr int AG_STAGE_BYTES = 2 * AG_X_BYTES;
-constexpr int AG_SMEM_BYTES = 1024 + AG_F * 2 * AG_F_BYTES + AG_STAGES * (AG_STAGE_BYTES + AG_STAT_BYTES);
+constexpr int AG_SMEM_BYTES = 1024 + AG_F * (2 * AG_F_BYTES + AG_F_STAT_BYTES) + AG_STAGES * (AG_STAGE_BYTES + AG_STAT_BYTES);
 constexpr uint32_t AG_TMEM = 512, AG_DP = 64, AG_ACC = 384;               // slot: S, then dP; behind the slots two gradients of 64 columns
 
 struct AttnGradParams {
@@ -173,6 +175,12 @@ __device__ __forceinline__ uint32_t packed_bf16(uint64_t v) {
     return pack_bf16(a, c);
 }
 
+// The block is launched with 96 registers a thread; the warps that issue and store give theirs to the softmax warps
+template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+constexpr int AG_REGS = 96, AG_REG_SOFTMAX = 128, AG_REG_ISSUE = 48, AG_REG_STORE = 48;
+static_assert(128 * (3 * AG_REG_SOFTMAX + AG_REG_ISSUE + AG_REG_STORE) <= AG_THREADS * AG_REGS, "more registers than the block is launched with");
+
 // A group's share of a tile, `edge`: the first column (of queries) or the last (of keys) that the thread's row sees: scores -> P (bf16, over them) -> with dP, dS (bf16, over that).  `mine`: the slot's columns in the warp's lanes.
 template <bool KEYS>
 __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uint32_t parity, uint32_t mine, uint32_t stat, int stage, uint32_t stage_parity,
@@ -234,24 +242,26 @@ __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uin
     }
     if (!wait_quick(smem_u32(&sh.dp[slot]), parity, &sh.abort)) return false;
     tc::fence_after_sync();
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {                     // (the second half's columns are read before any are written: 32 bf16 columns lie in 16)
+    {                                                    // 16 columns on their way while 16 are used (563 -> 559 us); read before dS lies there (32 of bf16 take 16)
         uint32_t s[2][16], pk[16];
-        tc::ld16(mine + AG_DP + hf * 32, s[0]);
-        tc::ld16(mine + AG_DP + hf * 32 + 16, s[1]);
+        tc::ld16(mine + AG_DP, s[0]);
         tc::wait_ld(s[0]);
-        tc::wait_ld(s[1]);
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-            uint64_t l[2];
-            of_columns(stat + AG_STAT_BYTES / 2, hf * 32 + e, d2, l[0], l[1]);
+        for (int c = 0; c < 4; ++c) {
+            if (c < 3) tc::ld16(mine + AG_DP + (c + 1) * 16, s[(c + 1) % 2]);
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-                pk[e / 2 + j] = packed_bf16(mul_f32x2(
-                    pr[hf * 16 + e / 2 + j],
-                    add_f32x2(pack_f32x2(__uint_as_float(s[e / 16][e % 16 + 2 * j]), __uint_as_float(s[e / 16][e % 16 + 2 * j + 1])), l[j])));
+            for (int e = 0; e < 16; e += 4) {
+                uint64_t l[2];
+                of_columns(stat + AG_STAT_BYTES / 2, c * 16 + e, d2, l[0], l[1]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    pk[c % 2 * 8 + e / 2 + j] = packed_bf16(mul_f32x2(
+                        pr[c * 8 + e / 2 + j],
+                        add_f32x2(pack_f32x2(__uint_as_float(s[c % 2][e + 2 * j]), __uint_as_float(s[c % 2][e + 2 * j + 1])), l[j])));
+            }
+            if (c < 3) tc::wait_ld(s[(c + 1) % 2]);
+            if (c % 2) tc::st16(mine + AG_DP + c / 2 * 16, pk);
         }
-        tc::st16(mine + AG_DP + hf * 16, pk);
     }
     tc::wait_st();
     tc::fence_before_sync();
@@ -267,7 +277,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
     __shared__ __align__(8) AttnGradShared sh;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sF = smem0, sX = smem0 + AG_F * 2 * AG_F_BYTES, sStat = sX + AG_STAGES * AG_STAGE_BYTES;
+    const uint32_t sF = smem0, sX = smem0 + AG_F * 2 * AG_F_BYTES, sStat = sX + AG_STAGES * AG_STAGE_BYTES, sFStat = sStat + AG_STAGES * AG_STAT_BYTES;
     if (tid == 0) {
         for (int i = 0; i < AG_STAGES; ++i) {
             mbar_init(smem_u32(&sh.full[i]), 1);
@@ -279,7 +289,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(smem_u32(&sh.done[i]), 1);
-            mbar_init(smem_u32(&sh.acc_free[i]), 12);     // one arrive per softmax warp
+            mbar_init(smem_u32(&sh.acc_free[i]), 4);      // one arrive per warp that stores gradients
         }
         for (int i = 0; i < AG_SLOTS; ++i) {
             mbar_init(smem_u32(&sh.s[i]), 1);
@@ -303,13 +313,14 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
     grid_dependency_wait();
 
     // number `u` of this CTA's blocks.  The ring is long enough: the loader is at most AG_F blocks ahead of the MMAs, of any three tiles that
-    // follow one another each group has had one, and a group comes back to the block before its own at most.  (Three tiles may belong to
-    // three blocks: so many F are kept.)
+    // follow one another each group has had one, and the products of a block wait until the gradients two blocks before are stored.  (Three
+    // tiles may belong to three blocks: so many F are kept.)
     auto unit_at = [&](uint32_t u, bool& ok) -> const AttnGradUnit& {
         ok = mbar_wait(smem_u32(&sh.unit[u % AG_UNITS]), u / AG_UNITS & 1u, &sh.abort);
         return sh.units[u % AG_UNITS];
     };
 
+    if (warp >= 12 && warp < 16) registers_down<AG_REG_ISSUE>();
     if (warp == 13) {
         // ---------------------------------------------------------- blocks, TMA producer
         if (elect_one()) {
@@ -326,7 +337,13 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                 ok = mbar_wait(smem_u32(&sh.f_empty[u % AG_F]), (u / AG_F & 1u) ^ 1u, &sh.abort);
                 if (!ok) break;
                 const uint32_t f_full = smem_u32(&sh.f_full[u % AG_F]), f_dst = sF + u % AG_F * 2 * AG_F_BYTES;
-                mbar_arrive_expect_tx(f_full, 2 * AG_F_BYTES);
+                mbar_arrive_expect_tx(f_full, 2 * AG_F_BYTES + (w.keys ? 0 : AG_F_STAT_BYTES));
+                if (!w.keys) {                            // the rows' own statistics (asked for by each thread they took 700 cycles: 563 -> 559 us)
+                    const float* from = p.stats + ((size_t)w.b * p.Hq + w.hf) * 2 * p.padded + w.f0;
+                    const uint32_t to = sFStat + u % AG_F * AG_F_STAT_BYTES;
+                    bulk_load(to, from, AG_F_STAT_BYTES / 2, f_full);
+                    bulk_load(to + AG_F_STAT_BYTES / 2, from + p.padded, AG_F_STAT_BYTES / 2, f_full);
+                }
 #pragma unroll
                 for (int j = 0; j < AG_BF / AG_BX; ++j) {
                     tma_load_4d(f_dst + j * AG_X_BYTES, f1, 0, w.hf, w.f0 + j * AG_BX, w.b, f_full);
@@ -429,38 +446,31 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                 }
             }
         }
-    } else {
-        // ------------------------------------------------ softmax groups
-        const int group = warp / 4, row = tid % 128;
-        const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), mine = lanes + group * 128;
-        const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
-        uint32_t n0 = 0;                                  // the block's first tile among all of this CTA's
-        bool ok = true;
-        // 16 columns of a block's gradients: dV and dK (keys) or dQ, of which a group has every third
-        auto gradients = [&](uint32_t u) {
-            const AttnGradUnit& w = sh.units[u % AG_UNITS];
+    } else if (warp >= 16) {
+        // ------------------------------------------------ gradients: thread = row
+        registers_down<AG_REG_STORE>();
+        const int row = tid % 128;
+        const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16);
+        for (uint32_t u = 0;; ++u) {
+            bool ok = true;
+            const AttnGradUnit& w = unit_at(u, ok);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok || w.steps == 0) break;
             const bool keys = w.keys;
             const int f = w.f0 + row, heads = keys ? p.Hkv : p.Hq;
             const size_t at = (((size_t)w.b * p.S + f) * heads + w.hf) * AG_D, all = (size_t)p.B * p.S * p.Hkv * AG_D;
             const float4* table = reinterpret_cast<const float4*>(p.table + (size_t)min(f, p.S - 1) * (AG_D / 2));
-            const int c0 = keys ? group : 4 + group;
-            float4 angle[4], next[4];
-            auto ask = [&](int c, float4 (&to)[4]) {      // (dV is not turned; 64 bytes of a line that the next columns share)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) to[e] = c >= 4 && c < 8 ? table[c % 4 * 4 + e] : make_float4(1.f, 0.f, 1.f, 0.f);
-            };
-            ask(c0, next);
-            if (!wait_quick(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) return false;
+            if (!mbar_wait_warp(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) break;
             tc::fence_after_sync();
 #pragma unroll 1
-            for (int c = c0; c < 8; c += AG_SLOTS) {
+            for (int c = keys ? 0 : 4; c < 8; ++c) {
                 const int col = c % 4 * 16;
                 const bool dv = c < 4;
+                float4 angle[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) angle[e] = dv ? make_float4(1.f, 0.f, 1.f, 0.f) : table[c % 4 * 4 + e];
                 uint32_t r[16];
                 tc::ld16(lanes + AG_ACC + (keys ? c / 4 : u & 1u) * 64 + col, r);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) angle[e] = next[e];
-                ask(c + AG_SLOTS, next);
                 tc::wait_ld(r);
                 if (f < p.S) {
                     if (keys && p.parts > 1) {
@@ -481,7 +491,6 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                         to[1] = make_uint4(o[4], o[5], o[6], o[7]);
                     }
                 }
-                __syncwarp();
             }
             tc::fence_before_sync();
             __syncwarp();
@@ -489,15 +498,21 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                 if (keys || (u & 1u) == 0) mbar_arrive(smem_u32(&sh.acc_free[0]));
                 if (keys || (u & 1u) == 1) mbar_arrive(smem_u32(&sh.acc_free[1]));
             }
-            return true;
-        };
+        }
+    } else {
+        // ------------------------------------------------ softmax groups
+        registers_up<AG_REG_SOFTMAX>();
+        const int group = warp / 4, row = tid % 128;
+        const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), mine = lanes + group * 128;
+        const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
+        uint32_t n0 = 0;                                  // the block's first tile among all of this CTA's
+        bool ok = true;
         for (uint32_t u = 0; ok; ++u) {
             const AttnGradUnit& w = unit_at(u, ok);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int steps = w.steps, f0 = w.f0, f = f0 + row, x_lo = w.x_lo, width = w.x_hi - x_lo;
             const int i0 = (int)((group + AG_SLOTS - n0 % AG_SLOTS) % AG_SLOTS);
-            bool owed = u > 0;                            // the gradients of the block before
             // the group's tiles; from which column on (queries) or up to which (keys) its rows see everything
             auto tiles = [&](auto keys, uint64_t lse2, uint64_t d2, int mine_sees, int all_see) {
                 constexpr bool KEYS = decltype(keys)::value;
@@ -512,10 +527,6 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                         return false;
                     x0 += AG_SLOTS * AG_BX;
                     while (x0 >= behind) x0 -= width * AG_BX;
-                    if (owed) {
-                        owed = false;
-                        if (!gradients(u - 1)) return false;
-                    }
                 }
                 return true;
             };
@@ -523,12 +534,15 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
             } else if (w.keys) {
                 ok = tiles(std::true_type{}, 0, 0, p.causal ? f - p.offset : 0, p.causal ? f0 + AG_BF - 1 - p.offset : 0);
             } else {                                      // -lse * log2(e) and -d of the row, twice (rows behind S are padded)
-                const float* of = p.stats + ((size_t)w.b * p.Hq + w.hf) * 2 * p.padded + f;
-                const float lse = of[0], d = of[p.padded];
+                ok = wait_quick(smem_u32(&sh.f_full[u % AG_F]), u / AG_F & 1u, &sh.abort);
+                if (!ok) break;
+                float lse, d;
+                const uint32_t of = sFStat + u % AG_F * AG_F_STAT_BYTES + row * 4;
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(lse) : "r"(of));
+                asm volatile("ld.shared.f32 %0, [%1];" : "=f"(d) : "r"(of + AG_F_STAT_BYTES / 2));
                 const long long sees = p.causal ? p.offset : p.S;
                 ok = tiles(std::false_type{}, pack_f32x2(lse, lse), pack_f32x2(d, d), (int)min((long long)p.S - 1, f + sees), (int)min((long long)p.S - 1, f0 + sees));
             }
-            if (ok && owed) ok = gradients(u - 1);
             if (steps == 0) break;
             n0 += steps;
         }
@@ -670,6 +684,9 @@ extern "C" int bn_attn_prefill_bf16_backward(const void* dout, const void* q, co
     int dev = 0;
     cudaGetDevice(&dev);
     if (configured_dev != dev) {
+        cudaFuncAttributes attr;                                               // (with fewer registers at launch the softmax warps would wait for theirs)
+        if (cudaFuncGetAttributes(&attr, attn_grad_kernel) != cudaSuccess || attr.numRegs < AG_REGS)
+            return fail(BN_ERR_CUDA, "%s: the kernel is launched with fewer registers than it shares out", what);
         if (int rc = allow_smem(attn_grad_kernel, AG_SMEM_BYTES, what, AG_SMEM_BYTES)) return rc;
         configured_dev = dev;
     }
