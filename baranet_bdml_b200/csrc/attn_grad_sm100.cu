@@ -16,14 +16,16 @@
 // are B operands twice, along both of their dimensions.
 // One CTA per SM takes blocks from a counter, the longest first, and goes on to the next without a pause: three F are kept, tiles of X
 // come through a ring.  Tensor memory: three slots of S and dP (128 columns) and 128 columns of gradients, so three tiles are under way:
-// warps 0-11 are three groups that take tiles in turn (thread = row, 64 columns); warp 13 loads by TMA; warps 12, 14 and 15 have a thread
-// each that issues the products of S, of the gradients and of dP; warps 16-19 store a block's gradients under the tiles of the next.  (One
-// thread for all products took 1950 cycles a tile for its waits and commits of 100 to 200 cycles each, where the products take 530 to 690.)
+// warps 0-15 are two groups that take tiles in turn (thread = row and half of the columns; three groups of four warps with a row's 64 columns
+// each: 544 instead of 538 us at 8 x 2048; three of eight, whose 72 registers a thread are too few, 560); warp 17 loads by TMA; warps 16, 18
+// and 19 have a thread each that issues the products of S, of the gradients and of dP; warps 20-23 store a block's gradients under the tiles of
+// the next.  (One thread for all products took 1950 cycles a tile for its waits and commits of 100 to 200 cycles each, where the products take
+// 530 to 690.)
 // A slot's S is free for the next tile as soon as P X2 has been computed, or a query block's group has read it, so S of a tile is there
 // before its group is.
 // A block's gradients need warps of their own: groups that stored them, 16 columns at a time behind their first tile of the next block, were
-// late for their tiles by 3000 cycles a block, most of it code that had left the instruction cache (8 x 2048 591 -> 571 us, and 562 with the
-// registers that the warps which issue and store do without: 128 a softmax thread instead of 120, so that nearly nothing is spilled).
+// late for their tiles by 3000 cycles a block, most of it code that had left the instruction cache (8 x 2048 591 -> 562 us).  Registers are
+// shared out by role, so that the softmax warps spill nothing (eight fewer a thread: 571).
 // Launch 3, where the heads of a group are shared by several blocks: their fp32 sums of dK and dV are added in order.
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
 #include <type_traits>
@@ -37,7 +39,8 @@ namespace bn {
 
 using namespace ptx;
 
-constexpr int AG_D = 64, AG_BF = 128, AG_BX = 64, AG_STAGES = 6, AG_SLOTS = 3, AG_F = 3, AG_THREADS = 640, AG_UNITS = 8;
+constexpr int AG_D = 64, AG_BF = 128, AG_BX = 64, AG_STAGES = 6, AG_SLOTS = 3, AG_F = 3, AG_UNITS = 8;
+constexpr int AG_COLS = AG_BX / 2, AG_GROUPS = 2, AG_SOFT = 8 * AG_GROUPS, AG_THREADS = (AG_SOFT + 8) * 32;      // a thread's columns; groups, their warps
 constexpr int AG_F_BYTES = AG_BF * AG_D * 2, AG_X_BYTES = AG_BX * AG_D * 2, AG_STAT_BYTES = AG_BX * 8, AG_F_STAT_BYTES = AG_BF * 8;
 constexpr int AG_STAGE_BYTES = 2 * AG_X_BYTES;
 constexpr int AG_SMEM_BYTES = 1024 + AG_F * (2 * AG_F_BYTES + AG_F_STAT_BYTES) + AG_STAGES * (AG_STAGE_BYTES + AG_STAT_BYTES);
@@ -175,13 +178,14 @@ __device__ __forceinline__ uint32_t packed_bf16(uint64_t v) {
     return pack_bf16(a, c);
 }
 
-// The block is launched with 96 registers a thread; the warps that issue and store give theirs to the softmax warps
+// The block is launched with 80 registers a thread; the warps that issue and store give some to the softmax warps
 template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-constexpr int AG_REGS = 96, AG_REG_SOFTMAX = 128, AG_REG_ISSUE = 48, AG_REG_STORE = 48;
-static_assert(128 * (3 * AG_REG_SOFTMAX + AG_REG_ISSUE + AG_REG_STORE) <= AG_THREADS * AG_REGS, "more registers than the block is launched with");
+constexpr int AG_REGS = 80, AG_REG_SOFTMAX = 96, AG_REG_ISSUE = 48, AG_REG_STORE = 48;
+static_assert(128 * (AG_SOFT / 4 * AG_REG_SOFTMAX + AG_REG_ISSUE + AG_REG_STORE) <= AG_THREADS * AG_REGS, "more registers than the block is launched with");
 
-// A group's share of a tile, `edge`: the first column (of queries) or the last (of keys) that the thread's row sees: scores -> P (bf16, over them) -> with dP, dS (bf16, over that).  `mine`: the slot's columns in the warp's lanes.
+// A thread's share of a tile, `edge`: the first of its columns (of queries) or the last (of keys) that its row sees: scores -> P (bf16, over
+// them) -> with dP, dS (bf16, over that).  `mine`: the thread's columns of the slot, in its warp's lanes; `stat`: of them too.
 template <bool KEYS>
 __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uint32_t parity, uint32_t mine, uint32_t stat, int stage, uint32_t stage_parity,
                                                uint64_t lse2, uint64_t d2, uint64_t scale2, bool masked, int edge, int lane) {
@@ -193,33 +197,31 @@ __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uin
     if (!wait_quick(smem_u32(&sh.s[slot]), parity, &sh.abort)) return false;
     if (KEYS && !wait_quick(smem_u32(&sh.full[stage]), stage_parity, &sh.abort)) return false;      // (the statistics; they came before)
     tc::fence_after_sync();
-    uint64_t pr[32];
+    uint64_t pr[AG_COLS / 2];
     {
-        uint32_t s[2][32];
-        tc::ld32(mine, s[0]);
-        tc::ld32(mine + 32, s[1]);
-        tc::wait_ld(s[0]);
-        tc::wait_ld(s[1]);
+        uint32_t s[AG_COLS];
+        tc::ld32(mine, s);
+        tc::wait_ld(s);
         if (!KEYS) {
             tc::fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&sh.p[slot]));
         }
 #pragma unroll
-        for (int e = 0; e < 64; e += 4) {
+        for (int e = 0; e < AG_COLS; e += 4) {
             uint64_t l[2];
             of_columns(stat, e, lse2, l[0], l[1]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 float a, c;
-                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e / 32][e % 32 + 2 * j]), __uint_as_float(s[e / 32][e % 32 + 2 * j + 1])), scale2, l[j]), a, c);
+                unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[e + 2 * j]), __uint_as_float(s[e + 2 * j + 1])), scale2, l[j]), a, c);
                 pr[e / 2 + j] = pack_f32x2(ex2(a), ex2(c));
             }
         }
     }
     if (masked) {                                        // (dS has the factor P, so one mask is enough)
 #pragma unroll
-        for (int e = 0; e < 32; ++e) {
+        for (int e = 0; e < AG_COLS / 2; ++e) {
             float a, c;
             unpack_f32x2(pr[e], a, c);
             if (KEYS ? 2 * e < edge : 2 * e > edge) a = 0.f;
@@ -227,14 +229,11 @@ __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uin
             pr[e] = pack_f32x2(a, c);
         }
     }
+    uint32_t pk[AG_COLS / 2];
     if (KEYS) {
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = packed_bf16(pr[hf * 16 + e]);
-            tc::st16(mine + hf * 16, pk);
-        }
+        for (int e = 0; e < AG_COLS / 2; ++e) pk[e] = packed_bf16(pr[e]);
+        tc::st16(mine, pk);
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
@@ -242,27 +241,21 @@ __device__ __forceinline__ bool attn_grad_tile(AttnGradShared& sh, int slot, uin
     }
     if (!wait_quick(smem_u32(&sh.dp[slot]), parity, &sh.abort)) return false;
     tc::fence_after_sync();
-    {                                                    // 16 columns on their way while 16 are used (563 -> 559 us); read before dS lies there (32 of bf16 take 16)
-        uint32_t s[2][16], pk[16];
-        tc::ld16(mine + AG_DP, s[0]);
-        tc::wait_ld(s[0]);
+    uint32_t dp[2][16];                                  // (the second half on its way while the first is used)
+    tc::ld16(mine + AG_DP, dp[0]);
+    tc::wait_ld(dp[0]);
+    tc::ld16(mine + AG_DP + 16, dp[1]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (c < 3) tc::ld16(mine + AG_DP + (c + 1) * 16, s[(c + 1) % 2]);
+    for (int e = 0; e < AG_COLS; e += 4) {
+        if (e == 16) tc::wait_ld(dp[1]);
+        uint64_t l[2];
+        of_columns(stat + AG_STAT_BYTES / 2, e, d2, l[0], l[1]);
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                uint64_t l[2];
-                of_columns(stat + AG_STAT_BYTES / 2, c * 16 + e, d2, l[0], l[1]);
-#pragma unroll
-                for (int j = 0; j < 2; ++j)
-                    pk[c % 2 * 8 + e / 2 + j] = packed_bf16(mul_f32x2(
-                        pr[c * 8 + e / 2 + j],
-                        add_f32x2(pack_f32x2(__uint_as_float(s[c % 2][e + 2 * j]), __uint_as_float(s[c % 2][e + 2 * j + 1])), l[j])));
-            }
-            if (c < 3) tc::wait_ld(s[(c + 1) % 2]);
-            if (c % 2) tc::st16(mine + AG_DP + c / 2 * 16, pk);
-        }
+        for (int j = 0; j < 2; ++j)
+            pk[e / 2 + j] = packed_bf16(mul_f32x2(
+                pr[e / 2 + j], add_f32x2(pack_f32x2(__uint_as_float(dp[e / 16][e % 16 + 2 * j]), __uint_as_float(dp[e / 16][e % 16 + 2 * j + 1])), l[j])));
     }
+    tc::st16(mine + AG_DP, pk);
     tc::wait_st();
     tc::fence_before_sync();
     __syncwarp();
@@ -294,15 +287,15 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
         for (int i = 0; i < AG_SLOTS; ++i) {
             mbar_init(smem_u32(&sh.s[i]), 1);
             mbar_init(smem_u32(&sh.dp[i]), 1);
-            mbar_init(smem_u32(&sh.p[i]), 4);
-            mbar_init(smem_u32(&sh.ds[i]), 4);
+            mbar_init(smem_u32(&sh.p[i]), 8);
+            mbar_init(smem_u32(&sh.ds[i]), 8);
             mbar_init(smem_u32(&sh.s_free[i]), 1);
         }
         for (int i = 0; i < AG_UNITS; ++i) mbar_init(smem_u32(&sh.unit[i]), 1);
         sh.abort = 0;
         fence_mbar_init();
     }
-    if (warp == 12) {
+    if (warp == AG_SOFT) {
         tc::tmem_alloc(smem_u32(&sh.tmem_base), AG_TMEM);
         tc::tmem_relinquish();
     }
@@ -312,7 +305,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
     const uint32_t tmem = sh.tmem_base;
     grid_dependency_wait();
 
-    // number `u` of this CTA's blocks.  The ring is long enough: the loader is at most AG_F blocks ahead of the MMAs, of any three tiles that
+    // number `u` of this CTA's blocks.  The ring is long enough: the loader is at most AG_F blocks ahead of the MMAs, of any two tiles that
     // follow one another each group has had one, and the products of a block wait until the gradients two blocks before are stored.  (Three
     // tiles may belong to three blocks: so many F are kept.)
     auto unit_at = [&](uint32_t u, bool& ok) -> const AttnGradUnit& {
@@ -320,8 +313,8 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
         return sh.units[u % AG_UNITS];
     };
 
-    if (warp >= 12 && warp < 16) registers_down<AG_REG_ISSUE>();
-    if (warp == 13) {
+    if (warp >= AG_SOFT && warp < AG_SOFT + 4) registers_down<AG_REG_ISSUE>();
+    if (warp == AG_SOFT + 1) {
         // ---------------------------------------------------------- blocks, TMA producer
         if (elect_one()) {
             int unit = blockIdx.x;
@@ -367,12 +360,12 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                 }
             }
         }
-    } else if (warp == 12 || warp == 15) {
-        // ------------------------------------------------------------ products of the scores: S (warp 12), dP (warp 15)
+    } else if (warp == AG_SOFT || warp == AG_SOFT + 3) {
+        // ------------------------------------------------------------ products of the scores: S (the first of these warps), dP
         constexpr uint32_t I_SCORE = tc::idesc_bf16(AG_BF, AG_BX, 0);
         const uint64_t d0 = tc::smem_desc_sw128(0);
         auto at = [&](uint32_t addr) { return d0 + (uint64_t)(addr >> 4); };
-        const uint32_t second = warp == 15;
+        const uint32_t second = warp == AG_SOFT + 3;
         if (elect_one()) {
             uint32_t n = 0, was_keys = 0, freed = 0;      // per slot: whether its last tile was one of keys; the parity of s_free
             bool ok = true;
@@ -406,13 +399,14 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                 }
             }
         }
-    } else if (warp == 14) {
+    } else if (warp == AG_SOFT + 2) {
         // ------------------------------------------------------------ products of the gradients
         constexpr uint32_t I_GRAD = tc::idesc_bf16(AG_BF, AG_D, 1);
         const uint64_t d0 = tc::smem_desc_sw128(0);
-        auto grad = [&](uint32_t column, uint32_t from, uint32_t sXi, bool first) {           // (P or dS) X
+        auto grad = [&](uint32_t column, uint32_t from, uint32_t sXi, bool first) {           // (P or dS) X: each half of P where its scores began
 #pragma unroll
-            for (int kk = 0; kk < AG_BX / 16; ++kk) tc::mma_ts(tmem + column, tmem + from + kk * 8, d0 + (uint64_t)((sXi + kk * 2048) >> 4), I_GRAD, !first || kk > 0);
+            for (int kk = 0; kk < AG_BX / 16; ++kk)
+                tc::mma_ts(tmem + column, tmem + from + kk / 2 * AG_COLS + kk % 2 * 8, d0 + (uint64_t)((sXi + kk * 2048) >> 4), I_GRAD, !first || kk > 0);
         };
         if (elect_one()) {
             uint32_t n = 0, uses0 = 0, uses1 = 0;
@@ -446,7 +440,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                 }
             }
         }
-    } else if (warp >= 16) {
+    } else if (warp >= AG_SOFT + 4) {
         // ------------------------------------------------ gradients: thread = row
         registers_down<AG_REG_STORE>();
         const int row = tid % 128;
@@ -502,8 +496,8 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
     } else {
         // ------------------------------------------------ softmax groups
         registers_up<AG_REG_SOFTMAX>();
-        const int group = warp / 4, row = tid % 128;
-        const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16), mine = lanes + group * 128;
+        const int group = warp / 8, row = tid % 128, half = warp / 4 % 2 * AG_COLS;
+        const uint32_t lanes = tmem + ((uint32_t)(warp % 4 * 32) << 16) + half;
         const uint64_t scale2 = pack_f32x2(p.scale_log2, p.scale_log2);
         uint32_t n0 = 0;                                  // the block's first tile among all of this CTA's
         bool ok = true;
@@ -512,20 +506,20 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             const int steps = w.steps, f0 = w.f0, f = f0 + row, x_lo = w.x_lo, width = w.x_hi - x_lo;
-            const int i0 = (int)((group + AG_SLOTS - n0 % AG_SLOTS) % AG_SLOTS);
+            const int i0 = (int)((group + AG_GROUPS - n0 % AG_GROUPS) % AG_GROUPS);
             // the group's tiles; from which column on (queries) or up to which (keys) its rows see everything
             auto tiles = [&](auto keys, uint64_t lse2, uint64_t d2, int mine_sees, int all_see) {
                 constexpr bool KEYS = decltype(keys)::value;
                 uint32_t n = n0 + i0;
                 int x0 = (x_lo + i0 % width) * AG_BX;
                 const int behind = (x_lo + width) * AG_BX;
-                for (int i = i0; i < steps; i += AG_SLOTS, n += AG_SLOTS) {
+                for (int i = i0; i < steps; i += AG_GROUPS, n += AG_GROUPS) {
                     const uint32_t st = n % AG_STAGES;
                     const bool masked = KEYS ? x0 < all_see : x0 + AG_BX - 1 > all_see;
-                    if (!attn_grad_tile<KEYS>(sh, group, n / AG_SLOTS & 1u, mine, sStat + st * AG_STAT_BYTES, st, n / AG_STAGES & 1u, lse2, d2, scale2, masked,
-                                              mine_sees - x0, lane))
+                    if (!attn_grad_tile<KEYS>(sh, n % AG_SLOTS, n / AG_SLOTS & 1u, lanes + n % AG_SLOTS * 128, sStat + st * AG_STAT_BYTES + half * 4, st,
+                                              n / AG_STAGES & 1u, lse2, d2, scale2, masked, mine_sees - x0 - half, lane))
                         return false;
-                    x0 += AG_SLOTS * AG_BX;
+                    x0 += AG_GROUPS * AG_BX;
                     while (x0 >= behind) x0 -= width * AG_BX;
                 }
                 return true;
@@ -551,7 +545,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
     tc::fence_before_sync();
     __syncthreads();
     if (tid == 0 && sh.abort && p.error_word) atomicExch(p.error_word, BN_ERR_TIMEOUT);
-    if (warp == 12) {
+    if (warp == AG_SOFT) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, AG_TMEM);
     }
