@@ -59,70 +59,84 @@ struct AttnGradParams {
 // a pair of a gradient by a rotated row, by the row itself
 __device__ __forceinline__ uint32_t turned_back(float a, float b, float cos, float sin) { return pack_bf16(a * cos + b * sin, b * cos - a * sin); }
 
-// Rotated copies of q and k, the table of cos and sin, and a query's lse and d side by side.  A block has 16 positions and a share of the
-// heads; 8 neighbouring lanes have a head's 64 values.
-constexpr int AP_POS = 16, AP_HEADS = 32, AP_THREADS = 256;
+// Rotated copies of q and k, the table of cos and sin, and a query's lse and d side by side.  A block has 4 positions and a share of the
+// heads, a warp one position: 8 lanes have a head's 64 values, 4 heads at a time, and their angles in registers; 12 loads of 16 bytes
+// under way, the first while the angles are computed.  Memory bounds it: 55 us at 8 x 2048, 4.9 TB/s (16 positions and angles in shared
+// memory 73; 8 positions 59, 8 heads more under way 78, loads behind the angles 57).
+constexpr int AP_POS = 4, AP_HEADS = 32, AP_THREADS = 32 * AP_POS, AP_BATCH = 4;
 __global__ void __launch_bounds__(AP_THREADS)
 attn_grad_prepare_kernel(const __nv_bfloat16* q, const __nv_bfloat16* k, const __nv_bfloat16* out, const __nv_bfloat16* dout, const float* lse, __nv_bfloat16* qrot,
                          __nv_bfloat16* krot, float2* table, float* stats, int* counter, int taken, int S, int padded, int Hq, int Hkv, float theta, int offset) {
-    __shared__ float2 cs[AP_POS][AG_D / 2];
     __shared__ float sums[AP_HEADS][AP_POS + 1];
     grid_dependency_wait();
     if (blockIdx.x + blockIdx.y + blockIdx.z + threadIdx.x == 0) *counter = taken;
-    const int s0 = blockIdx.x * AP_POS, b = blockIdx.y, share = blockIdx.z, shares = gridDim.z;
-    for (int e = threadIdx.x; e < AP_POS * (AG_D / 2); e += AP_THREADS) {
-        const int s = e / (AG_D / 2), i = e % (AG_D / 2);
-        const float angle = (s0 + s + offset) * rope_inv_freq(i, AG_D, theta);
-        const float2 v = make_float2(cosf(angle), sinf(angle));
-        cs[s][i] = v;
-        if (b == 0 && share == 0 && s0 + s < S) table[(size_t)(s0 + s) * (AG_D / 2) + i] = v;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, c = lane % 8;
+    const int s0 = blockIdx.x * AP_POS, pos = s0 + warp, b = blockIdx.y, share = blockIdx.z, shares = gridDim.z;
+    const bool live = pos < S;                            // (of the warp)
+    const int h0 = (int)((long long)Hq * share / shares), h1 = (int)((long long)Hq * (share + 1) / shares);
+    uint4 x[AP_BATCH], o[AP_BATCH], d[AP_BATCH];
+    auto load = [&](int hc, int i) {                      // heads hc + i, hc + i + 4, ..
+        const size_t at = (((size_t)b * S + pos) * Hq + hc + i) * 8 + c;
+#pragma unroll
+        for (int j = 0; j < AP_BATCH; ++j)
+            if (live && i + 4 * j < AP_HEADS && hc + i + 4 * j < h1) {
+                x[j] = reinterpret_cast<const uint4*>(q)[at + j * 32];
+                o[j] = reinterpret_cast<const uint4*>(out)[at + j * 32];
+                d[j] = reinterpret_cast<const uint4*>(dout)[at + j * 32];
+            } else {
+                x[j] = o[j] = d[j] = make_uint4(0, 0, 0, 0);
+            }
+    };
+    load(h0, lane / 8);                                   // (under way while the angles are computed)
+    float2 cs[4];
+    {
+        const float angle = (pos + offset) * rope_inv_freq(lane, AG_D, theta);
+        const float2 mine = make_float2(cosf(angle), sinf(angle));
+        if (b == 0 && share == 0 && live) table[(size_t)pos * (AG_D / 2) + lane] = mine;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) cs[t] = make_float2(__shfl_sync(0xffffffffu, mine.x, c * 4 + t), __shfl_sync(0xffffffffu, mine.y, c * 4 + t));
     }
-    __syncthreads();
-    auto rotate = [&](uint4 x, int s, int c) {
+    auto rotate = [&](uint4 x) {
         uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            const float2 v = cs[s][c * 4 + t];
             const float x0 = bf16_lo(w[t]), x1 = bf16_hi(w[t]);
-            w[t] = pack_bf16(x0 * v.x - x1 * v.y, x0 * v.y + x1 * v.x);
+            w[t] = pack_bf16(x0 * cs[t].x - x1 * cs[t].y, x0 * cs[t].y + x1 * cs[t].x);
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     };
-    const int h0 = (int)((long long)Hq * share / shares), h1 = (int)((long long)Hq * (share + 1) / shares);
     for (int hc = h0; hc < h1; hc += AP_HEADS) {
         const int heads = min(AP_HEADS, h1 - hc);
-#pragma unroll 2
-        for (int e = threadIdx.x; e < AP_POS * heads * 8; e += AP_THREADS) {          // (a multiple of 32: whole warps)
-            const int c = e % 8, h = e / 8 % heads, s = e / 8 / heads, pos = s0 + s;
-            float sum = 0.f;
-            if (pos < S) {
-                const size_t at = (((size_t)b * S + pos) * Hq + hc + h) * 8 + c;
-                const uint4 x = reinterpret_cast<const uint4*>(q)[at], o = reinterpret_cast<const uint4*>(out)[at], d = reinterpret_cast<const uint4*>(dout)[at];
-                reinterpret_cast<uint4*>(qrot)[at] = rotate(x, s, c);
-                const uint32_t ow[4] = {o.x, o.y, o.z, o.w}, dw[4] = {d.x, d.y, d.z, d.w};
+        for (int i = lane / 8; live && i - lane / 8 < heads; i += 4 * AP_BATCH) {
+            const size_t at = (((size_t)b * S + pos) * Hq + hc + i) * 8 + c;
+#pragma unroll
+            for (int j = 0; j < AP_BATCH; ++j) {
+                if (i + 4 * j < heads) reinterpret_cast<uint4*>(qrot)[at + j * 32] = rotate(x[j]);
+                const uint32_t ow[4] = {o[j].x, o[j].y, o[j].z, o[j].w}, dw[4] = {d[j].x, d[j].y, d[j].z, d[j].w};
+                float sum = 0.f;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) sum = fmaf(bf16_lo(ow[t]), bf16_lo(dw[t]), fmaf(bf16_hi(ow[t]), bf16_hi(dw[t]), sum));
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+                if (c == 0 && i + 4 * j < heads) sums[i + 4 * j][warp] = sum;
             }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 4);
-            if (c == 0) sums[h][s] = sum;
+            if (i - lane / 8 + 4 * AP_BATCH < heads) load(hc, i + 4 * AP_BATCH);
+            else if (hc + AP_HEADS < h1) load(hc + AP_HEADS, lane / 8);
         }
         __syncthreads();
         for (int e = threadIdx.x; e < AP_POS * heads; e += AP_THREADS) {              // positions side by side, as lse and stats have them
-            const int s = e % AP_POS, h = e / AP_POS, pos = s0 + s;
-            float* to = stats + ((size_t)b * Hq + hc + h) * 2 * padded + pos;
-            to[0] = pos < S ? lse[((size_t)b * Hq + hc + h) * S + pos] * -1.4426950408889634f : -INFINITY;
-            to[padded] = pos < S ? -sums[h][s] : 0.f;
+            const int s = e % AP_POS, h = e / AP_POS, at = s0 + s;
+            float* to = stats + ((size_t)b * Hq + hc + h) * 2 * padded + at;
+            to[0] = at < S ? lse[((size_t)b * Hq + hc + h) * S + at] * -1.4426950408889634f : -INFINITY;
+            to[padded] = at < S ? -sums[h][s] : 0.f;
         }
         __syncthreads();
     }
-    const int g0 = (int)((long long)Hkv * share / shares), groups = (int)((long long)Hkv * (share + 1) / shares) - g0;
-    for (int e = threadIdx.x; e < AP_POS * groups * 8; e += AP_THREADS) {
-        const int c = e % 8, g = g0 + e / 8 % groups, s = e / 8 / groups, pos = s0 + s;
-        if (pos >= S) continue;
+    const int g0 = (int)((long long)Hkv * share / shares), g1 = (int)((long long)Hkv * (share + 1) / shares);
+    for (int g = g0 + lane / 8; live && g < g1; g += 4) {
         const size_t at = (((size_t)b * S + pos) * Hkv + g) * 8 + c;
-        reinterpret_cast<uint4*>(krot)[at] = rotate(reinterpret_cast<const uint4*>(k)[at], s, c);
+        reinterpret_cast<uint4*>(krot)[at] = rotate(reinterpret_cast<const uint4*>(k)[at]);
     }
 }
 
