@@ -25,7 +25,7 @@
 // before its group is.
 // A block's gradients need warps of their own: groups that stored them, 16 columns at a time behind their first tile of the next block, were
 // late for their tiles by 3000 cycles a block, most of it code that had left the instruction cache (8 x 2048 591 -> 562 us).  Registers are
-// shared out by role, so that the softmax warps spill nothing (eight fewer a thread: 571).
+// shared out by role, so that no warp spills (softmax warps of eight registers fewer: 571).
 // Launch 3, where the heads of a group are shared by several blocks: their fp32 sums of dK and dV are added in order.
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
 #include <type_traits>
@@ -195,7 +195,7 @@ __device__ __forceinline__ uint32_t packed_bf16(uint64_t v) {
 // The block is launched with 80 registers a thread; the warps that issue and store give some to the softmax warps
 template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-constexpr int AG_REGS = 80, AG_REG_SOFTMAX = 96, AG_REG_ISSUE = 48, AG_REG_STORE = 48;
+constexpr int AG_REGS = 80, AG_REG_SOFTMAX = 88, AG_REG_ISSUE = 56, AG_REG_STORE = 72;
 static_assert(128 * (AG_SOFT / 4 * AG_REG_SOFTMAX + AG_REG_ISSUE + AG_REG_STORE) <= AG_THREADS * AG_REGS, "more registers than the block is launched with");
 
 // A thread's share of a tile, `edge`: the first of its columns (of queries) or the last (of keys) that its row sees: scores -> P (bf16, over
@@ -468,18 +468,30 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
             const int f = w.f0 + row, heads = keys ? p.Hkv : p.Hq;
             const size_t at = (((size_t)w.b * p.S + f) * heads + w.hf) * AG_D, all = (size_t)p.B * p.S * p.Hkv * AG_D;
             const float4* table = reinterpret_cast<const float4*>(p.table + (size_t)min(f, p.S - 1) * (AG_D / 2));
+            float4 angle[4], next[4];
+            auto ask = [&](int c, float4 (&to)[4]) {      // (dV is not turned)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[e] = c >= 4 && c < 8 ? table[c % 4 * 4 + e] : make_float4(1.f, 0.f, 1.f, 0.f);
+            };
+            ask(keys ? 0 : 4, next);
             if (!mbar_wait_warp(smem_u32(&sh.done[u & 1]), u >> 1 & 1u, &sh.abort)) break;
             tc::fence_after_sync();
 #pragma unroll 1
             for (int c = keys ? 0 : 4; c < 8; ++c) {
                 const int col = c % 4 * 16;
+                const uint32_t acc = keys ? c / 4 : u & 1u;
                 const bool dv = c < 4;
-                float4 angle[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) angle[e] = dv ? make_float4(1.f, 0.f, 1.f, 0.f) : table[c % 4 * 4 + e];
                 uint32_t r[16];
-                tc::ld16(lanes + AG_ACC + (keys ? c / 4 : u & 1u) * 64 + col, r);
+                tc::ld16(lanes + AG_ACC + acc * 64 + col, r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) angle[e] = next[e];
+                ask(c + 1, next);
                 tc::wait_ld(r);
+                if (c % 4 == 3) {                         // the next block may have this gradient's columns (both at the end: 3 x 1371 124 -> 121 us)
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&sh.acc_free[acc]));
+                }
                 if (f < p.S) {
                     if (keys && p.parts > 1) {
                         float4* to = reinterpret_cast<float4*>(p.partial + (w.part * 2 + (dv ? 0 : 1)) * all + at + col);
@@ -500,12 +512,6 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
                     }
                 }
             }
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (keys || (u & 1u) == 0) mbar_arrive(smem_u32(&sh.acc_free[0]));
-                if (keys || (u & 1u) == 1) mbar_arrive(smem_u32(&sh.acc_free[1]));
-            }
         }
     } else {
         // ------------------------------------------------ softmax groups
@@ -525,7 +531,7 @@ attn_grad_kernel(const __grid_constant__ CUtensorMap q_rows, const __grid_consta
             auto tiles = [&](auto keys, uint64_t lse2, uint64_t d2, int mine_sees, int all_see) {
                 constexpr bool KEYS = decltype(keys)::value;
                 uint32_t n = n0 + i0;
-                int x0 = (x_lo + i0 % width) * AG_BX;
+                int x0 = (x_lo + (i0 < width ? i0 : 0)) * AG_BX;              // (i0 is 0 or 1)
                 const int behind = (x_lo + width) * AG_BX;
                 for (int i = i0; i < steps; i += AG_GROUPS, n += AG_GROUPS) {
                     const uint32_t st = n % AG_STAGES;
