@@ -758,16 +758,15 @@ def status_word(device) -> torch.Tensor:
 # Training: the loss over a vocabulary and gradients.  Nothing here is recorded by torch's autograd: a caller keeps what a
 # backward call asks for and passes it on.
 # ---------------------------------------------------------------------------------------------------------------------
-def _operands(what: str, *tensors: torch.Tensor) -> torch.device:
-    """All of them contiguous bf16 on the current device (whose current stream the launches go to)"""
-    for t in tensors:
-        _need(t, torch.bfloat16, what)
-    return _here(what, *tensors)
-
-
-def _here(what: str, *tensors: torch.Tensor) -> torch.device:
+def _operands(what: str, *tensors: torch.Tensor, dtype=torch.bfloat16) -> torch.device:
+    """All of them contiguous, of one type, on the current device (whose current stream the launches go to)"""
     dev = tensors[0].device
-    if any(t.device != dev for t in tensors) or dev.index != torch.cuda.current_device():
+    for t in tensors:
+        if t.dtype != dtype or t.device != dev or not t.is_contiguous():
+            _need(t, dtype, what)
+            raise RuntimeError(f"{what}: all tensors must lie on the current device")
+    if dev.type != "cuda" or dev.index != torch.cuda.current_device():
+        _need(tensors[0], dtype, what)
         raise RuntimeError(f"{what}: all tensors must lie on the current device")
     return dev
 
@@ -805,10 +804,9 @@ def _loss_shapes(what: str, x: torch.Tensor, weight_t: torch.Tensor, *per_row: t
     if x.dim() != 2 or weight_t.dim() != 2 or x.shape[1] != weight_t.shape[1]:
         raise RuntimeError(f"MatMul: inner dimensions mismatch {tuple(x.shape)} x {tuple(weight_t.shape)}^T")
     for t, dtype in zip(per_row, (torch.int32, torch.float32, torch.float32)):
-        _need(t, dtype, what)
+        _operands(what, t, dtype=dtype)
         if t.shape != (x.shape[0],):
             raise RuntimeError(f"{what}: targets, log-sum-exp and gradient must have one value for each of {x.shape[0]} rows")
-    _here(what, x, *per_row)
     return dev
 
 
@@ -820,10 +818,9 @@ def linear_cross_entropy(x: torch.Tensor, weight_t: torch.Tensor, targets: torch
     what = "linear_cross_entropy"
     dev = _loss_shapes(what, x, weight_t, targets)
     if id_error is not None:
-        _need(id_error, torch.int32, what)
-        _here(what, x, id_error)
+        _operands(what, id_error, dtype=torch.int32)
     (rows, hidden), vocab, lib = x.shape, weight_t.shape[0], _lib.load()
-    loss, lse = (torch.empty((rows,), dtype=torch.float32, device=dev) for _ in range(2))
+    loss, lse = (x.new_empty((rows,), dtype=torch.float32) for _ in range(2))
     ws = _scratch(lib.bn_linear_cross_entropy_bf16_workspace_bytes(rows, vocab, hidden), dev)
     _lib.check(lib.bn_linear_cross_entropy_bf16(x.data_ptr(), weight_t.data_ptr(), targets.data_ptr(), loss.data_ptr(), lse.data_ptr(), rows, vocab,
                                                 hidden, ws.data_ptr(), ws.numel(), _ptr(id_error), _gemm_error_ptr(dev, None), _stream()))
@@ -875,8 +872,7 @@ def attn_prefill_bf16_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Ten
     what that call gave for the same arguments, `dout` the gradient of `out`.  k and v have the sums over their group's query heads."""
     what = "attn_prefill_bf16_backward"
     dev = _operands(what, dout, q, k, v, out)
-    _need(lse, torch.float32, what)
-    _here(what, q, lse)
+    _operands(what, lse, dtype=torch.float32)
     if q.dim() != 4 or v.dim() != 4:
         raise RuntimeError(f"{what}: q must be (B, S, Hq, D), k and v (B, S, Hkv, D)")
     (B, S, Hq, D), Hkv, lib = q.shape, v.shape[2], _lib.load()
