@@ -288,7 +288,8 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
         const uint32_t lane_base = ((uint32_t)(warp % 4 * 32)) << 16;
         const uint32_t out0 = smem0 + n_stages * p.ring.stage_bytes + warp * (grad_out_bytes(EPI == GE_GLU) / EW);
         int out_turn = 0;
-        // the warp's next buffer, when what was sent from it before has been read
+        // the warp's next buffer, when what was sent from it before has been read: all but the newest group have been, and the newest is the
+        // other buffer's, so every buffer that is taken has to be sent
         auto out_buffer = [&] {
             if (lane == 0) bulk_wait_group_read<1>();
             __syncwarp();
@@ -326,6 +327,7 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
             const Item w = item(q, t);
             const int M = q.M, N = q.N;
             const int gm = w.m * TILE_M + rank * GG_BM + row, n0 = w.n * columns + half * (columns / 2);
+            const int y = w.m * TILE_M + rank * GG_BM + warp % 4 * 32;          // the warp's first row
             const bool live = gm < M;
             // what a row needs beside its products, fetched while those run
             int target = -1;
@@ -364,8 +366,9 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
             if (!ok) break;
             tc::fence_after_sync();
             const uint32_t tacc = tmem + lane_base + acc * GG_BN + half * (columns / 2);
-            const int y = w.m * TILE_M + rank * GG_BM + warp % 4 * 32;          // the warp's first row
-            if (EPI == GE_DLOGITS || (PRODUCTS && !q.partial)) {
+            if (y >= M) {
+                // no row of this warp is one of the result's: nothing to take from tensor memory, nothing to send
+            } else if (EPI == GE_DLOGITS || (PRODUCTS && !q.partial)) {
                 const float factor = PRODUCTS ? common_factor(q.factor) : 1.f;
 #pragma unroll 1
                 for (int c = 0; c < p.bn / 64; ++c) {
@@ -390,7 +393,7 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
                         }
                         put_row(buf, hf, r);
                     }
-                    if (y < M) send([&] { tma_store_2d(w.part ? &maps.c1 : &maps.c0, buf, n0 + c * 64, y); });
+                    send([&] { tma_store_2d(w.part ? &maps.c1 : &maps.c0, buf, n0 + c * 64, y); });
                 }
             } else if (PRODUCTS) {
                 const bool add = q.add;
@@ -403,11 +406,10 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
                     tc::wait_ld(r);
 #pragma unroll
                     for (int v = 0; v < 8; ++v) put16(buf, v, r[v * 4], r[v * 4 + 1], r[v * 4 + 2], r[v * 4 + 3]);
-                    if (y < M)
-                        send([&] {
-                            if (add) tma_add_3d(&maps.c0, buf, n0 + c * 32, y, w.split);
-                            else tma_store_3d(&maps.c0, buf, n0 + c * 32, y, w.split);
-                        });
+                    send([&] {
+                        if (add) tma_add_3d(&maps.c0, buf, n0 + c * 32, y, w.split);
+                        else tma_store_3d(&maps.c0, buf, n0 + c * 32, y, w.split);
+                    });
                 }
             } else if (EPI == GE_LOSS) {
                 // one pass: the sum is kept relative to the largest logit so far
@@ -482,12 +484,11 @@ gemm_grad_kernel(const __grid_constant__ AllMaps all, const __grid_constant__ Gr
                         put_at(u_buf + at, u4[0], u4[1], u4[2], u4[3]);
                     }
                     if (c + 1 < p.bn / 128) load_dh(col0 + 32);            // (the next tile's: before its products are waited for)
-                    if (y < M)
-                        send([&] {
-                            tma_store_2d(&maps.c0, h_buf, col0, y);
-                            tma_store_2d(&maps.c1, g_buf, col0, y);
-                            tma_store_2d(&maps.c2, u_buf, col0, y);
-                        });
+                    send([&] {
+                        tma_store_2d(&maps.c0, h_buf, col0, y);
+                        tma_store_2d(&maps.c1, g_buf, col0, y);
+                        tma_store_2d(&maps.c2, u_buf, col0, y);
+                    });
                 }
             }
             tc::fence_before_sync();
