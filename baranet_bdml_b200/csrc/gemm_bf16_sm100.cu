@@ -20,7 +20,8 @@
 // mygrad/llama/llama_layers.py:217-232, SiLU as op_silu.cuh:7-15; GELU for other models): Bt holds, per 256-row tile, 128
 // rows of the gate weight followed by the 128 rows of the up weight for the same intermediate indices, so one thread finds
 // gate and up of an output element in the same accumulator row and writes act(gate) * up -- the two GEMMs, the activation
-// and the product in one launch.
+// and the product in one launch.  The two weights may also be given as they are, (inter, K) each: a tile of Bt is then 128 rows of the
+// one and 128 of the other, by a tensor map each, and nothing has to be packed again when a weight changes.
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
 #include "common.cuh"
 #include "gemm_rows.cuh"
@@ -77,13 +78,14 @@ struct GemmParams {
     long long mul_ld;
     int act;
     const float* bias;         // EPI_BIAS: C = act(accumulator + bias), bias (n_out) or null
+    int separate;              // EPI_GLU: the gate weight and the up weight have a tensor map each
 };
 
 
 template <int EPI, int GM_BN, bool PAIR = false>
 __global__ void __launch_bounds__(GM_THREADS, 1)
 gemm_bf16_nt_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
-                    const GemmParams p) {
+                    const __grid_constant__ CUtensorMap tmap_up, const GemmParams p) {
     using Shape = GemmShape<GM_BN, PAIR>;
     constexpr int GM_NSTAGE = Shape::NSTAGE, GM_STAGE_BYTES = Shape::STAGE_BYTES;
     constexpr uint32_t GM_TMEM_COLS = Shape::TMEM_COLS;
@@ -145,6 +147,7 @@ gemm_bf16_nt_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
     if (warp == 5 && lane == 0) {
         prefetch_tensormap(&tmap_a);
         prefetch_tensormap(&tmap_b);
+        if (EPI >= EPI_GLU && p.separate) prefetch_tensormap(&tmap_up);
         if (EPI == EPI_PARTIAL && first < n_tiles) {
             int ks0, ks1;
             k_range(first, ks0, ks1);
@@ -172,12 +175,18 @@ gemm_bf16_nt_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_con
                         const uint32_t full = in_rank(smem_u32(&bar_full[stage]), 0);
                         if (rank == 0) mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), 2 * GM_STAGE_BYTES);
                         tma_load_2d_pair(sA, &tmap_a, ks * GM_BK, m0, full);
-                        tma_load_2d_pair(sB, &tmap_b, ks * GM_BK, n0, full);
+                        if (EPI >= EPI_GLU && p.separate) tma_load_2d_pair(sB, rank ? &tmap_up : &tmap_b, ks * GM_BK, n0 / GM_BN * (GM_BN / 2), full);
+                        else tma_load_2d_pair(sB, &tmap_b, ks * GM_BK, n0, full);
                         continue;
                     }
                     mbar_arrive_expect_tx(smem_u32(&bar_full[stage]), GM_STAGE_BYTES);
                     tma_load_2d(sA, &tmap_a, ks * GM_BK, m0, smem_u32(&bar_full[stage]));
-                    tma_load_2d(sB, &tmap_b, ks * GM_BK, n0, smem_u32(&bar_full[stage]));
+                    if (EPI >= EPI_GLU && p.separate) {
+                        tma_load_2d(sB, &tmap_b, ks * GM_BK, n0 / 2, smem_u32(&bar_full[stage]));
+                        tma_load_2d(sB + Shape::B_BYTES / 2, &tmap_up, ks * GM_BK, n0 / 2, smem_u32(&bar_full[stage]));
+                    } else {
+                        tma_load_2d(sB, &tmap_b, ks * GM_BK, n0, smem_u32(&bar_full[stage]));
+                    }
                 }
             }
         }
@@ -542,7 +551,7 @@ static void splitk_plan(int M, int N, int K, int sms, int* splits, int* k_per_sp
 // Launches the kernel on `grid` CTAs (PAIR: clusters of two), as a programmatic dependent unless what is ahead has to be complete or the
 // attribute is refused
 template <int EPI, int BN, bool PAIR = false>
-static int gemm_run(const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, unsigned grid, cudaStream_t st) {
+static int gemm_run(const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& up, const GemmParams& p, unsigned grid, cudaStream_t st) {
     constexpr size_t smem = GemmShape<BN, PAIR>::SMEM_BYTES;
     static thread_local int configured_dev = -1;
     int dev = 0;
@@ -572,7 +581,7 @@ static int gemm_run(const CUtensorMap& a, const CUtensorMap& b, const GemmParams
     }
     cfg.attrs = attr;
     cfg.numAttrs = n;
-    cudaError_t e = launch_config(cfg, PAIR ? 1 : 0, gemm_bf16_nt_kernel<EPI, BN, PAIR>, a, b, p);
+    cudaError_t e = launch_config(cfg, PAIR ? 1 : 0, gemm_bf16_nt_kernel<EPI, BN, PAIR>, a, b, up, p);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return fail(BN_ERR_CUDA, "gemm: %s", cudaGetErrorString(e));
@@ -594,20 +603,22 @@ static bool gemm_pairs(int M, int N, int K) {
 }
 
 template <int EPI>
-static int gemm_run256(bool pairs, const CUtensorMap& a, const CUtensorMap& b, const GemmParams& p, unsigned grid, cudaStream_t st) {
-    return pairs ? gemm_run<EPI, 256, true>(a, b, p, grid, st) : gemm_run<EPI, 256>(a, b, p, grid, st);
+static int gemm_run256(bool pairs, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& up, const GemmParams& p, unsigned grid, cudaStream_t st) {
+    return pairs ? gemm_run<EPI, 256, true>(a, b, up, p, grid, st) : gemm_run<EPI, 256>(a, b, up, p, grid, st);
 }
 
 static int gemm_launch(const void* a, const void* bt, void* c, int M, int N, int K, int n_out, int epi, int* error_word,
                        bn_stream_t stream, const char* what, float* partial = nullptr, int splits = 1,
                        int k_per_split = 0, const QkvEpilogue* qkv = nullptr, float* c32 = nullptr,
-                       const void* mul = nullptr, long long mul_ld = 0, int act = BN_ACT_NONE, const float* bias = nullptr) {
+                       const void* mul = nullptr, long long mul_ld = 0, int act = BN_ACT_NONE, const float* bias = nullptr,
+                       const void* up = nullptr) {
     if (!a || !bt || (!c && !c32)) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     if (M < 0 || N < 0 || K < 0 || n_out < 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape M=%d N=%d K=%d", what, M, N, K);
     if (n_out % 8 || K % 8)
         return fail(BN_ERR_UNSUPPORTED, "%s: N=%d and K=%d must be multiples of 8 (16-byte rows)", what, n_out, K);
     if ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(bt) | reinterpret_cast<uintptr_t>(c) |
-         reinterpret_cast<uintptr_t>(c32) | reinterpret_cast<uintptr_t>(mul) | reinterpret_cast<uintptr_t>(bias)) & 15)
+         reinterpret_cast<uintptr_t>(c32) | reinterpret_cast<uintptr_t>(mul) | reinterpret_cast<uintptr_t>(bias) |
+         reinterpret_cast<uintptr_t>(up)) & 15)
         return fail(BN_ERR_INVALID_ARG, "%s: a/bt/c must be 16-byte aligned", what);
     if (mul && (mul_ld < n_out || mul_ld % 8))
         return fail(BN_ERR_INVALID_ARG, "%s: row stride %lld of the factor (a multiple of 8, at least %d)", what, mul_ld, n_out);
@@ -620,13 +631,13 @@ static int gemm_launch(const void* a, const void* bt, void* c, int M, int N, int
         return e == cudaSuccess ? BN_OK : fail(BN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
     }
     if (epi != EPI_QKV && epi != EPI_PLAIN && gemm_rows_ok(M, n_out, K, epi >= EPI_GLU)) {
-        RowsGemm r{a, bt, static_cast<__nv_bfloat16*>(c), c32, static_cast<const __nv_bfloat16*>(mul), bias, error_word, mul_ld, M, N, K,
+        RowsGemm r{a, bt, up, static_cast<__nv_bfloat16*>(c), c32, static_cast<const __nv_bfloat16*>(mul), bias, error_word, mul_ld, M, N, K,
                    n_out, epi >= EPI_GLU ? epi - EPI_GLU : act, epi >= EPI_GLU};
         return gemm_rows(r, as_stream(stream), what);
     }
     const int bn = epi == EPI_PARTIAL ? 64 : 256, sms = sm_count();
     const bool pairs = epi != EPI_PARTIAL && gemm_pairs(M, N, K);
-    CUtensorMap tmap_a, tmap_b;
+    CUtensorMap tmap_a, tmap_b, tmap_up;
     {
         const uint64_t dims[2] = {(uint64_t)K, (uint64_t)M}, strides[1] = {(uint64_t)K * 2};
         const uint32_t box[2] = {GM_BK, GM_BM};
@@ -635,29 +646,32 @@ static int gemm_launch(const void* a, const void* bt, void* c, int M, int N, int
             return rc;
     }
     {
-        const uint64_t dims[2] = {(uint64_t)K, (uint64_t)N}, strides[1] = {(uint64_t)K * 2};
-        const uint32_t box[2] = {GM_BK, (uint32_t)(pairs ? bn / 2 : bn)};
+        const uint64_t dims[2] = {(uint64_t)K, (uint64_t)(up ? n_out : N)}, strides[1] = {(uint64_t)K * 2};
+        const uint32_t box[2] = {GM_BK, (uint32_t)(pairs || up ? bn / 2 : bn)};
         if (int rc = make_tensor_map(&tmap_b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, bt, dims, strides, box,
                                      CU_TENSOR_MAP_SWIZZLE_128B))
             return rc;
+        tmap_up = tmap_b;
+        if (up)
+            if (int rc = make_tensor_map(&tmap_up, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, up, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
     }
     const int tile_m = pairs ? 2 * GM_BM : GM_BM, places = pairs ? sms / 2 : sms;
     const long long n_items = (long long)((M + tile_m - 1) / tile_m) * ((N + bn - 1) / bn) * splits;
     GemmParams p{static_cast<__nv_bfloat16*>(c), error_word, M, N, K, n_out, partial, splits, k_per_split, QkvEpilogue{},
-                 static_cast<const __nv_bfloat16*>(mul), mul_ld, act, bias};
+                 static_cast<const __nv_bfloat16*>(mul), mul_ld, act, bias, up != nullptr};
     if (epi == EPI_F32) p.partial = c32;
     if (qkv) p.qkv = *qkv;
     const unsigned grid = (unsigned)(n_items < places ? n_items : places) * (pairs ? 2 : 1);
     cudaStream_t st = as_stream(stream);
     int rc = BN_OK;
-    if (epi == EPI_PLAIN) rc = gemm_run256<EPI_PLAIN>(pairs, tmap_a, tmap_b, p, grid, st);
-    else if (epi == EPI_GLU_SILU) rc = gemm_run256<EPI_GLU_SILU>(pairs, tmap_a, tmap_b, p, grid, st);
-    else if (epi == EPI_GLU_GELU) rc = gemm_run256<EPI_GLU_GELU>(pairs, tmap_a, tmap_b, p, grid, st);
-    else if (epi == EPI_F32) rc = gemm_run256<EPI_F32>(pairs, tmap_a, tmap_b, p, grid, st);
-    else if (epi == EPI_ACTMUL) rc = gemm_run256<EPI_ACTMUL>(pairs, tmap_a, tmap_b, p, grid, st);
-    else if (epi == EPI_BIAS) rc = gemm_run256<EPI_BIAS>(pairs, tmap_a, tmap_b, p, grid, st);
-    else if (epi == EPI_QKV) rc = gemm_run256<EPI_QKV>(pairs, tmap_a, tmap_b, p, grid, st);
-    else rc = gemm_run<EPI_PARTIAL, 64>(tmap_a, tmap_b, p, grid, st);
+    if (epi == EPI_PLAIN) rc = gemm_run256<EPI_PLAIN>(pairs, tmap_a, tmap_b, tmap_up, p, grid, st);
+    else if (epi == EPI_GLU_SILU) rc = gemm_run256<EPI_GLU_SILU>(pairs, tmap_a, tmap_b, tmap_up, p, grid, st);
+    else if (epi == EPI_GLU_GELU) rc = gemm_run256<EPI_GLU_GELU>(pairs, tmap_a, tmap_b, tmap_up, p, grid, st);
+    else if (epi == EPI_F32) rc = gemm_run256<EPI_F32>(pairs, tmap_a, tmap_b, tmap_up, p, grid, st);
+    else if (epi == EPI_ACTMUL) rc = gemm_run256<EPI_ACTMUL>(pairs, tmap_a, tmap_b, tmap_up, p, grid, st);
+    else if (epi == EPI_BIAS) rc = gemm_run256<EPI_BIAS>(pairs, tmap_a, tmap_b, tmap_up, p, grid, st);
+    else if (epi == EPI_QKV) rc = gemm_run256<EPI_QKV>(pairs, tmap_a, tmap_b, tmap_up, p, grid, st);
+    else rc = gemm_run<EPI_PARTIAL, 64>(tmap_a, tmap_b, tmap_b, p, grid, st);
     if (rc) return rc;
     if (epi == EPI_PARTIAL) {
         if (int rc = launch_status(what)) return rc;
@@ -686,6 +700,15 @@ extern "C" int bn_gemm_glu_bf16_nt(const void* x, const void* gate_up_t, void* h
     if (inter < 0) return fail(BN_ERR_INVALID_ARG, "%s: bad shape inter=%d", what, inter);
     if (act != BN_ACT_SILU && act != BN_ACT_GELU_TANH) return fail(BN_ERR_UNSUPPORTED, "%s: activation %d", what, act);
     return gemm_launch(x, gate_up_t, h, M, (inter + 127) / 128 * 256, K, inter, EPI_GLU + act, error_word, stream, what);
+}
+
+extern "C" int bn_gemm_swiglu_bf16_nt_separate(const void* x, const void* gate_t, const void* up_t, void* h, int M, int inter, int K, int* error_word,
+                                               bn_stream_t stream) {
+    const char* what = "bn_gemm_swiglu_bf16_nt_separate";
+    if (!up_t) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (inter < 0 || inter > INT32_MAX / 2 - 256) return fail(BN_ERR_INVALID_ARG, "%s: bad shape inter=%d", what, inter);
+    return gemm_launch(x, gate_t, h, M, (inter + 127) / 128 * 256, K, inter, EPI_GLU_SILU, error_word, stream, what, nullptr, 1, 0, nullptr, nullptr,
+                       nullptr, 0, BN_ACT_NONE, nullptr, up_t);
 }
 
 extern "C" int bn_gemm_bf16_nt_f32(const void* a, const void* bt, float* c, int M, int N, int K, int* error_word,

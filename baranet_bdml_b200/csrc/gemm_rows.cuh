@@ -8,7 +8,8 @@ namespace bn {
 constexpr int GR_MAX_ROWS = 128;
 
 struct RowsGemm {
-    const void *a, *w;             // (M, K), and (N, K): the output's columns, or (glu) their gate and up rows 128 by 128
+    const void *a, *w;             // (M, K), and (N, K): the output's columns, or (glu) their gate and up rows 128 by 128, or
+    const void* up;                // (glu, optional) the up weight, (n_out, K), and w is the gate weight, (n_out, K)
     __nv_bfloat16* c;              // (M, n_out), or
     float* c32;                    // the sums themselves
     const __nv_bfloat16* mul;      // optional: c = act(sum) * mul, (M, mul_ld)

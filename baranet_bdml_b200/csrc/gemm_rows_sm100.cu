@@ -47,8 +47,8 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
 
 template <int MT, int NW>
 __global__ void __launch_bounds__(GR_THREADS)
-gemm_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_a, const RowsGemm p, int ranks,
-                 int k_per_rank) {
+gemm_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_up, const __grid_constant__ CUtensorMap tmap_a,
+                 const RowsGemm p, int ranks, int k_per_rank) {
     using Sh = RowsShape<MT, NW>;
     constexpr int NSTAGE = Sh::NSTAGE;
     extern __shared__ uint8_t smem_raw[];
@@ -59,6 +59,9 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const uint32_t smem0 = (smem_u32(smem_raw) + 1023u) & ~1023u;
     const int rank = blockIdx.x % ranks, n0 = blockIdx.x / ranks * GR_BN;     // n0: first output column
+    // the tile's rows of weight q: of the packed gate and up they take turns, 128 by 128
+    const CUtensorMap* const w_map[2] = {&tmap_w, p.up ? &tmap_up : &tmap_w};
+    const int w_row = NW == 2 && !p.up ? 2 * n0 : n0, w_next = p.up ? 0 : GR_BN;
     const int k_steps = (p.K + GR_BK - 1) / GR_BK, ks0 = min(rank * k_per_rank, k_steps), ks1 = min(k_steps, ks0 + k_per_rank);
 
     if (tid == 0) {
@@ -79,7 +82,7 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
         prefetch_tensormap(&tmap_a);
         for (int ks = ks0; ks < ks1; ++ks)
 #pragma unroll
-            for (int q = 0; q < NW; ++q) tma_prefetch_2d(&tmap_w, ks * GR_BK, NW * n0 + q * GR_BN);
+            for (int q = 0; q < NW; ++q) tma_prefetch_2d(w_map[q], ks * GR_BK, w_row + q * w_next);
     }
     tc::fence_before_sync();
     __syncthreads();
@@ -98,7 +101,7 @@ gemm_rows_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_consta
                 const uint32_t full = smem_u32(&bar_full[stage]), sW = smem0 + stage * Sh::STAGE_BYTES;
                 mbar_arrive_expect_tx(full, Sh::STAGE_BYTES);
 #pragma unroll
-                for (int q = 0; q < NW; ++q) tma_load_2d(sW + q * Sh::W_BYTES, &tmap_w, ks * GR_BK, NW * n0 + q * GR_BN, full);
+                for (int q = 0; q < NW; ++q) tma_load_2d(sW + q * Sh::W_BYTES, w_map[q], ks * GR_BK, w_row + q * w_next, full);
                 tma_load_2d(sW + NW * Sh::W_BYTES, &tmap_a, ks * GR_BK, 0, full);
             }
         }
@@ -242,10 +245,13 @@ static int rows_launch(const RowsGemm& p, cudaStream_t st, const char* what) {
         if (e != cudaSuccess) return fail(BN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
         configured_dev = dev;
     }
-    CUtensorMap mw, ma;
-    const uint64_t dims_w[2] = {(uint64_t)p.K, (uint64_t)p.N}, dims_a[2] = {(uint64_t)p.K, (uint64_t)p.M}, stride[1] = {(uint64_t)p.K * 2};
+    CUtensorMap mw, mu, ma;
+    const uint64_t dims_w[2] = {(uint64_t)p.K, (uint64_t)(p.up ? p.n_out : p.N)}, dims_a[2] = {(uint64_t)p.K, (uint64_t)p.M}, stride[1] = {(uint64_t)p.K * 2};
     const uint32_t box_w[2] = {GR_BK, GR_BN}, box_a[2] = {GR_BK, MT};
     if (int rc = make_tensor_map(&mw, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.w, dims_w, stride, box_w, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+    mu = mw;
+    if (p.up)
+        if (int rc = make_tensor_map(&mu, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.up, dims_w, stride, box_w, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
     if (int rc = make_tensor_map(&ma, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.a, dims_a, stride, box_a, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
     const int tiles = (p.n_out + GR_BN - 1) / GR_BN, steps = (p.K + GR_BK - 1) / GR_BK;
     const int ranks = rows_ranks(tiles, steps, rows_resident(Sh::PER_SM));
@@ -262,7 +268,7 @@ static int rows_launch(const RowsGemm& p, cudaStream_t st, const char* what) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    cudaError_t e = launch_config(cfg, 1, gemm_rows_kernel<MT, NW>, mw, ma, p, ranks, (steps + ranks - 1) / ranks);
+    cudaError_t e = launch_config(cfg, 1, gemm_rows_kernel<MT, NW>, mw, mu, ma, p, ranks, (steps + ranks - 1) / ranks);
     if (e != cudaSuccess) {
         (void)cudaGetLastError();
         return fail(BN_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));

@@ -277,11 +277,10 @@ class MLPBF16:
     """The SwiGLU feed-forward block (mygrad/llama/llama_layers.py:194-235: gate_proj, up_proj, down_proj;
     `(SiLU(x @ gate) * (x @ up)) @ down`) on the tensor-core path: one fused gate/up GEMM with the SiLU * mul epilogue
     and one down GEMM.  Weights are held transposed in bf16; `gate_proj` / `up_proj` / `down_proj` keep the reference's
-    names.  x: torch bf16 (tokens, hidden) on the GPU.  A call keeps nothing for a backward pass: `backward` takes x again."""
+    names.  x: torch bf16 (tokens, hidden) on the GPU.  A call keeps nothing for a backward pass: `backward` takes x again; both read the
+    three weights where they lie, as they are at the time (a captured call: at the replay)."""
 
     def __init__(self, config, is_cuda: bool = True):
-        import torch
-        from . import ops
         if not is_cuda:
             raise RuntimeError("MatMul: only GPU implementation available")
         self.config = config
@@ -290,7 +289,6 @@ class MLPBF16:
         init = _init_weight_t
         self.gate_proj, self.up_proj, self.down_proj = init(hidden, inter), init(hidden, inter), init(inter, hidden)
         self.intermediate_size = inter
-        self._gate_up = ops.pack_gate_up(self.gate_proj, self.up_proj)
 
     def __call__(self, x, few_rows: bool = False):
         from . import ops
@@ -299,7 +297,7 @@ class MLPBF16:
             # a decode step with at most 16 rows: both products are weight streams
             h = ops.gemm_swiglu_bf16_nt_skinny(x, self.gate_proj, self.up_proj)
             return ops.gemm_bf16_nt_skinny(h, self.down_proj)
-        h = ops.gemm_swiglu_bf16_nt(x, self._gate_up, self.intermediate_size)
+        h = ops.gemm_swiglu_bf16_nt_separate(x, self.gate_proj, self.up_proj)
         # the down projection has few output tiles: with few rows (a decode step) the split-K form streams its weight
         # with all SMs
         return ops.linear_bf16(h, self.down_proj) if few_rows else ops.gemm_bf16_nt(h, self.down_proj)

@@ -402,7 +402,6 @@ class LLaMAModelBF16(CausalLM):
             at.v_proj, at.o_proj = put(p + "self_attn.v_proj", kv, H), put(p + "self_attn.o_proj", H, H)
             mlp.gate_proj, mlp.up_proj = put(p + "mlp.gate_proj", inter, H), put(p + "mlp.up_proj", inter, H)
             mlp.down_proj = put(p + "mlp.down_proj", H, inter)
-            mlp._gate_up = ops.pack_gate_up(mlp.gate_proj, mlp.up_proj)
             layer.input_layernorm_weight = put(p + "input_layernorm", H)
             layer.post_attention_layernorm_weight = put(p + "post_attention_layernorm", H)
         self.norm_weight = put("norm", H)

@@ -228,6 +228,10 @@ BN_API int bn_gemm_qkv_append_bf16_skinny(const void* x, const void* wqkv_t, int
  * that follows is bn_gemm_bf16_nt. */
 BN_API int bn_gemm_swiglu_bf16_nt(const void* x, const void* gate_up_t, void* h, int M, int inter, int K,
                                   int* error_word, bn_stream_t stream);
+/* The same with the two weights as they are stored, gate_t and up_t (inter, K) bf16 each, 16-byte aligned: for weights that change
+ * between calls (a training step), which would have to be packed again. */
+BN_API int bn_gemm_swiglu_bf16_nt_separate(const void* x, const void* gate_t, const void* up_t, void* h, int M, int inter, int K,
+                                           int* error_word, bn_stream_t stream);
 
 /* y = x / sqrt(mean(x^2) + eps) * w, row by row; x, y (rows, hidden), w (hidden) with element strides.
  * Same arithmetic order as the reference kernel (256 partial fused-multiply-add chains, its reduction tree, IEEE
