@@ -180,7 +180,8 @@ class GroupedQueryAttentionBF16:
     is `bn_gemm_bf16_nt`: three kernel launches.  Same constructor arguments, attribute names and
     `__call__(hidden_states, position_offset, use_causal_mask)` as mygrad/llama/llama_layers.py:46-191;
     hidden_states is a torch bf16 tensor (B, S, hidden) or (S, hidden) on the GPU.  A call keeps nothing for a backward
-    pass: `backward` takes the input again."""
+    pass: `backward` takes the input again; both read the weights as they are at the time (a captured call: at the replay,
+    of the tensors that were the layer's at the capture)."""
 
     def __init__(self, config, is_cuda: bool = True):
         import torch
@@ -196,21 +197,35 @@ class GroupedQueryAttentionBF16:
         init = _init_weight_t
         self.q_proj, self.k_proj = init(self.hidden_size, self.hidden_size), init(self.hidden_size, kv)
         self.v_proj, self.o_proj = init(self.hidden_size, kv), init(self.hidden_size, self.hidden_size)
-        self._qkv_t = None          # Wq^T, Wk^T, Wv^T stacked: built at the first fused call from the three above
+        self.stack_qkv()
         self._ws_table = None       # (S, theta, position_offset) of the cos/sin table in the scratch buffer
         self.rotary_emb = RotaryEmbedding(self.head_dim, max_position_embeddings=config.max_position_embeddings,
                                           base=config.rope_theta)
         self.scale = 1.0 / np.sqrt(self.head_dim)
         self._ws = None
 
-    def packed_qkv(self):
-        """(Hq + 2 Hkv) * D rows: the three projection weights (held transposed) one after the other.  Rebuilt when
-        one of them has been replaced (they are plain attributes, as in the reference layer)."""
+    def stack_qkv(self):
+        """Moves the three projection weights (held transposed) into one tensor, (Hq + 2 Hkv) * D rows, of which the attributes
+        are parts from then on.  The constructor does so; after an assignment to one of the attributes it saves the copy that
+        every call makes otherwise."""
         import torch
-        key = (self.q_proj.data_ptr(), self.k_proj.data_ptr(), self.v_proj.data_ptr())
-        if self._qkv_t is None or self._qkv_t[0] != key:
-            self._qkv_t = (key, torch.cat([self.q_proj, self.k_proj, self.v_proj], dim=0).contiguous())
-        return self._qkv_t[1]
+        weights = (self.q_proj, self.k_proj, self.v_proj)
+        self._qkv_t = torch.cat(weights)
+        ends = np.cumsum([w.shape[0] for w in weights])
+        self.q_proj, self.k_proj, self.v_proj = (self._qkv_t[end - w.shape[0]:end] for w, end in zip(weights, ends))
+
+    def packed_qkv(self):
+        """The three projection weights one after the other, as they are now: the tensor that they are parts of, or, where one
+        of them has been assigned from outside (they are plain attributes, as in the reference layer), a copy for this call.
+        No copy outlives its call: neither an address nor a count of writes tells reliably that a weight is still the same."""
+        import torch
+        weights, stack, row = (self.q_proj, self.k_proj, self.v_proj), self._qkv_t, 0
+        for w in weights:
+            if w.data_ptr() != stack.data_ptr() + row * stack.stride(0) * stack.element_size() or w.dtype != stack.dtype or \
+                    w.dim() != 2 or w.shape[1] != stack.shape[1] or not w.is_contiguous():
+                return torch.cat(weights)
+            row += w.shape[0]
+        return stack if row == stack.shape[0] else torch.cat(weights)
 
     def attend(self, x2, B: int, S: int, position_offset: int = 0, use_causal_mask: bool = True, cache=None,
                workspace=None):
@@ -265,8 +280,7 @@ class GroupedQueryAttentionBF16:
         dattn = ops.gemm_bf16_nn(dy, self.o_proj).view(B, S, nq, D)
         do = ops.gemm_bf16_tn(dy, attn.view(n, nq * D))
         dqkv = torch.cat([g.view(n, -1) for g in ops.attn_prefill_bf16_backward(dattn, q, k, v, attn, lse, **how)], dim=1)
-        # (the weights as they are now: the packed copy of the forward pass knows only of tensors that were replaced)
-        dx = ops.gemm_bf16_nn(dqkv, torch.cat([self.q_proj, self.k_proj, self.v_proj])).view(hidden_states.shape)
+        dx = ops.gemm_bf16_nn(dqkv, self.packed_qkv()).view(hidden_states.shape)
         return dx, [*ops.gemm_bf16_tn(dqkv, x2).split([nq * D, nkv * D, nkv * D]), do]
 
     def parameters(self):

@@ -400,6 +400,7 @@ class LLaMAModelBF16(CausalLM):
             p, at, mlp = f"layers.{i}.", layer.self_attn, layer.mlp
             at.q_proj, at.k_proj = put(p + "self_attn.q_proj", H, H), put(p + "self_attn.k_proj", kv, H)
             at.v_proj, at.o_proj = put(p + "self_attn.v_proj", kv, H), put(p + "self_attn.o_proj", H, H)
+            at.stack_qkv()
             mlp.gate_proj, mlp.up_proj = put(p + "mlp.gate_proj", inter, H), put(p + "mlp.up_proj", inter, H)
             mlp.down_proj = put(p + "mlp.down_proj", H, inter)
             layer.input_layernorm_weight = put(p + "input_layernorm", H)
