@@ -26,7 +26,7 @@
 //             order: the same bits in every run
 //   LOSS      logits: of every row's columns in a tile the maximum and the sum of exponentials, and the target's logit: the logits stay in
 //             tensor memory
-//   DLOGITS   logits again -> g (exp(z - lse) - [v = target]) over the first row's g, as bf16
+//   DLOGITS   logits again -> g (exp(z - lse) - [v = target]) over the first row's g (its significand), as bf16
 //   GLU       columns [0,128) gate, [128,256) up of the same indices, and dh, fp32 -> dgate, dup and the product that the forward pass had
 // Every mbarrier wait is bounded; on expiry the kernel raises the caller's error word, frees TMEM and returns.
 #include <type_traits>
@@ -89,11 +89,13 @@ struct GradParams {
 struct GradMaps { CUtensorMap a0, a1, b0, b1, c0, c1, c2; };
 struct AllMaps { GradMaps job[GG_JOBS]; };
 
-// What the logits' gradients are divided by before they are rounded, and their products multiplied by: the first row's gradient, so that a
-// mean's 1 / rows, which all rows have, is not rounded to bf16 in every one of them alike (errors of 2.9e-3 instead of 2.4e-3)
+// What the logits' gradients are divided by before they are rounded, and their products multiplied by: the first row's gradient without its
+// power of two, 1 <= |factor| < 2, so that a mean's 1 / rows, which all rows have, is not rounded to bf16 in every one of them alike
+// (errors of 2.9e-3 instead of 2.4e-3), and no other row's gradient leaves the range that it has itself.  0, subnormal numbers, infinities
+// and NaN: 1.
 __device__ __forceinline__ float common_factor(const float* grad) {
-    const float g = grad ? *grad : 1.f, size = fabsf(g);
-    return size >= 0x1p-40f && size <= 0x1p40f ? g : 1.f;
+    const uint32_t bits = grad ? __float_as_uint(*grad) : 0u, exponent = bits & 0x7f800000u;
+    return exponent == 0 || exponent == 0x7f800000u ? 1.f : __uint_as_float((bits & 0x807fffffu) | 0x3f800000u);
 }
 
 __device__ __forceinline__ float log2e() { return 1.4426950408889634f; }

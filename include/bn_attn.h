@@ -627,7 +627,7 @@ BN_API int bn_linear_cross_entropy_bf16(const void* x, const void* weight_t, con
                                         int hidden, void* workspace, size_t workspace_bytes, int* id_error, int* error_word,
                                         bn_stream_t stream);
 /* Its gradients: dz[r][v] = grad_loss[r] (exp(z[r][v] - lse[r]) - [v = targets[r]]), a piece of the vocabulary at a time and as bf16
- * multiples of grad_loss[0]; dx (rows, hidden) = dz @ weight_t, dweight_t (vocab, hidden) = dz^T @ x, bf16.  Either may be NULL.
+ * multiples of grad_loss[0]'s significand; dx (rows, hidden) = dz @ weight_t, dweight_t (vocab, hidden) = dz^T @ x, bf16.  Either may be NULL.
  * lse from the call above.  Every row of x has to be finite, for one without a target is a factor of 0 in dweight_t's sums.  rows = 0
  * gives a zero dweight_t. */
 BN_API size_t bn_linear_cross_entropy_backward_bf16_workspace_bytes(int rows, int vocab, int hidden);

@@ -57,10 +57,9 @@ def test_product_across_the_weights_rows_by_elements(lib, M, N, K):
     ops.gemm_status()
 
 
-@pytest.mark.parametrize("rows,hidden,vocab", [(64, 2048, 10007), (16, 2048, 10007), (1531, 1000, 10007), (600, 2048, 32000), (2100, 1032, 30522)])
-def test_loss_gradients_by_elements(lib, rows, hidden, vocab):
+def check_loss_gradients(x, w, targets, grad):
     from baranet_bdml_b200 import ops
-    x, w, targets, grad = loss_inputs(rows, hidden, vocab, rows + vocab)
+    rows, hidden, vocab = *x.shape, w.shape[0]
     _, lse = ops.linear_cross_entropy(x, w, targets)
     got = ops.linear_cross_entropy_backward(x, w, targets, lse, grad)
     X, W, t = x.double(), w.double(), targets.long()
@@ -70,7 +69,7 @@ def test_loss_gradients_by_elements(lib, rows, hidden, vocab):
     off = sums(hidden) * 2 * (X.abs() @ W.abs().T).amax().item() + 4 * UNIT * (z.abs().max().item() + total.abs().max().item()) + 2 * UNIT
     size = torch.where(t >= 0, grad.double(), 0.0).abs()[:, None]
     p = torch.exp(z - total[:, None])
-    p_off = size * (p * 1.01 * off + UNIT)                # (the difference to 1 at the target rounds too)
+    p_off = size * (p * 1.01 * off + UNIT) + 2.0 ** -126  # (the difference to 1 at the target rounds too; what is below normal numbers may be lost)
     p[torch.arange(rows, device="cuda"), t.clamp(min=0)] -= 1.0
     dz = p * torch.where(t >= 0, grad.double(), 0.0)[:, None]
     dz_off = p_off + (HALF * 1.01 + sums(max(rows, vocab))) * dz.abs()
@@ -78,6 +77,20 @@ def test_loss_gradients_by_elements(lib, rows, hidden, vocab):
     within(got[1], dz.T @ X, dz_off.T @ X.abs())
     again(lambda: ops.linear_cross_entropy_backward(x, w, targets, lse, grad), got)
     ops.gemm_status()
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [(64, 2048, 10007), (16, 2048, 10007), (1531, 1000, 10007), (600, 2048, 32000), (2100, 1032, 30522)])
+def test_loss_gradients_by_elements(lib, rows, hidden, vocab):
+    check_loss_gradients(*loss_inputs(rows, hidden, vocab, rows + vocab))
+
+
+@pytest.mark.parametrize("first,others", [(1.5 * 2.0 ** -40, 1e30), (1.3 * 2.0 ** 40, 1e-30), (-1e-30, 1e-3), (1e-45, 1.0), (0.0, 1e-3), (-3e38, 1e-6)])
+def test_gradients_of_any_size_beside_the_first_rows(lib, first, others):
+    """Rows' gradients far above or below the first one's, which they are written as multiples of."""
+    x, w, targets, grad = loss_inputs(100, 264, 1000, 12)
+    grad = grad * 100 * others * torch.where(torch.arange(100, device="cuda") % 3 == 0, -1.0, 1.0)
+    grad[0], targets[0] = first, -100 if abs(first) > 1e38 else 5
+    check_loss_gradients(x, w, targets, grad)
 
 
 @pytest.mark.parametrize("rows,hidden,inter,act", [(64, 1000, 2712, "silu"), (1371, 1000, 2712, "gelu_tanh"), (5000, 2048, 5632, "silu")])
