@@ -93,12 +93,9 @@ def test_gradients_of_any_size_beside_the_first_rows(lib, first, others):
     check_loss_gradients(x, w, targets, grad)
 
 
-@pytest.mark.parametrize("rows,hidden,inter,act", [(64, 1000, 2712, "silu"), (1371, 1000, 2712, "gelu_tanh"), (5000, 2048, 5632, "silu")])
-def test_gated_block_gradients_by_elements(lib, rows, hidden, inter, act):
+def check_gated(x, dy, gate, up, down, act):
     from baranet_bdml_b200 import ops
-    rng = np.random.default_rng(rows + inter)
-    x, dy = bf16(rng, rows, hidden), bf16(rng, rows, hidden, std=1.0 / rows)
-    gate, up, down = bf16(rng, inter, hidden, std=hidden ** -0.5), bf16(rng, inter, hidden, std=hidden ** -0.5), bf16(rng, hidden, inter, std=inter ** -0.5)
+    rows, inter, hidden = x.shape[0], *gate.shape
     got = ops.gated_ff_backward(dy, x, gate, up, down, act=act)
     X, DY, G, U, D = (t.double() for t in (x, dy, gate, up, down))
     g, u, dh = X @ G.T, X @ U.T, DY @ D
@@ -120,3 +117,32 @@ def test_gated_block_gradients_by_elements(lib, rows, hidden, inter, act):
     within(got[3], DY.T @ h, DY.abs().T @ h_off)
     again(lambda: ops.gated_ff_backward(dy, x, gate, up, down, act=act), got)
     ops.gemm_status()
+
+
+@pytest.mark.parametrize("rows,hidden,inter,act", [(64, 1000, 2712, "silu"), (1371, 1000, 2712, "gelu_tanh"), (5000, 2048, 5632, "silu")])
+def test_gated_block_gradients_by_elements(lib, rows, hidden, inter, act):
+    rng = np.random.default_rng(rows + inter)
+    x, dy = bf16(rng, rows, hidden), bf16(rng, rows, hidden, std=1.0 / rows)
+    check_gated(x, dy, bf16(rng, inter, hidden, std=hidden ** -0.5), bf16(rng, inter, hidden, std=hidden ** -0.5),
+                bf16(rng, hidden, inter, std=inter ** -0.5), act)
+
+
+# few tiles and a long K: a weight's gradient of a narrow layer over many tokens
+@pytest.mark.parametrize("M,N,K", [(256, 256, 16384), (256, 2048, 16384), (8, 8, 16383), (264, 520, 5001)])
+def test_product_of_two_transposed_operands_with_a_long_sum(lib, M, N, K):
+    from baranet_bdml_b200 import ops
+    rng = np.random.default_rng(M + K)
+    a, b = bf16(rng, K, M), bf16(rng, K, N, std=K ** -0.5)
+    got = ops.gemm_bf16_tn(a, b)
+    within(got, a.double().T @ b.double(), sums(K) * (a.double().abs().T @ b.double().abs()))
+    again(lambda: [ops.gemm_bf16_tn(a, b)], [got])
+    ops.gemm_status()
+
+
+def test_gated_block_gradients_of_a_narrow_layer(lib):
+    from baranet_bdml_b200 import ops
+    rng = np.random.default_rng(9)
+    rows, hidden, inter = 16384, 256, 512
+    x, dy = bf16(rng, rows, hidden), bf16(rng, rows, hidden, std=1.0 / rows)
+    weights = bf16(rng, inter, hidden, std=hidden ** -0.5), bf16(rng, inter, hidden, std=hidden ** -0.5), bf16(rng, hidden, inter, std=inter ** -0.5)
+    check_gated(x, dy, *weights, "silu")
