@@ -254,13 +254,16 @@ class LLaMAModelBF16(CausalLM):
 
     # ------------------------------------------------------------------ pieces
     def embed(self, input_ids: torch.Tensor, check: bool = True, error: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """(n,) int32 token ids on the device -> (n, hidden) bf16 (gather on the device).  `check=False` skips the
+        """(n,) token ids -> (n, hidden) bf16 (gather on the device; ids that lie elsewhere are copied there).  `check=False` skips the
         host read of the out-of-range flag (a synchronisation), for use inside a CUDA graph, or where the caller reads
         the flag, a zeroed int32 `error` of its own, later."""
-        ids = input_ids.to(torch.int32).contiguous()
+        dev = self.embed_tokens.device
+        if dev.index != torch.cuda.current_device():
+            raise RuntimeError(f"embed: the model lies on {dev}, which is not the current device")
+        ids = input_ids.to(device=dev, dtype=torch.int32).contiguous()
         n, H = ids.numel(), self.config.hidden_size
-        out = torch.empty((n, H), dtype=torch.bfloat16, device="cuda")
-        err = torch.zeros(1, dtype=torch.int32, device="cuda") if check and error is None else error
+        out = torch.empty((n, H), dtype=torch.bfloat16, device=dev)
+        err = torch.zeros(1, dtype=torch.int32, device=dev) if check and error is None else error
         _lib.check(_lib.load().bn_embedding_gather_f32_bf16(self.embed_tokens.data_ptr(), H, ids.data_ptr(), out.data_ptr(), H,
                                                             n, H, self.config.vocab_size, None if err is None else err.data_ptr(),
                                                             ops._stream()))
@@ -288,7 +291,8 @@ class LLaMAModelBF16(CausalLM):
         """The log-probability that the model gives each id behind the first: (B, S) ids -> (B, S - 1) fp32.  The logits, which
         `__call__` returns as B * S * vocab numbers, are kept nowhere."""
         B, S = input_ids.shape
-        H, ids = self.config.hidden_size, input_ids.to(torch.int32)
+        # (an id that leaves 32 bits is outside the vocabulary, not the one that its low bits name)
+        H, ids = self.config.hidden_size, input_ids.to(self.embed_tokens.device, torch.int64).clamp(-1, self.config.vocab_size).to(torch.int32)
         if S < 2:
             raise RuntimeError(f"score: {S} ids in a sequence; the first has no probability, so at least two are needed")
         h = self.embed(ids.reshape(-1)).view(B, S, H)
@@ -297,7 +301,7 @@ class LLaMAModelBF16(CausalLM):
             h, pending = layer.forward_parts(h, 0, True, pending=pending)
         _, normed = ops.add_rmsnorm_bf16(h.reshape(B * S, H), pending.reshape(B * S, H), self.norm_weight, self.config.rms_norm_eps,
                                          want_sum=False)
-        targets = torch.full((B, S), -1, dtype=torch.int32, device="cuda")       # the last position has none
+        targets = torch.full((B, S), -1, dtype=torch.int32, device=ids.device)   # the last position has none
         targets[:, :-1] = ids[:, 1:]
         loss, _ = ops.linear_cross_entropy(normed, self.lm_head, targets.view(-1))
         return -loss.view(B, S)[:, :-1]
