@@ -349,14 +349,13 @@ def gemm_swiglu_bf16_nt(x: torch.Tensor, gate_up_t: torch.Tensor, inter: int, *,
 def gemm_swiglu_bf16_nt_separate(x: torch.Tensor, gate_t: torch.Tensor, up_t: torch.Tensor) -> torch.Tensor:
     """silu(x @ Wgate) * (x @ Wup) -> (M, inter) bf16 in one launch, the two weights (inter, K) as they are at the call."""
     what = "gemm_swiglu_bf16_nt_separate"
-    for t, n in ((x, "x"), (gate_t, "gate_t"), (up_t, "up_t")):
-        _need(t, torch.bfloat16, f"{what}({n})")
+    dev = _operands(what, x, gate_t, up_t)
     if x.dim() != 2 or gate_t.dim() != 2 or gate_t.shape[1] != x.shape[1] or up_t.shape != gate_t.shape:
         raise RuntimeError(f"{what}: x must be (M, K), gate and up weights (inter, K)")
     (M, K), inter = x.shape, gate_t.shape[0]
-    out = torch.empty((M, inter), dtype=torch.bfloat16, device=x.device)
+    out = torch.empty((M, inter), dtype=torch.bfloat16, device=dev)
     _lib.check(_lib.load().bn_gemm_swiglu_bf16_nt_separate(x.data_ptr(), gate_t.data_ptr(), up_t.data_ptr(), out.data_ptr(), M, inter, K,
-                                                           _gemm_error_ptr(x.device, None), _stream()))
+                                                           _gemm_error_ptr(dev, None), _stream()))
     return out
 
 
