@@ -91,8 +91,8 @@ struct AllMaps { GradMaps job[GG_JOBS]; };
 
 // What the logits' gradients are divided by before they are rounded, and their products multiplied by: the first row's gradient without its
 // power of two, 1 <= |factor| < 2, so that a mean's 1 / rows, which all rows have, is not rounded to bf16 in every one of them alike
-// (errors of 2.9e-3 instead of 2.4e-3), and no other row's gradient leaves the range that it has itself.  0, subnormal numbers, infinities
-// and NaN: 1.
+// (errors of 1.9 - 2.2e-3 instead of 1.66e-3, which the last rounding alone makes), and no other row's gradient leaves the range that it
+// has itself.  0, subnormal numbers, infinities and NaN: 1.
 __device__ __forceinline__ float common_factor(const float* grad) {
     const uint32_t bits = grad ? __float_as_uint(*grad) : 0u, exponent = bits & 0x7f800000u;
     return exponent == 0 || exponent == 0x7f800000u ? 1.f : __uint_as_float((bits & 0x807fffffu) | 0x3f800000u);
@@ -813,8 +813,9 @@ int zero(void* p, size_t bytes, cudaStream_t st, const char* what) {
 }
 
 // Columns of the vocabulary that a piece of the backward pass takes: the piece's logit gradients, 2 bytes each, stay at 128 MB, about what
-// L2 holds, but never fewer than 4096 columns: every piece reads and writes the rows' fp32 gradients again (rows x hidden x 8 bytes
-// against 6 x rows x 4096 x hidden operations: a tenth of the products' time).
+// L2 holds, or at 4096 columns where that is more (above 16384 rows): every piece reads and writes the rows' fp32 gradients again (rows x
+// hidden x 8 bytes against 6 x rows x columns x hidden operations: of 4096 columns a tenth of the products' time).  Pieces are of equal
+// size, so they have more than half as many columns: 4500 of 16500 rows are two of 2304, whose traffic is then a fifth.
 int piece_columns(int rows, int vocab) {
     long long want = (64LL << 20) / rows / 256 * 256;
     if (want < 4096) want = 4096;
@@ -998,7 +999,7 @@ static Plan plan_gradients(Product (&p)[3], int rows, int hidden, int inter) {
 }
 
 // h, dgate and dup (bf16); dh and, when that has been used, the sums of dx (fp32): dh rounded to bf16 would add half of the error that the
-// gradients have from their own roundings (2.9e-3 instead of 2.4e-3), and its ranges of K are added where it is read
+// gradients have from their own roundings (2.9e-3 instead of 2.35e-3), and its ranges of K are added where it is read
 extern "C" size_t bn_gated_ff_backward_bf16_workspace_bytes(int rows, int hidden, int inter) {
     if (rows <= 0 || hidden <= 0 || inter <= 0 || longer(rows, hidden, inter)) return 0;
     Product dh, p[3];

@@ -362,8 +362,8 @@ static int skinny_launch(const SkinnyParams& p, cudaStream_t st, const char* wha
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    // us before and now, the kernel that stays second.  Gated pairs: 2048 -> 2048 5.4, 4.1, -> 5632 11.7, 9.0 (between
-    // them, where three CTAs a multiprocessor hold all groups at once, the slower by a fifteenth).  Others with 8 rows: 2048 -> 256 2.2, 2.1, -> 4608 5.4, 4.9, 4096 -> 2048 5.4, 4.6,
+    // us before and now, the kernel that stays second.  Gated pairs: 2048 -> 2048 5.4, 4.1, -> 5632 11.7, 9.0, between
+    // them, where three CTAs a multiprocessor hold all groups at once, 6.0, 6.4.  Others with 8 rows: 2048 -> 256 2.2, 2.1, -> 4608 5.4, 4.9, 4096 -> 2048 5.4, 4.6,
     // 7424 -> 2048 8.6, 7.3, but 1024 -> 4608 3.3, 3.5 (1024 -> 6144, in two waves, 5.0, 4.1); with 16 rows the groups have
     // to share CTAs before the rows kept pay: 2048 -> 512 2.6, 3.0, -> 2048 4.0, 4.1, -> 2560 5.7, 5.0
     const int groups = p.N / 8;

@@ -628,6 +628,7 @@ BN_API int bn_linear_cross_entropy_bf16(const void* x, const void* weight_t, con
                                         bn_stream_t stream);
 /* Its gradients: dz[r][v] = grad_loss[r] (exp(z[r][v] - lse[r]) - [v = targets[r]]), a piece of the vocabulary at a time and as bf16
  * multiples of grad_loss[0]'s significand; dx (rows, hidden) = dz @ weight_t, dweight_t (vocab, hidden) = dz^T @ x, bf16.  Either may be NULL.
+ * Rounded to bf16 on the way: dz, so multiplied; sums are fp32.
  * lse from the call above.  Every row of x has to be finite, for one without a target is a factor of 0 in dweight_t's sums.  rows = 0
  * gives a zero dweight_t. */
 BN_API size_t bn_linear_cross_entropy_backward_bf16_workspace_bytes(int rows, int vocab, int hidden);
@@ -637,7 +638,8 @@ BN_API int bn_linear_cross_entropy_backward_bf16(const void* x, const void* weig
 
 /* Gradients of y = (act(x @ gate_t^T) * (x @ up_t^T)) @ down_t^T, what bn_gemm_glu_bf16_nt and the product behind it compute
  * (MLP.__call__, mygrad/llama/llama_layers.py:194-235): dy, x, dx (rows, hidden); gate_t, up_t, dgate_t, dup_t (inter, hidden);
- * down_t, ddown_t (hidden, inter).  gate and up are computed again from x.  act BN_ACT_SILU or BN_ACT_GELU_TANH; hidden and inter
+ * down_t, ddown_t (hidden, inter).  gate and up are computed again from x.  Rounded to bf16 on the way: act(gate) * up and the gradients of
+ * gate and up, operands of the last products; gate, up and the gradient of their product stay fp32.  act BN_ACT_SILU or BN_ACT_GELU_TANH; hidden and inter
  * multiples of 8; operands 16-byte, workspace 256-byte aligned.  rows = 0 gives zero weight gradients. */
 BN_API size_t bn_gated_ff_backward_bf16_workspace_bytes(int rows, int hidden, int inter);
 BN_API int bn_gated_ff_backward_bf16(const void* dy, const void* x, const void* gate_t, const void* up_t, const void* down_t, void* dx,
@@ -646,7 +648,8 @@ BN_API int bn_gated_ff_backward_bf16(const void* dy, const void* x, const void* 
 
 /* Gradients of bn_attn_prefill_bf16 by q, k and v as that call takes them (pre-RoPE), given its output, its lse and the output's gradient:
  *   q, out, dout, dq (B, S, Hq, D) bf16;  k, v, dk, dv (B, S, Hkv, D) bf16;  lse (B, Hq, S) fp32, natural log.
- * k and v have the sums over the query heads of their group.  Arguments as there; operands must be finite: a masked score has no
+ * k and v have the sums over the query heads of their group.  Rounded to bf16 on the way: the rotated q and k (in which bn_attn_prefill_bf16
+ * computes too), P and dS, operands of the last products (errors of 4.0e-3, where the last rounding alone makes 1.7e-3).  Arguments as there; operands must be finite: a masked score has no
  * gradient, but its key and query are factors of its tile's products.  Tensors 16-byte, workspace 256-byte aligned. */
 BN_API size_t bn_attn_prefill_bf16_backward_workspace_bytes(int B, int S, int Hq, int Hkv, int D, int causal);
 BN_API int bn_attn_prefill_bf16_backward(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse, void* dq,
