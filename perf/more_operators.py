@@ -18,7 +18,7 @@ own = False
 
 HEADS, KV_HEADS, DIM, THETA, VOCAB = 32, 4, 64, 10000.0, 32000
 PAGE, BLOCK = 16, 2112
-LEAST, MOST = 2.0 ** -100, 2.0 ** 120                  # of a scale
+LEAST, MOST = 2.0 ** -100, 2.0 ** 122                  # of a scale
 
 
 def listed():
