@@ -17,6 +17,7 @@ LIB_PATH = os.environ.get("BN_ATTN_LIB") or os.path.join(_HERE, "libbn_attn.so")
 BN_OK, BN_ERR_INVALID_ARG, BN_ERR_UNSUPPORTED, BN_ERR_CUDA, BN_ERR_ARCH, BN_ERR_TIMEOUT, BN_ERR_WORKSPACE = range(7)
 BN_HEADS_COLLAPSED, BN_HEADS_PER_HEAD = 0, 1
 BN_PAGE_TOKENS = 16
+BN_KV8_BLOCK, BN_KV8_E4M3, BN_KV8_INT8 = 2112, 0, 1
 BN_ACT_NONE, BN_ACT_SILU, BN_ACT_GELU_TANH, BN_ACT_RELU2 = range(4)
 BN_LINEAR_F32_CHAINS, BN_LINEAR_F32_SUMS, BN_LINEAR_F32_PARTS = 0, 1, 2
 
@@ -129,6 +130,11 @@ SIGNATURES = {
     "bn_gated_ff_backward_bf16": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _sz, _p, _p]),
     "bn_attn_prefill_bf16_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "bn_attn_prefill_bf16_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _f, _i, _i, _p, _sz, _p, _p]),
+    "bn_kv8_append": (_i, [_p, _i64, _p, _i, _i, _p, _p, _i, _p, _i64, _p, _i64, _i, _i, _i, _i, _i, _f, _p]),
+    "bn_kv8_gather": (_i, [_p, _i64, _p, _i, _i, _p, _p, _p, _i, _i, _p, _p, _i, _i, _i, _i, _p]),
+    "bn_attn_decode_kv8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
+    "bn_attn_decode_kv8": (_i, [_p, _p, _i64, _p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _f, _i, _i, _i, _p, _sz, _p]),
+    "bn_sample_rows": (_i, [_p, _i64, _i, _p, _p, _f, _p, _i, _p, _f, _p, _f, _p, _i, _i, _p]),
     "bn_gated_group_norm": (_i, [_p, _i64, _i, _p, _i64, _p, _p, _i64, _i, _i, _i, _f, _i, _p]),
 }
 

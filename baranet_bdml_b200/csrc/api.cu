@@ -76,6 +76,8 @@ int bn_workspace_status(const void* workspace, bn_stream_t stream) {
     if (e != cudaSuccess) return bn::fail(BN_ERR_CUDA, "bn_workspace_status: %s", cudaGetErrorString(e));
     if (word == BN_ERR_TIMEOUT)
         return bn::fail(BN_ERR_TIMEOUT, "a bounded device-side wait ran out; the result is invalid");
+    if (word == BN_ERR_INVALID_ARG)
+        return bn::fail(BN_ERR_INVALID_ARG, "a page table named a page outside the pool; the result is invalid");
     return BN_OK;
 }
 

@@ -1,0 +1,192 @@
+// The 8-bit paged cache (kv8.cuh): new tokens are rotated, scaled and rounded as they are written, and read back as bf16 or fp32.
+// The reference keeps no cache (mygrad/llama/llama_model.py:136-144); this one holds twice the tokens of the bf16 cache (kv_cache.cu).
+#include "kv8.cuh"
+
+namespace bn {
+
+constexpr int KV8_LANES = 8;                  // lanes that share one token's 64 numbers of a head: 8 each, 16 bytes of bf16
+constexpr int KV8_PER = KV8_D / KV8_LANES;
+
+template <typename T> __device__ __forceinline__ void load8(const T* p, bool wide, float (&x)[8]) {
+    if (wide) {
+        float a[4], b[4];
+        load4(p, a);
+        load4(p + 4, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { x[i] = a[i]; x[i + 4] = b[i]; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = to_f(p[i]);
+    }
+}
+
+// the largest magnitude of the lanes of a group, as bits (so that a NaN is larger than all numbers)
+__device__ __forceinline__ uint32_t group_most(const float (&x)[8]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = 1; o < KV8_LANES; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return m;
+}
+
+struct Kv8AppendParams {
+    uint8_t* pool;
+    int64_t pool_pages;
+    const int32_t *page_table, *seq_ids, *positions;
+    const void *k, *v;
+    int64_t k_stride, v_stride;
+    int num_seqs, max_pages, T, Hkv, rotate, wide;
+    RotationFreqs freqs;
+};
+
+// a group of lanes per (token, key head)
+template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8AppendParams p) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / KV8_LANES;
+    const int part = threadIdx.x % KV8_LANES;
+    const bool there = unit < (int64_t)p.T * p.Hkv;
+    const int t = there ? (int)(unit / p.Hkv) : 0, g = there ? (int)(unit % p.Hkv) : 0;
+    const int pos = p.positions[t], seq = p.seq_ids[t], slot = pos % BN_PAGE_TOKENS;
+    int page = -1;
+    if (there && pos >= 0 && pos / BN_PAGE_TOKENS < p.max_pages && seq >= 0 && seq < p.num_seqs)
+        page = p.page_table[(int64_t)seq * p.max_pages + pos / BN_PAGE_TOKENS];
+    float k[8], v[8];
+    load8(static_cast<const T*>(p.k) + t * p.k_stride + g * KV8_D + part * KV8_PER, p.wide, k);
+    load8(static_cast<const T*>(p.v) + t * p.v_stride + g * KV8_D + part * KV8_PER, p.wide, v);
+    if (p.rotate) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float c, s;
+            rotation(pos, p.freqs.f[part * 4 + i], &c, &s);
+            const float a = k[2 * i], b = k[2 * i + 1];
+            k[2 * i] = a * c - b * s;
+            k[2 * i + 1] = a * s + b * c;
+        }
+    }
+    const float ks = kv8_scale<VALUES>(group_most(k)), vs = kv8_scale<VALUES>(group_most(v));
+    if (page < 0 || page >= p.pool_pages) return;
+    uint8_t* block = p.pool + ((int64_t)page * p.Hkv + g) * BN_KV8_BLOCK;
+    auto pack = [](const float (&x)[8], float s) {
+        return make_uint2(kv8_pack<VALUES>(x[0], x[1], x[2], x[3], s), kv8_pack<VALUES>(x[4], x[5], x[6], x[7], s));
+    };
+    *reinterpret_cast<uint2*>(block + slot * KV8_D + part * KV8_PER) = pack(k, ks);
+    *reinterpret_cast<uint2*>(block + KV8_V + slot * KV8_D + kv8_v_place(slot, part * KV8_PER)) = pack(v, vs);
+    if (part == 0) *reinterpret_cast<uint32_t*>(block + KV8_SCALES + slot * 4) = __float_as_uint(ks) >> 16 | (__float_as_uint(vs) & 0xffff0000u);
+}
+
+struct Kv8GatherParams {
+    const uint8_t* pool;
+    int64_t pool_pages;
+    const int32_t *page_table, *seq_lens, *seq_ids, *starts;
+    void *k, *v;
+    int64_t units;
+    int num_seqs, max_pages, n_tokens, Hkv;
+};
+
+// a group of lanes per (row of the result, key head)
+template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8GatherParams p) {
+    ptx::grid_dependency_wait();
+    ptx::grid_launch_dependents();
+    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / KV8_LANES;
+    const int part = threadIdx.x % KV8_LANES;
+    if (unit >= p.units) return;
+    const int64_t row = unit / p.Hkv;
+    const int g = (int)(unit % p.Hkv), i = (int)(row / p.n_tokens);
+    const int64_t pos = (int64_t)p.starts[i] + row % p.n_tokens;
+    const int seq = p.seq_ids[i];
+    int page = -1;
+    if (seq >= 0 && seq < p.num_seqs && pos >= 0 && pos < p.seq_lens[seq] && pos / BN_PAGE_TOKENS < p.max_pages)
+        page = p.page_table[(int64_t)seq * p.max_pages + pos / BN_PAGE_TOKENS];
+    const bool there = page >= 0 && page < p.pool_pages;
+    const int slot = there ? (int)(pos % BN_PAGE_TOKENS) : 0;
+    const uint8_t* block = p.pool + ((int64_t)(there ? page : 0) * p.Hkv + g) * BN_KV8_BLOCK;
+    uint2 kb = make_uint2(0u, 0u), vb = kb;
+    uint32_t scales = 0u;
+    if (there) {
+        kb = *reinterpret_cast<const uint2*>(block + slot * KV8_D + part * KV8_PER);
+        vb = *reinterpret_cast<const uint2*>(block + KV8_V + slot * KV8_D + kv8_v_place(slot, part * KV8_PER));
+        scales = *reinterpret_cast<const uint32_t*>(block + KV8_SCALES + slot * 4);
+    }
+    auto put = [&](void* out, uint2 b, float scale) {
+        T* dst = static_cast<T*>(out) + unit * KV8_D + part * KV8_PER;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            uint32_t lo, hi;
+            kv8_halves<VALUES>(w ? b.y : b.x, lo, hi);
+            const float2 x = halves_to_floats(lo), y = halves_to_floats(hi);
+            const float o[4] = {there ? x.x * scale : 0.f, there ? x.y * scale : 0.f, there ? y.x * scale : 0.f, there ? y.y * scale : 0.f};
+            store4(dst + 4 * w, o);
+        }
+    };
+    put(p.k, kb, ptx::bf16_lo(scales));
+    put(p.v, vb, ptx::bf16_hi(scales));
+}
+
+}  // namespace bn
+
+using namespace bn;
+
+static int kv8_shape(const char* what, const void* pool, int64_t pool_pages, const int32_t* page_table, int num_seqs, int max_pages, int Hkv, int D,
+                     int values) {
+    if (!pool || !page_table) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (pool_pages <= 0 || num_seqs <= 0 || max_pages <= 0 || Hkv <= 0)
+        return fail(BN_ERR_INVALID_ARG, "%s: bad sizes pool_pages=%lld num_seqs=%d max_pages=%d Hkv=%d", what, (long long)pool_pages, num_seqs, max_pages,
+                    Hkv);
+    if (D != KV8_D) return fail(BN_ERR_UNSUPPORTED, "%s: head_dim=%d (64 supported)", what, D);
+    if (values != BN_KV8_E4M3 && values != BN_KV8_INT8) return fail(BN_ERR_INVALID_ARG, "%s: values=%d (0 = e4m3, 1 = int8)", what, values);
+    if (reinterpret_cast<uintptr_t>(pool) & 15) return fail(BN_ERR_INVALID_ARG, "%s: the pool must be 16-byte aligned", what);
+    return BN_OK;
+}
+
+extern "C" int bn_kv8_append(void* pool, int64_t pool_pages, const int32_t* page_table, int num_seqs, int max_pages, const int32_t* seq_ids,
+                             const int32_t* positions, int T, const void* k_new, int64_t k_row_stride, const void* v_new, int64_t v_row_stride,
+                             int dtype, int values, int rotate, int Hkv, int D, float theta, bn_stream_t stream) {
+    const char* what = "bn_kv8_append";
+    if (int rc = kv8_shape(what, pool, pool_pages, page_table, num_seqs, max_pages, Hkv, D, values)) return rc;
+    if (!seq_ids || !positions || !k_new || !v_new) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    if (T < 0 || (int64_t)T * Hkv > 0x7fffffffLL * 16) return fail(BN_ERR_INVALID_ARG, "%s: T=%d tokens of %d heads", what, T, Hkv);
+    if (dtype != 0 && dtype != 1) return fail(BN_ERR_INVALID_ARG, "%s: dtype=%d (0 = fp32, 1 = bf16)", what, dtype);
+    if (rotate && !(theta > 0.f)) return fail(BN_ERR_INVALID_ARG, "%s: theta=%g", what, theta);
+    if (int rc = require_sm100()) return rc;
+    if (T == 0) return BN_OK;
+    Kv8AppendParams p;
+    p.pool = static_cast<uint8_t*>(pool);
+    p.pool_pages = pool_pages;
+    p.page_table = page_table; p.seq_ids = seq_ids; p.positions = positions;
+    p.k = k_new; p.v = v_new; p.k_stride = k_row_stride; p.v_stride = v_row_stride;
+    p.num_seqs = num_seqs; p.max_pages = max_pages; p.T = T; p.Hkv = Hkv; p.rotate = rotate;
+    p.wide = ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 15) == 0 && ((k_row_stride | v_row_stride) % 8) == 0;
+    if (rotate) p.freqs = rotation_freqs(theta);
+    auto* kernel = dtype == 0 ? (values == BN_KV8_E4M3 ? kv8_append_kernel<float, BN_KV8_E4M3> : kv8_append_kernel<float, BN_KV8_INT8>)
+                              : (values == BN_KV8_E4M3 ? kv8_append_kernel<__nv_bfloat16, BN_KV8_E4M3> : kv8_append_kernel<__nv_bfloat16, BN_KV8_INT8>);
+    const unsigned blocks = (unsigned)(((int64_t)T * Hkv * KV8_LANES + 255) / 256);
+    launch_dependent(kernel, blocks, 256, 0, as_stream(stream), p);
+    return launch_status(what);
+}
+
+extern "C" int bn_kv8_gather(const void* pool, int64_t pool_pages, const int32_t* page_table, int num_seqs, int max_pages, const int32_t* seq_lens,
+                             const int32_t* seq_ids, const int32_t* starts, int n_seqs, int n_tokens, void* k_out, void* v_out, int out_dtype,
+                             int values, int Hkv, int D, bn_stream_t stream) {
+    const char* what = "bn_kv8_gather";
+    if (int rc = kv8_shape(what, pool, pool_pages, page_table, num_seqs, max_pages, Hkv, D, values)) return rc;
+    if (!seq_lens || !seq_ids || !starts || !k_out || !v_out) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
+    const int64_t units = (int64_t)n_seqs * n_tokens * Hkv;
+    if (n_seqs < 0 || n_tokens < 0 || units > 0x7fffffffLL * 16) return fail(BN_ERR_INVALID_ARG, "%s: bad sizes n_seqs=%d n_tokens=%d", what, n_seqs, n_tokens);
+    if (out_dtype != 0 && out_dtype != 1) return fail(BN_ERR_INVALID_ARG, "%s: out_dtype=%d (0 = fp32, 1 = bf16)", what, out_dtype);
+    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)
+        return fail(BN_ERR_INVALID_ARG, "%s: the outputs must be 16-byte aligned", what);
+    if (int rc = require_sm100()) return rc;
+    if (units == 0) return BN_OK;
+    Kv8GatherParams p;
+    p.pool = static_cast<const uint8_t*>(pool);
+    p.pool_pages = pool_pages;
+    p.page_table = page_table; p.seq_lens = seq_lens; p.seq_ids = seq_ids; p.starts = starts;
+    p.k = k_out; p.v = v_out; p.units = units;
+    p.num_seqs = num_seqs; p.max_pages = max_pages; p.n_tokens = n_tokens; p.Hkv = Hkv;
+    auto* kernel = out_dtype == 0 ? (values == BN_KV8_E4M3 ? kv8_gather_kernel<float, BN_KV8_E4M3> : kv8_gather_kernel<float, BN_KV8_INT8>)
+                                  : (values == BN_KV8_E4M3 ? kv8_gather_kernel<__nv_bfloat16, BN_KV8_E4M3> : kv8_gather_kernel<__nv_bfloat16, BN_KV8_INT8>);
+    launch_dependent(kernel, (unsigned)((units * KV8_LANES + 255) / 256), 256, 0, as_stream(stream), p);
+    return launch_status(what);
+}

@@ -1,0 +1,88 @@
+// The 8-bit paged cache: what a block holds, and how numbers become 8 bits and back.
+//
+// A block is one (page, key head), BN_KV8_BLOCK bytes in a row:
+//     [   0, 1024)  K  [16 tokens][64]
+//     [1024, 2048)  V  [16 tokens][64], the 16-byte piece c of token t in place c ^ (t / 2 % 4)
+//     [2048, 2112)  [16 tokens] (K scale, V scale), bf16
+// so that a block is one bulk copy into shared memory, keys are read from there 16 bytes a lane without bank conflicts, and eight
+// tokens' pieces of V lie in eight different groups of banks for ldmatrix.
+//
+// A scale belongs to one token and key head.  One for a page would have to grow with a later token of the page, whose older tokens
+// would then be rounded a second time, and what a token is read back as would depend on tokens that came after it or were taken
+// back; the finer scales cost 64 bytes of 2112.
+//   e4m3: the smallest power of two that leaves no magnitude above 448 (a float format gains nothing from other factors, and division
+//         by it is exact)
+//   int8: the largest magnitude / 127, rounded up to bf16
+// both kept within 2^-100 .. 2^122.  A token with an infinity or a NaN has the scale NaN.
+#pragma once
+
+#include "common.cuh"
+#include "hybrid.cuh"
+#include "ptx.cuh"
+
+namespace bn {
+
+constexpr int KV8_D = 64;
+constexpr int KV8_V = 1024, KV8_SCALES = 2048;
+constexpr uint32_t KV8_LEAST = (127 - 100) << 23, KV8_MOST = (127 + 122) << 23;
+static_assert(KV8_SCALES + BN_PAGE_TOKENS * 4 == BN_KV8_BLOCK, "block of the 8-bit cache");
+
+// where byte d of a token's values lies in its row of V
+__host__ __device__ __forceinline__ constexpr int kv8_v_place(int token, int d) { return (((d >> 4) ^ ((token >> 1) & 3)) << 4) | (d & 15); }
+
+// the frequencies of the 32 rotation pairs
+struct RotationFreqs {
+    double f[KV8_D / 2];
+};
+inline RotationFreqs rotation_freqs(float theta) {
+    RotationFreqs r;
+    for (int i = 0; i < KV8_D / 2; ++i) r.f[i] = pow((double)theta, -2.0 * i / KV8_D);
+    return r;
+}
+
+template <int VALUES> __device__ __forceinline__ float kv8_scale(uint32_t most_bits) {
+    if (most_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
+    uint32_t b;
+    if (VALUES == BN_KV8_E4M3) {
+        // most = 1.m * 2^e: 2^(e - 8) leaves 1.m * 2^8, too much above 1.75
+        const int e = (int)(most_bits >> 23) - 8 + ((most_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+        b = e > 0 ? (uint32_t)e << 23 : 0u;
+    } else {
+        b = (__float_as_uint(__fdiv_ru(__uint_as_float(most_bits), 127.f)) + 0xffffu) & 0xffff0000u;
+    }
+    return __uint_as_float(min(max(b, KV8_LEAST), KV8_MOST));
+}
+
+// four numbers / scale, rounded to nearest (ties to even), as four bytes
+template <int VALUES> __device__ __forceinline__ uint32_t kv8_pack(float a, float b, float c, float d, float scale) {
+    if (scale != scale) return 0u;
+    if (VALUES == BN_KV8_E4M3) {
+        const float inv = __uint_as_float((254u << 23) - __float_as_uint(scale));      // exact: a power of two
+        uint16_t lo, hi;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b * inv), "f"(a * inv));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d * inv), "f"(c * inv));
+        return (uint32_t)lo | (uint32_t)hi << 16;
+    }
+    auto one = [&](float v) { return (uint32_t)(max(-127, min(127, __float2int_rn(__fdiv_rn(v, scale)))) & 0xff); };
+    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+}
+
+// bytes (0, 1) and (2, 3) of a word as two fp16 each
+template <int VALUES> __device__ __forceinline__ void kv8_halves(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if (VALUES == BN_KV8_E4M3) {
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+    } else {
+        // 0x6400 | u is 1024 + u in fp16; u = value + 128
+        const uint32_t u = w ^ 0x80808080u;
+        uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(0x64806480u));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(0x64806480u));
+    }
+}
+__device__ __forceinline__ float2 halves_to_floats(uint32_t h) {
+    float2 f;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(f.x), "=f"(f.y) : "r"(h));
+    return f;
+}
+
+}  // namespace bn

@@ -20,6 +20,7 @@ from . import _lib
 from .ops import Workspace, _need, _stream
 
 PAGE_TOKENS = _lib.BN_PAGE_TOKENS
+KV8_VALUES = {"e4m3": _lib.BN_KV8_E4M3, "int8": _lib.BN_KV8_INT8}
 
 
 class ZeroedTogether:
@@ -83,12 +84,14 @@ class PagedKVCache:
         key = (B, Hq, max_seq_len, chunk_tokens)
         ws = self._ws.get(key)
         if ws is None:
-            n = _lib.load().bn_attn_decode_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len,
-                                                          chunk_tokens)
+            n = self._workspace_bytes(B, Hq, max_seq_len, chunk_tokens)
             if n == 0:
                 raise RuntimeError("bn_attn_decode_paged: unsupported shape")
             ws = self._ws[key] = Workspace(n, self.pool.device)
         return ws
+
+    def _workspace_bytes(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int) -> int:
+        return _lib.load().bn_attn_decode_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len, chunk_tokens)
 
     def status(self) -> None:
         """Raises if a decode launch on any of this cache's scratch buffers gave up on a bounded wait."""
@@ -118,6 +121,123 @@ class PagedKVCache:
             out.data_ptr() if out is not None else None, out_f32.data_ptr() if out_f32 is not None else None,
             lse.data_ptr() if lse is not None else None, B, Hq, self.num_kv_heads, D, float(scale), self.theta,
             int(bool(rope_q)), int(max_seq_len), int(chunk_tokens), ws.ptr, ws.nbytes, _stream()))
+        return out if out is not None else out_f32
+
+
+class QuantizedKVCache(PagedKVCache):
+    """The paged cache in 8 bits, `values` "e4m3" or "int8", a scale for each token and key head: about half the bytes of the bf16
+    cache, for each of which attention takes as long.  e4m3 numbers are off by up to 2^-4 of themselves, int8 numbers by up to
+    1 / 254 of the largest of their token and head.  Pool: [page][kv_head][2112 bytes], laid out as bn_kv8_append has it.
+
+    All tensors of a call lie on the cache's device, which is the current one."""
+
+    def __init__(self, num_pages: int, num_seqs: int, max_pages_per_seq: int, num_kv_heads: int = 4, head_dim: int = 64,
+                 theta: float = 10000.0, device="cuda", storage=None, values: str = "e4m3"):
+        if values not in KV8_VALUES:
+            raise RuntimeError(f"QuantizedKVCache: values {values!r} (e4m3 or int8)")
+        if head_dim != 64:
+            raise RuntimeError(f"QuantizedKVCache: head_dim={head_dim} (64 supported)")
+        pool, table, lens = (num_pages, num_kv_heads, _lib.BN_KV8_BLOCK), (num_seqs, max_pages_per_seq), (num_seqs,)
+        if storage is None:
+            storage = (torch.zeros(pool, dtype=torch.uint8, device=device), torch.zeros(table, dtype=torch.int32, device=device),
+                       torch.zeros(lens, dtype=torch.int32, device=device))
+        for t, shape, dtype in zip(storage, (pool, table, lens), (torch.uint8, torch.int32, torch.int32)):
+            if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+                raise RuntimeError(f"QuantizedKVCache: storage must be a contiguous {dtype} tensor of {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+        super().__init__(num_pages, num_seqs, max_pages_per_seq, num_kv_heads, head_dim, theta, device, storage)
+        self.values = values
+
+    def _here(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
+        dev = self.pool.device
+        if dev.type != "cuda":
+            raise RuntimeError(f"{what}: only GPU implementation available")
+        if dev.index != torch.cuda.current_device() or any(t is not None and t.device != dev for t in tensors):
+            raise RuntimeError(f"{what}: all tensors must lie on the cache's device, and it must be the current one")
+
+    def _ids(self, what: str, n: int, *tensors: torch.Tensor) -> None:
+        for t in tensors:
+            _need(t, torch.int32, what)
+            if t.numel() != n:
+                raise RuntimeError(f"{what}: {t.numel()} ids, positions or lengths where there are {n} rows")
+
+    def append(self, seq_ids: torch.Tensor, positions: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, *, rotated: bool = False) -> None:
+        """Writes tokens (sequence seq_ids[t], position positions[t]), k_new and v_new (T, Hkv*D) fp32 or bf16, K rotated at its
+        position unless `rotated` says that it is.  A (sequence, position) may occur once; tokens outside the cache are left
+        out.  Does not touch seq_lens (the caller advances them)."""
+        what = "kv append"
+        if k_new.dtype not in (torch.float32, torch.bfloat16) or v_new.dtype != k_new.dtype:
+            raise RuntimeError(f"{what}: k/v must both be fp32 or both bf16")
+        self._here(what, seq_ids, positions, k_new, v_new)
+        T, width = k_new.shape[0], self.num_kv_heads * self.head_dim
+        for t in (k_new, v_new):
+            if t.dim() != 2 or t.shape != (T, width) or t.stride(1) != 1:
+                raise RuntimeError(f"{what}: k/v must be rows of {width} contiguous elements, as many of each")
+        self._ids(what, T, seq_ids, positions)
+        if T == 0:
+            return
+        _lib.check(_lib.load().bn_kv8_append(
+            self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, seq_ids.data_ptr(), positions.data_ptr(), T,
+            k_new.data_ptr(), k_new.stride(0), v_new.data_ptr(), v_new.stride(0), 0 if k_new.dtype == torch.float32 else 1, KV8_VALUES[self.values],
+            int(not rotated), self.num_kv_heads, self.head_dim, self.theta, _stream()))
+
+    def gather(self, seq_ids: torch.Tensor, starts: torch.Tensor, n_tokens: int, *, dtype=torch.bfloat16):
+        """What the cache holds of sequence seq_ids[i] from position starts[i] on: K (rotated, as it is stored) and V, each
+        (len(seq_ids), n_tokens, Hkv, D) bf16 or fp32; zeros from seq_lens on."""
+        what = "kv gather"
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise RuntimeError(f"{what}: {dtype} (float32 or bfloat16)")
+        if n_tokens < 0:
+            raise RuntimeError(f"{what}: {n_tokens} tokens")
+        self._here(what, seq_ids, starts)
+        n = seq_ids.numel()
+        self._ids(what, n, seq_ids, starts)
+        k, v = (torch.empty((n, n_tokens, self.num_kv_heads, self.head_dim), dtype=dtype, device=self.pool.device) for _ in range(2))
+        if k.numel():
+            _lib.check(_lib.load().bn_kv8_gather(
+                self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, self.seq_lens.data_ptr(),
+                seq_ids.data_ptr(), starts.data_ptr(), n, n_tokens, k.data_ptr(), v.data_ptr(), 0 if dtype == torch.float32 else 1,
+                KV8_VALUES[self.values], self.num_kv_heads, self.head_dim, _stream()))
+        return k, v
+
+    def _workspace_bytes(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int) -> int:
+        return _lib.load().bn_attn_decode_kv8_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len, chunk_tokens)
+
+    def decode(self, q: torch.Tensor, *, num_heads: int, scale: Optional[float] = None, rope_q: bool = True,
+               q_positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               out_f32: Optional[torch.Tensor] = None, lse: Optional[torch.Tensor] = None,
+               max_seq_len: Optional[int] = None, chunk_tokens: int = 0, seq_lens: Optional[torch.Tensor] = None,
+               page_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """q (B, Hq, D) bf16 (pre-RoPE when rope_q) -> out (B, Hq, D) bf16, as PagedKVCache.decode."""
+        what = "decode"
+        _need(q, torch.bfloat16, f"{what}(q)")
+        seq_lens = self.seq_lens if seq_lens is None else seq_lens
+        page_table = self.page_table if page_table is None else page_table
+        self._here(what, q, seq_lens, page_table, q_positions, out, out_f32, lse)
+        if q.dim() != 3 or q.shape[1] != num_heads or q.shape[2] != self.head_dim:
+            raise RuntimeError(f"{what}: q must be (B, {num_heads}, {self.head_dim}), got {tuple(q.shape)}")
+        B, Hq, D = q.shape
+        self._ids(what, B, seq_lens, *([] if q_positions is None else [q_positions]))
+        _need(page_table, torch.int32, f"{what}(page_table)")
+        if page_table.dim() != 2 or page_table.shape[0] < B:
+            raise RuntimeError(f"{what}: a page table of {tuple(page_table.shape)} for {B} sequences")
+        for t, dtype, shape in ((out, torch.bfloat16, q.shape), (out_f32, torch.float32, q.shape), (lse, torch.float32, q.shape[:2])):
+            if t is not None:
+                _need(t, dtype, f"{what}(out)")
+                if t.numel() != shape.numel():
+                    raise RuntimeError(f"{what}: an output of {tuple(t.shape)} where {tuple(shape)} is written")
+        if out is None and out_f32 is None:
+            out = torch.empty_like(q)
+        if max_seq_len is None:
+            max_seq_len = page_table.shape[1] * PAGE_TOKENS
+        if scale is None:
+            scale = 1.0 / (D ** 0.5)
+        if B:
+            ws = self.workspace(B, Hq, max_seq_len, chunk_tokens)
+            _lib.check(_lib.load().bn_attn_decode_kv8(
+                q.data_ptr(), self.pool.data_ptr(), self.num_pages, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),
+                q_positions.data_ptr() if q_positions is not None else None, out.data_ptr() if out is not None else None,
+                out_f32.data_ptr() if out_f32 is not None else None, lse.data_ptr() if lse is not None else None, KV8_VALUES[self.values], B, Hq,
+                self.num_kv_heads, D, float(scale), self.theta, int(bool(rope_q)), int(max_seq_len), int(chunk_tokens), ws.ptr, ws.nbytes, _stream()))
         return out if out is not None else out_f32
 
 

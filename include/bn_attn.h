@@ -52,6 +52,11 @@ extern "C" {
 /* tokens per KV-cache page */
 #define BN_PAGE_TOKENS 16
 
+/* the 8-bit cache: bytes of a block (one page of one key head), and what its numbers are */
+#define BN_KV8_BLOCK 2112
+#define BN_KV8_E4M3 0
+#define BN_KV8_INT8 1
+
 /* activations of the fused products */
 #define BN_ACT_NONE 0
 #define BN_ACT_SILU 1
@@ -388,6 +393,55 @@ BN_API int bn_attn_decode_paged_static(const void* q, const void* pool, int64_t 
  * or BN_ERR_TIMEOUT when a call gave up on a bounded wait; in that case the header and the counters are cleared
  * here, so the next call starts clean.  Allocates nothing; it synchronises, so keep it off the hot path. */
 BN_API int bn_attn_decode_paged_static_status(bn_stream_t stream);
+
+/* Paged KV cache in 8 bits: about half the bytes of the bf16 cache.  One pool per layer, 16-byte aligned:
+ *   pool[page][kv_head][BN_KV8_BLOCK bytes] =
+ *     K [16 tokens][64] | V [16 tokens][64] | [16 tokens](K scale, V scale) bf16
+ * The 16-byte piece c of token t's V lies in place c ^ (t / 2 % 4).  A number is its byte (`values`: BN_KV8_E4M3 or
+ * BN_KV8_INT8) times the scale of its token and key head:
+ *   e4m3  the smallest power of two that leaves no magnitude above 448
+ *   int8  largest magnitude / 127, rounded up to bf16
+ * between 2^-100 and 2^122 (int8 magnitudes beyond 127 * 2^122 saturate).  A token with an infinity or a NaN gets the scale
+ * NaN: attention that reads it gives NaN, as it does from the bf16 cache.  D must be 64.  page_table (num_seqs, max_pages).
+ *
+ * bn_kv8_append: for t in [0, T) the token of sequence seq_ids[t] at position positions[t]; k_new, v_new rows of Hkv * D, row strides
+ * in elements, dtype 0 = fp32, 1 = bf16.  rotate != 0: K is rotated at its position first (angles in fp64); 0: it is rotated
+ * already.  Each number is rounded once, to nearest.  A token whose sequence, position or page lies outside is left out; a
+ * (sequence, position) may occur once in a call.
+ *
+ * bn_kv8_gather: row j of sequence seq_ids[i] in k_out, v_out (n_seqs, n_tokens, Hkv, D; out_dtype 0 = fp32, 1 = bf16) is the cached
+ * token at starts[i] + j, K rotated as it is stored; zeros for positions outside [0, seq_lens[seq_ids[i]]). */
+BN_API int bn_kv8_append(void* pool, int64_t pool_pages, const int32_t* page_table, int num_seqs, int max_pages,
+                         const int32_t* seq_ids, const int32_t* positions, int T, const void* k_new, int64_t k_row_stride,
+                         const void* v_new, int64_t v_row_stride, int dtype, int values, int rotate, int Hkv, int D,
+                         float theta, bn_stream_t stream);
+BN_API int bn_kv8_gather(const void* pool, int64_t pool_pages, const int32_t* page_table, int num_seqs, int max_pages,
+                         const int32_t* seq_lens, const int32_t* seq_ids, const int32_t* starts, int n_seqs, int n_tokens,
+                         void* k_out, void* v_out, int out_dtype, int values, int Hkv, int D, bn_stream_t stream);
+
+/* bn_attn_decode_paged over the 8-bit cache: the same arguments and `values`.  q is rotated with angles in fp64.  A page number
+ * outside the pool raises BN_ERR_INVALID_ARG in the scratch buffer's error word (bn_workspace_status); what is returned then
+ * is of no use.  The scratch buffer is zero-filled once before its first use, and belongs to one call at a time. */
+BN_API size_t bn_attn_decode_kv8_workspace_bytes(int B, int Hq, int Hkv, int D, int max_seq_len, int chunk_tokens);
+BN_API int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_pages, const int32_t* page_table, int max_pages,
+                              const int32_t* seq_lens, const int32_t* q_positions, void* out, float* out_f32, float* lse,
+                              int values, int B, int Hq, int Hkv, int D, float scale, float theta, int rope_q,
+                              int max_seq_len, int chunk_tokens, void* workspace, size_t workspace_bytes,
+                              bn_stream_t stream);
+
+/* Token ids from logits (rows, cols) fp32 (dtype 0) or bf16 (1), row stride in elements, and one random number in [0, 1) a row
+ * (values outside are taken as the nearest end): the temperature / top-k sampling of generate()
+ * (mygrad/llama/llama_model.py:144-160) on the device, with top-p and min-p.  With w_i = exp((x_i - max x) / temperature), in the
+ * order of the value, the lower index first among equals:
+ *   the first top_k (0: all); of these, those before which less than top_p of their sum lies (1: all); of these, w >= min_p.
+ *   The first always stays.
+ *   out[r] = the lowest index for which the sum of what is kept, up to and with it, exceeds uniform[r] times all that is kept.
+ * Weights are fp64 and summed as whole numbers, so that a result does not depend on how the work is divided.  temperature 0: the
+ * first maximum.  NaN counts as -inf; a row with nothing above -inf gives 0; +inf entries share the weight.
+ * temperature, top_k, top_p, min_p: one value a row (device), or NULL for the value beside it.  cols <= 2^20. */
+BN_API int bn_sample_rows(const void* logits, int64_t row_stride, int dtype, const float* uniform, const float* temperature,
+                          float temperature_all, const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
+                          const float* min_p, float min_p_all, int32_t* out, int rows, int cols, bn_stream_t stream);
 
 /* Log-sum-exp merge of P partial attention results (split-KV across GPUs):
  *   outs (P, n, D) fp32 normalised partial outputs, lses (P, n) natural log
