@@ -34,9 +34,14 @@ __host__ __device__ __forceinline__ constexpr int kv8_v_place(int token, int d) 
 struct RotationFreqs {
     double f[KV8_D / 2];
 };
-inline RotationFreqs rotation_freqs(float theta) {
-    RotationFreqs r;
-    for (int i = 0; i < KV8_D / 2; ++i) r.f[i] = pow((double)theta, -2.0 * i / KV8_D);
+// (a thread's last ones are at hand: 32 powers cost the host 2 us)
+inline const RotationFreqs& rotation_freqs(float theta) {
+    static thread_local float known = 0.f;
+    static thread_local RotationFreqs r;
+    if (theta != known) {
+        for (int i = 0; i < KV8_D / 2; ++i) r.f[i] = pow((double)theta, -2.0 * i / KV8_D);
+        known = theta;
+    }
     return r;
 }
 
@@ -77,6 +82,17 @@ template <int VALUES> __device__ __forceinline__ void kv8_halves(uint32_t w, uin
         uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
         asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(0x64806480u));
         asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(y), "r"(0x64806480u));
+    }
+}
+// the same of bytes (0, 2) and (1, 3): a word of ldmatrix.trans holds two elements of a token, then those of the next token
+template <int VALUES> __device__ __forceinline__ void kv8_token_pairs(uint32_t w, uint32_t& first, uint32_t& second) {
+    if (VALUES == BN_KV8_E4M3) {
+        kv8_halves<VALUES>(__byte_perm(w, 0u, 0x3120), first, second);
+    } else {
+        const uint32_t u = w ^ 0x80808080u;
+        uint32_t x = __byte_perm(u, 0x64646464u, 0x4240), y = __byte_perm(u, 0x64646464u, 0x4341);
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(first) : "r"(x), "r"(0x64806480u));
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(second) : "r"(y), "r"(0x64806480u));
     }
 }
 __device__ __forceinline__ float2 halves_to_floats(uint32_t h) {
