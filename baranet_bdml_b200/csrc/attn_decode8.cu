@@ -28,13 +28,14 @@ constexpr int DEC8_NSTAGES = 6;
 constexpr int DEC8_CWARPS = 8;                                       // consumer warps
 constexpr int DEC8_PPW = DEC8_PAGES / DEC8_CWARPS;                   // pages per warp and stage
 constexpr int DEC8_CTHREADS = DEC8_CWARPS * 32;
-constexpr int DEC8_TPH = DEC8_CTHREADS / DEC_G;                      // threads per head where heads are laid over the consumers: a warp
-constexpr int DEC8_THREADS = (DEC8_CWARPS + 2) * 32;                 // + producer warp + combine warp
+constexpr int DEC8_PWARPS = 4;                                       // producer warps
+constexpr int DEC8_PPP = DEC8_PAGES / DEC8_PWARPS;                   // pages per producer warp and stage
+constexpr int DEC8_THREADS = (DEC8_CWARPS + DEC8_PWARPS + 1) * 32;   // + combine warp
 constexpr int DEC8_SMEM_BYTES = DEC8_NSTAGES * DEC8_STAGE_BYTES + 128;
 constexpr int DEC8_DEFAULT_MIN_TOKENS = 1024;                        // a CTA's range is never shorter than this
 constexpr int DEC8_WHOLE_MAX_STAGES = 8;                             // sequences up to this many stages are never split (if there are enough)
 constexpr float DEC8_HEADROOM = 8.f;                                 // p' <= 2^8
-static_assert(DEC8_TPH == 32, "a warp per query head");
+static_assert(DEC8_CTHREADS == DEC_G * DEC_D / 2, "a thread per head and two dimensions where warps are merged");
 
 struct Decode8Params {
     const __nv_bfloat16* q;
@@ -61,7 +62,8 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     __shared__ int s_nmax;                      // stages of the longest sequence
     __shared__ float mrg_m[DEC8_CWARPS][DEC_G], mrg_l[DEC8_CWARPS][DEC_G];
     __shared__ __align__(16) float mrg_o[DEC8_CWARPS][DEC_G][DEC_D + 2];   // written and read as float2
-    __shared__ __align__(16) uint32_t s_q[DEC_G][DEC_D / 2];    // rotated query heads of the current segment, pairs of fp16
+    __shared__ __align__(16) uint32_t s_q[DEC_G][3 * DEC_D / 4]; // rotated query heads of the current segment: three e4m3 parts, or fp16
+    constexpr uint32_t QUERY_TOP = VALUES == BN_KV8_E4M3 ? 7 : 14;
     __shared__ float s_factor[DEC_G];                           // scale * log2(e) * what q was divided by
     __shared__ int s_abort;
 
@@ -70,7 +72,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 
     if (tid == 0) {
         for (int s = 0; s < DEC8_NSTAGES; ++s) {
-            mbar_init(smem_u32(&full_bar[s]), 1);
+            mbar_init(smem_u32(&full_bar[s]), DEC8_PWARPS);
             mbar_init(smem_u32(&empty_bar[s]), DEC8_CWARPS);
         }
         mbar_init(smem_u32(&merge_bar), DEC8_CWARPS);
@@ -94,10 +96,11 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     const int range_lo = active ? sc.range_begin(blockIdx.x) : 0;
     const int range_hi = active ? sc.range_begin(blockIdx.x + 1) : 0;
 
-    if (warp == DEC8_CWARPS) {
+    if (warp >= DEC8_CWARPS && warp < DEC8_CWARPS + DEC8_PWARPS) {
         // ------------------------------------------------------------ producer
         // page numbers are read two stages (a 128-byte line of the table) at a time, one such group ahead of their use
         constexpr int GRP = 32 / DEC8_PAGES;
+        const int mine = (warp - DEC8_CWARPS) * DEC8_PPP + lane % DEC8_PPP;      // the lane's page of a stage
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true, bad = false;
@@ -122,15 +125,15 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                     if ((grp + 1) * GRP < sg.s1) ids_pref = load_group(sg, grp + 1);
                     else if (have_next) ids_pref = load_group(sg_next, sg_next.s0 / GRP);
                 }
-                int page = __shfl_sync(0xffffffffu, ids, (s % GRP) * DEC8_PAGES + (lane % DEC8_PAGES));
+                int page = __shfl_sync(0xffffffffu, ids, (s % GRP) * DEC8_PAGES + mine);
                 if (page < 0 || page >= p.pool_pages) { page = 0; bad = true; }
                 if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, &s_abort)) { ok = false; break; }
-                const int npages = min(DEC8_PAGES, n_pages_seq - s * DEC8_PAGES);
+                const int npages = max(0, min(DEC8_PPP, n_pages_seq - s * DEC8_PAGES - (warp - DEC8_CWARPS) * DEC8_PPP));
                 const uint32_t fb = smem_u32(&full_bar[stage]);
                 if (lane == 0) mbar_arrive_expect_tx(fb, (uint32_t)npages * BN_KV8_BLOCK);
                 __syncwarp();
                 if (lane < npages)
-                    bulk_load_hint(ring + stage * DEC8_STAGE_BYTES + lane * BN_KV8_BLOCK,
+                    bulk_load_hint(ring + stage * DEC8_STAGE_BYTES + mine * BN_KV8_BLOCK,
                                    p.pool + ((int64_t)page * p.Hkv + sg.g) * BN_KV8_BLOCK, BN_KV8_BLOCK, fb, stream_policy);
                 if (++stage == DEC8_NSTAGES) { stage = 0; phase ^= 1u; }
             }
@@ -143,7 +146,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         return;
     }
 
-    if (warp == DEC8_CWARPS + 1) {
+    if (warp == DEC8_CWARPS + DEC8_PWARPS) {
         // -------------------------------------------------------- combine warp
         SegmentIter iter;
         iter.init(range_lo, range_hi);
@@ -160,15 +163,15 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     }
 
     // --------------------------------------------------------------- consumers
-    // where a head's 64 results (or query elements) are laid over a warp: head `warp`, dims 2 * lane, + 1
-    const int hd = 2 * lane;
+    // where the heads' 64 results are laid over the consumers: a warp has a head, a lane two dimensions
+    const int td = 2 * lane;
     // sequences without tokens get a zero output from whoever passes by
     for (int bgi = blockIdx.x; bgi < p.B * p.Hkv; bgi += gridDim.x) {
         const int b = bgi / p.Hkv, g = bgi % p.Hkv;
         if (sc.nst(b) > 0 || warp >= p.n_rep) continue;
         const size_t row = (size_t)b * p.Hq + (size_t)g * p.n_rep + warp;
-        if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + hd) = 0u;
-        if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + hd) = make_float2(0.f, 0.f);
+        if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + td) = 0u;
+        if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + td) = make_float2(0.f, 0.f);
         if (p.lse && lane == 0) p.lse[row] = -INFINITY;
     }
 
@@ -185,7 +188,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     };
     auto load_q_raw = [&](const Segment& sg) -> uint32_t {
         if (warp >= p.n_rep) return 0u;
-        return *reinterpret_cast<const uint32_t*>(p.q + ((size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep + warp) * DEC_D + hd);
+        return *reinterpret_cast<const uint32_t*>(p.q + ((size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep + warp) * DEC_D + 2 * lane);
     };
     auto store_q = [&](const Segment& sgq, uint32_t raw) {
         float x0 = bf16_lo(raw), x1 = bf16_hi(raw);
@@ -196,12 +199,27 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
             const float y1 = x0 * s + x1 * c;
             x0 = y0; x1 = y1;
         }
-        // the head's largest magnitude to [2^14, 2^15)
         const uint32_t most = __reduce_max_sync(0xffffffffu, max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu));
-        const uint32_t e = max(most >> 23, 20u);
-        const float up = __uint_as_float((268u - e) << 23);
-        s_q[warp][lane] = pack_f16(x0 * up, x1 * up);
-        if (lane == 0) s_factor[warp] = p.scale_log2 * __uint_as_float((e - 14u) << 23);
+        const uint32_t e = max(most >> 23, 30u);
+        const float up = __uint_as_float((254u + QUERY_TOP - e) << 23);        // the head's largest magnitude to 2^QUERY_TOP and above
+        x0 *= up;
+        x1 *= up;
+        if (VALUES == BN_KV8_E4M3) {
+#pragma unroll
+            for (int part = 0; part < 3; ++part) {
+                uint16_t two;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(x1), "f"(x0));
+                reinterpret_cast<uint16_t*>(&s_q[warp][part * (DEC_D / 4)])[lane] = two;
+                uint32_t back;
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(two));
+                const float2 f = halves_to_floats(back);
+                x0 -= f.x;
+                x1 -= f.y;
+            }
+        } else {
+            reinterpret_cast<uint32_t*>(s_q[warp])[lane] = pack_f16(x0, x1);
+        }
+        if (lane == 0) s_factor[warp] = p.scale_log2 * (e == 255u ? NAN : __uint_as_float((e - QUERY_TOP) << 23));     // (an infinity would saturate)
     };
 
     SegmentIter iter;
@@ -217,15 +235,20 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         // look one segment ahead so that its query is already on the way
         const bool have_next = iter.next(sc, sg_next);
         const uint32_t q_raw_next = have_next ? load_q_raw(sg_next) : 0u;
-        // Q^T fragments: dims 16 c + 4 kk .. + 3 of head lane / 4, c = lane % 4
-        uint32_t qb[8];
-        {
-            const uint4 a = *reinterpret_cast<const uint4*>(&s_q[lane / 4][8 * (lane % 4)]), b = *reinterpret_cast<const uint4*>(&s_q[lane / 4][8 * (lane % 4) + 4]);
-            qb[0] = a.x; qb[1] = a.y; qb[2] = a.z; qb[3] = a.w; qb[4] = b.x; qb[5] = b.y; qb[6] = b.z; qb[7] = b.w;
+        // Q^T fragments: dims 16 c .. 16 c + 15 of head lane / 4, c = lane % 4
+        uint32_t qb[VALUES == BN_KV8_E4M3 ? 12 : 8];
+#pragma unroll
+        for (int i = 0; i < (VALUES == BN_KV8_E4M3 ? 3 : 2); ++i) {
+            // (a part's 16 elements are one 16-byte piece of e4m3, or half of the two pieces of fp16)
+            const uint4 a = VALUES == BN_KV8_E4M3 ? *reinterpret_cast<const uint4*>(&s_q[lane / 4][i * (DEC_D / 4) + 4 * (lane % 4)])
+                                                  : *reinterpret_cast<const uint4*>(&s_q[lane / 4][8 * (lane % 4) + 4 * i]);
+            qb[4 * i] = a.x; qb[4 * i + 1] = a.y; qb[4 * i + 2] = a.z; qb[4 * i + 3] = a.w;
         }
         const float fA = s_factor[hA], fB = s_factor[hA + 1];
 
-        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+        // weights are 2^(s - m_run) (times vs for the product): no larger than 2^8 where m_run is renewed, and it is renewed before
+        // they pass 2^14
+        float m_run[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f};
         float o[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -234,93 +257,113 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 
         for (int s = sg.s0; s < sg.s1; ++s) {
             if (!mbar_wait_warp(smem_u32(&full_bar[stage]), phase, &s_abort)) { ok = false; break; }
-            const int ntok = min(DEC8_STAGE_TOKENS, sg.L - s * DEC8_STAGE_TOKENS);
-            const uint32_t sbase = ring + stage * DEC8_STAGE_BYTES + warp * DEC8_PPW * BN_KV8_BLOCK;
-            float sv[DEC8_PPW][4], vs[DEC8_PPW][2];
-            int nv[DEC8_PPW];
-            float tmax[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int pi = 0; pi < DEC8_PPW; ++pi) {
-                nv[pi] = max(0, min(BN_PAGE_TOKENS, ntok - (warp * DEC8_PPW + pi) * BN_PAGE_TOKENS));
-                const uint32_t block = sbase + pi * BN_KV8_BLOCK;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sv[pi][j] = 0.f;
-                if (nv[pi] == 0) continue;
-                if (VALUES == BN_KV8_E4M3 && nv[pi] < BN_PAGE_TOKENS) {
-                    // ragged last page: the unwritten V rows may hold a NaN, and 0 * NaN must not reach O
-                    for (int e = lane; e < (BN_PAGE_TOKENS - nv[pi]) * 4; e += 32)
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(block + KV8_V + nv[pi] * KV8_D + e * 16), "r"(0) : "memory");
+            // tokens of the warp's pages
+            const int mine = min(DEC8_STAGE_TOKENS, sg.L - s * DEC8_STAGE_TOKENS) - warp * DEC8_PPW * BN_PAGE_TOKENS;
+            if (mine > 0) {
+                const uint32_t sbase = ring + stage * DEC8_STAGE_BYTES + warp * DEC8_PPW * BN_KV8_BLOCK;
+                // thread owns heads hA, hA + 1 and tokens lane / 4 (+ 8) of each page
+                float sv[DEC8_PPW][4], pr[DEC8_PPW][4], vs[DEC8_PPW][2];
+                bool renew = m_run[0] == -INFINITY || m_run[1] == -INFINITY;
+                const bool ragged = mine < DEC8_PPW * BN_PAGE_TOKENS;
+                if (VALUES == BN_KV8_E4M3 && ragged) {
+                    // what lies behind the last token may be a NaN, and 0 * NaN must not reach O (whole pages may not have been loaded)
+                    for (int e = mine * 4 + lane; e < DEC8_PPW * BN_PAGE_TOKENS * 4; e += 32)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(sbase + (e / 64) * BN_KV8_BLOCK + KV8_V + (e % 64) * 16), "r"(0) : "memory");
                     fence_proxy_async_smem();          // the next copy into this stage comes after
                     __syncwarp();
                 }
-                const uint32_t row = block + (lane / 4) * KV8_D + (lane % 4) * 16, sc0 = block + KV8_SCALES + (lane / 4) * 4;
-                uint32_t a[4], b[4];
-                lds_v4(row, a);
-                lds_v4(row + 8 * KV8_D, b);
-                const uint32_t s0 = lds(sc0), s1 = lds(sc0 + 32);
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk) {
-                    uint32_t a0, a1, a2, a3;
-                    kv8_halves<VALUES>(a[kk], a0, a2);
-                    kv8_halves<VALUES>(b[kk], a1, a3);
-                    mma_f16_16816(sv[pi], a0, a1, a2, a3, qb[2 * kk], qb[2 * kk + 1]);
+                for (int pi = 0; pi < DEC8_PPW; ++pi) {
+                    const uint32_t block = sbase + pi * BN_KV8_BLOCK;
+                    const uint32_t row = block + (lane / 4) * KV8_D + (lane % 4) * 16, sc0 = block + KV8_SCALES + (lane / 4) * 4;
+                    uint32_t a[4], b[4];
+                    lds_v4(row, a);
+                    lds_v4(row + 8 * KV8_D, b);
+                    const uint32_t s0 = lds(sc0), s1 = lds(sc0 + 32);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sv[pi][j] = 0.f;
+                    if (VALUES == BN_KV8_E4M3) {
+#pragma unroll
+                        for (int part = 0; part < 3; ++part)
+#pragma unroll
+                            for (int kk = 0; kk < 2; ++kk)
+                                mma_e4m3_16832(sv[pi], a[2 * kk], b[2 * kk], a[2 * kk + 1], b[2 * kk + 1], qb[4 * part + 2 * kk], qb[4 * part + 2 * kk + 1]);
+                    } else {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) {
+                            uint32_t a0, a1, a2, a3;
+                            kv8_halves<VALUES>(a[kk], a0, a2);
+                            kv8_halves<VALUES>(b[kk], a1, a3);
+                            mma_f16_16816(sv[pi], a0, a1, a2, a3, qb[2 * kk], qb[2 * kk + 1]);
+                        }
+                    }
+                    const float k0 = bf16_lo(s0), k1 = bf16_lo(s1);
+                    vs[pi][0] = bf16_hi(s0); vs[pi][1] = bf16_hi(s1);
+                    sv[pi][0] *= k0 * fA; sv[pi][1] *= k0 * fB; sv[pi][2] *= k1 * fA; sv[pi][3] *= k1 * fB;
                 }
-                // thread owns heads hA, hA + 1 and tokens lane / 4 (+ 8) of each page
-                const float k0 = bf16_lo(s0), k1 = bf16_lo(s1);
-                vs[pi][0] = bf16_hi(s0); vs[pi][1] = bf16_hi(s1);
-                sv[pi][0] *= k0 * fA; sv[pi][1] *= k0 * fB; sv[pi][2] *= k1 * fA; sv[pi][3] *= k1 * fB;
-                if (nv[pi] < BN_PAGE_TOKENS) {
+                if (ragged) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        if (lane / 4 + 8 * i >= nv[pi]) { sv[pi][2 * i] = sv[pi][2 * i + 1] = -INFINITY; vs[pi][i] = 0.f; }
+                    for (int i = 0; i < 2 * DEC8_PPW; ++i)
+                        if (lane / 4 + 8 * i >= mine) { sv[i / 2][2 * (i % 2)] = sv[i / 2][2 * (i % 2) + 1] = -INFINITY; vs[i / 2][i % 2] = 0.f; }
                 }
-                const float e0 = lg2(fmaxf(vs[pi][0], 8.0779357e-28f)), e1 = lg2(fmaxf(vs[pi][1], 8.0779357e-28f));     // 2^-90
-                tmax[0] = fmaxf(tmax[0], fmaxf(sv[pi][0] + e0, sv[pi][2] + e1));
-                tmax[1] = fmaxf(tmax[1], fmaxf(sv[pi][1] + e0, sv[pi][3] + e1));
-            }
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 4));
-                tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 8));
-                tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 16));
-            }
-            float less[2];                      // what is taken off the scores
+                for (int pi = 0; pi < DEC8_PPW; ++pi) {
+                    float most = 0.f;
 #pragma unroll
-            for (int hh = 0; hh < 2; ++hh) {
-                const float m_new = fmaxf(m_run[hh], tmax[hh] - DEC8_HEADROOM);
-                less[hh] = m_new == -INFINITY ? 0.f : m_new;
-                if (m_new != m_run[hh]) {     // the running maximum moves rarely after the first stages
-                    const float alpha = ex2(m_run[hh] - less[hh]);
-                    m_run[hh] = m_new;
-                    l_run[hh] *= alpha;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) { o[i][hh] *= alpha; o[i][hh + 2] *= alpha; }
+                    for (int j = 0; j < 4; ++j) {
+                        pr[pi][j] = ex2(sv[pi][j] - less[j & 1]);
+                        most = fmaxf(most, pr[pi][j]);
+                    }
+                    // (2^-86: the sum of weights does without vs, and has to stay a number where vs is very small)
+                    renew |= most * fmaxf(fmaxf(vs[pi][0], vs[pi][1]), 1.2924697e-26f) > 16384.f;
                 }
-            }
+                if (__any_sync(0xffffffffu, renew)) {
+                    float tmax[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int pi = 0; pi < DEC8_PPW; ++pi) {
-                if (nv[pi] == 0) continue;
-                float pr[4];
+                    for (int pi = 0; pi < DEC8_PPW; ++pi)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    pr[j] = ex2(sv[pi][j] - less[j & 1]);
-                    l_run[j & 1] += pr[j];
-                    pr[j] *= vs[pi][j >> 1];
+                        for (int j = 0; j < 4; ++j)
+                            tmax[j & 1] = fmaxf(tmax[j & 1], sv[pi][j] + lg2(fmaxf(vs[pi][j >> 1], 8.0779357e-28f)));      // 2^-90
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh) {
+                        tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 4));
+                        tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 8));
+                        tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 16));
+                        const float m_new = fmaxf(m_run[hh], tmax[hh] - DEC8_HEADROOM);
+                        less[hh] = m_new == -INFINITY ? 0.f : m_new;
+                        const float alpha = ex2(m_run[hh] - less[hh]);
+                        m_run[hh] = m_new;
+                        l_run[hh] *= alpha;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) { o[i][hh] *= alpha; o[i][hh + 2] *= alpha; }
+                    }
+#pragma unroll
+                    for (int pi = 0; pi < DEC8_PPW; ++pi)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) pr[pi][j] = ex2(sv[pi][j] - less[j & 1]);
                 }
-                const uint32_t b0 = movmatrix_trans(pack_f16(pr[0], pr[1]));
-                const uint32_t b1 = movmatrix_trans(pack_f16(pr[2], pr[3]));
-                const int tok = (lane % 8) + ((lane / 8) & 1) * 8;
-                const uint32_t vrow = sbase + pi * BN_KV8_BLOCK + KV8_V + tok * KV8_D;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    // matrices: tokens 0-7 and 8-15 of 16 dims, the same of the next 16
-                    uint32_t r[4], a0, a1, a2, a3;
-                    ldmatrix_x4_trans(vrow + (((half * 2 + (lane / 16)) ^ ((tok >> 1) & 3)) << 4), r[0], r[1], r[2], r[3]);
+                for (int pi = 0; pi < DEC8_PPW; ++pi) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        kv8_token_pairs<VALUES>(r[2 * i], a0, a1);
-                        kv8_token_pairs<VALUES>(r[2 * i + 1], a2, a3);
-                        mma_f16_16816(o[half * 2 + i], a0, a1, a2, a3, b0, b1);
+                    for (int j = 0; j < 4; ++j) {
+                        l_run[j & 1] += pr[pi][j];
+                        pr[pi][j] *= vs[pi][j >> 1];
+                    }
+                    const uint32_t b0 = movmatrix_trans(pack_f16(pr[pi][0], pr[pi][1]));
+                    const uint32_t b1 = movmatrix_trans(pack_f16(pr[pi][2], pr[pi][3]));
+                    const int tok = (lane % 8) + ((lane / 8) & 1) * 8;
+                    const uint32_t vrow = sbase + pi * BN_KV8_BLOCK + KV8_V + tok * KV8_D;
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        // matrices: tokens 0-7 and 8-15 of 16 dims, the same of the next 16
+                        uint32_t r[4], a0, a1, a2, a3;
+                        ldmatrix_x4_trans(vrow + (((half * 2 + (lane / 16)) ^ ((tok >> 1) & 3)) << 4), r[0], r[1], r[2], r[3]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            kv8_token_pairs<VALUES>(r[2 * i], a0, a1);
+                            kv8_token_pairs<VALUES>(r[2 * i + 1], a2, a3);
+                            mma_f16_16816(o[half * 2 + i], a0, a1, a2, a3, b0, b1);
+                        }
                     }
                 }
             }
@@ -357,7 +400,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         for (int w = 0; w < DEC8_CWARPS; ++w) {
             const float scl = ex2(mrg_m[w][warp] - ms);
             lsum += mrg_l[w][warp] * scl;
-            const float2 po = *reinterpret_cast<const float2*>(&mrg_o[w][warp][hd]);
+            const float2 po = *reinterpret_cast<const float2*>(&mrg_o[w][warp][td]);
             acc[0] += po.x * scl; acc[1] += po.y * scl;
         }
         const int bgi = sg.b * p.Hkv + sg.g;
@@ -366,8 +409,8 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 const size_t row = (size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep + warp;
                 const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
                 const float r0 = acc[0] * inv, r1 = acc[1] * inv;
-                if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + hd) = pack_bf16(r0, r1);
-                if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + hd) = make_float2(r0, r1);
+                if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + td) = pack_bf16(r0, r1);
+                if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + td) = make_float2(r0, r1);
                 if (p.lse && lane == 0) p.lse[row] = lsum > 0.f ? (mstar + log2f(lsum)) * LN2 : -INFINITY;
             }
         } else {
@@ -376,7 +419,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 p.part_m[slot * DEC_G + warp] = mstar;
                 p.part_l[slot * DEC_G + warp] = lsum;
             }
-            *reinterpret_cast<float2*>(p.part_o + (slot * DEC_G + warp) * DEC_D + hd) = make_float2(acc[0], acc[1]);
+            *reinterpret_cast<float2*>(p.part_o + (slot * DEC_G + warp) * DEC_D + td) = make_float2(acc[0], acc[1]);
             // hand the partial to the combine warp and go on
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&part_bar));
