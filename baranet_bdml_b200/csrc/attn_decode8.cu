@@ -1,21 +1,28 @@
 // Single-token decode attention over the 8-bit paged cache (kv8.cuh), HBM bound:
 //     s_t = scale <RoPE(q), K_t> ks_t,   p = softmax(s),   out = sum_t p_t vs_t V_t,   lse = log sum exp s
 //
-// The schedule, the ring of stages and the merge are those of attn_decode.cu (decode_schedule.cuh): one persistent CTA per SM takes an
-// equal share of all 256-token stages, a producer warp fills a ring of shared memory, eight consumer warps take two pages of a stage
-// each, a tenth warp merges what several CTAs hold.  What 8 bits change:
-//   * A block (page, key head) is one bulk copy of 2112 bytes, scales included: no tensor map.
-//   * Both products are m16n8k16 MMAs of fp16, which holds every e4m3 and int8 number exactly:
-//       S^T (16 tokens x 8 heads) = K (16 x 64) Q^T,     O^T (64 x 8 heads) += V^T (64 x 16 tokens) P^T.
-//     The sum over k may run in any order, so a lane reads 16 bytes of a key's row at once (dims 16 c .. 16 c + 15 are its k's of all
-//     four MMAs) and q is laid out to match; V goes through ldmatrix.trans as pairs of bytes, which a byte permutation turns into
-//     pairs of tokens.  Two bytes become two fp16 by one conversion (e4m3) or two operations (int8).
+// The schedule is that of attn_decode.cu (decode_schedule.cuh): one persistent CTA per SM takes an equal share of all 256-token stages, as a
+// list of segments = (sequence, key head, run of stages).  Half the bytes leave half the time per token, so that what the consumers
+// do beside the two products has to go elsewhere:
+//   * two producer warps keep a ring of stages filled.  A block (page, key head) is one bulk copy of 2112 bytes, scales included; one
+//     warp issues one in 44 ns, two one in 30, and 52 is what DRAM needs for it (4 x 262144 tokens 122 -> 101 us with more than one);
+//   * a query warp rotates and converts the next segment's queries while the consumers work on the one before;
+//   * eight consumer warps, two groups of four that take stages in turn, four pages of a stage each: with two pages each, whose
+//     instruction chains are as long, 95 us instead of 91;
+//   * two merger warps, four heads each, join the consumers' (m, l, O) of a segment, write the result or a partial, and, where they hold the
+//     last of a (sequence, head)'s partials, join those; buffers are double, so that nobody waits for them.
+// Both products are m16n8k16 MMAs of fp16, which holds every e4m3 and int8 number exactly:
+//     S^T (16 tokens x 8 heads) = K (16 x 64) Q^T,     O^T (64 x 8 heads) += V^T (64 x 16 tokens) P^T.
+//   * The sum over k may run in any order, so a lane reads 16 bytes of a key's row at once (dims 16 c .. 16 c + 15 are its k's of all four
+//     MMAs) and q is laid out to match; V goes through ldmatrix.trans as pairs of bytes, which a byte permutation turns into pairs of
+//     tokens.  Two bytes become two fp16 by one conversion (e4m3) or two operations (int8).  (Scores by e4m3 MMAs, q in three parts, take
+//     fewer instructions and longer: 105 us instead of 97.)
 //   * q is rounded to fp16 as a multiple of a power of two that brings the head's largest element to 2^14 (a relative error of 2^-11; the
 //     2^28 below that keep it).
-//   * A token's value scale goes into its weight: p' = 2^(s - m) vs, with m the running maximum of s + log2 vs, not of s.  So p' is
-//     never above 2^8 and the tokens that count most in the result have the most bits of fp16, however far scales and weights are
-//     apart (2^-11 for 22 binades).  The sum of weights l runs in fp32 without vs; s - m + 8 is at most 98 (log2 vs counts as -90 at
-//     least), so it leaves no room for an overflow below 2^29 tokens.
+//   * A token's value scale goes into its weight: p' = 2^(s - m) vs, with m the running maximum of s + log2 vs - 8, not of s.  So the
+//     tokens that count most in the result have the most bits of fp16, however far scales and weights are apart.  m is only renewed
+//     when a weight would pass 2^14 (a vote instead of a reduction in every stage).  The sum of weights l runs in fp32 without vs: log2 vs
+//     counts as -90 at least there and a weight without vs renews m beyond 2^100, so l has room for 2^27 tokens.
 #include "decode_schedule.cuh"
 #include "kv8.cuh"
 
@@ -24,18 +31,23 @@ namespace bn {
 constexpr int DEC8_STAGE_TOKENS = 256;
 constexpr int DEC8_PAGES = DEC8_STAGE_TOKENS / BN_PAGE_TOKENS;       // of a stage
 constexpr int DEC8_STAGE_BYTES = DEC8_PAGES * BN_KV8_BLOCK;          // 33792
-constexpr int DEC8_NSTAGES = 6;
-constexpr int DEC8_CWARPS = 8;                                       // consumer warps
-constexpr int DEC8_PPW = DEC8_PAGES / DEC8_CWARPS;                   // pages per warp and stage
-constexpr int DEC8_CTHREADS = DEC8_CWARPS * 32;
-constexpr int DEC8_PWARPS = 4;                                       // producer warps
+constexpr int DEC8_NSTAGES = 4;
+constexpr int DEC8_GROUPS = 2;                                       // groups of consumer warps, which take stages in turn
+constexpr int DEC8_GWARPS = 4;                                       // warps of a group
+constexpr int DEC8_CWARPS = DEC8_GROUPS * DEC8_GWARPS;
+constexpr int DEC8_PPW = DEC8_PAGES / DEC8_GWARPS;                   // pages per warp and stage
+constexpr int DEC8_PWARPS = 2;                                       // producers
 constexpr int DEC8_PPP = DEC8_PAGES / DEC8_PWARPS;                   // pages per producer warp and stage
-constexpr int DEC8_THREADS = (DEC8_CWARPS + DEC8_PWARPS + 1) * 32;   // + combine warp
+constexpr int DEC8_MWARPS = 2;                                       // mergers
+constexpr int DEC8_HPM = DEC_G / DEC8_MWARPS;                        // heads per merger
+constexpr int DEC8_QUERY_WARP = DEC8_CWARPS + DEC8_PWARPS, DEC8_MERGER = DEC8_QUERY_WARP + 1;
+constexpr int DEC8_THREADS = (DEC8_MERGER + DEC8_MWARPS) * 32;
 constexpr int DEC8_SMEM_BYTES = DEC8_NSTAGES * DEC8_STAGE_BYTES + 128;
 constexpr int DEC8_DEFAULT_MIN_TOKENS = 1024;                        // a CTA's range is never shorter than this
 constexpr int DEC8_WHOLE_MAX_STAGES = 8;                             // sequences up to this many stages are never split (if there are enough)
-constexpr float DEC8_HEADROOM = 8.f;                                 // p' <= 2^8
-static_assert(DEC8_CTHREADS == DEC_G * DEC_D / 2, "a thread per head and two dimensions where warps are merged");
+// a group has to have waited for every fill of the slots that it reads: with another's fills in between, the parity that it waits for
+// may be that of the fill before the last
+static_assert(DEC8_NSTAGES % DEC8_GROUPS == 0, "slots belong to groups");
 
 struct Decode8Params {
     const __nv_bfloat16* q;
@@ -45,26 +57,32 @@ struct Decode8Params {
     __nv_bfloat16* out;
     float *out_f32, *lse;
     DecodeHeader* hdr;
-    int* tickets;
+    int* tickets;                               // [merger][sequence][key head]
     float *part_m, *part_l, *part_o;
     int B, Hq, Hkv, n_rep, max_pages, max_seq_len, min_stages, max_parts, rope_q;
     float scale_log2;
     RotationFreqs freqs;
 };
 
+// results of one head: lane -> dims 2 * lane, + 1
+__device__ __forceinline__ void decode8_store(const Decode8Params& p, size_t row, int lane, float m, float l, float a, float b) {
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + 2 * lane) = pack_bf16(a * inv, b * inv);
+    if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + 2 * lane) = make_float2(a * inv, b * inv);
+    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+}
+
 template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8_kernel(const __grid_constant__ Decode8Params p) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t full_bar[DEC8_NSTAGES];
-    __shared__ __align__(8) uint64_t empty_bar[DEC8_NSTAGES];
-    __shared__ __align__(8) uint64_t merge_bar, part_bar;
+    __shared__ __align__(8) uint64_t full_bar[DEC8_NSTAGES], empty_bar[DEC8_NSTAGES];
+    __shared__ __align__(8) uint64_t q_full[2], q_free[2], mrg_full[2], mrg_free[2];
     __shared__ int s_prefix[DEC_MAX_SEQS + 1];
     __shared__ int s_len[DEC_MAX_SEQS];
     __shared__ int s_nmax;                      // stages of the longest sequence
-    __shared__ float mrg_m[DEC8_CWARPS][DEC_G], mrg_l[DEC8_CWARPS][DEC_G];
-    __shared__ __align__(16) float mrg_o[DEC8_CWARPS][DEC_G][DEC_D + 2];   // written and read as float2
-    __shared__ __align__(16) uint32_t s_q[DEC_G][3 * DEC_D / 4]; // rotated query heads of the current segment: three e4m3 parts, or fp16
-    constexpr uint32_t QUERY_TOP = VALUES == BN_KV8_E4M3 ? 7 : 14;
-    __shared__ float s_factor[DEC_G];                           // scale * log2(e) * what q was divided by
+    __shared__ float mrg_m[2][DEC8_CWARPS][DEC_G], mrg_l[2][DEC8_CWARPS][DEC_G];
+    __shared__ __align__(16) float mrg_o[2][DEC8_CWARPS][DEC_G][DEC_D + 2];   // written and read as float2
+    __shared__ __align__(16) uint32_t s_q[2][DEC_G][DEC_D / 2]; // rotated query heads of a segment, pairs of fp16
+    __shared__ float s_factor[2][DEC_G];                        // scale * log2(e) * what q was divided by
     __shared__ int s_abort;
 
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -73,10 +91,14 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     if (tid == 0) {
         for (int s = 0; s < DEC8_NSTAGES; ++s) {
             mbar_init(smem_u32(&full_bar[s]), DEC8_PWARPS);
-            mbar_init(smem_u32(&empty_bar[s]), DEC8_CWARPS);
+            mbar_init(smem_u32(&empty_bar[s]), DEC8_GWARPS);
         }
-        mbar_init(smem_u32(&merge_bar), DEC8_CWARPS);
-        mbar_init(smem_u32(&part_bar), DEC8_CWARPS);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(smem_u32(&q_full[s]), 1);
+            mbar_init(smem_u32(&q_free[s]), DEC8_CWARPS);
+            mbar_init(smem_u32(&mrg_full[s]), DEC8_CWARPS);
+            mbar_init(smem_u32(&mrg_free[s]), DEC8_MWARPS);
+        }
         s_abort = 0;
         fence_mbar_init();
     }
@@ -93,20 +115,19 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     sc.whole = s_nmax <= DEC8_WHOLE_MAX_STAGES && p.B * p.Hkv >= 16;
     sc.G = sc.whole ? min((int)gridDim.x, p.B * p.Hkv) : max(1, min((int)gridDim.x, sc.T / p.min_stages));
     const bool active = sc.T > 0 && (int)blockIdx.x < sc.G;
-    const int range_lo = active ? sc.range_begin(blockIdx.x) : 0;
-    const int range_hi = active ? sc.range_begin(blockIdx.x + 1) : 0;
+    SegmentIter iter;
+    iter.init(active ? sc.range_begin(blockIdx.x) : 0, active ? sc.range_begin(blockIdx.x + 1) : 0);
+    Segment sg;
 
-    if (warp >= DEC8_CWARPS && warp < DEC8_CWARPS + DEC8_PWARPS) {
-        // ------------------------------------------------------------ producer
+    if (warp >= DEC8_CWARPS && warp < DEC8_QUERY_WARP) {
+        // ----------------------------------------------------------- producers
         // page numbers are read two stages (a 128-byte line of the table) at a time, one such group ahead of their use
         constexpr int GRP = 32 / DEC8_PAGES;
-        const int mine = (warp - DEC8_CWARPS) * DEC8_PPP + lane % DEC8_PPP;      // the lane's page of a stage
+        const int first = (warp - DEC8_CWARPS) * DEC8_PPP, mine = first + lane % DEC8_PPP;      // of a stage's pages: the warp's and the lane's
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true, bad = false;
-        SegmentIter iter;
-        iter.init(range_lo, range_hi);
-        Segment sg, sg_next;
+        Segment sg_next;
         bool have = iter.next(sc, sg, false);
         auto load_group = [&](const Segment& sgm, int grp) {
             const int e = grp * 32 + lane;
@@ -127,8 +148,8 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 }
                 int page = __shfl_sync(0xffffffffu, ids, (s % GRP) * DEC8_PAGES + mine);
                 if (page < 0 || page >= p.pool_pages) { page = 0; bad = true; }
-                if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1u, &s_abort)) { ok = false; break; }
-                const int npages = max(0, min(DEC8_PPP, n_pages_seq - s * DEC8_PAGES - (warp - DEC8_CWARPS) * DEC8_PPP));
+                if (!mbar_wait_warp(smem_u32(&empty_bar[stage]), phase ^ 1u, &s_abort)) { ok = false; break; }
+                const int npages = max(0, min(DEC8_PPP, n_pages_seq - s * DEC8_PAGES - first));
                 const uint32_t fb = smem_u32(&full_bar[stage]);
                 if (lane == 0) mbar_arrive_expect_tx(fb, (uint32_t)npages * BN_KV8_BLOCK);
                 __syncwarp();
@@ -146,108 +167,147 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         return;
     }
 
-    if (warp == DEC8_CWARPS + DEC8_PWARPS) {
-        // -------------------------------------------------------- combine warp
-        SegmentIter iter;
-        iter.init(range_lo, range_hi);
-        Segment sg;
-        uint32_t pphase = 0;
-        while (iter.next(sc, sg)) {
-            if (sg.n_parts == 1) continue;
-            if (!mbar_wait(smem_u32(&part_bar), pphase, &s_abort)) break;
-            pphase ^= 1u;
-            decode_combine(p, sg, lane);
+    if (warp == DEC8_QUERY_WARP) {
+        // ---------------------------------------------------------- query warp: lane -> dims 2 * lane, + 1, of all heads
+        for (int n = 0; iter.next(sc, sg, false); ++n) {
+            const int buf = n % 2;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + ((size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep) * (DEC_D / 2) + lane;
+            uint32_t raw[DEC_G];
+#pragma unroll
+            for (int h = 0; h < DEC_G; ++h) raw[h] = h < p.n_rep ? src[h * (DEC_D / 2)] : 0u;
+            float c = 1.f, s = 0.f;
+            if (p.rope_q) rotation(p.q_positions ? p.q_positions[sg.b] : sg.L - 1, p.freqs.f[lane], &c, &s);
+            if (!mbar_wait_warp(smem_u32(&q_free[buf]), (n / 2 & 1) ^ 1u, &s_abort)) break;
+#pragma unroll
+            for (int h = 0; h < DEC_G; ++h) {
+                const float x0 = bf16_lo(raw[h]), x1 = bf16_hi(raw[h]);
+                const float y0 = x0 * c - x1 * s, y1 = x0 * s + x1 * c;
+                const uint32_t most = __reduce_max_sync(0xffffffffu, max(__float_as_uint(y0) & 0x7fffffffu, __float_as_uint(y1) & 0x7fffffffu));
+                const uint32_t e = max(most >> 23, 30u);
+                const float up = __uint_as_float((254u + 14u - e) << 23);              // the largest magnitude to 2^14 and above
+                s_q[buf][h][lane] = pack_f16(y0 * up, y1 * up);
+                if (lane == 0) s_factor[buf][h] = p.scale_log2 * __uint_as_float((e - 14u) << 23);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&q_full[buf]));
+        }
+        if (lane == 0 && s_abort) atomicExch(&p.hdr->error, BN_ERR_TIMEOUT);
+        return;
+    }
+
+    if (warp >= DEC8_MERGER) {
+        // ------------------------------------------------------------- mergers
+        const int h0 = (warp - DEC8_MERGER) * DEC8_HPM;
+        // sequences without tokens get a zero output from whoever passes by
+        for (int bgi = blockIdx.x; bgi < p.B * p.Hkv; bgi += gridDim.x) {
+            const int b = bgi / p.Hkv, g = bgi % p.Hkv;
+            if (sc.nst(b) > 0) continue;
+#pragma unroll
+            for (int h = h0; h < h0 + DEC8_HPM; ++h)
+                if (h < p.n_rep) decode8_store(p, (size_t)b * p.Hq + (size_t)g * p.n_rep + h, lane, 0.f, 0.f, 0.f, 0.f);
+        }
+        for (int n = 0; iter.next(sc, sg); ++n) {
+            const int buf = n % 2;
+            if (!mbar_wait_warp(smem_u32(&mrg_full[buf]), n / 2 & 1, &s_abort)) break;
+            float m[DEC8_HPM], l[DEC8_HPM], a[DEC8_HPM], b[DEC8_HPM];
+#pragma unroll
+            for (int i = 0; i < DEC8_HPM; ++i) {
+                const int h = h0 + i;
+                m[i] = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < DEC8_CWARPS; ++w) m[i] = fmaxf(m[i], mrg_m[buf][w][h]);
+                const float base = m[i] == -INFINITY ? 0.f : m[i];
+                l[i] = a[i] = b[i] = 0.f;
+#pragma unroll
+                for (int w = 0; w < DEC8_CWARPS; ++w) {
+                    const float scl = ex2(mrg_m[buf][w][h] - base);
+                    const float2 o = *reinterpret_cast<const float2*>(&mrg_o[buf][w][h][2 * lane]);
+                    l[i] += mrg_l[buf][w][h] * scl;
+                    a[i] += o.x * scl;
+                    b[i] += o.y * scl;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&mrg_free[buf]));
+            const int bgi = sg.b * p.Hkv + sg.g;
+            const size_t row = (size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep;
+            if (sg.n_parts > 1) {
+                const size_t part = ((size_t)bgi * p.max_parts + ((int)blockIdx.x - sg.c_first)) * DEC_G;
+#pragma unroll
+                for (int i = 0; i < DEC8_HPM; ++i) {
+                    if (lane == 0) { p.part_m[part + h0 + i] = m[i]; p.part_l[part + h0 + i] = l[i]; }
+                    *reinterpret_cast<float2*>(p.part_o + (part + h0 + i) * DEC_D + 2 * lane) = make_float2(a[i], b[i]);
+                }
+                __threadfence();
+                __syncwarp();
+                int* ticket = p.tickets + (size_t)(warp - DEC8_MERGER) * DEC_MAX_SEQS * p.Hkv + bgi;
+                int t = 0;
+                if (lane == 0) t = atomicAdd(ticket, 1);
+                if (__shfl_sync(0xffffffffu, t, 0) != sg.n_parts - 1) continue;
+                __threadfence();
+                if (lane == 0) *ticket = 0;            // leave the scratch clean for the next launch
+                // this CTA stored the last part: joined in the order of the parts, whoever is last
+#pragma unroll
+                for (int i = 0; i < DEC8_HPM; ++i) { m[i] = -INFINITY; l[i] = a[i] = b[i] = 0.f; }
+                constexpr int AHEAD = 4;               // parts whose loads are under way together
+                for (int c0 = 0; c0 < sg.n_parts; c0 += AHEAD) {
+                    float pm[AHEAD][DEC8_HPM], pl[AHEAD][DEC8_HPM];
+                    float2 po[AHEAD][DEC8_HPM];
+#pragma unroll
+                    for (int c = 0; c < AHEAD; ++c)
+#pragma unroll
+                        for (int i = 0; i < DEC8_HPM; ++i) {
+                            const bool on = c0 + c < sg.n_parts;
+                            const size_t e = ((size_t)bgi * p.max_parts + (on ? c0 + c : 0)) * DEC_G + h0 + i;
+                            pm[c][i] = on ? __ldcg(p.part_m + e) : -INFINITY;
+                            pl[c][i] = on ? __ldcg(p.part_l + e) : 0.f;
+                            po[c][i] = on ? __ldcg(reinterpret_cast<const float2*>(p.part_o + e * DEC_D + 2 * lane)) : make_float2(0.f, 0.f);
+                        }
+#pragma unroll
+                    for (int i = 0; i < DEC8_HPM; ++i) {
+                        float top = m[i];
+#pragma unroll
+                        for (int c = 0; c < AHEAD; ++c) top = fmaxf(top, pm[c][i]);
+                        const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[i] - base);
+                        m[i] = top;
+                        l[i] *= keep; a[i] *= keep; b[i] *= keep;
+#pragma unroll
+                        for (int c = 0; c < AHEAD; ++c) {
+                            const float scl = ex2(pm[c][i] - base);
+                            l[i] += pl[c][i] * scl;
+                            a[i] += po[c][i].x * scl;
+                            b[i] += po[c][i].y * scl;
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < DEC8_HPM; ++i)
+                if (h0 + i < p.n_rep) decode8_store(p, row + h0 + i, lane, m[i], l[i], a[i], b[i]);
         }
         if (lane == 0 && s_abort) atomicExch(&p.hdr->error, BN_ERR_TIMEOUT);
         return;
     }
 
     // --------------------------------------------------------------- consumers
-    // where the heads' 64 results are laid over the consumers: a warp has a head, a lane two dimensions
-    const int td = 2 * lane;
-    // sequences without tokens get a zero output from whoever passes by
-    for (int bgi = blockIdx.x; bgi < p.B * p.Hkv; bgi += gridDim.x) {
-        const int b = bgi / p.Hkv, g = bgi % p.Hkv;
-        if (sc.nst(b) > 0 || warp >= p.n_rep) continue;
-        const size_t row = (size_t)b * p.Hq + (size_t)g * p.n_rep + warp;
-        if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + td) = 0u;
-        if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + td) = make_float2(0.f, 0.f);
-        if (p.lse && lane == 0) p.lse[row] = -INFINITY;
-    }
-
-    int stage = 0;
-    uint32_t phase = 0, mphase = 0;
+    const int group = warp / DEC8_GWARPS, gwarp = warp % DEC8_GWARPS;
     const int hA = 2 * (lane % 4);       // the two heads whose softmax state this thread carries
-    const uint32_t mb = smem_u32(&merge_bar);
-    auto group_sync = [&]() -> bool {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(mb);
-        const bool ok = mbar_wait_warp(mb, mphase, &s_abort);
-        mphase ^= 1u;
-        return ok;
-    };
-    auto load_q_raw = [&](const Segment& sg) -> uint32_t {
-        if (warp >= p.n_rep) return 0u;
-        return *reinterpret_cast<const uint32_t*>(p.q + ((size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep + warp) * DEC_D + 2 * lane);
-    };
-    auto store_q = [&](const Segment& sgq, uint32_t raw) {
-        float x0 = bf16_lo(raw), x1 = bf16_hi(raw);
-        if (p.rope_q) {
-            float c, s;
-            rotation(p.q_positions ? p.q_positions[sgq.b] : sgq.L - 1, p.freqs.f[lane], &c, &s);
-            const float y0 = x0 * c - x1 * s;
-            const float y1 = x0 * s + x1 * c;
-            x0 = y0; x1 = y1;
-        }
-        const uint32_t most = __reduce_max_sync(0xffffffffu, max(__float_as_uint(x0) & 0x7fffffffu, __float_as_uint(x1) & 0x7fffffffu));
-        const uint32_t e = max(most >> 23, 30u);
-        const float up = __uint_as_float((254u + QUERY_TOP - e) << 23);        // the head's largest magnitude to 2^QUERY_TOP and above
-        x0 *= up;
-        x1 *= up;
-        if (VALUES == BN_KV8_E4M3) {
-#pragma unroll
-            for (int part = 0; part < 3; ++part) {
-                uint16_t two;
-                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(two) : "f"(x1), "f"(x0));
-                reinterpret_cast<uint16_t*>(&s_q[warp][part * (DEC_D / 4)])[lane] = two;
-                uint32_t back;
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(back) : "h"(two));
-                const float2 f = halves_to_floats(back);
-                x0 -= f.x;
-                x1 -= f.y;
-            }
-        } else {
-            reinterpret_cast<uint32_t*>(s_q[warp])[lane] = pack_f16(x0, x1);
-        }
-        if (lane == 0) s_factor[warp] = p.scale_log2 * (e == 255u ? NAN : __uint_as_float((e - QUERY_TOP) << 23));     // (an infinity would saturate)
-    };
-
-    SegmentIter iter;
-    iter.init(range_lo, range_hi);
-    Segment sg, sg_next;
-    bool have = iter.next(sc, sg);
+    int before = 0;                      // stages of the range that lie before the segment
     bool ok = true;
-    if (have) {
-        store_q(sg, load_q_raw(sg));
-        ok = group_sync();
-    }
-    while (ok && have) {
-        // look one segment ahead so that its query is already on the way
-        const bool have_next = iter.next(sc, sg_next);
-        const uint32_t q_raw_next = have_next ? load_q_raw(sg_next) : 0u;
+    for (int n = 0; ok && iter.next(sc, sg, false); ++n) {
+        const int buf = n % 2;
+        if (!mbar_wait_warp(smem_u32(&q_full[buf]), n / 2 & 1, &s_abort)) break;
         // Q^T fragments: dims 16 c .. 16 c + 15 of head lane / 4, c = lane % 4
-        uint32_t qb[VALUES == BN_KV8_E4M3 ? 12 : 8];
+        uint32_t qb[8];
 #pragma unroll
-        for (int i = 0; i < (VALUES == BN_KV8_E4M3 ? 3 : 2); ++i) {
-            // (a part's 16 elements are one 16-byte piece of e4m3, or half of the two pieces of fp16)
-            const uint4 a = VALUES == BN_KV8_E4M3 ? *reinterpret_cast<const uint4*>(&s_q[lane / 4][i * (DEC_D / 4) + 4 * (lane % 4)])
-                                                  : *reinterpret_cast<const uint4*>(&s_q[lane / 4][8 * (lane % 4) + 4 * i]);
+        for (int i = 0; i < 2; ++i) {
+            const uint4 a = *reinterpret_cast<const uint4*>(&s_q[buf][lane / 4][8 * (lane % 4) + 4 * i]);
             qb[4 * i] = a.x; qb[4 * i + 1] = a.y; qb[4 * i + 2] = a.z; qb[4 * i + 3] = a.w;
         }
-        const float fA = s_factor[hA], fB = s_factor[hA + 1];
+        const float fA = s_factor[buf][hA], fB = s_factor[buf][hA + 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&q_free[buf]));
 
-        // weights are 2^(s - m_run) (times vs for the product): no larger than 2^8 where m_run is renewed, and it is renewed before
-        // they pass 2^14
         float m_run[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f};
         float o[4][4];
 #pragma unroll
@@ -255,12 +315,13 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
 
-        for (int s = sg.s0; s < sg.s1; ++s) {
-            if (!mbar_wait_warp(smem_u32(&full_bar[stage]), phase, &s_abort)) { ok = false; break; }
+        for (int s = sg.s0 + ((before ^ group) & 1); s < sg.s1; s += DEC8_GROUPS) {
+            const int nth = before + s - sg.s0, stage = nth % DEC8_NSTAGES;
+            if (!mbar_wait_warp(smem_u32(&full_bar[stage]), (nth / DEC8_NSTAGES) & 1, &s_abort)) { ok = false; break; }
             // tokens of the warp's pages
-            const int mine = min(DEC8_STAGE_TOKENS, sg.L - s * DEC8_STAGE_TOKENS) - warp * DEC8_PPW * BN_PAGE_TOKENS;
+            const int mine = min(DEC8_STAGE_TOKENS, sg.L - s * DEC8_STAGE_TOKENS) - gwarp * DEC8_PPW * BN_PAGE_TOKENS;
             if (mine > 0) {
-                const uint32_t sbase = ring + stage * DEC8_STAGE_BYTES + warp * DEC8_PPW * BN_KV8_BLOCK;
+                const uint32_t sbase = ring + stage * DEC8_STAGE_BYTES + gwarp * DEC8_PPW * BN_KV8_BLOCK;
                 // thread owns heads hA, hA + 1 and tokens lane / 4 (+ 8) of each page
                 float sv[DEC8_PPW][4], pr[DEC8_PPW][4], vs[DEC8_PPW][2];
                 bool renew = m_run[0] == -INFINITY || m_run[1] == -INFINITY;
@@ -282,20 +343,12 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                     const uint32_t s0 = lds(sc0), s1 = lds(sc0 + 32);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) sv[pi][j] = 0.f;
-                    if (VALUES == BN_KV8_E4M3) {
 #pragma unroll
-                        for (int part = 0; part < 3; ++part)
-#pragma unroll
-                            for (int kk = 0; kk < 2; ++kk)
-                                mma_e4m3_16832(sv[pi], a[2 * kk], b[2 * kk], a[2 * kk + 1], b[2 * kk + 1], qb[4 * part + 2 * kk], qb[4 * part + 2 * kk + 1]);
-                    } else {
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) {
-                            uint32_t a0, a1, a2, a3;
-                            kv8_halves<VALUES>(a[kk], a0, a2);
-                            kv8_halves<VALUES>(b[kk], a1, a3);
-                            mma_f16_16816(sv[pi], a0, a1, a2, a3, qb[2 * kk], qb[2 * kk + 1]);
-                        }
+                    for (int kk = 0; kk < 4; ++kk) {
+                        uint32_t a0, a1, a2, a3;
+                        kv8_halves<VALUES>(a[kk], a0, a2);
+                        kv8_halves<VALUES>(b[kk], a1, a3);
+                        mma_f16_16816(sv[pi], a0, a1, a2, a3, qb[2 * kk], qb[2 * kk + 1]);
                     }
                     const float k0 = bf16_lo(s0), k1 = bf16_lo(s1);
                     vs[pi][0] = bf16_hi(s0); vs[pi][1] = bf16_hi(s1);
@@ -329,7 +382,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                         tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 4));
                         tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 8));
                         tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 16));
-                        const float m_new = fmaxf(m_run[hh], tmax[hh] - DEC8_HEADROOM);
+                        const float m_new = fmaxf(m_run[hh], tmax[hh] - 8.f);
                         less[hh] = m_new == -INFINITY ? 0.f : m_new;
                         const float alpha = ex2(m_run[hh] - less[hh]);
                         m_run[hh] = m_new;
@@ -369,66 +422,30 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&empty_bar[stage]));
-            if (++stage == DEC8_NSTAGES) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
+        before += sg.s1 - sg.s0;
 
-        // ------------------------------------------------ merge the warps
+        // hand (m, l, O) to the mergers
 #pragma unroll
         for (int hh = 0; hh < 2; ++hh) {
             l_run[hh] += __shfl_xor_sync(0xffffffffu, l_run[hh], 4);
             l_run[hh] += __shfl_xor_sync(0xffffffffu, l_run[hh], 8);
             l_run[hh] += __shfl_xor_sync(0xffffffffu, l_run[hh], 16);
         }
+        if (!mbar_wait_warp(smem_u32(&mrg_free[buf]), (n / 2 & 1) ^ 1u, &s_abort)) break;
         if (lane < 4) {
-            mrg_m[warp][hA] = m_run[0]; mrg_m[warp][hA + 1] = m_run[1];
-            mrg_l[warp][hA] = l_run[0]; mrg_l[warp][hA + 1] = l_run[1];
+            mrg_m[buf][warp][hA] = m_run[0]; mrg_m[buf][warp][hA + 1] = m_run[1];
+            mrg_l[buf][warp][hA] = l_run[0]; mrg_l[buf][warp][hA + 1] = l_run[1];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int d = i * 16 + 2 * (lane / 4);
-            *reinterpret_cast<float2*>(&mrg_o[warp][hA][d]) = make_float2(o[i][0], o[i][2]);
-            *reinterpret_cast<float2*>(&mrg_o[warp][hA + 1][d]) = make_float2(o[i][1], o[i][3]);
+            *reinterpret_cast<float2*>(&mrg_o[buf][warp][hA][d]) = make_float2(o[i][0], o[i][2]);
+            *reinterpret_cast<float2*>(&mrg_o[buf][warp][hA + 1][d]) = make_float2(o[i][1], o[i][3]);
         }
-        if (!group_sync()) break;
-        float mstar = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < DEC8_CWARPS; ++w) mstar = fmaxf(mstar, mrg_m[w][warp]);
-        const float ms = mstar == -INFINITY ? 0.f : mstar;
-        float lsum = 0.f, acc[2] = {0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < DEC8_CWARPS; ++w) {
-            const float scl = ex2(mrg_m[w][warp] - ms);
-            lsum += mrg_l[w][warp] * scl;
-            const float2 po = *reinterpret_cast<const float2*>(&mrg_o[w][warp][td]);
-            acc[0] += po.x * scl; acc[1] += po.y * scl;
-        }
-        const int bgi = sg.b * p.Hkv + sg.g;
-        if (sg.n_parts == 1) {
-            if (warp < p.n_rep) {
-                const size_t row = (size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep + warp;
-                const float inv = lsum > 0.f ? 1.f / lsum : 0.f;
-                const float r0 = acc[0] * inv, r1 = acc[1] * inv;
-                if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + td) = pack_bf16(r0, r1);
-                if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + td) = make_float2(r0, r1);
-                if (p.lse && lane == 0) p.lse[row] = lsum > 0.f ? (mstar + log2f(lsum)) * LN2 : -INFINITY;
-            }
-        } else {
-            const size_t slot = (size_t)bgi * p.max_parts + ((int)blockIdx.x - sg.c_first);
-            if (lane == 0) {
-                p.part_m[slot * DEC_G + warp] = mstar;
-                p.part_l[slot * DEC_G + warp] = lsum;
-            }
-            *reinterpret_cast<float2*>(p.part_o + (slot * DEC_G + warp) * DEC_D + td) = make_float2(acc[0], acc[1]);
-            // hand the partial to the combine warp and go on
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&part_bar));
-        }
-        // the next segment's query replaces this one's (every warp took its fragments long ago)
-        if (have_next) store_q(sg_next, q_raw_next);
-        if (!group_sync()) break;              // mrg_* free again, s_q visible
-        sg = sg_next;
-        have = have_next;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&mrg_full[buf]));
     }
     if (s_abort && lane == 0) atomicExch(&p.hdr->error, BN_ERR_TIMEOUT);
 }
@@ -444,7 +461,7 @@ static int dec8_min_tokens(int chunk_tokens) {
 
 extern "C" size_t bn_attn_decode_kv8_workspace_bytes(int B, int Hq, int Hkv, int D, int max_seq_len, int chunk_tokens) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || D != KV8_D || max_seq_len < 0 || chunk_tokens < 0 || chunk_tokens % 128) return 0;
-    return decode_layout(B, Hkv, max_seq_len, dec8_min_tokens(chunk_tokens), regular_ticket_slots(Hkv)).total;
+    return decode_layout(B, Hkv, max_seq_len, dec8_min_tokens(chunk_tokens), DEC8_MWARPS * regular_ticket_slots(Hkv)).total;
 }
 
 extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_pages, const int32_t* page_table, int max_pages,
@@ -473,7 +490,7 @@ extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_
     if (int rc = require_sm100()) return rc;
     if (B == 0) return BN_OK;
     const int min_tokens = dec8_min_tokens(chunk_tokens);
-    const DecodeLayout L = decode_layout(B, Hkv, max_seq_len, min_tokens, regular_ticket_slots(Hkv));
+    const DecodeLayout L = decode_layout(B, Hkv, max_seq_len, min_tokens, DEC8_MWARPS * regular_ticket_slots(Hkv));
     if (!workspace || workspace_bytes < L.total) return fail(BN_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", what, workspace_bytes, L.total);
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(BN_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", what);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
