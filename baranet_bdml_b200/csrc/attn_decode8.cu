@@ -9,8 +9,10 @@
 //   * a query warp rotates and converts the next segment's queries while the consumers work on the one before;
 //   * eight consumer warps, two groups of four that take stages in turn, four pages of a stage each: with two pages each, whose
 //     instruction chains are as long, 95 us instead of 91;
-//   * two merger warps, four heads each, join the consumers' (m, l, O) of a segment, write the result or a partial, and, where they hold the
-//     last of a (sequence, head)'s partials, join those; buffers are double, so that nobody waits for them.
+//   * four merger warps, two heads each, join the consumers' (m, l, O) of a segment, write the result or a partial, and, where they hold
+//     the last of a (sequence, head)'s partials, join those; buffers are double, so that nobody waits for them.
+//     (Two mergers of four heads: 24.1 -> 24.9 us for 64 sequences of 1024 to 4096 tokens.  Taking the segment that a range's end cuts first, so
+//     that its partials are joined before the CTAs end, costs more at the start than it saves at the end: 22.9 -> 24.1 us.)
 // Both products are m16n8k16 MMAs of fp16, which holds every e4m3 and int8 number exactly:
 //     S^T (16 tokens x 8 heads) = K (16 x 64) Q^T,     O^T (64 x 8 heads) += V^T (64 x 16 tokens) P^T.
 //   * The sum over k may run in any order, so a lane reads 16 bytes of a key's row at once (dims 16 c .. 16 c + 15 are its k's of all four
@@ -38,13 +40,13 @@ constexpr int DEC8_CWARPS = DEC8_GROUPS * DEC8_GWARPS;
 constexpr int DEC8_PPW = DEC8_PAGES / DEC8_GWARPS;                   // pages per warp and stage
 constexpr int DEC8_PWARPS = 2;                                       // producers
 constexpr int DEC8_PPP = DEC8_PAGES / DEC8_PWARPS;                   // pages per producer warp and stage
-constexpr int DEC8_MWARPS = 2;                                       // mergers
+constexpr int DEC8_MWARPS = 4;                                       // mergers
 constexpr int DEC8_HPM = DEC_G / DEC8_MWARPS;                        // heads per merger
 constexpr int DEC8_QUERY_WARP = DEC8_CWARPS + DEC8_PWARPS, DEC8_MERGER = DEC8_QUERY_WARP + 1;
 constexpr int DEC8_THREADS = (DEC8_MERGER + DEC8_MWARPS) * 32;
 constexpr int DEC8_SMEM_BYTES = DEC8_NSTAGES * DEC8_STAGE_BYTES + 128;
-constexpr int DEC8_DEFAULT_MIN_TOKENS = 1024;                        // a CTA's range is never shorter than this
-constexpr int DEC8_WHOLE_MAX_STAGES = 8;                             // sequences up to this many stages are never split (if there are enough)
+constexpr int DEC8_MAX_CTAS = 256;
+constexpr int DEC8_CUT_STAGES = 4;                                   // what a cut segment costs, in stages
 // a group has to have waited for every fill of the slots that it reads: with another's fills in between, the parity that it waits for
 // may be that of the fill before the last
 static_assert(DEC8_NSTAGES % DEC8_GROUPS == 0, "slots belong to groups");
@@ -57,9 +59,10 @@ struct Decode8Params {
     __nv_bfloat16* out;
     float *out_f32, *lse;
     DecodeHeader* hdr;
-    int* tickets;                               // [merger][sequence][key head]
-    float *part_m, *part_l, *part_o;
-    int B, Hq, Hkv, n_rep, max_pages, max_seq_len, min_stages, max_parts, rope_q;
+    int* tickets;                               // [merger][CTA that holds the segment's first part]
+    float *part_m, *part_l, *part_o;            // [CTA][0: the segment began before its range, 1: it ends behind it][head] ([dim])
+    int B, Hq, Hkv, n_rep, max_pages, max_seq_len, min_stages, rope_q;
+    int most_heads;                             // (sequence, key head)s of a CTA that takes whole ones
     float scale_log2;
     RotationFreqs freqs;
 };
@@ -112,8 +115,10 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     sc.Hkv = p.Hkv;
     sc.B = p.B;
     sc.T = p.Hkv * s_prefix[p.B];
-    sc.whole = s_nmax <= DEC8_WHOLE_MAX_STAGES && p.B * p.Hkv >= 16;
-    sc.G = sc.whole ? min((int)gridDim.x, p.B * p.Hkv) : max(1, min((int)gridDim.x, sc.T / p.min_stages));
+    // whole (sequence, key head)s for every CTA where equal shares would save less than their cuts cost
+    const int grid = gridDim.x;
+    sc.whole = (int64_t)p.most_heads * s_nmax * grid <= sc.T + DEC8_CUT_STAGES * grid;
+    sc.G = sc.whole ? min(grid, p.B * p.Hkv) : max(1, min(grid, p.min_stages == 1 ? sc.T : sc.T / p.min_stages));
     const bool active = sc.T > 0 && (int)blockIdx.x < sc.G;
     SegmentIter iter;
     iter.init(active ? sc.range_begin(blockIdx.x) : 0, active ? sc.range_begin(blockIdx.x + 1) : 0);
@@ -206,7 +211,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
             for (int h = h0; h < h0 + DEC8_HPM; ++h)
                 if (h < p.n_rep) decode8_store(p, (size_t)b * p.Hq + (size_t)g * p.n_rep + h, lane, 0.f, 0.f, 0.f, 0.f);
         }
-        for (int n = 0; iter.next(sc, sg); ++n) {
+        for (int n = 0; iter.next(sc, sg, true); ++n) {
             const int buf = n % 2;
             if (!mbar_wait_warp(smem_u32(&mrg_full[buf]), n / 2 & 1, &s_abort)) break;
             float m[DEC8_HPM], l[DEC8_HPM], a[DEC8_HPM], b[DEC8_HPM];
@@ -229,10 +234,9 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&mrg_free[buf]));
-            const int bgi = sg.b * p.Hkv + sg.g;
             const size_t row = (size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep;
             if (sg.n_parts > 1) {
-                const size_t part = ((size_t)bgi * p.max_parts + ((int)blockIdx.x - sg.c_first)) * DEC_G;
+                const int part = ((int)blockIdx.x * 2 + ((int)blockIdx.x == sg.c_first)) * DEC_G;
 #pragma unroll
                 for (int i = 0; i < DEC8_HPM; ++i) {
                     if (lane == 0) { p.part_m[part + h0 + i] = m[i]; p.part_l[part + h0 + i] = l[i]; }
@@ -240,7 +244,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 }
                 __threadfence();
                 __syncwarp();
-                int* ticket = p.tickets + (size_t)(warp - DEC8_MERGER) * DEC_MAX_SEQS * p.Hkv + bgi;
+                int* ticket = p.tickets + (warp - DEC8_MERGER) * DEC8_MAX_CTAS + sg.c_first;
                 int t = 0;
                 if (lane == 0) t = atomicAdd(ticket, 1);
                 if (__shfl_sync(0xffffffffu, t, 0) != sg.n_parts - 1) continue;
@@ -249,7 +253,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 // this CTA stored the last part: joined in the order of the parts, whoever is last
 #pragma unroll
                 for (int i = 0; i < DEC8_HPM; ++i) { m[i] = -INFINITY; l[i] = a[i] = b[i] = 0.f; }
-                constexpr int AHEAD = 4;               // parts whose loads are under way together
+                constexpr int AHEAD = 8;               // parts whose loads are under way together
                 for (int c0 = 0; c0 < sg.n_parts; c0 += AHEAD) {
                     float pm[AHEAD][DEC8_HPM], pl[AHEAD][DEC8_HPM];
                     float2 po[AHEAD][DEC8_HPM];
@@ -258,7 +262,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 #pragma unroll
                         for (int i = 0; i < DEC8_HPM; ++i) {
                             const bool on = c0 + c < sg.n_parts;
-                            const size_t e = ((size_t)bgi * p.max_parts + (on ? c0 + c : 0)) * DEC_G + h0 + i;
+                            const int e = ((sg.c_first + (on ? c0 + c : 0)) * 2 + (!on || c0 + c == 0)) * DEC_G + h0 + i;
                             pm[c][i] = on ? __ldcg(p.part_m + e) : -INFINITY;
                             pl[c][i] = on ? __ldcg(p.part_l + e) : 0.f;
                             po[c][i] = on ? __ldcg(reinterpret_cast<const float2*>(p.part_o + e * DEC_D + 2 * lane)) : make_float2(0.f, 0.f);
@@ -454,14 +458,14 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 
 using namespace bn;
 
-static int dec8_min_tokens(int chunk_tokens) {
-    const int t = chunk_tokens > 0 ? chunk_tokens : DEC8_DEFAULT_MIN_TOKENS;
-    return (int)(((int64_t)t + DEC8_STAGE_TOKENS - 1) / DEC8_STAGE_TOKENS) * DEC8_STAGE_TOKENS;   // whole stages
-}
+// Scratch: the error word, a ticket per merger and CTA, two partial results per CTA (a range cuts two segments at most)
+constexpr size_t DEC8_PARTS = (size_t)2 * DEC8_MAX_CTAS * DEC_G;
+constexpr size_t DEC8_TICKETS_AT = 256, DEC8_PARTS_AT = DEC8_TICKETS_AT + DEC8_MWARPS * DEC8_MAX_CTAS * sizeof(int);
+constexpr size_t DEC8_SCRATCH_BYTES = DEC8_PARTS_AT + DEC8_PARTS * (DEC_D + 2) * sizeof(float);
 
 extern "C" size_t bn_attn_decode_kv8_workspace_bytes(int B, int Hq, int Hkv, int D, int max_seq_len, int chunk_tokens) {
     if (B <= 0 || Hq <= 0 || Hkv <= 0 || D != KV8_D || max_seq_len < 0 || chunk_tokens < 0 || chunk_tokens % 128) return 0;
-    return decode_layout(B, Hkv, max_seq_len, dec8_min_tokens(chunk_tokens), DEC8_MWARPS * regular_ticket_slots(Hkv)).total;
+    return DEC8_SCRATCH_BYTES;
 }
 
 extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_pages, const int32_t* page_table, int max_pages,
@@ -489,9 +493,8 @@ extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_
         return fail(BN_ERR_INVALID_ARG, "%s: pool/q/out buffers must be 16/8/8/16-byte aligned", what);
     if (int rc = require_sm100()) return rc;
     if (B == 0) return BN_OK;
-    const int min_tokens = dec8_min_tokens(chunk_tokens);
-    const DecodeLayout L = decode_layout(B, Hkv, max_seq_len, min_tokens, DEC8_MWARPS * regular_ticket_slots(Hkv));
-    if (!workspace || workspace_bytes < L.total) return fail(BN_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", what, workspace_bytes, L.total);
+    if (!workspace || workspace_bytes < DEC8_SCRATCH_BYTES)
+        return fail(BN_ERR_WORKSPACE, "%s: workspace of %zu bytes given, %zu needed", what, workspace_bytes, DEC8_SCRATCH_BYTES);
     if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(BN_ERR_INVALID_ARG, "%s: workspace must be 256-byte aligned", what);
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     Decode8Params p;
@@ -502,13 +505,12 @@ extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_
     p.out = static_cast<__nv_bfloat16*>(out);
     p.out_f32 = out_f32; p.lse = lse;
     p.hdr = reinterpret_cast<DecodeHeader*>(ws);
-    p.tickets = reinterpret_cast<int*>(ws + L.tickets);
-    p.part_m = reinterpret_cast<float*>(ws + L.part_m);
-    p.part_l = reinterpret_cast<float*>(ws + L.part_l);
-    p.part_o = reinterpret_cast<float*>(ws + L.part_o);
+    p.tickets = reinterpret_cast<int*>(ws + DEC8_TICKETS_AT);
+    p.part_m = reinterpret_cast<float*>(ws + DEC8_PARTS_AT);
+    p.part_l = p.part_m + DEC8_PARTS;
+    p.part_o = p.part_l + DEC8_PARTS;
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.n_rep = Hq / Hkv; p.max_pages = max_pages; p.max_seq_len = max_seq_len;
-    p.min_stages = min_tokens / DEC8_STAGE_TOKENS;
-    p.max_parts = L.max_parts;
+    p.min_stages = chunk_tokens > DEC8_STAGE_TOKENS ? (chunk_tokens + DEC8_STAGE_TOKENS - 1) / DEC8_STAGE_TOKENS : 1;
     p.rope_q = rope_q;
     p.scale_log2 = scale * LOG2E;
     if (rope_q) p.freqs = rotation_freqs(theta);
@@ -523,8 +525,9 @@ extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_
         configured_dev = dev;
     }
     // no more CTAs than ranges of the minimum length can exist
-    const long long max_ranges = (long long)B * Hkv * ((max_seq_len + (long long)min_tokens - 1) / min_tokens + 1);
-    const int grid = (int)(max_ranges < sm_count() ? (max_ranges > 0 ? max_ranges : 1) : sm_count());
+    const long long min_tokens = (long long)p.min_stages * DEC8_STAGE_TOKENS, ranges = (long long)B * Hkv * ((max_seq_len + min_tokens - 1) / min_tokens + 1);
+    const int most = sm_count() < DEC8_MAX_CTAS ? sm_count() : DEC8_MAX_CTAS, grid = (int)(ranges < most ? ranges : most);
+    p.most_heads = (int)(((int64_t)B * Hkv + grid - 1) / grid);
     launch_dependent(values == BN_KV8_E4M3 ? decode8_kernel<BN_KV8_E4M3> : decode8_kernel<BN_KV8_INT8>, (unsigned)grid, DEC8_THREADS, DEC8_SMEM_BYTES,
                      as_stream(stream), p);
     return launch_status(what);

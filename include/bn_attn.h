@@ -421,7 +421,8 @@ BN_API int bn_kv8_gather(const void* pool, int64_t pool_pages, const int32_t* pa
 
 /* bn_attn_decode_paged over the 8-bit cache: the same arguments and `values`.  q is rotated with angles in fp64.  A page number
  * outside the pool raises BN_ERR_INVALID_ARG in the scratch buffer's error word (bn_workspace_status); what is returned then
- * is of no use.  The scratch buffer is zero-filled once before its first use, and belongs to one call at a time. */
+ * is of no use.  chunk_tokens: 0 = default 256.  The scratch buffer (1.1 MB, whatever the sizes) is zero-filled once before its
+ * first use, and belongs to one call at a time; any calls may share it in turn. */
 BN_API size_t bn_attn_decode_kv8_workspace_bytes(int B, int Hq, int Hkv, int D, int max_seq_len, int chunk_tokens);
 BN_API int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_pages, const int32_t* page_table, int max_pages,
                               const int32_t* seq_lens, const int32_t* q_positions, void* out, float* out_f32, float* lse,
