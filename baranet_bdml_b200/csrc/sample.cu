@@ -11,11 +11,14 @@
 // computed in fp64 (2^f by a table of 32 and five terms of the exponential series, |error| < 3e-15) and summed as 64-bit whole numbers of
 // 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight above 0 counts at least one such unit.
 //
-// A cluster of CTAs per row, each with a part of the row in shared memory: read once, 4 bytes a token.  The last element that is kept is
-// found by a histogram of 1024 steps of the value below the maximum (counts for top-k, weights as three 16-bit limbs for top-p, whose
-// sums fit the 32-bit atomics that shared memory has), each CTA joining a part of the steps through distributed shared memory; the few
-// elements of the step that the border falls into are ranked among each other.  Where they are many (equal logits, far outliers), the step
-// is divided again by (value, index) until they are not.  Fp64 is only spent on what top-k has left.
+// A cluster of CTAs per row, each with a part of the row in shared memory (as integers in the values' order): read once.  The border of
+// top-k or top-p is found by a histogram of 512 steps of the value below the maximum (counts, or counts and weights as three 16-bit
+// limbs, whose sums fit the 32-bit atomics that shared memory has), which every CTA joins for itself through distributed shared memory.
+// Where no more than 512 tokens lie in the steps down to the border, all that is left is done with a list of them, in every CTA alike:
+// ranks, sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and the row is passed over once
+// more for the choice.  A step with too many (equal logits, far outliers) is divided again by (value, index) until it has not.  Fp64 is
+// only spent on what top-k has left.  What bounds it: a cluster's barriers, about 1 us each, of which there are three with a short list
+// and five without, and, for many rows, fp64 and the histogram's atomics.
 #include <math.h>
 
 #include "hybrid.cuh"
@@ -24,15 +27,13 @@ namespace bn {
 
 using namespace ptx;
 
-constexpr int SMP_THREADS = 1024;
+constexpr int SMP_THREADS = 512;
 constexpr int SMP_WARPS = SMP_THREADS / 32;
-constexpr int SMP_BINS = 1024;
+constexpr int SMP_BINS = SMP_THREADS;                 // a thread has one
+constexpr int SMP_LIST = SMP_THREADS;                 // elements that are ranked among each other, a thread each
 constexpr int SMP_CLUSTER = 8;                        // CTAs per row at most
-constexpr int SMP_LIST = 512;                         // elements that are ranked among each other
-constexpr int SMP_KEPT = 16384;                       // tokens per CTA whose weights fit into shared memory beside the logits
 constexpr int SMP_MOST = 49152;                       // tokens per CTA
-constexpr size_t SMP_MOST_SMEM = (size_t)SMP_KEPT * 12;
-static_assert(SMP_MOST_SMEM >= (size_t)SMP_MOST * 4, "either form of a part fits");
+constexpr size_t SMP_MOST_SMEM = (size_t)SMP_MOST * 4;
 constexpr int SMP_MOST_COLS = SMP_MOST * SMP_CLUSTER;
 
 struct SampleParams {
@@ -48,30 +49,34 @@ struct SampleParams {
 
 // 32 bits in the order of the values; NaN and -inf: 0, which nothing else is
 __device__ __forceinline__ uint32_t order_of(float v) {
-    const uint32_t b = __float_as_uint(v);
-    if (!(v > -INFINITY)) return 0u;
-    if (b == 0x80000000u) return 0x80000000u;             // -0 is 0
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    const uint32_t b = __float_as_uint(v + 0.f);          // (-0 is 0)
+    const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
+    return v > -INFINITY ? o : 0u;
 }
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
-__device__ __forceinline__ uint64_t key_of(float v, int i) { return (uint64_t)order_of(v) << 32 | (uint32_t)~i; }
 
 struct SampleShared {
     uint32_t hist[4][SMP_BINS];                        // counts, and the limbs of weights
-    uint64_t list_key[SMP_LIST], list_w[SMP_LIST];     // this CTA's elements of the step
+    uint64_t list_key[SMP_LIST], list_w[SMP_LIST];     // this CTA's elements
     uint64_t all_key[SMP_LIST], all_w[SMP_LIST];       // the cluster's
-    uint64_t from[2][SMP_CLUSTER][4];                  // what the CTAs tell each other
-    uint64_t red[2][2][SMP_WARPS];
+    uint64_t from[2][SMP_CLUSTER * SMP_WARPS][2];      // what all warps of the cluster tell each other
+    uint64_t warp_sum[2][SMP_WARPS];
+    uint32_t warp_cnt[2][SMP_WARPS];
+    struct { uint64_t above; uint32_t lane1, count, upto; } border[SMP_WARPS];
+    uint64_t kept_sum;
     double table[32];                                  // 2^(j / 32)
-    uint64_t found[3];
     int list_n;
 };
 
-template <typename T, bool KEEP> __global__ void __launch_bounds__(SMP_THREADS, 1) sample_rows_kernel(const SampleParams p) {
-    extern __shared__ __align__(16) uint8_t smem_raw[];
+__device__ __forceinline__ uint64_t warp_total(uint64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SampleParams p) {
+    extern __shared__ __align__(16) uint32_t so[];     // the part's orders
     __shared__ SampleShared sh;
-    float* sx = reinterpret_cast<float*>(smem_raw);
-    uint64_t* sw = reinterpret_cast<uint64_t*>(smem_raw + (size_t)p.slice * 4);      // KEEP: weights
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     uint32_t ncta;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ncta));
@@ -81,106 +86,106 @@ template <typename T, bool KEEP> __global__ void __launch_bounds__(SMP_THREADS, 
     grid_dependency_wait();
     grid_launch_dependents();
 
-    int turn = 0, rturn = 0;
-    // tells every CTA of the cluster up to three numbers; they are in sh.from[turn ^ 1] afterwards
-    auto tell = [&](uint64_t a, uint64_t b, uint64_t c) {
-        if (tid < C) {
-            const uint32_t at = in_rank(smem_u32(&sh.from[turn][rank][0]), tid);
+    // every warp of the cluster tells all CTAs two numbers; in sh.from[turn ^ 1] behind the barrier
+    int turn = 0, turn2 = 0;
+    auto tell = [&](uint64_t a, uint64_t b) {
+        if (lane < C) {
+            const uint32_t at = in_rank(smem_u32(&sh.from[turn][rank * SMP_WARPS + warp][0]), lane);
             st_cluster_u64(at, a);
             st_cluster_u64(at + 8, b);
-            st_cluster_u64(at + 16, c);
         }
         cluster_sync();
         turn ^= 1;
     };
-    // over the block, in every thread
-    auto block_max2 = [&](uint64_t& a, uint64_t& b) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-            b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-        }
-        if (lane == 0) { sh.red[rturn][0][warp] = a; sh.red[rturn][1][warp] = b; }
-        __syncthreads();
-        a = sh.red[rturn][0][lane];
-        b = sh.red[rturn][1][lane];
-        rturn ^= 1;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-            b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
-        }
-    };
-    // sum of what the lower threads have, and of all
-    auto block_scan = [&](uint64_t v, uint64_t& total) -> uint64_t {
+    // sums over the lower threads of the block, of a wide number and a narrow one, and over all
+    auto block_scan = [&](uint64_t v, uint32_t w, uint64_t& total, uint32_t& below_w) -> uint64_t {
         uint64_t run = v;
+        uint32_t runw = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t t = __shfl_up_sync(0xffffffffu, run, o);
-            if (lane >= o) run += t;
+            const uint32_t tw = __shfl_up_sync(0xffffffffu, runw, o);
+            if (lane >= o) { run += t; runw += tw; }
         }
-        if (lane == 31) sh.red[rturn][0][warp] = run;
+        if (lane == 31) { sh.warp_sum[turn2][warp] = run; sh.warp_cnt[turn2][warp] = runw; }
         __syncthreads();
-        uint64_t w = sh.red[rturn][0][lane];
-        rturn ^= 1;
+        uint64_t s = lane < SMP_WARPS ? sh.warp_sum[turn2][lane] : 0;
+        uint32_t sw = lane < SMP_WARPS ? sh.warp_cnt[turn2][lane] : 0;
+        turn2 ^= 1;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t t = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += t;
+        for (int o = 1; o < SMP_WARPS; o <<= 1) {
+            const uint64_t t = __shfl_up_sync(0xffffffffu, s, o);
+            const uint32_t tw = __shfl_up_sync(0xffffffffu, sw, o);
+            if (lane >= o) { s += t; sw += tw; }
         }
-        total = __shfl_sync(0xffffffffu, w, 31);
-        const uint64_t below = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+        total = __shfl_sync(0xffffffffu, s, SMP_WARPS - 1);
+        const uint64_t below = __shfl_sync(0xffffffffu, s, max(warp - 1, 0));
+        const uint32_t belowc = __shfl_sync(0xffffffffu, sw, max(warp - 1, 0));
+        below_w = runw - w + (warp ? belowc : 0);
         return run - v + (warp ? below : 0);
     };
 
     // ------------------------------------------------------------------ the row's part, its largest and its smallest element
-    uint64_t best = 0, least = 0;                      // least: of the complement of the order
+    uint32_t top = 0, top_at = 0xffffffffu, low = 0xffffffffu;
     {
         const T* x = static_cast<const T*>(p.x) + r * p.row_stride + first;
-        auto see = [&](float v, int i) {
-            const uint32_t o = order_of(v);
-            if (o) {
-                best = max(best, (uint64_t)o << 32 | (uint32_t)~(first + i));
-                least = max(least, (uint64_t)(uint32_t)~o);
-            }
+        auto see = [&](uint32_t o, int i) {
+            if (o > top) { top = o; top_at = first + i; }          // (a thread's indices ascend: the first of equals stays)
+            if (o) low = min(low, o);
         };
         const bool wide = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
         if (wide) {
+#pragma unroll 4
             for (int i = 4 * tid; i + 4 <= n; i += 4 * SMP_THREADS) {
                 float v[4];
                 load4(x + i, v);
-                *reinterpret_cast<float4*>(sx + i) = make_float4(v[0], v[1], v[2], v[3]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) see(v[e], i + e);
+                const uint4 o = make_uint4(order_of(v[0]), order_of(v[1]), order_of(v[2]), order_of(v[3]));
+                *reinterpret_cast<uint4*>(so + i) = o;
+                see(o.x, i); see(o.y, i + 1); see(o.z, i + 2); see(o.w, i + 3);
             }
         }
+#pragma unroll 4
         for (int i = (wide ? n / 4 * 4 : 0) + tid; i < n; i += SMP_THREADS) {
-            const float v = to_f(x[i]);
-            sx[i] = v;
-            see(v, i);
+            const uint32_t o = order_of(to_f(x[i]));
+            so[i] = o;
+            see(o, i);
         }
+        const uint32_t all = __reduce_max_sync(0xffffffffu, top);
+        top_at = __reduce_min_sync(0xffffffffu, top == all ? top_at : 0xffffffffu);
+        top = all;
+        low = __reduce_min_sync(0xffffffffu, low);
     }
-    block_max2(best, least);
-    tell(best, least, 0);
-    for (int c = 0; c < C; ++c) {
-        best = max(best, sh.from[turn ^ 1][c][0]);
-        least = max(least, sh.from[turn ^ 1][c][1]);
+    tell((uint64_t)top << 32 | top_at, low);
+    top = 0;
+    for (int i = lane; i < C * SMP_WARPS; i += 32) {
+        const uint64_t a = sh.from[turn ^ 1][i][0];
+        const uint32_t o = (uint32_t)(a >> 32);
+        if (o > top || (o == top && (uint32_t)a < top_at)) { top = o; top_at = (uint32_t)a; }
+        low = min(low, (uint32_t)sh.from[turn ^ 1][i][1]);
+    }
+    {
+        const uint32_t all = __reduce_max_sync(0xffffffffu, top);
+        top_at = __reduce_min_sync(0xffffffffu, top == all ? top_at : 0xffffffffu);
+        top = all;
+        low = __reduce_min_sync(0xffffffffu, low);
     }
     const float temp = p.temperature ? p.temperature[r] : p.temperature1;
-    if (best == 0 || !(temp > 0.f)) {
-        if (rank == 0 && tid == 0) p.out[r] = best == 0 ? 0 : (int)~(uint32_t)best;
+    const int top_k = p.top_k ? p.top_k[r] : p.top_k1;
+    if (top == 0 || !(temp > 0.f) || top_k == 1) {
+        if (rank == 0 && tid == 0) p.out[r] = top == 0 ? 0 : (int)top_at;
         return;                                        // (nothing reaches into another CTA behind the last barrier)
     }
-    const float peak = value_of((uint32_t)(best >> 32)), depth = peak - value_of(~(uint32_t)least);
+    const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
+    const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);
+    const float peak = value_of(top), depth = peak - value_of(low);
     const double per = 1.4426950408889634 / (double)temp;
     const int unit = p.unit_bits;
-    const int top_k = p.top_k ? p.top_k[r] : p.top_k1;
-    const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
+    const double floor_w = (double)min_p * (double)(1ull << unit);
 
     // 2^((v - peak) / T * log2 e + unit), whole and at least 1; 0 where fp64 has none
-    auto weigh = [&](float v) -> uint64_t {
-        if (v == peak) return 1ull << unit;
-        const double t = ((double)v - (double)peak) * per;
+    auto weigh = [&](uint32_t order) -> uint64_t {
+        if (order == top) return 1ull << unit;
+        const double t = ((double)value_of(order) - (double)peak) * per;
         if (!(t >= -1074.5)) return 0;
         if (t < -(double)(unit + 1)) return 1;
         const double rounded = t + 0x1.8p47;           // to a multiple of 1 / 32, which is the low word
@@ -195,39 +200,37 @@ template <typename T, bool KEEP> __global__ void __launch_bounds__(SMP_THREADS, 
         return max(m, (uint64_t)1);
     };
 
-    uint64_t last = 0;                                 // all with a key of at least this are kept
-    bool weighed = false;
-    auto key_at = [&](int i) { return key_of(sx[i], first + i); };
-    auto kept = [&](uint64_t key) { return key >> 32 != 0 && key >= last; };
-    auto weight_at = [&](int i) -> uint64_t { return KEEP && weighed ? sw[i] : weigh(sx[i]); };
-    // a warp has a run of its CTA's part, so that its sum is one of neighbours
-    const int run = (n + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n, begin + run);
+    // kept: above `last` in the order, or `last` itself
+    uint32_t last_order = 1, last_at = 0xffffffffu;
+    auto kept = [&](uint32_t o, int i) { return o > last_order || (o == last_order && (uint32_t)(first + i) <= last_at); };
+    auto key_of = [&](uint32_t o, int i) { return (uint64_t)o << 32 | (uint32_t)~(first + i); };
 
-    // `last` becomes the key of the last element before which there is less than `limit`
-    auto cut = [&](bool by_weight, double limit, float range) {
+    // The last element before which there is less than a limit: top_k by count, top_p times their sum by weight.  True: the choice has
+    // been made with the list.
+    auto cut = [&](bool by_weight, float range) -> bool {
         uint64_t above = 0, hi = 0, lo = 0;            // what lies above the step; the step as a range of keys, once it is one
-        int shift = -1, step = 0;
+        int shift = -1, step = 0, m = 0;
+        double limit = (double)top_k;
+        bool listed = false;
         const float scale = range > 0.f ? SMP_BINS / range : 0.f;
-        auto step_of = [&](uint64_t key, float v) -> int {
-            if (shift >= 0) return (int)((hi - key) >> shift);
-            return v == peak ? 0 : min(SMP_BINS - 1, __float2int_rd((peak - v) * scale));
+        auto in_range = [&](uint32_t o, int i) { return kept(o, i) && (shift < 0 || (key_of(o, i) <= hi && key_of(o, i) >= lo)); };
+        auto step_of = [&](uint32_t o, int i) -> int {
+            if (shift >= 0) return (int)((hi - key_of(o, i)) >> shift);
+            return o == top ? 0 : min(SMP_BINS - 1, __float2int_rd((peak - value_of(o)) * scale));
         };
-        auto in_range = [&](uint64_t key) { return kept(key) && (shift < 0 || (key <= hi && key >= lo)); };
-        uint64_t count = 0;
         for (;;) {
-            for (int i = tid; i < SMP_BINS; i += SMP_THREADS) {
-                sh.hist[0][i] = 0;
-                if (by_weight) sh.hist[1][i] = sh.hist[2][i] = sh.hist[3][i] = 0;
-            }
+            sh.hist[0][tid] = 0;
+            if (by_weight) sh.hist[1][tid] = sh.hist[2][tid] = sh.hist[3][tid] = 0;
             if (tid == 0) sh.list_n = 0;
             __syncthreads();
+#pragma unroll 4
             for (int i = tid; i < n; i += SMP_THREADS) {
-                const uint64_t key = key_at(i);
-                if (!in_range(key)) continue;
-                const int b = step_of(key, sx[i]);
+                const uint32_t o = so[i];
+                if (!in_range(o, i)) continue;
+                const int b = step_of(o, i);
                 atomicAdd(&sh.hist[0][b], 1u);
                 if (by_weight) {
-                    const uint64_t w = weight_at(i);
+                    const uint64_t w = weigh(o);
                     atomicAdd(&sh.hist[1][b], (uint32_t)w & 0xffffu);
                     if (w >> 16) {
                         atomicAdd(&sh.hist[2][b], (uint32_t)(w >> 16) & 0xffffu);
@@ -236,133 +239,162 @@ template <typename T, bool KEEP> __global__ void __launch_bounds__(SMP_THREADS, 
                 }
             }
             cluster_sync();
-            // a part of the steps for each CTA, a step a thread
-            const int steps = SMP_BINS / C;
-            uint64_t cnt = 0, sum = 0;
-            if (tid < steps) {
-                for (int c = 0; c < C; ++c) {
-                    const uint32_t at = in_rank(smem_u32(&sh.hist[0][rank * steps + tid]), c);
-                    cnt += ld_cluster_u32(at);
-                    if (by_weight)
-                        sum += ld_cluster_u32(at + SMP_BINS * 4) + ((uint64_t)ld_cluster_u32(at + SMP_BINS * 8) << 16) +
-                               ((uint64_t)ld_cluster_u32(at + SMP_BINS * 12) << 32);
-                }
-                if (!by_weight) sum = cnt;
+            uint32_t cnt = 0;
+            uint64_t sum = 0;
+#pragma unroll
+            for (int c = 0; c < SMP_CLUSTER; ++c) {
+                if (c >= C) break;
+                const uint32_t at = in_rank(smem_u32(&sh.hist[0][tid]), c);
+                cnt += ld_cluster_u32(at);
+                if (by_weight)
+                    sum += ld_cluster_u32(at + SMP_BINS * 4) + ((uint64_t)ld_cluster_u32(at + SMP_BINS * 8) << 16) +
+                           ((uint64_t)ld_cluster_u32(at + SMP_BINS * 12) << 32);
             }
-            uint64_t total, before = block_scan(sum, total);
-            tell(total, 0, 0);
-            for (int c = 0; c < rank; ++c) before += sh.from[turn ^ 1][c][0];
-            before += above;
-            // the last step of the part that has elements and less than the limit above it
-            uint64_t mine = tid < steps && cnt > 0 && (double)before < limit ? (uint64_t)(rank * steps + tid + 1) : 0, none = 0;
-            const uint64_t own = mine;
-            if (tid == 0) sh.found[1] = sh.found[2] = 0;
-            block_max2(mine, none);
-            if (mine != 0 && own == mine) { sh.found[1] = before; sh.found[2] = cnt; }
+            if (!by_weight) sum = cnt;
+            uint64_t total;
+            uint32_t upto;
+            const uint64_t before = block_scan(sum, cnt, total, upto) + above;
+            if (by_weight && shift < 0) limit = fmax((double)top_p * (double)total, 0.5);
+            // the last step that has elements and less than the limit above it
+            const uint32_t here = __ballot_sync(0xffffffffu, cnt > 0 && (double)before < limit);
+            if (lane == (here ? 31 - __clz(here) : 0)) {
+                sh.border[warp].above = before;
+                sh.border[warp].lane1 = here ? lane + 1 : 0;
+                sh.border[warp].count = cnt;
+                sh.border[warp].upto = upto + cnt;
+            }
             __syncthreads();
-            tell(mine, sh.found[1], sh.found[2]);
-            uint64_t at = 0;
-            for (int c = 0; c < C; ++c)
-                if (sh.from[turn ^ 1][c][0] > at) {
-                    at = sh.from[turn ^ 1][c][0];
-                    above = sh.from[turn ^ 1][c][1];
-                    count = sh.from[turn ^ 1][c][2];
-                }
-            step = (int)at - 1;
-            if (count <= SMP_LIST) break;
+            const uint32_t warps = __ballot_sync(0xffffffffu, lane < SMP_WARPS && sh.border[lane % SMP_WARPS].lane1 != 0);
+            const int w = 31 - __clz(warps);
+            above = sh.border[w].above;
+            step = w * 32 + sh.border[w].lane1 - 1;
+            m = sh.border[w].count;
+            if (shift < 0 && sh.border[w].upto <= SMP_LIST) { m = sh.border[w].upto; listed = true; }
+            if (m <= SMP_LIST) break;
             // too many to be ranked: the step's range of keys, to be divided
             if (shift < 0) {
-                uint64_t top = 0, bottom = 0;
+                uint64_t most = 0, least = 0;          // (least: of the complement)
                 for (int i = tid; i < n; i += SMP_THREADS) {
-                    const uint64_t key = key_at(i);
-                    if (in_range(key) && step_of(key, sx[i]) == step) { top = max(top, key); bottom = max(bottom, ~key); }
+                    const uint32_t o = so[i];
+                    if (in_range(o, i) && step_of(o, i) == step) { most = max(most, key_of(o, i)); least = max(least, ~key_of(o, i)); }
                 }
-                block_max2(top, bottom);
-                tell(top, bottom, 0);
-                for (int c = 0; c < C; ++c) {
-                    top = max(top, sh.from[turn ^ 1][c][0]);
-                    bottom = max(bottom, sh.from[turn ^ 1][c][1]);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                    least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
                 }
-                hi = top;
-                lo = ~bottom;
+                tell(most, least);
+                for (int i = 0; i < C * SMP_WARPS; ++i) {
+                    most = max(most, sh.from[turn ^ 1][i][0]);
+                    least = max(least, sh.from[turn ^ 1][i][1]);
+                }
+                hi = most;
+                lo = ~least;
             } else {
                 hi -= (uint64_t)step << shift;
                 lo = max(lo, hi - (((uint64_t)1 << shift) - 1));
+                cluster_sync();                        // the others have read this CTA's histogram
             }
-            shift = max(0, 64 - __clzll((long long)(hi - lo)) - 10);
+            shift = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
         }
-        // rank them among each other
+        // the list: the step's elements, or all down to it
+#pragma unroll 4
         for (int i = tid; i < n; i += SMP_THREADS) {
-            const uint64_t key = key_at(i);
-            if (!in_range(key) || step_of(key, sx[i]) != step) continue;
+            const uint32_t o = so[i];
+            if (!in_range(o, i)) continue;
+            const int b = step_of(o, i);
+            if (b > step || (b < step && !listed)) continue;
             const int at = atomicAdd(&sh.list_n, 1);
-            sh.list_key[at] = key;
-            sh.list_w[at] = by_weight ? weight_at(i) : 1;
+            sh.list_key[at] = key_of(o, i);
+            sh.list_w[at] = by_weight || listed ? weigh(o) : 1;
         }
         cluster_sync();
-        int m = 0;
-        for (int c = 0; c < C; ++c) {
-            const int here = (int)ld_cluster_u32(in_rank(smem_u32(&sh.list_n), c));
-            for (int i = tid; i < here; i += SMP_THREADS) {
-                sh.all_key[m + i] = ld_cluster_u64(in_rank(smem_u32(&sh.list_key[i]), c));
-                sh.all_w[m + i] = ld_cluster_u64(in_rank(smem_u32(&sh.list_w[i]), c));
+        {
+            // the thread's element of the cluster's list: which CTA's, and which there
+            uint32_t here = lane < C ? ld_cluster_u32(in_rank(smem_u32(&sh.list_n), min(lane, C - 1))) : 0;
+            int c = 0, at = tid;
+            for (int i = 0; i < C; ++i) {
+                const int k = (int)__shfl_sync(0xffffffffu, here, i);
+                if (c == i && at >= k) { at -= k; ++c; }
             }
-            m += here;
+            if (tid < m) {
+                sh.all_key[tid] = ld_cluster_u64(in_rank(smem_u32(&sh.list_key[at]), c));
+                sh.all_w[tid] = ld_cluster_u64(in_rank(smem_u32(&sh.list_w[at]), c));
+            }
         }
         __syncthreads();
-        uint64_t low = 0, none = 0;
-        if (tid < m) {
-            const uint64_t key = sh.all_key[tid];
-            uint64_t before = above;
-            for (int i = 0; i < m; ++i)
-                if (sh.all_key[i] > key) before += sh.all_w[i];
-            if ((double)before < limit) low = ~key;
+        int rank_of = 0;
+        const uint64_t key = tid < m ? sh.all_key[tid] : 0, weight = tid < m ? sh.all_w[tid] : 0;
+        if (warp * 32 < m) {
+#pragma unroll 4
+            for (int i = 0; i < m; ++i) rank_of += sh.all_key[i] > key;
         }
-        block_max2(low, none);
-        last = ~low;
+        // in order, where the histogram was
+        uint64_t* in_key = reinterpret_cast<uint64_t*>(sh.hist[0]);
+        uint64_t* in_w = in_key + SMP_LIST;
+        if (tid < m) { in_key[rank_of] = key; in_w[rank_of] = weight; }
+        __syncthreads();
+        const uint64_t w = tid < m ? in_w[tid] : 0;
+        uint64_t total;
+        uint32_t unused;
+        if (!listed) {
+            const uint64_t before = block_scan(w, 0, total, unused) + above;
+            const int stay = __syncthreads_count(tid < m && (double)before < limit);
+            const uint64_t k = in_key[stay - 1];
+            last_order = (uint32_t)(k >> 32);
+            last_at = ~(uint32_t)k;
+            cluster_sync();                            // the others have read this CTA's list (and histogram)
+            return false;
+        }
+        const int few = !by_weight && top_k < m ? top_k : m;
+        const uint64_t before = block_scan(tid < few ? w : 0, 0, total, unused);
+        if (!by_weight) limit = fmax((double)top_p * (double)total, 0.5);
+        const int stay = __syncthreads_count(tid < few && (tid == 0 || ((!(top_p < 1.f) || (double)before < limit) && !((double)w < floor_w))));
+        if (tid == stay - 1) sh.kept_sum = before + w;
+        __syncthreads();
+        const uint64_t all = sh.kept_sum, reach = min((uint64_t)(u * (double)all), all - 1);
+        if (rank == 0 && tid < stay) {
+            const uint32_t mine = (uint32_t)in_key[tid];       // (the complement of the index: larger is earlier)
+            uint64_t earlier = 0;
+#pragma unroll 4
+            for (int i = 0; i < stay; ++i) earlier += (uint32_t)in_key[i] > mine ? in_w[i] : 0;
+            if (earlier <= reach && reach < earlier + w) p.out[r] = (int)~mine;
+        }
+        return true;
     };
 
-    if (top_k > 0 && top_k < p.cols) cut(false, (double)top_k, fminf(depth, 128.f));
-    if (top_p < 1.f) {
-        uint64_t sum = 0, total;
-        for (int i = tid; i < n; i += SMP_THREADS) {
-            const uint64_t w = kept(key_at(i)) ? weigh(sx[i]) : 0;
-            if (KEEP) sw[i] = w;
-            sum += w;
-        }
-        weighed = true;                                // (read by other threads behind the barriers of the sums)
-        block_scan(sum, total);
-        tell(total, 0, 0);
-        total = 0;
-        for (int c = 0; c < C; ++c) total += sh.from[turn ^ 1][c][0];
-        cut(true, fmax((double)top_p * (double)total, 0.5), fminf(depth, 64.f * temp));
+    bool chosen = false;
+    if (top_k > 0 && top_k < p.cols) chosen = cut(false, fminf(depth, 128.f));
+    if (!chosen && top_p < 1.f) chosen = cut(true, fminf(depth, 64.f * temp));
+    if (chosen) {
+        cluster_sync();                                // the others have read this CTA's list
+        return;
     }
 
-    // ------------------------------------------------------------------------------------------------------------- the choice
-    const double floor_w = (double)min_p * (double)(1ull << unit);
+    // ------------------------------------------------------------------------------------------- the choice from the whole row
     auto counted = [&](int i) -> uint64_t {
-        const uint64_t key = key_at(i);
-        if (!kept(key)) return 0;
-        const uint64_t w = weight_at(i);
-        return (double)w < floor_w && key != best ? 0 : w;
+        const uint32_t o = so[i];
+        if (!kept(o, i)) return 0;
+        const uint64_t w = weigh(o);
+        return (double)w < floor_w && (uint32_t)(first + i) != top_at ? 0 : w;
     };
-    uint64_t mine = 0, total;
+    // a warp has a run of its CTA's part, so that its sum is one of neighbours
+    const int run = (n + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n, begin + run);
+    uint64_t mine = 0;
+#pragma unroll 4
     for (int i = begin + lane; i < end; i += 32) mine += counted(i);
-    uint64_t below = block_scan(mine, total);
-    tell(total, 0, 0);
-    uint64_t all = 0, before = 0;
-    for (int c = 0; c < C; ++c) {
-        if (c == rank) before = all;
-        all += sh.from[turn ^ 1][c][0];
+    mine = warp_total(mine);
+    tell(mine, 0);
+    uint64_t all = 0, below = 0;
+    for (int i = lane; i < C * SMP_WARPS; i += 32) {
+        const uint64_t v = sh.from[turn ^ 1][i][0];
+        all += v;
+        if (i < rank * SMP_WARPS + warp) below += v;
     }
-    const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);
+    all = warp_total(all);
+    below = warp_total(below);
     const uint64_t reach = min((uint64_t)(u * (double)all), all - 1);
-    // sums before the warp and up to its end
-    below = __shfl_sync(0xffffffffu, below, 0) + before;
-    uint64_t own = mine;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) own += __shfl_xor_sync(0xffffffffu, own, o);
-    if (reach < below || reach >= below + own) return;
+    if (reach < below || reach >= below + mine) return;
     for (int i = begin + lane; i - lane < end; i += 32) {
         uint64_t sum = i < end ? counted(i) : 0;
 #pragma unroll
@@ -406,12 +438,10 @@ extern "C" int bn_sample_rows(const void* logits, int64_t row_stride, int dtype,
     while ((1ll << (62 - p.unit_bits)) < cols) --p.unit_bits;
     // as many CTAs for a row as there are SMs for, but no fewer than its tokens need, and parts of 1024 tokens at least
     int c = 1;
-    while (c < SMP_CLUSTER && (cols > c * SMP_KEPT || ((int64_t)rows * 2 * c <= sm_count() && cols > c * 1024))) c *= 2;
+    while (c < SMP_CLUSTER && (cols > c * SMP_MOST || ((int64_t)rows * 2 * c <= sm_count() && cols > c * 1024))) c *= 2;
     p.slice = ((cols + c - 1) / c + 3) / 4 * 4;
-    const bool keep = p.slice <= SMP_KEPT;
-    const size_t smem = (size_t)p.slice * (keep ? 12 : 4);
-    auto* kernel = dtype == 0 ? (keep ? sample_rows_kernel<float, true> : sample_rows_kernel<float, false>)
-                              : (keep ? sample_rows_kernel<__nv_bfloat16, true> : sample_rows_kernel<__nv_bfloat16, false>);
+    const size_t smem = (size_t)p.slice * 4;
+    auto* kernel = dtype == 0 ? sample_rows_kernel<float> : sample_rows_kernel<__nv_bfloat16>;
     if (int rc = allow_smem(kernel, smem, what, SMP_MOST_SMEM, sizeof(SampleShared))) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * c));
