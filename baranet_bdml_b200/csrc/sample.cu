@@ -8,7 +8,7 @@
 // What is kept is always a prefix of the order, so that it is named by its last element.
 //
 // Sums decide which side of a border a token falls on, so they have to come out the same however the row is divided: weights are
-// computed in fp64 (2^f by a table of 32 and five terms of the exponential series, |error| < 3e-15) and summed as 64-bit whole numbers of
+// computed in fp64 (2^f for |f| <= 1/2 by twelve terms of the exponential series, whose rest is below 2e-16) and summed as 64-bit whole numbers of
 // 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight above 0 counts at least one such unit.
 //
 // A cluster of CTAs per row, each with a part of the row in shared memory (as integers in the values' order): read once.  The border of
@@ -33,6 +33,7 @@ constexpr int SMP_BINS = SMP_THREADS;                 // a thread has one
 constexpr int SMP_LIST = SMP_THREADS;                 // elements that are ranked among each other, a thread each
 constexpr int SMP_CLUSTER = 8;                        // CTAs per row at most
 constexpr int SMP_MOST = 49152;                       // tokens per CTA
+constexpr int SMP_TWO = 20480;                        // tokens per CTA of which an SM takes two
 constexpr size_t SMP_MOST_SMEM = (size_t)SMP_MOST * 4;
 constexpr int SMP_MOST_COLS = SMP_MOST * SMP_CLUSTER;
 
@@ -57,14 +58,14 @@ __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_flo
 
 struct SampleShared {
     uint32_t hist[4][SMP_BINS];                        // counts, and the limbs of weights
-    uint64_t list_key[SMP_LIST], list_w[SMP_LIST];     // this CTA's elements
+    uint64_t list_key[SMP_LIST];                       // this CTA's elements
     uint64_t all_key[SMP_LIST], all_w[SMP_LIST];       // the cluster's
     uint64_t from[2][SMP_CLUSTER * SMP_WARPS][2];      // what all warps of the cluster tell each other
     uint64_t warp_sum[2][SMP_WARPS];
     uint32_t warp_cnt[2][SMP_WARPS];
     struct { uint64_t above; uint32_t lane1, count, upto; } border[SMP_WARPS];
     uint64_t kept_sum;
-    double table[32];                                  // 2^(j / 32)
+    uint32_t rank[SMP_LIST];
     int list_n;
 };
 
@@ -81,21 +82,24 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
     uint32_t ncta;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ncta));
     const int C = (int)ncta, rank = (int)cluster_rank(), r = blockIdx.x / C;
-    const int first = rank * p.slice, n = max(0, min(p.slice, p.cols - first));
-    if (tid < 32) sh.table[tid] = exp2(tid / 32.0);
+    const int first = rank * p.slice, n = max(0, min(p.slice, p.cols - first)), n4 = (n + 3) / 4;
     grid_dependency_wait();
     grid_launch_dependents();
 
     // every warp of the cluster tells all CTAs two numbers; in sh.from[turn ^ 1] behind the barrier
     int turn = 0, turn2 = 0;
-    auto tell = [&](uint64_t a, uint64_t b) {
+    auto cluster_arrive_tell = [&](uint64_t a, uint64_t b) {
         if (lane < C) {
             const uint32_t at = in_rank(smem_u32(&sh.from[turn][rank * SMP_WARPS + warp][0]), lane);
             st_cluster_u64(at, a);
             st_cluster_u64(at + 8, b);
         }
-        cluster_sync();
+        cluster_arrive();
         turn ^= 1;
+    };
+    auto tell = [&](uint64_t a, uint64_t b) {
+        cluster_arrive_tell(a, b);
+        cluster_wait();
     };
     // sums over the lower threads of the block, of a wide number and a narrow one, and over all
     auto block_scan = [&](uint64_t v, uint32_t w, uint64_t& total, uint32_t& below_w) -> uint64_t {
@@ -133,6 +137,7 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             if (o > top) { top = o; top_at = first + i; }          // (a thread's indices ascend: the first of equals stays)
             if (o) low = min(low, o);
         };
+        if (tid < n4 * 4 - n) so[n + tid] = 0;         // (behind the last one: whole pieces of four)
         const bool wide = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
         if (wide) {
 #pragma unroll 4
@@ -155,7 +160,19 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         top = all;
         low = __reduce_min_sync(0xffffffffu, low);
     }
-    tell((uint64_t)top << 32 | top_at, low);
+    // (what the row's numbers alone say is worked out while the barrier is waited for)
+    cluster_arrive_tell((uint64_t)top << 32 | top_at, low);
+    const float temp = p.temperature ? p.temperature[r] : p.temperature1;
+    const int top_k = p.top_k ? p.top_k[r] : p.top_k1;
+    const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
+    const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);
+    const double per = 1.4426950408889634 / (double)temp;
+    const int unit = p.unit_bits;
+    const double floor_w = (min_p > 1.f ? 1.0 : (double)min_p) * (double)(1ull << unit);
+    // Further below the maximum than `deep` the weights of all the row's tokens together are less than 1 - top_p of the largest: the
+    // border of top-p lies above
+    const float deep = temp * (logf((float)p.cols) - logf(1.f - top_p) + 1.f);
+    cluster_wait();
     top = 0;
     for (int i = lane; i < C * SMP_WARPS; i += 32) {
         const uint64_t a = sh.from[turn ^ 1][i][0];
@@ -169,35 +186,36 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         top = all;
         low = __reduce_min_sync(0xffffffffu, low);
     }
-    const float temp = p.temperature ? p.temperature[r] : p.temperature1;
-    const int top_k = p.top_k ? p.top_k[r] : p.top_k1;
     if (top == 0 || !(temp > 0.f) || top_k == 1) {
         if (rank == 0 && tid == 0) p.out[r] = top == 0 ? 0 : (int)top_at;
         return;                                        // (nothing reaches into another CTA behind the last barrier)
     }
-    const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
-    const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);
     const float peak = value_of(top), depth = peak - value_of(low);
-    const double per = 1.4426950408889634 / (double)temp;
-    const int unit = p.unit_bits;
-    const double floor_w = (double)min_p * (double)(1ull << unit);
 
-    // 2^((v - peak) / T * log2 e + unit), whole and at least 1; 0 where fp64 has none
+    // 2^((v - peak) / T * log2 e + unit), whole and at least 1; 0 where fp64 has none.  No branches: a warp weighs different values, and
+    // a thread's four at a time are worked out side by side
     auto weigh = [&](uint32_t order) -> uint64_t {
-        if (order == top) return 1ull << unit;
         const double t = ((double)value_of(order) - (double)peak) * per;
-        if (!(t >= -1074.5)) return 0;
-        if (t < -(double)(unit + 1)) return 1;
-        const double rounded = t + 0x1.8p47;           // to a multiple of 1 / 32, which is the low word
-        const int k = __double2loint(rounded);
-        const double f = t - (rounded - 0x1.8p47);
+        const double near = fmax(t, -(double)(unit + 1));          // (a NaN, infinity less infinity, comes out as the bound)
+        const double rounded = near + 0x1.8p52;                    // to a whole number, which is the low word
+        const double f = near - (rounded - 0x1.8p52);
         // (ln 2)^i / i!
-        double w = fma(f, fma(f, fma(f, fma(f, fma(f, 1.3333558146428443e-3, 9.6181291076284772e-3), 5.5504108664821580e-2), 0.24022650695910072),
-                              0.69314718055994531), 1.0);
-        w *= sh.table[k & 31];
-        w = __hiloint2double(__double2hiint(w) + (((k >> 5) + unit) << 20), __double2loint(w));
-        const uint64_t m = (uint64_t)__double_as_longlong(w + 0x1p52) - 0x4330000000000000ull;
-        return max(m, (uint64_t)1);
+        double w = 2.5678435993488196e-11;
+        w = fma(w, f, 4.4455382718708101e-10);
+        w = fma(w, f, 7.0549116208011209e-09);
+        w = fma(w, f, 1.0178086009239696e-07);
+        w = fma(w, f, 1.3215486790144305e-06);
+        w = fma(w, f, 1.5252733804059838e-05);
+        w = fma(w, f, 1.5403530393381606e-04);
+        w = fma(w, f, 1.3333558146428441e-03);
+        w = fma(w, f, 9.6181291076284769e-03);
+        w = fma(w, f, 5.5504108664821576e-02);
+        w = fma(w, f, 2.4022650695910069e-01);
+        w = fma(w, f, 6.9314718055994529e-01);
+        w = fma(w, f, 1.0);
+        w = __hiloint2double(__double2hiint(w) + ((__double2loint(rounded) + unit) << 20), __double2loint(w));
+        const uint64_t m = max((uint64_t)(__double_as_longlong(w + 0x1p52) - 0x4330000000000000ll), (uint64_t)1);
+        return order == top ? 1ull << unit : t >= -1074.5 ? m : 0;
     };
 
     // kept: above `last` in the order, or `last` itself
@@ -212,31 +230,52 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         int shift = -1, step = 0, m = 0;
         double limit = (double)top_k;
         bool listed = false;
+        // (an order below that of the rounded edge is below the edge itself)
+        const uint32_t deep_order = by_weight && range < depth ? order_of(peak - range) : 0;
         const float scale = range > 0.f ? SMP_BINS / range : 0.f;
         auto in_range = [&](uint32_t o, int i) { return kept(o, i) && (shift < 0 || (key_of(o, i) <= hi && key_of(o, i) >= lo)); };
-        auto step_of = [&](uint32_t o, int i) -> int {
-            if (shift >= 0) return (int)((hi - key_of(o, i)) >> shift);
-            return o == top ? 0 : min(SMP_BINS - 1, __float2int_rd((peak - value_of(o)) * scale));
+        // (the rounding is to the nearest step: any will do that never puts the larger value behind the smaller)
+        auto step_of_order = [&](uint32_t o) -> int {
+            return o == top ? 0 : (int)(__float_as_uint(fminf((peak - value_of(o)) * scale, SMP_BINS - 1.f) + 8388608.f) & (SMP_BINS - 1));
         };
+        auto step_of = [&](uint32_t o, int i) -> int { return shift >= 0 ? (int)((hi - key_of(o, i)) >> shift) : step_of_order(o); };
         for (;;) {
             sh.hist[0][tid] = 0;
             if (by_weight) sh.hist[1][tid] = sh.hist[2][tid] = sh.hist[3][tid] = 0;
             if (tid == 0) sh.list_n = 0;
             __syncthreads();
-#pragma unroll 4
-            for (int i = tid; i < n; i += SMP_THREADS) {
-                const uint32_t o = so[i];
-                if (!in_range(o, i)) continue;
-                const int b = step_of(o, i);
-                atomicAdd(&sh.hist[0][b], 1u);
+            uint64_t rest = 0;
+            for (int q = tid; q < n4; q += SMP_THREADS) {
+                const uint4 four = *reinterpret_cast<const uint4*>(so + 4 * q);
+                const uint32_t os[4] = {four.x, four.y, four.z, four.w};
+                uint64_t ws[4];
                 if (by_weight) {
-                    const uint64_t w = weigh(o);
-                    atomicAdd(&sh.hist[1][b], (uint32_t)w & 0xffffu);
-                    if (w >> 16) {
-                        atomicAdd(&sh.hist[2][b], (uint32_t)(w >> 16) & 0xffffu);
-                        if (w >> 32) atomicAdd(&sh.hist[3][b], (uint32_t)(w >> 32));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint64_t w = weigh(os[e]);
+                        ws[e] = in_range(os[e], 4 * q + e) ? w : 0;
+                        rest += os[e] < deep_order ? ws[e] : 0;
                     }
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t o = os[e];
+                    if (o < deep_order || !in_range(o, 4 * q + e)) continue;
+                    const int b = step_of(o, 4 * q + e);
+                    atomicAdd(&sh.hist[0][b], 1u);
+                    if (by_weight) {
+                        const uint64_t w = ws[e];
+                        atomicAdd(&sh.hist[1][b], (uint32_t)w & 0xffffu);
+                        if (w >> 16) {
+                            atomicAdd(&sh.hist[2][b], (uint32_t)(w >> 16) & 0xffffu);
+                            if (w >> 32) atomicAdd(&sh.hist[3][b], (uint32_t)(w >> 32));
+                        }
+                    }
+                }
+            }
+            if (by_weight && deep_order > 1) {         // what lies deep counts in the sum alone
+                rest = warp_total(rest);
+                if (lane < 3) atomicAdd(&sh.hist[lane + 1][SMP_BINS - 1], lane == 0 ? (uint32_t)rest & 0xffffu : lane == 1 ? (uint32_t)(rest >> 16) & 0xffffu : (uint32_t)(rest >> 32));
             }
             cluster_sync();
             uint32_t cnt = 0;
@@ -298,15 +337,17 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             shift = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
         }
         // the list: the step's elements, or all down to it
-#pragma unroll 4
-        for (int i = tid; i < n; i += SMP_THREADS) {
-            const uint32_t o = so[i];
-            if (!in_range(o, i)) continue;
-            const int b = step_of(o, i);
-            if (b > step || (b < step && !listed)) continue;
-            const int at = atomicAdd(&sh.list_n, 1);
-            sh.list_key[at] = key_of(o, i);
-            sh.list_w[at] = by_weight || listed ? weigh(o) : 1;
+        for (int q = tid; q < n4; q += SMP_THREADS) {
+            const uint4 four = *reinterpret_cast<const uint4*>(so + 4 * q);
+            const uint32_t os[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (os[e] < deep_order || !in_range(os[e], 4 * q + e)) continue;
+                const int b = step_of(os[e], 4 * q + e);
+                if (b > step || (b < step && !listed)) continue;
+                const int at = min(atomicAdd(&sh.list_n, 1), SMP_LIST - 1);      // (m of them in the whole cluster)
+                sh.list_key[at] = key_of(os[e], 4 * q + e);
+            }
         }
         cluster_sync();
         {
@@ -317,18 +358,28 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
                 const int k = (int)__shfl_sync(0xffffffffu, here, i);
                 if (c == i && at >= k) { at -= k; ++c; }
             }
-            if (tid < m) {
-                sh.all_key[tid] = ld_cluster_u64(in_rank(smem_u32(&sh.list_key[at]), c));
-                sh.all_w[tid] = ld_cluster_u64(in_rank(smem_u32(&sh.list_w[at]), c));
-            }
+            if (tid < m) sh.all_key[tid] = ld_cluster_u64(in_rank(smem_u32(&sh.list_key[at]), c));
         }
         __syncthreads();
-        int rank_of = 0;
-        const uint64_t key = tid < m ? sh.all_key[tid] : 0, weight = tid < m ? sh.all_w[tid] : 0;
-        if (warp * 32 < m) {
+        // how many of m keys are larger than the thread's: all threads share the comparisons
+        auto rank_among = [&](const auto* keys, int m) -> int {
+            sh.rank[tid] = 0;
+            __syncthreads();
+            const int wide = (m + 31) / 32 * 32, shares = SMP_THREADS / wide, share = tid / wide, t = tid % wide;
+            if (share < shares && t < m) {
+                const int end = m * (share + 1) / shares;
+                const auto mine = keys[t];
+                uint32_t larger = 0;
 #pragma unroll 4
-            for (int i = 0; i < m; ++i) rank_of += sh.all_key[i] > key;
-        }
+                for (int i = m * share / shares; i < end; ++i) larger += keys[i] > mine;
+                atomicAdd(&sh.rank[t], larger);
+            }
+            __syncthreads();
+            return (int)sh.rank[tid];
+        };
+        const uint64_t key = tid < m ? sh.all_key[tid] : 0;
+        const uint64_t weight = tid >= m ? 0 : by_weight || listed ? weigh((uint32_t)(key >> 32)) : 1;
+        const int rank_of = rank_among(sh.all_key, m);
         // in order, where the histogram was
         uint64_t* in_key = reinterpret_cast<uint64_t*>(sh.hist[0]);
         uint64_t* in_w = in_key + SMP_LIST;
@@ -353,36 +404,77 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         if (tid == stay - 1) sh.kept_sum = before + w;
         __syncthreads();
         const uint64_t all = sh.kept_sum, reach = min((uint64_t)(u * (double)all), all - 1);
-        if (rank == 0 && tid < stay) {
-            const uint32_t mine = (uint32_t)in_key[tid];       // (the complement of the index: larger is earlier)
-            uint64_t earlier = 0;
-#pragma unroll 4
-            for (int i = 0; i < stay; ++i) earlier += (uint32_t)in_key[i] > mine ? in_w[i] : 0;
-            if (earlier <= reach && reach < earlier + w) p.out[r] = (int)~mine;
+        // in the order of the index (whose complement the key has), for the sums up to each
+        uint32_t* index = reinterpret_cast<uint32_t*>(sh.all_w);
+        uint64_t* by_index = sh.all_key;
+        if (tid < stay) index[tid] = (uint32_t)in_key[tid];
+        const int place = rank_among(index, stay);
+        const uint32_t mine = tid < stay ? index[tid] : 0;
+        __syncthreads();
+        if (tid < stay) {
+            by_index[place] = w;
+            index[place] = mine;
         }
+        __syncthreads();
+        const uint64_t w2 = tid < stay ? by_index[tid] : 0, earlier = block_scan(w2, 0, total, unused);
+        if (rank == 0 && tid < stay && earlier <= reach && reach < earlier + w2) p.out[r] = (int)~index[tid];
         return true;
     };
 
     bool chosen = false;
     if (top_k > 0 && top_k < p.cols) chosen = cut(false, fminf(depth, 128.f));
-    if (!chosen && top_p < 1.f) chosen = cut(true, fminf(depth, 64.f * temp));
+    if (!chosen && top_p < 1.f) chosen = cut(true, fminf(depth, deep));
     if (chosen) {
         cluster_sync();                                // the others have read this CTA's list
         return;
     }
 
     // ------------------------------------------------------------------------------------------- the choice from the whole row
-    auto counted = [&](int i) -> uint64_t {
-        const uint32_t o = so[i];
+    auto counted = [&](uint32_t o, int i) -> uint64_t {
         if (!kept(o, i)) return 0;
         const uint64_t w = weigh(o);
         return (double)w < floor_w && (uint32_t)(first + i) != top_at ? 0 : w;
     };
     // a warp has a run of its CTA's part, so that its sum is one of neighbours
-    const int run = (n + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n, begin + run);
+    const int run = (n4 + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n4, begin + run);      // in pieces of four
     uint64_t mine = 0;
-#pragma unroll 4
-    for (int i = begin + lane; i < end; i += 32) mine += counted(i);
+    if (last_order == 1) {
+        for (int q = begin + lane; q < end; q += 32) {
+            const uint4 four = *reinterpret_cast<const uint4*>(so + 4 * q);
+            mine += counted(four.x, 4 * q) + counted(four.y, 4 * q + 1) + counted(four.z, 4 * q + 2) + counted(four.w, 4 * q + 3);
+        }
+    } else {
+        // few are kept: they are put side by side, so that 32 at a time are weighed
+        uint32_t* queue = sh.hist[0] + warp * 64;
+        int held = 0;
+        auto weigh_queued = [&](int k) {               // the top's weight is above any floor
+            const uint64_t w = lane < k ? weigh(queue[lane]) : 0;
+            if (lane < k && (!((double)w < floor_w))) mine += w;
+            __syncwarp();
+        };
+        for (int q = begin; q < end; q += 32) {
+            const uint4 four = q + lane < end ? *reinterpret_cast<const uint4*>(so + 4 * (q + lane)) : make_uint4(0u, 0u, 0u, 0u);
+            if (!__any_sync(0xffffffffu, max(max(four.x, four.y), max(four.z, four.w)) >= last_order)) continue;
+            const uint32_t os[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const bool in = kept(os[e], 4 * (q + lane) + e);
+                const uint32_t who = __ballot_sync(0xffffffffu, in);
+                if (in) queue[held + __popc(who & ((1u << lane) - 1))] = os[e];
+                held += __popc(who);
+                __syncwarp();
+                if (held >= 32) {
+                    weigh_queued(32);
+                    held -= 32;
+                    const uint32_t o = lane < held ? queue[32 + lane] : 0;
+                    __syncwarp();
+                    if (lane < held) queue[lane] = o;
+                    __syncwarp();
+                }
+            }
+        }
+        weigh_queued(held);
+    }
     mine = warp_total(mine);
     tell(mine, 0);
     uint64_t all = 0, below = 0;
@@ -395,8 +487,11 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
     below = warp_total(below);
     const uint64_t reach = min((uint64_t)(u * (double)all), all - 1);
     if (reach < below || reach >= below + mine) return;
-    for (int i = begin + lane; i - lane < end; i += 32) {
-        uint64_t sum = i < end ? counted(i) : 0;
+    for (int q = begin + lane; q - lane < end; q += 32) {
+        const uint4 four = q < end ? *reinterpret_cast<const uint4*>(so + 4 * q) : make_uint4(0u, 0u, 0u, 0u);
+        const uint64_t w[4] = {counted(four.x, 4 * q), counted(four.y, 4 * q + 1), counted(four.z, 4 * q + 2), counted(four.w, 4 * q + 3)};
+        uint64_t sum = w[0] + w[1] + w[2] + w[3];
+        const uint64_t own = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t t = __shfl_up_sync(0xffffffffu, sum, o);
@@ -404,7 +499,12 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         }
         const uint32_t over = __ballot_sync(0xffffffffu, below + sum > reach);
         if (over) {
-            if (lane == __ffs(over) - 1) p.out[r] = first + i;
+            if (lane == __ffs(over) - 1) {
+                below += sum - own;
+                int e = 0;
+                while (e < 3 && below + w[e] <= reach) below += w[e++];
+                p.out[r] = first + 4 * q + e;
+            }
             return;
         }
         below += __shfl_sync(0xffffffffu, sum, 31);
@@ -438,7 +538,7 @@ extern "C" int bn_sample_rows(const void* logits, int64_t row_stride, int dtype,
     while ((1ll << (62 - p.unit_bits)) < cols) --p.unit_bits;
     // as many CTAs for a row as there are SMs for, but no fewer than its tokens need, and parts of 1024 tokens at least
     int c = 1;
-    while (c < SMP_CLUSTER && (cols > c * SMP_MOST || ((int64_t)rows * 2 * c <= sm_count() && cols > c * 1024))) c *= 2;
+    while (c < SMP_CLUSTER && (cols > c * SMP_MOST || (rows > 8 && cols > c * SMP_TWO) || ((int64_t)rows * 2 * c <= sm_count() && cols > c * 1024))) c *= 2;
     p.slice = ((cols + c - 1) / c + 3) / 4 * 4;
     const size_t smem = (size_t)p.slice * 4;
     auto* kernel = dtype == 0 ? sample_rows_kernel<float> : sample_rows_kernel<__nv_bfloat16>;
