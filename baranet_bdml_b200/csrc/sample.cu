@@ -8,17 +8,22 @@
 // What is kept is always a prefix of the order, so that it is named by its last element.
 //
 // Sums decide which side of a border a token falls on, so they have to come out the same however the row is divided: weights are
-// computed in fp64 (2^f for |f| <= 1/2 by twelve terms of the exponential series, whose rest is below 2e-16) and summed as 64-bit whole numbers of
-// 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight above 0 counts at least one such unit.
+// computed in fp64 (2^f for |f| <= 1/2 by twelve terms of the exponential series, whose rest is below 2e-16) and summed as 64-bit whole
+// numbers of 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight above 0 counts at least
+// one such unit.
 //
-// A cluster of CTAs per row, each with a part of the row in shared memory (as integers in the values' order): read once.  The border of
-// top-k or top-p is found by a histogram of 512 steps of the value below the maximum (counts, or counts and weights as three 16-bit
-// limbs, whose sums fit the 32-bit atomics that shared memory has), which every CTA joins for itself through distributed shared memory.
+// A cluster of CTAs per row, each with a part of the row in shared memory: read once.  The border of top-k is found by a histogram of
+// counts over 512 steps of the value below the maximum, which every CTA joins for itself through distributed shared memory.  For top-p the
+// same counts, with the largest and the smallest weight of each step, tell between which two steps the border must lie.  Every token is
+// then weighed once: those above and below only go into sums (exact in fp64, whole numbers below 2^53), those between into a second
+// histogram, of weights as three 16-bit limbs (whose sums fit the 32-bit atomics that shared memory has; 64-bit ones take 50 times as
+// long), and the places of all that may be kept are put side by side for the choice.
 // Where no more than 512 tokens lie in the steps down to the border, all that is left is done with a list of them, in every CTA alike:
-// ranks, sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and the row is passed over once
-// more for the choice.  A step with too many (equal logits, far outliers) is divided again by (value, index) until it has not.  Fp64 is
-// only spent on what top-k has left.  What bounds it: a cluster's barriers, about 1 us each, of which there are three with a short list
-// and five without, and, for many rows, fp64 and the histogram's atomics.
+// ranks, sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and what is kept is passed over once
+// more for the choice.  A step with too many (equal logits, far outliers) is divided again by (value, index) until it has not.
+// A batch pays for the instructions per token (256 rows of 32000: 270 of them and every weight through the histogram 107 us, and with the
+// tokens that could not matter by a bound on their number alone left out 155), few rows for barriers of the cluster, about 1 us each:
+// three with a short list, six without.
 #include <math.h>
 
 #include "hybrid.cuh"
@@ -32,9 +37,9 @@ constexpr int SMP_WARPS = SMP_THREADS / 32;
 constexpr int SMP_BINS = SMP_THREADS;                 // a thread has one
 constexpr int SMP_LIST = SMP_THREADS;                 // elements that are ranked among each other, a thread each
 constexpr int SMP_CLUSTER = 8;                        // CTAs per row at most
-constexpr int SMP_MOST = 49152;                       // tokens per CTA
-constexpr int SMP_TWO = 20480;                        // tokens per CTA of which an SM takes two
-constexpr size_t SMP_MOST_SMEM = (size_t)SMP_MOST * 4;
+constexpr int SMP_MOST = 32768;                       // tokens per CTA: 5 bytes of shared memory each
+constexpr int SMP_TWO = 16384;                        // tokens per CTA of which an SM takes two
+constexpr size_t SMP_MOST_SMEM = (size_t)SMP_MOST * 5;
 constexpr int SMP_MOST_COLS = SMP_MOST * SMP_CLUSTER;
 
 struct SampleParams {
@@ -48,11 +53,12 @@ struct SampleParams {
     int cols, slice, unit_bits;                        // slice: tokens per CTA, a multiple of 4
 };
 
-// 32 bits in the order of the values; NaN and -inf: 0, which nothing else is
+// a logit as it is kept: NaN is -inf, -0 is 0
+__device__ __forceinline__ float plain_logit(float v) { return v > -INFINITY ? v + 0.f : -INFINITY; }
+// 32 bits in the order of the values, and back
 __device__ __forceinline__ uint32_t order_of(float v) {
-    const uint32_t b = __float_as_uint(v + 0.f);          // (-0 is 0)
-    const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-    return v > -INFINITY ? o : 0u;
+    const uint32_t b = __float_as_uint(v);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_float(order & 0x80000000u ? order & 0x7fffffffu : ~order); }
 
@@ -64,6 +70,8 @@ struct SampleShared {
     uint64_t warp_sum[2][SMP_WARPS];
     uint32_t warp_cnt[2][SMP_WARPS];
     struct { uint64_t above; uint32_t lane1, count, upto; } border[SMP_WARPS];
+    struct { uint32_t lane1, lane2, upto; } between[SMP_WARPS];
+    uint64_t sums[SMP_WARPS][2];
     uint64_t kept_sum;
     uint32_t rank[SMP_LIST];
     int list_n;
@@ -76,19 +84,22 @@ __device__ __forceinline__ uint64_t warp_total(uint64_t v) {
 }
 
 template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SampleParams p) {
-    extern __shared__ __align__(16) uint32_t so[];     // the part's orders
+    extern __shared__ __align__(16) float sx[];        // the part's logits, and 16-bit places of up to half of them
     __shared__ SampleShared sh;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     uint32_t ncta;
     asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(ncta));
     const int C = (int)ncta, rank = (int)cluster_rank(), r = blockIdx.x / C;
     const int first = rank * p.slice, n = max(0, min(p.slice, p.cols - first)), n4 = (n + 3) / 4;
+    // a warp has a run of the part, so that its sum is one of neighbours; in pieces of four
+    const int run = (n4 + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n4, begin + run);
+    uint16_t* places = reinterpret_cast<uint16_t*>(sx + p.slice) + 2 * begin;      // of the warp's run, from its start
     grid_dependency_wait();
     grid_launch_dependents();
 
     // every warp of the cluster tells all CTAs two numbers; in sh.from[turn ^ 1] behind the barrier
     int turn = 0, turn2 = 0;
-    auto cluster_arrive_tell = [&](uint64_t a, uint64_t b) {
+    auto tell_and_go_on = [&](uint64_t a, uint64_t b) {
         if (lane < C) {
             const uint32_t at = in_rank(smem_u32(&sh.from[turn][rank * SMP_WARPS + warp][0]), lane);
             st_cluster_u64(at, a);
@@ -98,20 +109,20 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         turn ^= 1;
     };
     auto tell = [&](uint64_t a, uint64_t b) {
-        cluster_arrive_tell(a, b);
+        tell_and_go_on(a, b);
         cluster_wait();
     };
     // sums over the lower threads of the block, of a wide number and a narrow one, and over all
     auto block_scan = [&](uint64_t v, uint32_t w, uint64_t& total, uint32_t& below_w) -> uint64_t {
-        uint64_t run = v;
-        uint32_t runw = w;
+        uint64_t sum = v;
+        uint32_t sumw = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t t = __shfl_up_sync(0xffffffffu, run, o);
-            const uint32_t tw = __shfl_up_sync(0xffffffffu, runw, o);
-            if (lane >= o) { run += t; runw += tw; }
+            const uint64_t t = __shfl_up_sync(0xffffffffu, sum, o);
+            const uint32_t tw = __shfl_up_sync(0xffffffffu, sumw, o);
+            if (lane >= o) { sum += t; sumw += tw; }
         }
-        if (lane == 31) { sh.warp_sum[turn2][warp] = run; sh.warp_cnt[turn2][warp] = runw; }
+        if (lane == 31) { sh.warp_sum[turn2][warp] = sum; sh.warp_cnt[turn2][warp] = sumw; }
         __syncthreads();
         uint64_t s = lane < SMP_WARPS ? sh.warp_sum[turn2][lane] : 0;
         uint32_t sw = lane < SMP_WARPS ? sh.warp_cnt[turn2][lane] : 0;
@@ -125,43 +136,52 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         total = __shfl_sync(0xffffffffu, s, SMP_WARPS - 1);
         const uint64_t below = __shfl_sync(0xffffffffu, s, max(warp - 1, 0));
         const uint32_t belowc = __shfl_sync(0xffffffffu, sw, max(warp - 1, 0));
-        below_w = runw - w + (warp ? belowc : 0);
-        return run - v + (warp ? below : 0);
+        below_w = sumw - w + (warp ? belowc : 0);
+        return sum - v + (warp ? below : 0);
     };
 
     // ------------------------------------------------------------------ the row's part, its largest and its smallest element
-    uint32_t top = 0, top_at = 0xffffffffu, low = 0xffffffffu;
+    float top = -INFINITY, low = INFINITY;
+    uint32_t top_at = 0xffffffffu;
     {
         const T* x = static_cast<const T*>(p.x) + r * p.row_stride + first;
-        auto see = [&](uint32_t o, int i) {
-            if (o > top) { top = o; top_at = first + i; }          // (a thread's indices ascend: the first of equals stays)
-            if (o) low = min(low, o);
+        auto see = [&](float v, int i) {
+            if (v > top) { top = v; top_at = first + i; }          // (a thread's indices ascend: the first of equals stays)
+            low = fminf(low, v > -INFINITY ? v : INFINITY);
         };
-        if (tid < n4 * 4 - n) so[n + tid] = 0;         // (behind the last one: whole pieces of four)
+        if (tid < n4 * 4 - n) sx[n + tid] = -INFINITY; // (behind the last one: whole pieces of four)
         const bool wide = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
         if (wide) {
 #pragma unroll 4
             for (int i = 4 * tid; i + 4 <= n; i += 4 * SMP_THREADS) {
                 float v[4];
                 load4(x + i, v);
-                const uint4 o = make_uint4(order_of(v[0]), order_of(v[1]), order_of(v[2]), order_of(v[3]));
-                *reinterpret_cast<uint4*>(so + i) = o;
-                see(o.x, i); see(o.y, i + 1); see(o.z, i + 2); see(o.w, i + 3);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = plain_logit(v[e]);
+                    see(v[e], i + e);
+                }
+                *reinterpret_cast<float4*>(sx + i) = make_float4(v[0], v[1], v[2], v[3]);
             }
         }
 #pragma unroll 4
         for (int i = (wide ? n / 4 * 4 : 0) + tid; i < n; i += SMP_THREADS) {
-            const uint32_t o = order_of(to_f(x[i]));
-            so[i] = o;
-            see(o, i);
+            const float v = plain_logit(to_f(x[i]));
+            sx[i] = v;
+            see(v, i);
         }
-        const uint32_t all = __reduce_max_sync(0xffffffffu, top);
-        top_at = __reduce_min_sync(0xffffffffu, top == all ? top_at : 0xffffffffu);
-        top = all;
-        low = __reduce_min_sync(0xffffffffu, low);
     }
+    // over a warp: the largest, the lowest index that has it, the smallest
+    auto join = [&](uint32_t& top_order, uint32_t& low_order) {
+        const uint32_t all = __reduce_max_sync(0xffffffffu, top_order);
+        top_at = __reduce_min_sync(0xffffffffu, top_order == all ? top_at : 0xffffffffu);
+        top_order = all;
+        low_order = __reduce_min_sync(0xffffffffu, low_order);
+    };
+    uint32_t top_order = order_of(top), low_order = order_of(low);
+    join(top_order, low_order);
+    tell_and_go_on((uint64_t)top_order << 32 | top_at, low_order);
     // (what the row's numbers alone say is worked out while the barrier is waited for)
-    cluster_arrive_tell((uint64_t)top << 32 | top_at, low);
     const float temp = p.temperature ? p.temperature[r] : p.temperature1;
     const int top_k = p.top_k ? p.top_k[r] : p.top_k1;
     const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
@@ -169,131 +189,243 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
     const double per = 1.4426950408889634 / (double)temp;
     const int unit = p.unit_bits;
     const double floor_w = (min_p > 1.f ? 1.0 : (double)min_p) * (double)(1ull << unit);
-    // Further below the maximum than `deep` the weights of all the row's tokens together are less than 1 - top_p of the largest: the
-    // border of top-p lies above
-    const float deep = temp * (logf((float)p.cols) - logf(1.f - top_p) + 1.f);
     cluster_wait();
-    top = 0;
+    top_order = order_of(-INFINITY);
     for (int i = lane; i < C * SMP_WARPS; i += 32) {
         const uint64_t a = sh.from[turn ^ 1][i][0];
         const uint32_t o = (uint32_t)(a >> 32);
-        if (o > top || (o == top && (uint32_t)a < top_at)) { top = o; top_at = (uint32_t)a; }
-        low = min(low, (uint32_t)sh.from[turn ^ 1][i][1]);
+        if (o > top_order || (o == top_order && (uint32_t)a < top_at)) { top_order = o; top_at = (uint32_t)a; }
+        low_order = min(low_order, (uint32_t)sh.from[turn ^ 1][i][1]);
     }
-    {
-        const uint32_t all = __reduce_max_sync(0xffffffffu, top);
-        top_at = __reduce_min_sync(0xffffffffu, top == all ? top_at : 0xffffffffu);
-        top = all;
-        low = __reduce_min_sync(0xffffffffu, low);
-    }
-    if (top == 0 || !(temp > 0.f) || top_k == 1) {
-        if (rank == 0 && tid == 0) p.out[r] = top == 0 ? 0 : (int)top_at;
+    join(top_order, low_order);
+    const float peak = value_of(top_order), depth = peak - value_of(low_order);
+    if (peak == -INFINITY || !(temp > 0.f) || top_k == 1) {
+        if (rank == 0 && tid == 0) p.out[r] = peak == -INFINITY ? 0 : (int)top_at;
         return;                                        // (nothing reaches into another CTA behind the last barrier)
     }
-    const float peak = value_of(top), depth = peak - value_of(low);
 
-    // 2^((v - peak) / T * log2 e + unit), whole and at least 1; 0 where fp64 has none.  No branches: a warp weighs different values, and
-    // a thread's four at a time are worked out side by side
-    auto weigh = [&](uint32_t order) -> uint64_t {
-        const double t = ((double)value_of(order) - (double)peak) * per;
-        const double near = fmax(t, -(double)(unit + 1));          // (a NaN, infinity less infinity, comes out as the bound)
-        const double rounded = near + 0x1.8p52;                    // to a whole number, which is the low word
+    // 2^((v - peak) / T * log2 e) in units of 2^-unit, to the nearest whole number, at least 1; 0 where fp64 has none.  No branches: a
+    // warp weighs different values.
+    auto weigh_whole = [&](float v) -> double {
+        const double t = ((double)v - (double)peak) * per;
+        const double near = fmax(t, -(double)unit);    // (infinity less infinity comes out as the bound)
+        const double rounded = near + 0x1.8p52;        // to a whole number, which is the low word
         const double f = near - (rounded - 0x1.8p52);
-        // (ln 2)^i / i!
-        double w = 2.5678435993488196e-11;
-        w = fma(w, f, 4.4455382718708101e-10);
-        w = fma(w, f, 7.0549116208011209e-09);
-        w = fma(w, f, 1.0178086009239696e-07);
-        w = fma(w, f, 1.3215486790144305e-06);
-        w = fma(w, f, 1.5252733804059838e-05);
-        w = fma(w, f, 1.5403530393381606e-04);
-        w = fma(w, f, 1.3333558146428441e-03);
-        w = fma(w, f, 9.6181291076284769e-03);
-        w = fma(w, f, 5.5504108664821576e-02);
-        w = fma(w, f, 2.4022650695910069e-01);
-        w = fma(w, f, 6.9314718055994529e-01);
-        w = fma(w, f, 1.0);
+        // (ln 2)^i / i!, by halves: a chain of five instead of twelve
+        const double f2 = f * f, f4 = f2 * f2, f8 = f4 * f4;
+        const double a = fma(fma(5.5504108664821576e-02, f, 2.4022650695910069e-01), f2, fma(6.9314718055994529e-01, f, 1.0));
+        const double b = fma(fma(1.5252733804059838e-05, f, 1.5403530393381606e-04), f2, fma(1.3333558146428441e-03, f, 9.6181291076284769e-03));
+        const double d = fma(fma(4.4455382718708101e-10, f, 7.0549116208011209e-09), f2, fma(1.0178086009239696e-07, f, 1.3215486790144305e-06));
+        double w = fma(fma(2.5678435993488196e-11, f4, d), f8, fma(b, f4, a));
         w = __hiloint2double(__double2hiint(w) + ((__double2loint(rounded) + unit) << 20), __double2loint(w));
-        const uint64_t m = max((uint64_t)(__double_as_longlong(w + 0x1p52) - 0x4330000000000000ll), (uint64_t)1);
-        return order == top ? 1ull << unit : t >= -1074.5 ? m : 0;
+        w = (w + 0x1p52) - 0x1p52;
+        return v == peak ? (double)(1ull << unit) : t >= -1074.5 ? w : 0.0;
     };
+    auto weigh = [&](float v) -> uint64_t { return (uint64_t)(__double_as_longlong(weigh_whole(v) + 0x1p52) - 0x4330000000000000ll); };
 
     // kept: above `last` in the order, or `last` itself
-    uint32_t last_order = 1, last_at = 0xffffffffu;
-    auto kept = [&](uint32_t o, int i) { return o > last_order || (o == last_order && (uint32_t)(first + i) <= last_at); };
-    auto key_of = [&](uint32_t o, int i) { return (uint64_t)o << 32 | (uint32_t)~(first + i); };
+    float last = -INFINITY;
+    int last_at = -1;
+    auto kept = [&](float v, int i) { return v > last || (v == last && first + i <= last_at); };
+    auto key_of = [&](float v, int i) { return (uint64_t)order_of(v) << 32 | (uint32_t)~(first + i); };
+
+    // What `which` says of the warp's run is put side by side, its places in the order of the index, if that is half of it at most
+    int held = -1;                                     // of the warp's run; -1: all of it is looked at
+    auto compact = [&](auto which) {
+        int at = 0;
+        const uint32_t lower = (1u << lane) - 1;
+        for (int q0 = begin; q0 < end; q0 += 32) {
+            const int q = q0 + lane;
+            const float4 four = q < end ? *reinterpret_cast<const float4*>(sx + 4 * q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+            const float v[4] = {four.x, four.y, four.z, four.w};
+            bool in[4];
+            int before = at, own = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                in[e] = which(v[e], 4 * q + e);
+                const uint32_t who = __ballot_sync(0xffffffffu, in[e]);
+                before += __popc(who & lower);
+                at += __popc(who);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (in[e]) {
+                    if (before + own < 2 * (end - begin)) places[before + own] = (uint16_t)(4 * (q - begin) + e);
+                    ++own;
+                }
+        }
+        __syncwarp();
+        held = at <= 2 * (end - begin) ? at : -1;
+    };
+    // calls f(value, index in the part) for what the thread looks at
+    auto each = [&](auto f) {
+        if (held >= 0) {
+#pragma unroll 2
+            for (int j = lane; j < held; j += 32) {
+                const int i = 4 * begin + places[j];
+                f(sx[i], i);
+            }
+        } else {
+            for (int q = begin + lane; q < end; q += 32) {
+                const float4 four = *reinterpret_cast<const float4*>(sx + 4 * q);
+                f(four.x, 4 * q);
+                f(four.y, 4 * q + 1);
+                f(four.z, 4 * q + 2);
+                f(four.w, 4 * q + 3);
+            }
+        }
+    };
 
     // The last element before which there is less than a limit: top_k by count, top_p times their sum by weight.  True: the choice has
     // been made with the list.
     auto cut = [&](bool by_weight, float range) -> bool {
-        uint64_t above = 0, hi = 0, lo = 0;            // what lies above the step; the step as a range of keys, once it is one
-        int shift = -1, step = 0, m = 0;
+        uint64_t above = 0, hi = 0, lo = 0;            // what lies above the steps; their range of keys, where they divide one
+        int shift = -1, step = 0, m = 0, step1 = 0, step2 = SMP_BINS - 1;
         double limit = (double)top_k;
         bool listed = false;
-        // (an order below that of the rounded edge is below the edge itself)
-        const uint32_t deep_order = by_weight && range < depth ? order_of(peak - range) : 0;
         const float scale = range > 0.f ? SMP_BINS / range : 0.f;
-        auto in_range = [&](uint32_t o, int i) { return kept(o, i) && (shift < 0 || (key_of(o, i) <= hi && key_of(o, i) >= lo)); };
+        float edge = peak, scale2 = scale;             // of the steps between step1 and step2
         // (the rounding is to the nearest step: any will do that never puts the larger value behind the smaller)
-        auto step_of_order = [&](uint32_t o) -> int {
-            return o == top ? 0 : (int)(__float_as_uint(fminf((peak - value_of(o)) * scale, SMP_BINS - 1.f) + 8388608.f) & (SMP_BINS - 1));
+        auto step_below = [&](float d) -> int { return (int)(__float_as_uint(fminf(d, SMP_BINS - 1.f) + 8388608.f) & (SMP_BINS - 1)); };
+        auto coarse = [&](float v) -> int { return v == peak ? 0 : step_below((peak - v) * scale); };
+        auto in_step = [&](float v, int i) -> int {    // -1: not in the range
+            if (!kept(v, i)) return -1;
+            if (shift < 0) {
+                const int b = coarse(v);
+                return !by_weight ? b : b < step1 || b > step2 ? -1 : step_below(fmaxf((edge - v) * scale2, 0.f));
+            }
+            const uint64_t key = key_of(v, i);
+            return key > hi || key < lo ? -1 : (int)((hi - key) >> shift);
         };
-        auto step_of = [&](uint32_t o, int i) -> int { return shift >= 0 ? (int)((hi - key_of(o, i)) >> shift) : step_of_order(o); };
-        for (;;) {
+        auto clear = [&]() {
             sh.hist[0][tid] = 0;
             if (by_weight) sh.hist[1][tid] = sh.hist[2][tid] = sh.hist[3][tid] = 0;
             if (tid == 0) sh.list_n = 0;
             __syncthreads();
-            uint64_t rest = 0;
-            for (int q = tid; q < n4; q += SMP_THREADS) {
-                const uint4 four = *reinterpret_cast<const uint4*>(so + 4 * q);
-                const uint32_t os[4] = {four.x, four.y, four.z, four.w};
-                uint64_t ws[4];
-                if (by_weight) {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint64_t w = weigh(os[e]);
-                        ws[e] = in_range(os[e], 4 * q + e) ? w : 0;
-                        rest += os[e] < deep_order ? ws[e] : 0;
-                    }
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t o = os[e];
-                    if (o < deep_order || !in_range(o, 4 * q + e)) continue;
-                    const int b = step_of(o, 4 * q + e);
-                    atomicAdd(&sh.hist[0][b], 1u);
-                    if (by_weight) {
-                        const uint64_t w = ws[e];
-                        atomicAdd(&sh.hist[1][b], (uint32_t)w & 0xffffu);
-                        if (w >> 16) {
-                            atomicAdd(&sh.hist[2][b], (uint32_t)(w >> 16) & 0xffffu);
-                            if (w >> 32) atomicAdd(&sh.hist[3][b], (uint32_t)(w >> 32));
-                        }
-                    }
+        };
+        auto add = [&](int b, uint64_t w) {
+            atomicAdd(&sh.hist[0][b], 1u);
+            if (by_weight) {
+                atomicAdd(&sh.hist[1][b], (uint32_t)w & 0xffffu);
+                if (w >> 16) {
+                    atomicAdd(&sh.hist[2][b], (uint32_t)(w >> 16) & 0xffffu);
+                    if (w >> 32) atomicAdd(&sh.hist[3][b], (uint32_t)(w >> 32));
                 }
             }
-            if (by_weight && deep_order > 1) {         // what lies deep counts in the sum alone
-                rest = warp_total(rest);
-                if (lane < 3) atomicAdd(&sh.hist[lane + 1][SMP_BINS - 1], lane == 0 ? (uint32_t)rest & 0xffffu : lane == 1 ? (uint32_t)(rest >> 16) & 0xffffu : (uint32_t)(rest >> 32));
-            }
+        };
+        auto put = [&](float v, int i) {
+            const int at = min(atomicAdd(&sh.list_n, 1), SMP_LIST - 1);      // (m of them in the whole cluster)
+            sh.list_key[at] = key_of(v, i);
+        };
+        auto joined = [&](int row) -> uint32_t {       // the cluster's histogram at the thread's step
+            uint32_t sum = 0;
+#pragma unroll
+            for (int c = 0; c < SMP_CLUSTER; ++c)
+                if (c < C) sum += ld_cluster_u32(in_rank(smem_u32(&sh.hist[row][tid]), c));
+            return sum;
+        };
+
+        clear();
+        if (by_weight) {
+            each([&](float v, int i) {
+                if (kept(v, i)) atomicAdd(&sh.hist[0][coarse(v)], 1u);
+            });
             cluster_sync();
-            uint32_t cnt = 0;
-            uint64_t sum = 0;
+            const uint32_t cnt = joined(0);
+            // the step's weights lie between these, its sums between theirs (a thousandth of a step and 1e-4 for the roundings)
+            const float wide = range / SMP_BINS / temp, most = tid == 0 ? 1.f : __expf(-(tid - 0.501f) * wide), least = tid == SMP_BINS - 1 ? 0.f : __expf(-(tid + 0.501f) * wide);
+            float a = cnt * most, b = cnt ? cnt * least : 0.f;
+            uint32_t upto = cnt;
+            const float own_a = a, own_b = b;
 #pragma unroll
-            for (int c = 0; c < SMP_CLUSTER; ++c) {
-                if (c >= C) break;
-                const uint32_t at = in_rank(smem_u32(&sh.hist[0][tid]), c);
-                cnt += ld_cluster_u32(at);
-                if (by_weight)
-                    sum += ld_cluster_u32(at + SMP_BINS * 4) + ((uint64_t)ld_cluster_u32(at + SMP_BINS * 8) << 16) +
-                           ((uint64_t)ld_cluster_u32(at + SMP_BINS * 12) << 32);
+            for (int o = 1; o < 32; o <<= 1) {
+                const float ta = __shfl_up_sync(0xffffffffu, a, o), tb = __shfl_up_sync(0xffffffffu, b, o);
+                const uint32_t tc = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) { a += ta; b += tb; upto += tc; }
             }
-            if (!by_weight) sum = cnt;
+            if (lane == 31) { sh.sums[warp][0] = (uint64_t)__float_as_uint(a) << 32 | __float_as_uint(b); sh.sums[warp][1] = upto; }
+            __syncthreads();
+            float all_a = 0.f, all_b = 0.f, low_a = 0.f, low_b = 0.f;
+            for (int w = 0; w < SMP_WARPS; ++w) {
+                if (w == warp) { low_a = all_a; low_b = all_b; }
+                if (w < warp) upto += (uint32_t)sh.sums[w][1];
+                all_a += __uint_as_float((uint32_t)(sh.sums[w][0] >> 32));
+                all_b += __uint_as_float((uint32_t)sh.sums[w][0]);
+            }
+            const uint32_t first_ok = __ballot_sync(0xffffffffu, cnt && (a - own_a + low_a) * 1.0001f < top_p * all_b * 0.9999f);
+            const uint32_t last_ok = __ballot_sync(0xffffffffu, cnt && (b - own_b + low_b) * 0.9999f <= top_p * all_a * 1.0001f);
+            if (lane == (last_ok ? 31 - __clz(last_ok) : 0)) {
+                sh.between[warp].lane1 = first_ok ? 32 - __clz(first_ok) : 0;
+                sh.between[warp].lane2 = last_ok ? 32 - __clz(last_ok) : 0;
+                sh.between[warp].upto = upto;
+            }
+            __syncthreads();
+            const uint32_t w1 = __ballot_sync(0xffffffffu, lane < SMP_WARPS && sh.between[lane % SMP_WARPS].lane1 != 0);
+            const uint32_t w2 = __ballot_sync(0xffffffffu, lane < SMP_WARPS && sh.between[lane % SMP_WARPS].lane2 != 0);
+            step1 = w1 ? (31 - __clz(w1)) * 32 + (int)sh.between[31 - __clz(w1)].lane1 - 1 : 0;
+            step2 = w2 ? (31 - __clz(w2)) * 32 + (int)sh.between[31 - __clz(w2)].lane2 - 1 : 0;
+            m = w2 ? (int)sh.between[31 - __clz(w2)].upto : SMP_LIST + 1;
+            step1 = min(step1, step2);
+            listed = m <= SMP_LIST;
+            if (listed) step1 = step2 + 1;             // nothing between: sums and the list are all that is wanted
+            edge = step1 == 0 ? peak : peak - (step1 - 0.5f) / scale;
+            scale2 = scale * SMP_BINS / (step2 - step1 + 1);
+            cluster_sync();                            // the others have read this CTA's histogram
+            clear();
+            // every token is weighed, once
+            double sum_above = 0.0, sum_below = 0.0;
+            compact([&](float v, int i) {
+                const bool k = kept(v, i);
+                const int c = coarse(v);
+                const double w = k ? weigh_whole(v) : 0.0;
+                sum_below += c > step2 ? w : 0.0;
+                sum_above += c < step1 ? w : 0.0;
+                return k && c <= step2;
+            });
+            each([&](float v, int i) {
+                if (listed) {
+                    if (kept(v, i) && coarse(v) <= step2) put(v, i);
+                } else {
+                    const int b = in_step(v, i);
+                    if (b >= 0) add(b, weigh(v));
+                }
+            });
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                sum_above += __shfl_xor_sync(0xffffffffu, sum_above, o);
+                sum_below += __shfl_xor_sync(0xffffffffu, sum_below, o);
+            }
+            tell((uint64_t)sum_above, (uint64_t)sum_below);
+            uint64_t below = 0;
+            for (int i = lane; i < C * SMP_WARPS; i += 32) {
+                above += sh.from[turn ^ 1][i][0];
+                below += sh.from[turn ^ 1][i][1];
+            }
+            above = warp_total(above);
+            below = warp_total(below);
+            limit = (double)(above + below);           // (the sum of the others still to come)
+        } else {
+            each([&](float v, int i) {
+                const int b = in_step(v, i);
+                if (b >= 0) add(b, 0);
+            });
+            cluster_sync();
+        }
+        for (bool again = false; !(by_weight && listed); again = true) {
+            if (again) {
+                clear();
+                each([&](float v, int i) {
+                    const int b = in_step(v, i);
+                    if (b >= 0) add(b, by_weight ? weigh(v) : 0);
+                });
+                cluster_sync();
+            }
+            const uint32_t cnt = joined(0);
             uint64_t total;
             uint32_t upto;
+            const uint64_t sum = by_weight ? joined(1) + ((uint64_t)joined(2) << 16) + ((uint64_t)joined(3) << 32) : cnt;
             const uint64_t before = block_scan(sum, cnt, total, upto) + above;
-            if (by_weight && shift < 0) limit = fmax((double)top_p * (double)total, 0.5);
+            if (by_weight && !again) limit = fmax((double)top_p * (limit + (double)total), 0.5);
             // the last step that has elements and less than the limit above it
             const uint32_t here = __ballot_sync(0xffffffffu, cnt > 0 && (double)before < limit);
             if (lane == (here ? 31 - __clz(here) : 0)) {
@@ -308,15 +440,16 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             above = sh.border[w].above;
             step = w * 32 + sh.border[w].lane1 - 1;
             m = sh.border[w].count;
-            if (shift < 0 && sh.border[w].upto <= SMP_LIST) { m = sh.border[w].upto; listed = true; }
+            if (!by_weight && !again && sh.border[w].upto <= SMP_LIST) { m = sh.border[w].upto; listed = true; }
             if (m <= SMP_LIST) break;
             // too many to be ranked: the step's range of keys, to be divided
             if (shift < 0) {
                 uint64_t most = 0, least = 0;          // (least: of the complement)
-                for (int i = tid; i < n; i += SMP_THREADS) {
-                    const uint32_t o = so[i];
-                    if (in_range(o, i) && step_of(o, i) == step) { most = max(most, key_of(o, i)); least = max(least, ~key_of(o, i)); }
-                }
+                each([&](float v, int i) {
+                    if (in_step(v, i) != step) return;
+                    most = max(most, key_of(v, i));
+                    least = max(least, ~key_of(v, i));
+                });
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) {
                     most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -336,20 +469,17 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             }
             shift = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
         }
-        // the list: the step's elements, or all down to it
-        for (int q = tid; q < n4; q += SMP_THREADS) {
-            const uint4 four = *reinterpret_cast<const uint4*>(so + 4 * q);
-            const uint32_t os[4] = {four.x, four.y, four.z, four.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (os[e] < deep_order || !in_range(os[e], 4 * q + e)) continue;
-                const int b = step_of(os[e], 4 * q + e);
-                if (b > step || (b < step && !listed)) continue;
-                const int at = min(atomicAdd(&sh.list_n, 1), SMP_LIST - 1);      // (m of them in the whole cluster)
-                sh.list_key[at] = key_of(os[e], 4 * q + e);
-            }
+        if (by_weight && listed) {
+            limit = fmax((double)top_p * limit, 0.5);
+            above = 0;
+        } else {
+            // the list: the step's elements, or all down to it
+            each([&](float v, int i) {
+                const int b = in_step(v, i);
+                if (b >= 0 && b <= step && (b == step || listed)) put(v, i);
+            });
+            cluster_sync();
         }
-        cluster_sync();
         {
             // the thread's element of the cluster's list: which CTA's, and which there
             uint32_t here = lane < C ? ld_cluster_u32(in_rank(smem_u32(&sh.list_n), min(lane, C - 1))) : 0;
@@ -378,7 +508,7 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             return (int)sh.rank[tid];
         };
         const uint64_t key = tid < m ? sh.all_key[tid] : 0;
-        const uint64_t weight = tid >= m ? 0 : by_weight || listed ? weigh((uint32_t)(key >> 32)) : 1;
+        const uint64_t weight = tid >= m ? 0 : by_weight || listed ? weigh(value_of((uint32_t)(key >> 32))) : 1;
         const int rank_of = rank_among(sh.all_key, m);
         // in order, where the histogram was
         uint64_t* in_key = reinterpret_cast<uint64_t*>(sh.hist[0]);
@@ -392,8 +522,8 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             const uint64_t before = block_scan(w, 0, total, unused) + above;
             const int stay = __syncthreads_count(tid < m && (double)before < limit);
             const uint64_t k = in_key[stay - 1];
-            last_order = (uint32_t)(k >> 32);
-            last_at = ~(uint32_t)k;
+            last = value_of((uint32_t)(k >> 32));
+            last_at = (int)~(uint32_t)k;
             cluster_sync();                            // the others have read this CTA's list (and histogram)
             return false;
         }
@@ -423,58 +553,20 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
 
     bool chosen = false;
     if (top_k > 0 && top_k < p.cols) chosen = cut(false, fminf(depth, 128.f));
-    if (!chosen && top_p < 1.f) chosen = cut(true, fminf(depth, deep));
+    if (!chosen && top_p < 1.f) chosen = cut(true, fminf(fminf(depth, 64.f * temp), 3e38f));
     if (chosen) {
         cluster_sync();                                // the others have read this CTA's list
         return;
     }
+    if (held < 0 && last > -INFINITY) compact(kept);
 
-    // ------------------------------------------------------------------------------------------- the choice from the whole row
-    auto counted = [&](uint32_t o, int i) -> uint64_t {
-        if (!kept(o, i)) return 0;
-        const uint64_t w = weigh(o);
+    // ---------------------------------------------------------------------------------------- the choice from all that is kept
+    auto counted = [&](float v, int i) -> uint64_t {
+        const uint64_t w = kept(v, i) ? weigh(v) : 0;
         return (double)w < floor_w && (uint32_t)(first + i) != top_at ? 0 : w;
     };
-    // a warp has a run of its CTA's part, so that its sum is one of neighbours
-    const int run = (n4 + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n4, begin + run);      // in pieces of four
     uint64_t mine = 0;
-    if (last_order == 1) {
-        for (int q = begin + lane; q < end; q += 32) {
-            const uint4 four = *reinterpret_cast<const uint4*>(so + 4 * q);
-            mine += counted(four.x, 4 * q) + counted(four.y, 4 * q + 1) + counted(four.z, 4 * q + 2) + counted(four.w, 4 * q + 3);
-        }
-    } else {
-        // few are kept: they are put side by side, so that 32 at a time are weighed
-        uint32_t* queue = sh.hist[0] + warp * 64;
-        int held = 0;
-        auto weigh_queued = [&](int k) {               // the top's weight is above any floor
-            const uint64_t w = lane < k ? weigh(queue[lane]) : 0;
-            if (lane < k && (!((double)w < floor_w))) mine += w;
-            __syncwarp();
-        };
-        for (int q = begin; q < end; q += 32) {
-            const uint4 four = q + lane < end ? *reinterpret_cast<const uint4*>(so + 4 * (q + lane)) : make_uint4(0u, 0u, 0u, 0u);
-            if (!__any_sync(0xffffffffu, max(max(four.x, four.y), max(four.z, four.w)) >= last_order)) continue;
-            const uint32_t os[4] = {four.x, four.y, four.z, four.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool in = kept(os[e], 4 * (q + lane) + e);
-                const uint32_t who = __ballot_sync(0xffffffffu, in);
-                if (in) queue[held + __popc(who & ((1u << lane) - 1))] = os[e];
-                held += __popc(who);
-                __syncwarp();
-                if (held >= 32) {
-                    weigh_queued(32);
-                    held -= 32;
-                    const uint32_t o = lane < held ? queue[32 + lane] : 0;
-                    __syncwarp();
-                    if (lane < held) queue[lane] = o;
-                    __syncwarp();
-                }
-            }
-        }
-        weigh_queued(held);
-    }
+    each([&](float v, int i) { mine += counted(v, i); });
     mine = warp_total(mine);
     tell(mine, 0);
     uint64_t all = 0, below = 0;
@@ -487,11 +579,10 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
     below = warp_total(below);
     const uint64_t reach = min((uint64_t)(u * (double)all), all - 1);
     if (reach < below || reach >= below + mine) return;
-    for (int q = begin + lane; q - lane < end; q += 32) {
-        const uint4 four = q < end ? *reinterpret_cast<const uint4*>(so + 4 * q) : make_uint4(0u, 0u, 0u, 0u);
-        const uint64_t w[4] = {counted(four.x, 4 * q), counted(four.y, 4 * q + 1), counted(four.z, 4 * q + 2), counted(four.w, 4 * q + 3)};
-        uint64_t sum = w[0] + w[1] + w[2] + w[3];
-        const uint64_t own = sum;
+    const int looked = held >= 0 ? held : 4 * (end - begin);
+    for (int j = lane; j - lane < looked; j += 32) {
+        const int i = 4 * begin + (held < 0 || j >= looked ? j : places[j]);
+        uint64_t sum = j < looked ? counted(sx[i], i) : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t t = __shfl_up_sync(0xffffffffu, sum, o);
@@ -499,12 +590,7 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         }
         const uint32_t over = __ballot_sync(0xffffffffu, below + sum > reach);
         if (over) {
-            if (lane == __ffs(over) - 1) {
-                below += sum - own;
-                int e = 0;
-                while (e < 3 && below + w[e] <= reach) below += w[e++];
-                p.out[r] = first + 4 * q + e;
-            }
+            if (lane == __ffs(over) - 1) p.out[r] = first + i;
             return;
         }
         below += __shfl_sync(0xffffffffu, sum, 31);
@@ -540,7 +626,7 @@ extern "C" int bn_sample_rows(const void* logits, int64_t row_stride, int dtype,
     int c = 1;
     while (c < SMP_CLUSTER && (cols > c * SMP_MOST || (rows > 8 && cols > c * SMP_TWO) || ((int64_t)rows * 2 * c <= sm_count() && cols > c * 1024))) c *= 2;
     p.slice = ((cols + c - 1) / c + 3) / 4 * 4;
-    const size_t smem = (size_t)p.slice * 4;
+    const size_t smem = (size_t)p.slice * 5;
     auto* kernel = dtype == 0 ? sample_rows_kernel<float> : sample_rows_kernel<__nv_bfloat16>;
     if (int rc = allow_smem(kernel, smem, what, SMP_MOST_SMEM, sizeof(SampleShared))) return rc;
     cudaLaunchConfig_t cfg = {};
