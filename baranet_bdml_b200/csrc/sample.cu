@@ -15,7 +15,7 @@
 // A cluster of CTAs per row, each with a part of the row in shared memory: read once.  The border of top-k is found by a histogram of
 // counts over 512 steps of the value below the maximum, which every CTA joins for itself through distributed shared memory.  For top-p the
 // same counts, with the largest and the smallest weight of each step, tell between which two steps the border must lie.  Every token is
-// then weighed once: those above and below only go into sums (exact in fp64, whole numbers below 2^53), those between into a second
+// then weighed once: those above and below only go into sums, those between into a second
 // histogram, of weights as three 16-bit limbs (whose sums fit the 32-bit atomics that shared memory has; 64-bit ones take 50 times as
 // long), and the places of all that may be kept are put side by side for the choice.
 // Where no more than 512 tokens lie in the steps down to the border, all that is left is done with a list of them, in every CTA alike:
@@ -50,7 +50,7 @@ struct SampleParams {
     float temperature1, top_p1, min_p1;
     int top_k1;
     int32_t* out;
-    int cols, slice, unit_bits;                        // slice: tokens per CTA, a multiple of 4
+    int bf16, cols, slice, unit_bits;                        // slice: tokens per CTA, a multiple of 4
 };
 
 // a logit as it is kept: NaN is -inf, -0 is 0
@@ -83,7 +83,31 @@ __device__ __forceinline__ uint64_t warp_total(uint64_t v) {
     return v;
 }
 
-template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SampleParams p) {
+// The part's logits into shared memory; f sees each
+template <typename T, typename F> __device__ __forceinline__ void load_logits(const T* x, float* sx, int n, F f) {
+    const bool wide = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
+    if (wide) {
+#pragma unroll 4
+        for (int i = 4 * threadIdx.x; i + 4 <= n; i += 4 * SMP_THREADS) {
+            float v[4];
+            load4(x + i, v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = plain_logit(v[e]);
+                f(v[e], i + e);
+            }
+            *reinterpret_cast<float4*>(sx + i) = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    }
+#pragma unroll 4
+    for (int i = (wide ? n / 4 * 4 : 0) + threadIdx.x; i < n; i += SMP_THREADS) {
+        const float v = plain_logit(to_f(x[i]));
+        sx[i] = v;
+        f(v, i);
+    }
+}
+
+__global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SampleParams p) {
     extern __shared__ __align__(16) float sx[];        // the part's logits, and 16-bit places of up to half of them
     __shared__ SampleShared sh;
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -144,32 +168,14 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
     float top = -INFINITY, low = INFINITY;
     uint32_t top_at = 0xffffffffu;
     {
-        const T* x = static_cast<const T*>(p.x) + r * p.row_stride + first;
         auto see = [&](float v, int i) {
             if (v > top) { top = v; top_at = first + i; }          // (a thread's indices ascend: the first of equals stays)
             low = fminf(low, v > -INFINITY ? v : INFINITY);
         };
         if (tid < n4 * 4 - n) sx[n + tid] = -INFINITY; // (behind the last one: whole pieces of four)
-        const bool wide = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
-        if (wide) {
-#pragma unroll 4
-            for (int i = 4 * tid; i + 4 <= n; i += 4 * SMP_THREADS) {
-                float v[4];
-                load4(x + i, v);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = plain_logit(v[e]);
-                    see(v[e], i + e);
-                }
-                *reinterpret_cast<float4*>(sx + i) = make_float4(v[0], v[1], v[2], v[3]);
-            }
-        }
-#pragma unroll 4
-        for (int i = (wide ? n / 4 * 4 : 0) + tid; i < n; i += SMP_THREADS) {
-            const float v = plain_logit(to_f(x[i]));
-            sx[i] = v;
-            see(v, i);
-        }
+        const int64_t at = r * p.row_stride + first;
+        if (p.bf16) load_logits(static_cast<const __nv_bfloat16*>(p.x) + at, sx, n, see);
+        else load_logits(static_cast<const float*>(p.x) + at, sx, n, see);
     }
     // over a warp: the largest, the lowest index that has it, the smallest
     auto join = [&](uint32_t& top_order, uint32_t& low_order) {
@@ -182,7 +188,7 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
     join(top_order, low_order);
     tell_and_go_on((uint64_t)top_order << 32 | top_at, low_order);
     // (what the row's numbers alone say is worked out while the barrier is waited for)
-    const float temp = p.temperature ? p.temperature[r] : p.temperature1;
+    const float temp_given = p.temperature ? p.temperature[r] : p.temperature1, temp = temp_given > 3e38f ? 3e38f : temp_given;
     const int top_k = p.top_k ? p.top_k[r] : p.top_k1;
     const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
     const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);
@@ -198,30 +204,45 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
         low_order = min(low_order, (uint32_t)sh.from[turn ^ 1][i][1]);
     }
     join(top_order, low_order);
-    const float peak = value_of(top_order), depth = peak - value_of(low_order);
+    float peak = value_of(top_order), depth = peak - value_of(low_order);
     if (peak == -INFINITY || !(temp > 0.f) || top_k == 1) {
         if (rank == 0 && tid == 0) p.out[r] = peak == -INFINITY ? 0 : (int)top_at;
         return;                                        // (nothing reaches into another CTA behind the last barrier)
     }
+    if (peak == INFINITY) {                            // infinities share the weight
+        __syncthreads();
+        for (int i = tid; i < 4 * n4; i += SMP_THREADS) sx[i] = sx[i] == INFINITY ? 0.f : -INFINITY;
+        peak = depth = 0.f;
+        __syncthreads();
+    }
 
     // 2^((v - peak) / T * log2 e) in units of 2^-unit, to the nearest whole number, at least 1; 0 where fp64 has none.  No branches: a
-    // warp weighs different values.
-    auto weigh_whole = [&](float v) -> double {
+    // warp weighs different values.  The smallest values above one unit and above nothing are rounded up, so that they part exactly.
+    const float one_unit = __double2float_ru((double)peak - unit / per), nothing = __double2float_ru((double)peak - 1074.5 / per);
+    auto weigh = [&](float v) -> uint64_t {
         const double t = ((double)v - (double)peak) * per;
-        const double near = fmax(t, -(double)unit);    // (infinity less infinity comes out as the bound)
-        const double rounded = near + 0x1.8p52;        // to a whole number, which is the low word
-        const double f = near - (rounded - 0x1.8p52);
-        // (ln 2)^i / i!, by halves: a chain of five instead of twelve
-        const double f2 = f * f, f4 = f2 * f2, f8 = f4 * f4;
-        const double a = fma(fma(5.5504108664821576e-02, f, 2.4022650695910069e-01), f2, fma(6.9314718055994529e-01, f, 1.0));
-        const double b = fma(fma(1.5252733804059838e-05, f, 1.5403530393381606e-04), f2, fma(1.3333558146428441e-03, f, 9.6181291076284769e-03));
-        const double d = fma(fma(4.4455382718708101e-10, f, 7.0549116208011209e-09), f2, fma(1.0178086009239696e-07, f, 1.3215486790144305e-06));
-        double w = fma(fma(2.5678435993488196e-11, f4, d), f8, fma(b, f4, a));
-        w = __hiloint2double(__double2hiint(w) + ((__double2loint(rounded) + unit) << 20), __double2loint(w));
-        w = (w + 0x1p52) - 0x1p52;
-        return v == peak ? (double)(1ull << unit) : t >= -1074.5 ? w : 0.0;
+        const double rounded = t + (0x1.8p52 + unit);  // to a whole number, which, with unit, is the low word
+        const double f = t - (rounded - (0x1.8p52 + unit));
+        // (ln 2)^i / i!
+        double w = 2.5678435993488196e-11;
+        w = fma(w, f, 4.4455382718708101e-10);
+        w = fma(w, f, 7.0549116208011209e-09);
+        w = fma(w, f, 1.0178086009239696e-07);
+        w = fma(w, f, 1.3215486790144305e-06);
+        w = fma(w, f, 1.5252733804059838e-05);
+        w = fma(w, f, 1.5403530393381606e-04);
+        w = fma(w, f, 1.3333558146428441e-03);
+        w = fma(w, f, 9.6181291076284769e-03);
+        w = fma(w, f, 5.5504108664821576e-02);
+        w = fma(w, f, 2.4022650695910069e-01);
+        w = fma(w, f, 6.9314718055994529e-01);
+        w = fma(w, f, 1.0);
+        w = __hiloint2double(__double2hiint(w) + (__double2loint(rounded) << 20), __double2loint(w));
+        w += 0x1p52;                                   // (what is left are the low bits)
+        const uint32_t hi = v >= one_unit ? (uint32_t)__double2hiint(w) - 0x43300000u : 0u;
+        const uint32_t lo = v >= one_unit ? (uint32_t)__double2loint(w) : v >= nothing ? 1u : 0u;
+        return (uint64_t)hi << 32 | lo;
     };
-    auto weigh = [&](float v) -> uint64_t { return (uint64_t)(__double_as_longlong(weigh_whole(v) + 0x1p52) - 0x4330000000000000ll); };
 
     // kept: above `last` in the order, or `last` itself
     float last = -INFINITY;
@@ -367,43 +388,58 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             m = w2 ? (int)sh.between[31 - __clz(w2)].upto : SMP_LIST + 1;
             step1 = min(step1, step2);
             listed = m <= SMP_LIST;
-            if (listed) step1 = step2 + 1;             // nothing between: sums and the list are all that is wanted
             edge = step1 == 0 ? peak : peak - (step1 - 0.5f) / scale;
             scale2 = scale * SMP_BINS / (step2 - step1 + 1);
+            // the smallest value of the steps up to step2: a warp looks at 32 at once
+            uint32_t from = order_of(-INFINITY) + 1, to = order_of(peak);
+            while (from < to) {
+                const uint32_t apart = (to - from) / 32 + 1, at = from + lane * apart;
+                const uint32_t who = __ballot_sync(0xffffffffu, at >= to || coarse(value_of(at)) <= step2);
+                if (who == 0) { from += 31 * apart + 1; continue; }
+                const int f = __ffs(who) - 1;
+                to = min(to, from + f * apart);
+                if (f) from += (f - 1) * apart + 1;
+            }
+            const float lowest = value_of(to);
             cluster_sync();                            // the others have read this CTA's histogram
             clear();
-            // every token is weighed, once
-            double sum_above = 0.0, sum_below = 0.0;
-            compact([&](float v, int i) {
-                const bool k = kept(v, i);
-                const int c = coarse(v);
-                const double w = k ? weigh_whole(v) : 0.0;
-                sum_below += c > step2 ? w : 0.0;
-                sum_above += c < step1 ? w : 0.0;
-                return k && c <= step2;
-            });
+            // every token is weighed, once: what lies below the steps, and all
+            uint64_t all = 0, below = 0;
+            if (last == -INFINITY) {
+                compact([&](float v, int i) {
+                    const uint64_t w = weigh(v);
+                    all += w;
+                    if (v < lowest) below += w;
+                    return v >= lowest;
+                });
+            } else {
+                compact([&](float v, int i) {
+                    const bool k = kept(v, i);
+                    const uint64_t w = k ? weigh(v) : 0;
+                    all += w;
+                    if (v < lowest) below += w;
+                    return k && v >= lowest;
+                });
+            }
             each([&](float v, int i) {
                 if (listed) {
-                    if (kept(v, i) && coarse(v) <= step2) put(v, i);
+                    if (kept(v, i) && v >= lowest) put(v, i);
                 } else {
                     const int b = in_step(v, i);
                     if (b >= 0) add(b, weigh(v));
                 }
             });
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                sum_above += __shfl_xor_sync(0xffffffffu, sum_above, o);
-                sum_below += __shfl_xor_sync(0xffffffffu, sum_below, o);
-            }
-            tell((uint64_t)sum_above, (uint64_t)sum_below);
-            uint64_t below = 0;
+            all = warp_total(all);
+            below = warp_total(below);
+            tell(all, below);
+            all = below = 0;
             for (int i = lane; i < C * SMP_WARPS; i += 32) {
-                above += sh.from[turn ^ 1][i][0];
+                all += sh.from[turn ^ 1][i][0];
                 below += sh.from[turn ^ 1][i][1];
             }
-            above = warp_total(above);
-            below = warp_total(below);
-            limit = (double)(above + below);           // (the sum of the others still to come)
+            all = warp_total(all);
+            limit = fmax((double)top_p * (double)all, 0.5);
+            above = all - warp_total(below);           // (and less by what the steps hold)
         } else {
             each([&](float v, int i) {
                 const int b = in_step(v, i);
@@ -424,8 +460,9 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             uint64_t total;
             uint32_t upto;
             const uint64_t sum = by_weight ? joined(1) + ((uint64_t)joined(2) << 16) + ((uint64_t)joined(3) << 32) : cnt;
-            const uint64_t before = block_scan(sum, cnt, total, upto) + above;
-            if (by_weight && !again) limit = fmax((double)top_p * (limit + (double)total), 0.5);
+            uint64_t before = block_scan(sum, cnt, total, upto);
+            if (by_weight && !again) above -= total;
+            before += above;
             // the last step that has elements and less than the limit above it
             const uint32_t here = __ballot_sync(0xffffffffu, cnt > 0 && (double)before < limit);
             if (lane == (here ? 31 - __clz(here) : 0)) {
@@ -470,7 +507,6 @@ template <typename T> __global__ void __launch_bounds__(SMP_THREADS, 2) sample_r
             shift = max(0, 64 - __clzll((long long)(hi - lo)) - 9);
         }
         if (by_weight && listed) {
-            limit = fmax((double)top_p * limit, 0.5);
             above = 0;
         } else {
             // the list: the step's elements, or all down to it
@@ -627,8 +663,8 @@ extern "C" int bn_sample_rows(const void* logits, int64_t row_stride, int dtype,
     while (c < SMP_CLUSTER && (cols > c * SMP_MOST || (rows > 8 && cols > c * SMP_TWO) || ((int64_t)rows * 2 * c <= sm_count() && cols > c * 1024))) c *= 2;
     p.slice = ((cols + c - 1) / c + 3) / 4 * 4;
     const size_t smem = (size_t)p.slice * 5;
-    auto* kernel = dtype == 0 ? sample_rows_kernel<float> : sample_rows_kernel<__nv_bfloat16>;
-    if (int rc = allow_smem(kernel, smem, what, SMP_MOST_SMEM, sizeof(SampleShared))) return rc;
+    p.bf16 = dtype;
+    if (int rc = allow_smem(sample_rows_kernel, smem, what, SMP_MOST_SMEM, sizeof(SampleShared))) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * c));
     cfg.blockDim = dim3(SMP_THREADS);
@@ -642,6 +678,6 @@ extern "C" int bn_sample_rows(const void* logits, int64_t row_stride, int dtype,
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    (void)launch_config(cfg, 1, kernel, p);
+    (void)launch_config(cfg, 1, sample_rows_kernel, p);
     return launch_status(what);
 }
