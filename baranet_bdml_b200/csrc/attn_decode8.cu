@@ -174,6 +174,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 
     if (warp == DEC8_QUERY_WARP) {
         // ---------------------------------------------------------- query warp: lane -> dims 2 * lane, + 1, of all heads
+        const double freq = p.freqs.f[lane];           // (of 32 different parameters a warp reads one at a time: not in every segment)
         for (int n = 0; iter.next(sc, sg, false); ++n) {
             const int buf = n % 2;
             const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + ((size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep) * (DEC_D / 2) + lane;
@@ -181,7 +182,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 #pragma unroll
             for (int h = 0; h < DEC_G; ++h) raw[h] = h < p.n_rep ? src[h * (DEC_D / 2)] : 0u;
             float c = 1.f, s = 0.f;
-            if (p.rope_q) rotation(p.q_positions ? p.q_positions[sg.b] : sg.L - 1, p.freqs.f[lane], &c, &s);
+            if (p.rope_q) rotation(p.q_positions ? p.q_positions[sg.b] : sg.L - 1, freq, &c, &s);
             if (!mbar_wait_warp(smem_u32(&q_free[buf]), (n / 2 & 1) ^ 1u, &s_abort)) break;
 #pragma unroll
             for (int h = 0; h < DEC_G; ++h) {

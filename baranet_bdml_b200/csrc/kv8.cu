@@ -40,12 +40,16 @@ struct Kv8AppendParams {
     RotationFreqs freqs;
 };
 
-// a group of lanes per (token, key head)
-template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_append_kernel(const Kv8AppendParams p) {
+// A group of lanes per (token, key head).  Where the four groups of a warp have the same token (a multiple of four heads), each works out
+// a quarter of its cosines and sines: they are most of the instructions.
+template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_append_kernel(const __grid_constant__ Kv8AppendParams p) {
+    __shared__ double freq[KV8_D / 2];                 // (32 lanes that read 32 parameters take 32 turns: once a block, not once a warp)
+    if (threadIdx.x < KV8_D / 2) freq[threadIdx.x] = p.freqs.f[threadIdx.x];
+    __syncthreads();
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
     const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / KV8_LANES;
-    const int part = threadIdx.x % KV8_LANES;
+    const int part = threadIdx.x % KV8_LANES, group = threadIdx.x % 32 / KV8_LANES;
     const bool there = unit < (int64_t)p.T * p.Hkv;
     const int t = there ? (int)(unit / p.Hkv) : 0, g = there ? (int)(unit % p.Hkv) : 0;
     const int pos = p.positions[t], seq = p.seq_ids[t], slot = pos % BN_PAGE_TOKENS;
@@ -56,13 +60,24 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_app
     load8(static_cast<const T*>(p.k) + t * p.k_stride + g * KV8_D + part * KV8_PER, p.wide, k);
     load8(static_cast<const T*>(p.v) + t * p.v_stride + g * KV8_D + part * KV8_PER, p.wide, v);
     if (p.rotate) {
+        float c[4], s[4];
+        if (p.Hkv % 4 == 0) {
+            float c1, s1;
+            rotation(pos, freq[part * 4 + group], &c1, &s1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                c[i] = __shfl_sync(0xffffffffu, c1, i * KV8_LANES + part);
+                s[i] = __shfl_sync(0xffffffffu, s1, i * KV8_LANES + part);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rotation(pos, freq[part * 4 + i], &c[i], &s[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float c, s;
-            rotation(pos, p.freqs.f[part * 4 + i], &c, &s);
             const float a = k[2 * i], b = k[2 * i + 1];
-            k[2 * i] = a * c - b * s;
-            k[2 * i + 1] = a * s + b * c;
+            k[2 * i] = a * c[i] - b * s[i];
+            k[2 * i + 1] = a * s[i] + b * c[i];
         }
     }
     const float ks = kv8_scale<VALUES>(group_most(k)), vs = kv8_scale<VALUES>(group_most(v));
@@ -85,12 +100,13 @@ struct Kv8GatherParams {
     int num_seqs, max_pages, n_tokens, Hkv;
 };
 
-// a group of lanes per (row of the result, key head)
+// Four lanes per (row of the result, key head), 16 bytes of K and of V each
+constexpr int KV8_GLANES = 4;
 template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8GatherParams p) {
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / KV8_LANES;
-    const int part = threadIdx.x % KV8_LANES;
+    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / KV8_GLANES;
+    const int part = threadIdx.x % KV8_GLANES;
     if (unit >= p.units) return;
     const int64_t row = unit / p.Hkv;
     const int g = (int)(unit % p.Hkv), i = (int)(row / p.n_tokens);
@@ -101,23 +117,33 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_gat
         page = p.page_table[(int64_t)seq * p.max_pages + pos / BN_PAGE_TOKENS];
     const bool there = page >= 0 && page < p.pool_pages;
     const int slot = there ? (int)(pos % BN_PAGE_TOKENS) : 0;
-    const uint8_t* block = p.pool + ((int64_t)(there ? page : 0) * p.Hkv + g) * BN_KV8_BLOCK;
-    uint2 kb = make_uint2(0u, 0u), vb = kb;
+    uint4 kb = make_uint4(0u, 0u, 0u, 0u), vb = kb;
     uint32_t scales = 0u;
     if (there) {
-        kb = *reinterpret_cast<const uint2*>(block + slot * KV8_D + part * KV8_PER);
-        vb = *reinterpret_cast<const uint2*>(block + KV8_V + slot * KV8_D + kv8_v_place(slot, part * KV8_PER));
+        const uint8_t* block = p.pool + ((int64_t)page * p.Hkv + g) * BN_KV8_BLOCK;
+        kb = *reinterpret_cast<const uint4*>(block + slot * KV8_D + part * 16);
+        vb = *reinterpret_cast<const uint4*>(block + KV8_V + slot * KV8_D + kv8_v_place(slot, part * 16));
         scales = *reinterpret_cast<const uint32_t*>(block + KV8_SCALES + slot * 4);
     }
-    auto put = [&](void* out, uint2 b, float scale) {
-        T* dst = static_cast<T*>(out) + unit * KV8_D + part * KV8_PER;
+    auto put = [&](void* out, uint4 b, float scale) {
+        T* dst = static_cast<T*>(out) + unit * KV8_D + part * 16;
+        const uint32_t words[4] = {b.x, b.y, b.z, b.w};
+        float o[16];
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
+        for (int w = 0; w < 4; ++w) {
             uint32_t lo, hi;
-            kv8_halves<VALUES>(w ? b.y : b.x, lo, hi);
+            kv8_halves<VALUES>(words[w], lo, hi);
             const float2 x = halves_to_floats(lo), y = halves_to_floats(hi);
-            const float o[4] = {there ? x.x * scale : 0.f, there ? x.y * scale : 0.f, there ? y.x * scale : 0.f, there ? y.y * scale : 0.f};
-            store4(dst + 4 * w, o);
+            o[4 * w] = x.x * scale; o[4 * w + 1] = x.y * scale; o[4 * w + 2] = y.x * scale; o[4 * w + 3] = y.y * scale;
+        }
+        if (sizeof(T) == 2) {
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+                reinterpret_cast<uint4*>(dst)[w] = make_uint4(ptx::pack_bf16(o[8 * w], o[8 * w + 1]), ptx::pack_bf16(o[8 * w + 2], o[8 * w + 3]),
+                                                              ptx::pack_bf16(o[8 * w + 4], o[8 * w + 5]), ptx::pack_bf16(o[8 * w + 6], o[8 * w + 7]));
+        } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) reinterpret_cast<float4*>(dst)[w] = make_float4(o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]);
         }
     };
     put(p.k, kb, ptx::bf16_lo(scales));
@@ -161,8 +187,7 @@ extern "C" int bn_kv8_append(void* pool, int64_t pool_pages, const int32_t* page
     if (rotate) p.freqs = rotation_freqs(theta);
     auto* kernel = dtype == 0 ? (values == BN_KV8_E4M3 ? kv8_append_kernel<float, BN_KV8_E4M3> : kv8_append_kernel<float, BN_KV8_INT8>)
                               : (values == BN_KV8_E4M3 ? kv8_append_kernel<__nv_bfloat16, BN_KV8_E4M3> : kv8_append_kernel<__nv_bfloat16, BN_KV8_INT8>);
-    const unsigned blocks = (unsigned)(((int64_t)T * Hkv * KV8_LANES + 255) / 256);
-    launch_dependent(kernel, blocks, 256, 0, as_stream(stream), p);
+    launch_dependent(kernel, (unsigned)(((int64_t)T * Hkv * KV8_LANES + 255) / 256), 256, 0, as_stream(stream), p);
     return launch_status(what);
 }
 
@@ -187,6 +212,6 @@ extern "C" int bn_kv8_gather(const void* pool, int64_t pool_pages, const int32_t
     p.num_seqs = num_seqs; p.max_pages = max_pages; p.n_tokens = n_tokens; p.Hkv = Hkv;
     auto* kernel = out_dtype == 0 ? (values == BN_KV8_E4M3 ? kv8_gather_kernel<float, BN_KV8_E4M3> : kv8_gather_kernel<float, BN_KV8_INT8>)
                                   : (values == BN_KV8_E4M3 ? kv8_gather_kernel<__nv_bfloat16, BN_KV8_E4M3> : kv8_gather_kernel<__nv_bfloat16, BN_KV8_INT8>);
-    launch_dependent(kernel, (unsigned)((units * KV8_LANES + 255) / 256), 256, 0, as_stream(stream), p);
+    launch_dependent(kernel, (unsigned)((units * KV8_GLANES + 255) / 256), 256, 0, as_stream(stream), p);
     return launch_status(what);
 }

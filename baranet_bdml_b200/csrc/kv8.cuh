@@ -53,7 +53,9 @@ template <int VALUES> __device__ __forceinline__ float kv8_scale(uint32_t most_b
         const int e = (int)(most_bits >> 23) - 8 + ((most_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
         b = e > 0 ? (uint32_t)e << 23 : 0u;
     } else {
-        b = (__float_as_uint(__fdiv_ru(__uint_as_float(most_bits), 127.f)) + 0xffffu) & 0xffff0000u;
+        // the bf16 number at or below the quotient, or the next: 127 times it is exact
+        b = __float_as_uint(__uint_as_float(most_bits) * (1.f / 127.f)) & 0xffff0000u;
+        if (127.f * __uint_as_float(b) < __uint_as_float(most_bits)) b += 0x10000u;
     }
     return __uint_as_float(min(max(b, KV8_LEAST), KV8_MOST));
 }
@@ -68,8 +70,22 @@ template <int VALUES> __device__ __forceinline__ uint32_t kv8_pack(float a, floa
         asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d * inv), "f"(c * inv));
         return (uint32_t)lo | (uint32_t)hi << 16;
     }
-    auto one = [&](float v) { return (uint32_t)(max(-127, min(127, __float2int_rn(__fdiv_rn(v, scale)))) & 0xff); };
-    return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+    // x / scale to the nearest whole number: by the reciprocal, whose product is off by less than 2^-14, and by the division itself where
+    // that could put it on the other side of a tie
+    const float inv = __fdividef(1.f, scale), x[4] = {a, b, c, d};
+    uint32_t bits[4];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float q = fminf(fmaxf(x[i] * inv, -127.f), 127.f), whole = q + 12582912.f;          // 1.5 * 2^23: the whole number is in the low bits
+        near |= fabsf(q - (whole - 12582912.f)) > 0.5f - 6.1035156e-5f;
+        bits[i] = __float_as_uint(whole);
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bits[i] = __float_as_uint(fminf(fmaxf(__fdiv_rn(x[i], scale), -127.f), 127.f) + 12582912.f);
+    }
+    return __byte_perm(__byte_perm(bits[0], bits[1], 0x0040), __byte_perm(bits[2], bits[3], 0x0040), 0x5410);
 }
 
 // bytes (0, 1) and (2, 3) of a word as two fp16 each

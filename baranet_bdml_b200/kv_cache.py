@@ -84,14 +84,12 @@ class PagedKVCache:
         key = (B, Hq, max_seq_len, chunk_tokens)
         ws = self._ws.get(key)
         if ws is None:
-            n = self._workspace_bytes(B, Hq, max_seq_len, chunk_tokens)
+            n = _lib.load().bn_attn_decode_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len,
+                                                          chunk_tokens)
             if n == 0:
                 raise RuntimeError("bn_attn_decode_paged: unsupported shape")
             ws = self._ws[key] = Workspace(n, self.pool.device)
         return ws
-
-    def _workspace_bytes(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int) -> int:
-        return _lib.load().bn_attn_decode_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len, chunk_tokens)
 
     def status(self) -> None:
         """Raises if a decode launch on any of this cache's scratch buffers gave up on a bounded wait."""
@@ -148,15 +146,20 @@ class QuantizedKVCache(PagedKVCache):
         self.values = values
 
     def _here(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
-        dev = self.pool.device
-        if dev.type != "cuda":
+        dev = self.pool.get_device()
+        if dev < 0:
             raise RuntimeError(f"{what}: only GPU implementation available")
-        if dev.index != torch.cuda.current_device() or any(t is not None and t.device != dev for t in tensors):
-            raise RuntimeError(f"{what}: all tensors must lie on the cache's device, and it must be the current one")
-
-    def _ids(self, what: str, n: int, *tensors: torch.Tensor) -> None:
+        if dev != torch.cuda.current_device():
+            raise RuntimeError(f"{what}: the cache's device must be the current one")
         for t in tensors:
-            _need(t, torch.int32, what)
+            if t is not None and t.get_device() != dev:
+                raise RuntimeError(f"{what}: all tensors must lie on the cache's device")
+
+    @staticmethod
+    def _ids(what: str, n: int, *tensors: torch.Tensor) -> None:
+        for t in tensors:
+            if t.dtype != torch.int32 or not t.is_contiguous():
+                _need(t, torch.int32, what)
             if t.numel() != n:
                 raise RuntimeError(f"{what}: {t.numel()} ids, positions or lengths where there are {n} rows")
 
@@ -165,20 +168,21 @@ class QuantizedKVCache(PagedKVCache):
         position unless `rotated` says that it is.  A (sequence, position) may occur once; tokens outside the cache are left
         out.  Does not touch seq_lens (the caller advances them)."""
         what = "kv append"
-        if k_new.dtype not in (torch.float32, torch.bfloat16) or v_new.dtype != k_new.dtype:
+        f32 = k_new.dtype == torch.float32
+        if not (f32 or k_new.dtype == torch.bfloat16) or v_new.dtype != k_new.dtype:
             raise RuntimeError(f"{what}: k/v must both be fp32 or both bf16")
         self._here(what, seq_ids, positions, k_new, v_new)
-        T, width = k_new.shape[0], self.num_kv_heads * self.head_dim
-        for t in (k_new, v_new):
-            if t.dim() != 2 or t.shape != (T, width) or t.stride(1) != 1:
-                raise RuntimeError(f"{what}: k/v must be rows of {width} contiguous elements, as many of each")
+        shape, width = k_new.shape, self.num_kv_heads * self.head_dim
+        if len(shape) != 2 or shape[1] != width or v_new.shape != shape or k_new.stride(1) != 1 or v_new.stride(1) != 1:
+            raise RuntimeError(f"{what}: k/v must be rows of {width} contiguous elements, as many of each")
+        T = shape[0]
         self._ids(what, T, seq_ids, positions)
         if T == 0:
             return
         _lib.check(_lib.load().bn_kv8_append(
             self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, seq_ids.data_ptr(), positions.data_ptr(), T,
-            k_new.data_ptr(), k_new.stride(0), v_new.data_ptr(), v_new.stride(0), 0 if k_new.dtype == torch.float32 else 1, KV8_VALUES[self.values],
-            int(not rotated), self.num_kv_heads, self.head_dim, self.theta, _stream()))
+            k_new.data_ptr(), k_new.stride(0), v_new.data_ptr(), v_new.stride(0), 0 if f32 else 1, KV8_VALUES[self.values], int(not rotated),
+            self.num_kv_heads, self.head_dim, self.theta, _stream()))
 
     def gather(self, seq_ids: torch.Tensor, starts: torch.Tensor, n_tokens: int, *, dtype=torch.bfloat16):
         """What the cache holds of sequence seq_ids[i] from position starts[i] on: K (rotated, as it is stored) and V, each
@@ -191,16 +195,22 @@ class QuantizedKVCache(PagedKVCache):
         self._here(what, seq_ids, starts)
         n = seq_ids.numel()
         self._ids(what, n, seq_ids, starts)
-        k, v = (torch.empty((n, n_tokens, self.num_kv_heads, self.head_dim), dtype=dtype, device=self.pool.device) for _ in range(2))
-        if k.numel():
+        k, v = torch.empty((2, n, n_tokens, self.num_kv_heads, self.head_dim), dtype=dtype, device=self.pool.device).unbind(0)
+        if n and n_tokens:
             _lib.check(_lib.load().bn_kv8_gather(
                 self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, self.seq_lens.data_ptr(),
                 seq_ids.data_ptr(), starts.data_ptr(), n, n_tokens, k.data_ptr(), v.data_ptr(), 0 if dtype == torch.float32 else 1,
                 KV8_VALUES[self.values], self.num_kv_heads, self.head_dim, _stream()))
         return k, v
 
-    def _workspace_bytes(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int) -> int:
-        return _lib.load().bn_attn_decode_kv8_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len, chunk_tokens)
+    def workspace(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int = 0) -> Workspace:
+        """The decode scratch: one for all shapes, kept while the cache lives (a captured graph may hold its address)."""
+        n = _lib.load().bn_attn_decode_kv8_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len, chunk_tokens)
+        if n == 0:
+            raise RuntimeError("bn_attn_decode_kv8: unsupported shape")
+        if () not in self._ws:
+            self._ws[()] = Workspace(n, self.pool.device)
+        return self._ws[()]
 
     def decode(self, q: torch.Tensor, *, num_heads: int, scale: Optional[float] = None, rope_q: bool = True,
                q_positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -209,32 +219,38 @@ class QuantizedKVCache(PagedKVCache):
                page_table: Optional[torch.Tensor] = None) -> torch.Tensor:
         """q (B, Hq, D) bf16 (pre-RoPE when rope_q) -> out (B, Hq, D) bf16, as PagedKVCache.decode."""
         what = "decode"
-        _need(q, torch.bfloat16, f"{what}(q)")
-        seq_lens = self.seq_lens if seq_lens is None else seq_lens
-        page_table = self.page_table if page_table is None else page_table
+        if q.dtype != torch.bfloat16 or not q.is_contiguous():
+            _need(q, torch.bfloat16, f"{what}(q)")
+        if seq_lens is None:
+            seq_lens = self.seq_lens
+        if page_table is None:
+            page_table = self.page_table
         self._here(what, q, seq_lens, page_table, q_positions, out, out_f32, lse)
-        if q.dim() != 3 or q.shape[1] != num_heads or q.shape[2] != self.head_dim:
-            raise RuntimeError(f"{what}: q must be (B, {num_heads}, {self.head_dim}), got {tuple(q.shape)}")
-        B, Hq, D = q.shape
-        self._ids(what, B, seq_lens, *([] if q_positions is None else [q_positions]))
-        _need(page_table, torch.int32, f"{what}(page_table)")
-        if page_table.dim() != 2 or page_table.shape[0] < B:
+        shape = q.shape
+        if len(shape) != 3 or shape[1] != num_heads or shape[2] != self.head_dim:
+            raise RuntimeError(f"{what}: q must be (B, {num_heads}, {self.head_dim}), got {tuple(shape)}")
+        B, Hq, D = shape
+        self._ids(what, B, seq_lens)
+        if q_positions is not None:
+            self._ids(what, B, q_positions)
+        if page_table.dtype != torch.int32 or not page_table.is_contiguous():
+            _need(page_table, torch.int32, f"{what}(page_table)")
+        rows, width = page_table.shape if page_table.dim() == 2 else (-1, 0)
+        if rows < B:
             raise RuntimeError(f"{what}: a page table of {tuple(page_table.shape)} for {B} sequences")
-        for t, dtype, shape in ((out, torch.bfloat16, q.shape), (out_f32, torch.float32, q.shape), (lse, torch.float32, q.shape[:2])):
-            if t is not None:
-                _need(t, dtype, f"{what}(out)")
-                if t.numel() != shape.numel():
-                    raise RuntimeError(f"{what}: an output of {tuple(t.shape)} where {tuple(shape)} is written")
+        for t, dtype, n in ((out, torch.bfloat16, B * Hq * D), (out_f32, torch.float32, B * Hq * D), (lse, torch.float32, B * Hq)):
+            if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.numel() != n):
+                raise RuntimeError(f"{what}: an output must be a contiguous {dtype} tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
         if out is None and out_f32 is None:
             out = torch.empty_like(q)
         if max_seq_len is None:
-            max_seq_len = page_table.shape[1] * PAGE_TOKENS
+            max_seq_len = width * PAGE_TOKENS
         if scale is None:
             scale = 1.0 / (D ** 0.5)
         if B:
-            ws = self.workspace(B, Hq, max_seq_len, chunk_tokens)
+            ws = self._ws.get(()) or self.workspace(B, Hq, max_seq_len, chunk_tokens)
             _lib.check(_lib.load().bn_attn_decode_kv8(
-                q.data_ptr(), self.pool.data_ptr(), self.num_pages, page_table.data_ptr(), page_table.shape[1], seq_lens.data_ptr(),
+                q.data_ptr(), self.pool.data_ptr(), self.num_pages, page_table.data_ptr(), width, seq_lens.data_ptr(),
                 q_positions.data_ptr() if q_positions is not None else None, out.data_ptr() if out is not None else None,
                 out_f32.data_ptr() if out_f32 is not None else None, lse.data_ptr() if lse is not None else None, KV8_VALUES[self.values], B, Hq,
                 self.num_kv_heads, D, float(scale), self.theta, int(bool(rope_q)), int(max_seq_len), int(chunk_tokens), ws.ptr, ws.nbytes, _stream()))

@@ -745,40 +745,39 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0,
     int32 for top_k); a number is taken as fp32.  temperature 0: the first maximum.  Equals are taken in the order of their ids, NaN
     counts as -inf, and a row with nothing above -inf gives 0."""
     what = "sample_rows"
-    if not logits.is_cuda:
+    dev = logits.get_device()
+    if dev < 0:
         raise RuntimeError(f"{what}: only GPU implementation available")
-    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16) or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    f32, shape = logits.dtype == torch.float32, logits.shape
+    if len(shape) != 2 or not (f32 or logits.dtype == torch.bfloat16) or (shape[1] > 1 and logits.stride(1) != 1):
         raise RuntimeError(f"{what}: expected fp32 or bf16 logits (rows, vocab) with contiguous rows")
-    (rows, vocab), dev = logits.shape, logits.device
+    rows, vocab = shape
     if vocab == 0:
         raise RuntimeError(f"{what}: no columns to choose from")
-    if dev.index != torch.cuda.current_device():
+    if dev != torch.cuda.current_device():
         raise RuntimeError(f"{what}: all tensors must lie on the current device")
 
     def per_row(t, dtype):
-        _operands(what, t, dtype=dtype)
-        if t.shape != (rows,):
-            raise RuntimeError(f"{what}: {tuple(t.shape)} values where there are {rows} rows")
+        if t.dtype != dtype or t.get_device() != dev or t.shape != (rows,) or not t.is_contiguous():
+            raise RuntimeError(f"{what}: expected a contiguous {dtype} tensor of {rows} values on the current device, got {t.dtype} {tuple(t.shape)}")
         return t.data_ptr()
 
     args = []
     for v, dtype, lo, hi, name in ((temperature, torch.float32, 0.0, 3.0e38, "temperature"), (top_k, torch.int32, 0, 2 ** 31 - 1, "top_k"),
                                    (top_p, torch.float32, 0.0, 1.0, "top_p"), (min_p, torch.float32, 0.0, 1.0, "min_p")):
-        args += [per_row(v, dtype), type(lo)(0)] if isinstance(v, torch.Tensor) else [None, _within(what, name, v, lo, hi)]
+        if isinstance(v, torch.Tensor):
+            args += (per_row(v, dtype), type(lo)(0))
+        elif lo <= v <= hi:
+            args += (None, type(lo)(v))
+        else:
+            raise RuntimeError(f"{what}: {name}={v} (from {lo} to {hi})")
     u = per_row(uniform, torch.float32)
     if out is None:
-        out = torch.empty((rows,), dtype=torch.int32, device=dev)
-    per_row(out, torch.int32)
+        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
+    o = per_row(out, torch.int32)
     if rows:
-        _lib.check(_lib.load().bn_sample_rows(logits.data_ptr(), max(logits.stride(0), vocab) if rows == 1 else logits.stride(0),
-                                              0 if logits.dtype == torch.float32 else 1, u, *args, out.data_ptr(), rows, vocab, _stream()))
+        _lib.check(_lib.load().bn_sample_rows(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, 0 if f32 else 1, u, *args, o, rows, vocab, _stream()))
     return out
-
-
-def _within(what: str, name: str, v, lo, hi):
-    if not lo <= v <= hi:
-        raise RuntimeError(f"{what}: {name}={v} (from {lo} to {hi})")
-    return type(lo)(v)
 
 
 def tensors_of(value) -> list:
