@@ -130,6 +130,7 @@ SIGNATURES = {
     "bn_gated_ff_backward_bf16": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p, _sz, _p, _p]),
     "bn_attn_prefill_bf16_backward_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),
     "bn_attn_prefill_bf16_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _f, _i, _i, _p, _sz, _p, _p]),
+    "bn_attn_prefill_bf16_rotated_k": (_sz, [_i, _i, _i, _i]),
     "bn_kv8_append": (_i, [_p, _i64, _p, _i, _i, _p, _p, _i, _p, _i64, _p, _i64, _i, _i, _i, _i, _i, _f, _p]),
     "bn_kv8_gather": (_i, [_p, _i64, _p, _i, _i, _p, _p, _p, _i, _i, _p, _p, _i, _i, _i, _i, _p]),
     "bn_attn_decode_kv8_workspace_bytes": (_sz, [_i, _i, _i, _i, _i, _i]),

@@ -1222,6 +1222,11 @@ extern "C" size_t bn_attn_prefill_bf16_workspace_bytes(int B, int S, int Hq, int
     return prefill_layout(B, S, Hkv).total;
 }
 
+extern "C" size_t bn_attn_prefill_bf16_rotated_k(int B, int S, int Hkv, int D) {
+    if (B <= 0 || S <= 0 || Hkv <= 0 || D != PF_D) return 0;
+    return prefill_layout(B, S, Hkv).krot;
+}
+
 extern "C" int bn_attn_prefill_bf16_table(int B, int S, int Hkv, int D, float theta, int position_offset, void* workspace,
                                           size_t workspace_bytes, bn_stream_t stream) {
     if (B <= 0 || S <= 0 || Hkv <= 0 || position_offset < 0)

@@ -1,4 +1,4 @@
-"""Paged bf16 KV cache and single-token decode.
+"""Paged KV caches, bf16 and in 8 bits, and single-token decode.
 
 The reference has no cache: `generate()` recomputes the whole sequence for
 every new token and keeps the last row (mygrad/llama/llama_model.py:136-144).
@@ -21,6 +21,12 @@ from .ops import Workspace, _need, _stream
 
 PAGE_TOKENS = _lib.BN_PAGE_TOKENS
 KV8_VALUES = {"e4m3": _lib.BN_KV8_E4M3, "int8": _lib.BN_KV8_INT8}
+
+
+def token_rows(B: int, S: int, first: int = 0, device="cuda"):
+    """(sequence, position) of S tokens of each of B sequences, from position `first` on, row after row"""
+    seqs = torch.arange(B, dtype=torch.int32, device=device).repeat_interleave(S)
+    return seqs, torch.arange(first, first + S, dtype=torch.int32, device=device).repeat(B)
 
 
 class ZeroedTogether:

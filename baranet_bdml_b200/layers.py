@@ -228,12 +228,15 @@ class GroupedQueryAttentionBF16:
         return stack if row == stack.shape[0] else torch.cat(weights)
 
     def attend(self, x2, B: int, S: int, position_offset: int = 0, use_causal_mask: bool = True, cache=None,
-               workspace=None):
+               workspace=None, cache_rows=None):
         """x2 (B*S, hidden) bf16 -> attention output before o_proj, (B*S, hidden): ONE GEMM for q, k, v with the K
         rotation (and, with `cache`, the append of K and V at positions position_offset ..) in its epilogue, then the
         fused attention kernel on the rotated K it left in the scratch buffer.  head_dim 64.  A caller that passes
-        its own `workspace` keeps its cos/sin table current itself (ops.prefill_table)."""
+        its own `workspace` keeps its cos/sin table current itself (ops.prefill_table).  A cache in 8 bits takes the rotated
+        K and V in a launch of its own; `cache_rows`: (sequence, position) of the B*S rows, where the caller has them."""
         from . import ops
+        from .kv_cache import QuantizedKVCache, token_rows
+        eight = isinstance(cache, QuantizedKVCache)
         if workspace is None:
             key = (B, S)
             if self._ws is None or self._ws[0] != key:
@@ -245,7 +248,10 @@ class GroupedQueryAttentionBF16:
                 ops.prefill_table(workspace, B, S, self.num_kv_heads, self.head_dim, self.rotary_emb.base, position_offset)
                 self._ws_table = tkey
         q, v = ops.gemm_qkv_rope_bf16(x2, self.packed_qkv(), B, S, self.num_heads, self.num_kv_heads, self.head_dim,
-                                      workspace, position_offset=position_offset, cache=cache)
+                                      workspace, position_offset=position_offset, cache=None if eight else cache)
+        if eight:
+            cache.append(*(cache_rows or token_rows(B, S, position_offset, x2.device)), ops.rotated_k(workspace, B, S, self.num_kv_heads, self.head_dim),
+                         v.view(B * S, -1), rotated=True)
         attn = ops.attn_prefill_bf16(q, None, v, scale=float(self.scale), theta=self.rotary_emb.base,
                                      position_offset=position_offset, causal=use_causal_mask, workspace=workspace,
                                      reuse_rotated_k=True)

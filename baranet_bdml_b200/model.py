@@ -6,17 +6,19 @@ composed from the rows of this package: device-side embedding gather, `LLaMADeco
 and for every new token one row per sequence through the same weights with `bn_kv_append` + `bn_attn_decode_paged`
 instead of attention over the recomputed sequence (the reference recomputes the whole sequence for every token and
 keeps the last row, llama_model.py:136-144), then the final norm, the lm_head GEMM and a device-side argmax.
-Greedy decoding only (temperature / top-k sampling of the reference is host code).  Inference only.
+The next token is the first maximum, or sampled on the device (temperature and top-k as the reference's host code has them, top-p
+and min-p).  Inference only.
 """
 from __future__ import annotations
 
+from functools import partial
 from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
 
 from . import _lib, ops
-from .kv_cache import PAGE_TOKENS, PagedKVCache, SequenceSlots, ZeroedTogether
+from .kv_cache import KV8_VALUES, PAGE_TOKENS, PagedKVCache, QuantizedKVCache, SequenceSlots, ZeroedTogether, token_rows
 from .layers import LLaMAConfig, LLaMADecoderLayerBF16
 
 
@@ -52,38 +54,56 @@ class CausalLM:
                                                   rows, cols, ops._stream()))
         return out
 
-    def capture_decode_step(self):
-        """Captures `decode_step` + argmax for the current batch into a CUDA graph: a step is tens of launches that
+    def choose(self, logits: torch.Tensor, uniform: Optional[torch.Tensor] = None, **how) -> torch.Tensor:
+        """The next ids: the first maxima, or, given random numbers in [0, 1) (rows) fp32, ops.sample_rows with its `how`
+        (temperature, top_k, top_p, min_p)."""
+        if uniform is None:
+            if how:
+                raise RuntimeError("choose: sampling needs its random numbers")
+            return self.argmax(logits)
+        return ops.sample_rows(logits, uniform, **how)
+
+    def capture_decode_step(self, **how):
+        """Captures `decode_step` + `choose` for the current batch into a CUDA graph: a step is tens of launches that
         Python issues one by one (the host, not the GPU, bounds it); replayed from a graph they are one submission.
-        Returns step(token_ids) -> (logits, next_ids), both static buffers overwritten by the next call.  Lengths (and
-        states) advance inside the graph, so every replay is the next position."""
+        Returns step(token_ids) -> (logits, next_ids), both static buffers overwritten by the next call; with `how` (what
+        ops.sample_rows takes; tensors among them are read at the replay) step(token_ids, uniform).  Lengths (and states)
+        advance inside the graph, so every replay is the next position."""
         B = self.seq_lens.numel()
         static_tok = torch.zeros((B,), dtype=torch.int32, device="cuda")
+        static_u = torch.zeros((B,), dtype=torch.float32, device="cuda") if how else None
         saved = [t.clone() for t in self.state_tensors()]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):                      # warm-up outside the capture (workspaces, attributes)
-            self.decode_step(static_tok, check=False)
+            self.choose(self.decode_step(static_tok, check=False), static_u, **how)
         torch.cuda.current_stream().wait_stream(side)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             logits = self.decode_step(static_tok, check=False)
-            nxt = self.argmax(logits)
+            nxt = self.choose(logits, static_u, **how)
         torch.cuda.synchronize()
         for t, v in zip(self.state_tensors(), saved):      # warm-up and capture must not count as positions
             t.copy_(v)
 
-        def step(token_ids: torch.Tensor):
+        def step(token_ids: torch.Tensor, uniform: Optional[torch.Tensor] = None):
+            if (uniform is None) != (static_u is None):
+                raise RuntimeError("step: random numbers belong to a step that samples, and to no other")
             static_tok.copy_(token_ids)
+            if uniform is not None:
+                static_u.copy_(uniform)
             graph.replay()
             return logits, nxt
 
         step.graph = graph
         return step
 
-    def generate(self, input_ids, max_new_tokens: int = 50) -> List[List[int]]:
-        """Greedy `generate` (llama_model.py:112-168 with temperature -> 0): prompts (B, S) of equal length, or, where the
-        family takes them (`ragged_prompts`), a list of id lists of any lengths."""
+    def generate(self, input_ids, max_new_tokens: int = 50, *, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                 seed: Optional[int] = None) -> List[List[int]]:
+        """`generate` (llama_model.py:112-168): prompts (B, S) of equal length, or, where the family takes them
+        (`ragged_prompts`), a list of id lists of any lengths.  temperature 0: greedy; above, sampled as ops.sample_rows does it,
+        every sequence with random numbers of its own.  The same `seed` gives the same tokens; None: torch's generator of
+        the current device."""
         rows = [np.asarray(r, dtype=np.int32).reshape(-1) for r in (input_ids if np.ndim(input_ids[0]) else [input_ids])]
         if any(len(r) == 0 for r in rows):
             raise ValueError("generate: empty prompt")
@@ -94,11 +114,16 @@ class CausalLM:
             prompts = rows
         else:
             raise ValueError("generate: this model takes prompts of equal length")
+        how, uniform = {}, None
+        if temperature != 0.0:
+            how = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            gen = None if seed is None else torch.Generator(device="cuda").manual_seed(seed)
+            uniform = torch.rand((max_new_tokens, B), generator=gen, device="cuda")
         logits = self.prefill(prompts, longest + max_new_tokens)
         out = [list(map(int, r)) for r in rows]
         done = [False] * B
         for n in range(max_new_tokens):
-            nxt = self.argmax(logits)
+            nxt = self.choose(logits, None if uniform is None else uniform[n], **how)
             host = nxt.cpu().numpy()
             for b in range(B):
                 if not done[b]:
@@ -239,10 +264,13 @@ class SequenceLM(CausalLM):
 
 
 class LLaMAModelBF16(CausalLM):
-    def __init__(self, config: LLaMAConfig, is_cuda: bool = True):
+    """`kv_cache`: what the caches of the next prompt hold, "bf16", or "e4m3" or "int8" (8 bits and a scale for each token and key head;
+    the prompt's own attention runs in bf16 either way)."""
+
+    def __init__(self, config: LLaMAConfig, is_cuda: bool = True, kv_cache: str = "bf16"):
         if not is_cuda:
             raise RuntimeError("LLaMAModelBF16: only GPU implementation available")
-        self.config = config
+        self.config, self.kv_cache = config, kv_cache
         # embed_tokens as the reference initialises it (llama_model.py:44-50: normal, std 0.02), fp32 table
         self.embed_tokens = torch.from_numpy(
             (np.random.randn(config.vocab_size, config.hidden_size) * 0.02).astype(np.float32)).cuda()
@@ -307,19 +335,23 @@ class LLaMAModelBF16(CausalLM):
         return -loss.view(B, S)[:, :-1]
 
     def _alloc_caches(self, B: int, max_len: int):
-        cfg = self.config
+        cfg, kind = self.config, self.kv_cache
+        if kind != "bf16" and kind not in KV8_VALUES:
+            raise RuntimeError(f"LLaMAModelBF16: kv_cache {kind!r} (bf16, {', '.join(KV8_VALUES)})")
         pages_per_seq = (max_len + PAGE_TOKENS - 1) // PAGE_TOKENS
         self.caches = []              # those of an earlier prompt make room first
         # every block holds the same tokens: ONE length vector, advanced once per step; the pools are zeroed by one launch, and the
         # page tables are parts of one tensor
         n, pages = len(self.layers), B * pages_per_seq
         zeros = ZeroedTogether()
-        pools = [zeros((pages, cfg.num_key_value_heads, 2, PAGE_TOKENS, cfg.head_dim), dtype=torch.bfloat16, device="cuda") for _ in range(n)]
+        shape, dtype = ((2, PAGE_TOKENS, cfg.head_dim), torch.bfloat16) if kind == "bf16" else ((_lib.BN_KV8_BLOCK,), torch.uint8)
+        pools = [zeros((pages, cfg.num_key_value_heads, *shape), dtype=dtype, device="cuda") for _ in range(n)]
         zeros.fill()
         tables = torch.arange(pages, dtype=torch.int32, device="cuda").view(B, pages_per_seq).repeat(n, 1, 1)
         lens = torch.zeros((B,), dtype=torch.int32, device="cuda")
-        self.caches = [PagedKVCache(pages, B, pages_per_seq, cfg.num_key_value_heads, cfg.head_dim, cfg.rope_theta,
-                                    storage=(pools[i], tables[i], lens)) for i in range(n)]
+        make = PagedKVCache if kind == "bf16" else partial(QuantizedKVCache, values=kind)
+        self.caches = [make(pages, B, pages_per_seq, cfg.num_key_value_heads, cfg.head_dim, cfg.rope_theta,
+                            storage=(pools[i], tables[i], lens)) for i in range(n)]
         self.seq_lens = self.caches[0].seq_lens
         self.caches[0].seq_ids = torch.arange(B, dtype=torch.int32, device="cuda")      # as old as the caches: a captured step reads it
 
@@ -337,13 +369,14 @@ class LLaMAModelBF16(CausalLM):
         # one scratch buffer for all blocks (they run one after the other): cos/sin table written once
         ws = ops.prefill_workspace(B, S, cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim)
         ops.prefill_table(ws, B, S, cfg.num_key_value_heads, cfg.head_dim, cfg.rope_theta, 0)
+        rows = None if self.kv_cache == "bf16" else token_rows(B, S)
         for layer, cache in zip(self.layers, self.caches):
             x2 = h.reshape(B * S, H)
             residual, normed = ops.add_rmsnorm_bf16(x2, None if pending is None else pending.reshape(B * S, H),
                                                     layer.input_layernorm_weight, layer.eps)
             at = layer.self_attn
             # q/k/v in one GEMM whose epilogue rotates K and appends K and V to this block's cache
-            attn = at.attend(normed, B, S, 0, True, cache=cache, workspace=ws)
+            attn = at.attend(normed, B, S, 0, True, cache=cache, workspace=ws, cache_rows=rows)
             o = ops.gemm_bf16_nt(attn, at.o_proj)
             residual, normed = ops.add_rmsnorm_bf16(residual, o, layer.post_attention_layernorm_weight, layer.eps)
             h, pending = residual.view(B, S, H), layer.mlp(normed).view(B, S, H)
@@ -368,7 +401,11 @@ class LLaMAModelBF16(CausalLM):
             residual, normed = ops.add_rmsnorm_bf16(h, pending, layer.input_layernorm_weight, layer.eps)
             at = layer.self_attn
             kv = at.num_kv_heads * at.head_dim
-            if ops.skinny_ok(B, at.hidden_size + 2 * kv, normed.shape[1]):
+            if ops.skinny_ok(B, at.hidden_size + 2 * kv, normed.shape[1]) and isinstance(cache, QuantizedKVCache):
+                q, k, v = ops.gemm_bf16_nt_skinny(normed, at.packed_qkv(), splits=(at.num_heads * at.head_dim, kv, kv))
+                q = q.view(B, at.num_heads, at.head_dim)
+                cache.append(seq_ids, positions, k, v)
+            elif ops.skinny_ok(B, at.hidden_size + 2 * kv, normed.shape[1]):
                 # q, k, v as one stream of the concatenated weight; K rotated and K, V appended by the same launch
                 q = ops.gemm_qkv_append_bf16_skinny(normed, at.packed_qkv(), cache, seq_ids, positions, at.num_heads)
                 q = q.view(B, at.num_heads, at.head_dim)

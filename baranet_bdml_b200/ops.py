@@ -84,6 +84,15 @@ def prefill_table(workspace: Workspace, B: int, S: int, Hkv: int, D: int = 64, t
                                                       workspace.nbytes, _stream()))
 
 
+def rotated_k(workspace: Workspace, B: int, S: int, Hkv: int, D: int = 64) -> torch.Tensor:
+    """The rotated keys that a prefill scratch buffer holds, (B*S, Hkv*D) bf16: a part of it, as the last call left it"""
+    n = _lib.load().bn_attn_prefill_bf16_rotated_k(B, S, Hkv, D)
+    if n == 0:
+        raise RuntimeError(f"bn_attn_prefill_bf16: unsupported shape B={B} S={S} Hkv={Hkv} D={D}")
+    at = workspace.ptr - workspace.buf.data_ptr() + n
+    return workspace.buf[at:at + B * S * Hkv * D * 2].view(torch.bfloat16).view(B * S, Hkv * D)
+
+
 def gemm_qkv_rope_bf16(x: torch.Tensor, wqkv_t: torch.Tensor, B: int, S: int, Hq: int, Hkv: int, D: int,
                        workspace: Workspace, *, position_offset: int = 0, cache=None,
                        error_word: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -304,6 +304,10 @@ BN_API int bn_attn_prefill_bf16(const void* q, const void* k, const void* v, voi
                          int Hkv, int D, float scale, float theta, int position_offset, int causal, int flags,
                                 void* workspace, size_t workspace_bytes, bn_stream_t stream);
 
+/* Where in the scratch buffer of bn_attn_prefill_bf16 the rotated keys lie (bytes from its start): (B, S, Hkv, 64) bf16, as that call
+ * or bn_gemm_qkv_rope_bf16 left them, for a cache of another kind; 0 for a shape that the prefill does not take. */
+BN_API size_t bn_attn_prefill_bf16_rotated_k(int B, int S, int Hkv, int D);
+
 /* The q, k and v projections of the layer as ONE tensor-core GEMM with RoPE(K), the cache append and the K operand
  * of the attention kernel produced in its epilogue (mygrad/llama/llama_layers.py:157-163: three op_mm launches and
  * the K rotation; plus what bn_kv_append does):
