@@ -133,7 +133,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         uint32_t phase = 0;
         bool ok = true, bad = false;
         Segment sg_next;
-        bool have = iter.next(sc, sg, false);
+        bool have = iter.next<true>(sc, sg, false);
         auto load_group = [&](const Segment& sgm, int grp) {
             const int e = grp * 32 + lane;
             const int n_pages_seq = (sgm.L + BN_PAGE_TOKENS - 1) / BN_PAGE_TOKENS;
@@ -142,15 +142,10 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         const uint64_t stream_policy = l2_policy_evict_first();     // every cache byte is read once per launch
         int ids = have ? load_group(sg, sg.s0 / GRP) : 0, ids_pref = 0;
         while (ok && have) {
-            const bool have_next = iter.next(sc, sg_next, false);
+            bool have_next = false;
             const int n_pages_seq = (sg.L + BN_PAGE_TOKENS - 1) / BN_PAGE_TOKENS;
             for (int s = sg.s0; s < sg.s1; ++s) {
-                if (s == sg.s0 || s % GRP == 0) {
-                    if (s != sg.s0) ids = ids_pref;
-                    const int grp = s / GRP;
-                    if ((grp + 1) * GRP < sg.s1) ids_pref = load_group(sg, grp + 1);
-                    else if (have_next) ids_pref = load_group(sg_next, sg_next.s0 / GRP);
-                }
+                if (s != sg.s0 && s % GRP == 0) ids = ids_pref;
                 int page = __shfl_sync(0xffffffffu, ids, (s % GRP) * DEC8_PAGES + mine);
                 if (page < 0 || page >= p.pool_pages) { page = 0; bad = true; }
                 if (!mbar_wait_warp(smem_u32(&empty_bar[stage]), phase ^ 1u, &s_abort)) { ok = false; break; }
@@ -162,6 +157,16 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                     bulk_load_hint(ring + stage * DEC8_STAGE_BYTES + mine * BN_KV8_BLOCK,
                                    p.pool + ((int64_t)page * p.Hkv + sg.g) * BN_KV8_BLOCK, BN_KV8_BLOCK, fb, stream_policy);
                 if (++stage == DEC8_NSTAGES) { stage = 0; phase ^= 1u; }
+                // (behind the copies, so that the first of them does not wait for the next segment to be found)
+                if (s == sg.s0 || s % GRP == 0) {
+                    const int grp = s / GRP;
+                    if ((grp + 1) * GRP < sg.s1) {
+                        ids_pref = load_group(sg, grp + 1);
+                    } else {
+                        have_next = iter.next<true>(sc, sg_next, false);
+                        if (have_next) ids_pref = load_group(sg_next, sg_next.s0 / GRP);
+                    }
+                }
             }
             sg = sg_next;
             ids = ids_pref;
@@ -175,14 +180,14 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     if (warp == DEC8_QUERY_WARP) {
         // ---------------------------------------------------------- query warp: lane -> dims 2 * lane, + 1, of all heads
         const double freq = p.freqs.f[lane];           // (of 32 different parameters a warp reads one at a time: not in every segment)
-        for (int n = 0; iter.next(sc, sg, false); ++n) {
+        for (int n = 0; iter.next<true>(sc, sg, false); ++n) {
             const int buf = n % 2;
             const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + ((size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep) * (DEC_D / 2) + lane;
             uint32_t raw[DEC_G];
 #pragma unroll
             for (int h = 0; h < DEC_G; ++h) raw[h] = h < p.n_rep ? src[h * (DEC_D / 2)] : 0u;
             float c = 1.f, s = 0.f;
-            if (p.rope_q) rotation(p.q_positions ? p.q_positions[sg.b] : sg.L - 1, freq, &c, &s);
+            if (p.rope_q) kv8_rotation(p.q_positions ? p.q_positions[sg.b] : sg.L - 1, freq, &c, &s);
             if (!mbar_wait_warp(smem_u32(&q_free[buf]), (n / 2 & 1) ^ 1u, &s_abort)) break;
 #pragma unroll
             for (int h = 0; h < DEC_G; ++h) {
@@ -212,7 +217,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
             for (int h = h0; h < h0 + DEC8_HPM; ++h)
                 if (h < p.n_rep) decode8_store(p, (size_t)b * p.Hq + (size_t)g * p.n_rep + h, lane, 0.f, 0.f, 0.f, 0.f);
         }
-        for (int n = 0; iter.next(sc, sg, true); ++n) {
+        for (int n = 0; iter.next<true>(sc, sg, true); ++n) {
             const int buf = n % 2;
             if (!mbar_wait_warp(smem_u32(&mrg_full[buf]), n / 2 & 1, &s_abort)) break;
             float m[DEC8_HPM], l[DEC8_HPM], a[DEC8_HPM], b[DEC8_HPM];
@@ -299,7 +304,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     const int hA = 2 * (lane % 4);       // the two heads whose softmax state this thread carries
     int before = 0;                      // stages of the range that lie before the segment
     bool ok = true;
-    for (int n = 0; ok && iter.next(sc, sg, false); ++n) {
+    for (int n = 0; ok && iter.next<true>(sc, sg, false); ++n) {
         const int buf = n % 2;
         if (!mbar_wait_warp(smem_u32(&q_full[buf]), n / 2 & 1, &s_abort)) break;
         // Q^T fragments: dims 16 c .. 16 c + 15 of head lane / 4, c = lane % 4

@@ -63,7 +63,7 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_app
         float c[4], s[4];
         if (p.Hkv % 4 == 0) {
             float c1, s1;
-            rotation(pos, freq[part * 4 + group], &c1, &s1);
+            kv8_rotation(pos, freq[part * 4 + group], &c1, &s1);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 c[i] = __shfl_sync(0xffffffffu, c1, i * KV8_LANES + part);
@@ -71,7 +71,7 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_app
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rotation(pos, freq[part * 4 + i], &c[i], &s[i]);
+            for (int i = 0; i < 4; ++i) kv8_rotation(pos, freq[part * 4 + i], &c[i], &s[i]);
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -45,6 +45,17 @@ inline const RotationFreqs& rotation_freqs(float theta) {
     return r;
 }
 
+// cos and sin of position * frequency, each off by little more than a rounding: the product and its reduction to a turn are taken in fp64,
+// the functions (of half turns, which need no reduction of their own) in fp32, and what fp32 leaves of the angle is added to first order
+__device__ __forceinline__ void kv8_rotation(int position, double freq, float* c, float* s) {
+    const double turns = (double)position * freq * 0.15915494309189535, halves = 2.0 * (turns - rint(turns));
+    const float at = (float)halves, rest = (float)(halves - (double)at) * 3.14159265f;
+    float c0, s0;
+    sincospif(at, &s0, &c0);
+    *c = fmaf(-rest, s0, c0);
+    *s = fmaf(rest, c0, s0);
+}
+
 template <int VALUES> __device__ __forceinline__ float kv8_scale(uint32_t most_bits) {
     if (most_bits >= 0x7f800000u) return __uint_as_float(0x7fc00000u);
     uint32_t b;
