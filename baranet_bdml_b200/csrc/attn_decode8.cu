@@ -5,7 +5,8 @@
 // list of segments = (sequence, key head, run of stages).  Half the bytes leave half the time per token, so that what the consumers
 // do beside the two products has to go elsewhere:
 //   * two producer warps keep a ring of stages filled.  A block (page, key head) is one bulk copy of 2112 bytes, scales included; one
-//     warp issues one in 44 ns, two one in 30, and 52 is what DRAM needs for it (4 x 262144 tokens 122 -> 101 us with more than one);
+//     warp issues one in 44 ns, two one in 30, and 52 is what DRAM needs for it (4 x 262144 tokens 115 us with one, 91 with two; finding the
+//     next segment only behind the first copies starts 0.3 us sooner and streams 3 % slower);
 //   * a query warp rotates and converts the next segment's queries while the consumers work on the one before;
 //   * eight consumer warps, two groups of four that take stages in turn, four pages of a stage each: with two pages each, whose
 //     instruction chains are as long, 95 us instead of 91;
@@ -142,10 +143,15 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         const uint64_t stream_policy = l2_policy_evict_first();     // every cache byte is read once per launch
         int ids = have ? load_group(sg, sg.s0 / GRP) : 0, ids_pref = 0;
         while (ok && have) {
-            bool have_next = false;
+            const bool have_next = iter.next<true>(sc, sg_next, false);
             const int n_pages_seq = (sg.L + BN_PAGE_TOKENS - 1) / BN_PAGE_TOKENS;
             for (int s = sg.s0; s < sg.s1; ++s) {
-                if (s != sg.s0 && s % GRP == 0) ids = ids_pref;
+                if (s == sg.s0 || s % GRP == 0) {
+                    if (s != sg.s0) ids = ids_pref;
+                    const int grp = s / GRP;
+                    if ((grp + 1) * GRP < sg.s1) ids_pref = load_group(sg, grp + 1);
+                    else if (have_next) ids_pref = load_group(sg_next, sg_next.s0 / GRP);
+                }
                 int page = __shfl_sync(0xffffffffu, ids, (s % GRP) * DEC8_PAGES + mine);
                 if (page < 0 || page >= p.pool_pages) { page = 0; bad = true; }
                 if (!mbar_wait_warp(smem_u32(&empty_bar[stage]), phase ^ 1u, &s_abort)) { ok = false; break; }
@@ -157,16 +163,6 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                     bulk_load_hint(ring + stage * DEC8_STAGE_BYTES + mine * BN_KV8_BLOCK,
                                    p.pool + ((int64_t)page * p.Hkv + sg.g) * BN_KV8_BLOCK, BN_KV8_BLOCK, fb, stream_policy);
                 if (++stage == DEC8_NSTAGES) { stage = 0; phase ^= 1u; }
-                // (behind the copies, so that the first of them does not wait for the next segment to be found)
-                if (s == sg.s0 || s % GRP == 0) {
-                    const int grp = s / GRP;
-                    if ((grp + 1) * GRP < sg.s1) {
-                        ids_pref = load_group(sg, grp + 1);
-                    } else {
-                        have_next = iter.next<true>(sc, sg_next, false);
-                        if (have_next) ids_pref = load_group(sg_next, sg_next.s0 / GRP);
-                    }
-                }
             }
             sg = sg_next;
             ids = ids_pref;

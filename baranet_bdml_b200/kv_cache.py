@@ -209,14 +209,25 @@ class QuantizedKVCache(PagedKVCache):
                 KV8_VALUES[self.values], self.num_kv_heads, self.head_dim, _stream()))
         return k, v
 
+    def status(self) -> None:
+        """Raises if a decode launch gave up on a bounded wait, or met a page outside the pool; the scratch buffer starts afresh then."""
+        for ws in self._ws.values():
+            try:
+                ws.status()
+            except RuntimeError:
+                ws.buf.zero_()
+                raise
+
     def workspace(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int = 0) -> Workspace:
-        """The decode scratch: one for all shapes, kept while the cache lives (a captured graph may hold its address)."""
+        """The current stream's decode scratch, for all shapes, kept while the cache lives (a captured graph may hold its address:
+        graphs of one cache, which are captured on one stream, run one after the other)."""
         n = _lib.load().bn_attn_decode_kv8_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len, chunk_tokens)
         if n == 0:
             raise RuntimeError("bn_attn_decode_kv8: unsupported shape")
-        if () not in self._ws:
-            self._ws[()] = Workspace(n, self.pool.device)
-        return self._ws[()]
+        key = _stream()
+        if key not in self._ws:
+            self._ws[key] = Workspace(n, self.pool.device)
+        return self._ws[key]
 
     def decode(self, q: torch.Tensor, *, num_heads: int, scale: Optional[float] = None, rope_q: bool = True,
                q_positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -254,12 +265,13 @@ class QuantizedKVCache(PagedKVCache):
         if scale is None:
             scale = 1.0 / (D ** 0.5)
         if B:
-            ws = self._ws.get(()) or self.workspace(B, Hq, max_seq_len, chunk_tokens)
+            stream = _stream()
+            ws = self._ws.get(stream) or self.workspace(B, Hq, max_seq_len, chunk_tokens)
             _lib.check(_lib.load().bn_attn_decode_kv8(
                 q.data_ptr(), self.pool.data_ptr(), self.num_pages, page_table.data_ptr(), width, seq_lens.data_ptr(),
                 q_positions.data_ptr() if q_positions is not None else None, out.data_ptr() if out is not None else None,
                 out_f32.data_ptr() if out_f32 is not None else None, lse.data_ptr() if lse is not None else None, KV8_VALUES[self.values], B, Hq,
-                self.num_kv_heads, D, float(scale), self.theta, int(bool(rope_q)), int(max_seq_len), int(chunk_tokens), ws.ptr, ws.nbytes, _stream()))
+                self.num_kv_heads, D, float(scale), self.theta, int(bool(rope_q)), int(max_seq_len), int(chunk_tokens), ws.ptr, ws.nbytes, stream))
         return out if out is not None else out_f32
 
 

@@ -419,6 +419,27 @@ def test_streams_graphs_and_two_at_once(lib, values):
         assert all(torch.equal(a, b) for a, b in zip(again, step(caches[0])))
 
 
+@pytest.mark.parametrize("values", VALUES)
+def test_one_cache_on_two_streams(lib, values):
+    """Two batches of queries against one cache at the same time, each long enough to be split over CTAs and merged"""
+    lens = [9000, 5000, 7]
+    cache, table, rng = make(lens, 4, values, 40)
+    k, v = fill(cache, values, rng)
+    qs = [queries(rng, 3, 32) for _ in range(2)]
+    want = [check_decode(cache, k, v, table, lens, q)[1].clone() for q in qs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    on_gpu = [q.cuda() for q in qs]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(cache.decode(on_gpu[i], num_heads=32, out_f32=torch.empty((3, 32, 64), device="cuda")))
+    torch.cuda.synchronize()
+    cache.status()
+    assert all(torch.equal(g, w) for w, rows in zip(want, got) for g in rows)
+
+
 def test_refusals_on_the_gpu(lib):
     cache, table, rng = make([100], 2, "e4m3", 13)
     i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")      # noqa: E731
