@@ -21,9 +21,10 @@
 // Where no more than 512 tokens lie in the steps down to the border, all that is left is done with a list of them, in every CTA alike:
 // ranks, sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and what is kept is passed over once
 // more for the choice.  A step with too many (equal logits, far outliers) is divided again by (value, index) until it has not.
-// A batch pays for the instructions per token (256 rows of 32000: 270 of them and every weight through the histogram 107 us, and with the
-// tokens that could not matter by a bound on their number alone left out 155), few rows for barriers of the cluster, about 1 us each:
-// three with a short list, six without.
+// A batch pays for the instructions per token: 256 rows of 32000 with top-p of 0.9 take 83 us, 0.39 TB/s, at 62% of the instructions that
+// the SMs can issue (107 with every weight through the histogram, 155 with the tokens that cannot matter left out by a bound on their number
+// alone; the exponential series is 18 of the 83).  Few rows pay for barriers of the cluster, about 1 us each, three with a short list and six
+// without: a row of 32000 with top-k 50 takes 10.2 us, without any limit 6.1.
 #include <math.h>
 
 #include "hybrid.cuh"
@@ -36,6 +37,11 @@ constexpr int SMP_THREADS = 512;
 constexpr int SMP_WARPS = SMP_THREADS / 32;
 constexpr int SMP_BINS = SMP_THREADS;                 // a thread has one
 constexpr int SMP_LIST = SMP_THREADS;                 // elements that are ranked among each other, a thread each
+// Up to so many elements the row's choice is made with them alone: ranking m costs m^2 / 512 comparisons a thread, and saves other passes
+// and barriers.  By top-k alone (16 x 4000, us with the list and without, k of 100: 9.1, 9.2; 150: 10.2, 9.4; 300: 13.7, 9.4), by top-p
+// alone (what is kept up to 99: 11.9, 14.3; 291: 15.0, 14.3), and by top-k before top-p, which the list then does as well (k of 200: 10.2,
+// 16.9; 300: 12.0, 17.5; 480: 15.9, 19.2).
+constexpr int SMP_FEW_BY_COUNT = 128, SMP_FEW_BY_WEIGHT = 256;
 constexpr int SMP_CLUSTER = 8;                        // CTAs per row at most
 constexpr int SMP_MOST = 32768;                       // tokens per CTA: 5 bytes of shared memory each
 constexpr int SMP_TWO = 16384;                        // tokens per CTA of which an SM takes two
@@ -64,6 +70,7 @@ __device__ __forceinline__ float value_of(uint32_t order) { return __uint_as_flo
 
 struct SampleShared {
     uint32_t hist[4][SMP_BINS];                        // counts, and the limbs of weights
+    uint32_t coarse[SMP_BINS];                         // counts that say where to look
     uint64_t list_key[SMP_LIST];                       // this CTA's elements
     uint64_t all_key[SMP_LIST], all_w[SMP_LIST];       // the cluster's
     uint64_t from[2][SMP_CLUSTER * SMP_WARPS][2];      // what all warps of the cluster tell each other
@@ -304,11 +311,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
         int shift = -1, step = 0, m = 0, step1 = 0, step2 = SMP_BINS - 1;
         double limit = (double)top_k;
         bool listed = false;
-        const float scale = range > 0.f ? SMP_BINS / range : 0.f;
+        const float scale = range > 0.f ? fminf(SMP_BINS / range, 3e38f) : 0.f;      // (finite: what equals the maximum is in step 0)
         float edge = peak, scale2 = scale;             // of the steps between step1 and step2
         // (the rounding is to the nearest step: any will do that never puts the larger value behind the smaller)
         auto step_below = [&](float d) -> int { return (int)(__float_as_uint(fminf(d, SMP_BINS - 1.f) + 8388608.f) & (SMP_BINS - 1)); };
-        auto coarse = [&](float v) -> int { return v == peak ? 0 : step_below((peak - v) * scale); };
+        auto coarse = [&](float v) -> int { return step_below((peak - v) * scale); };
         auto in_step = [&](float v, int i) -> int {    // -1: not in the range
             if (!kept(v, i)) return -1;
             if (shift < 0) {
@@ -320,7 +327,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
         };
         auto clear = [&]() {
             sh.hist[0][tid] = 0;
-            if (by_weight) sh.hist[1][tid] = sh.hist[2][tid] = sh.hist[3][tid] = 0;
+            if (by_weight) sh.coarse[tid] = sh.hist[1][tid] = sh.hist[2][tid] = sh.hist[3][tid] = 0;
             if (tid == 0) sh.list_n = 0;
             __syncthreads();
         };
@@ -338,21 +345,27 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             const int at = min(atomicAdd(&sh.list_n, 1), SMP_LIST - 1);      // (m of them in the whole cluster)
             sh.list_key[at] = key_of(v, i);
         };
-        auto joined = [&](int row) -> uint32_t {       // the cluster's histogram at the thread's step
+        auto joined = [&](const uint32_t* row) -> uint32_t {       // the cluster's histogram at the thread's step
             uint32_t sum = 0;
 #pragma unroll
             for (int c = 0; c < SMP_CLUSTER; ++c)
-                if (c < C) sum += ld_cluster_u32(in_rank(smem_u32(&sh.hist[row][tid]), c));
+                if (c < C) sum += ld_cluster_u32(in_rank(smem_u32(row + tid), c));
             return sum;
         };
 
         clear();
         if (by_weight) {
-            each([&](float v, int i) {
-                if (kept(v, i)) atomicAdd(&sh.hist[0][coarse(v)], 1u);
-            });
+            if (last == -INFINITY) {
+                each([&](float v, int) {
+                    if (v > -INFINITY) atomicAdd(&sh.coarse[coarse(v)], 1u);
+                });
+            } else {
+                each([&](float v, int i) {
+                    if (kept(v, i)) atomicAdd(&sh.coarse[coarse(v)], 1u);
+                });
+            }
             cluster_sync();
-            const uint32_t cnt = joined(0);
+            const uint32_t cnt = joined(sh.coarse);
             // the step's weights lie between these, its sums between theirs (a thousandth of a step and 1e-4 for the roundings)
             const float wide = range / SMP_BINS / temp, most = tid == 0 ? 1.f : __expf(-(tid - 0.501f) * wide), least = tid == SMP_BINS - 1 ? 0.f : __expf(-(tid + 0.501f) * wide);
             float a = cnt * most, b = cnt ? cnt * least : 0.f;
@@ -387,7 +400,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             step2 = w2 ? (31 - __clz(w2)) * 32 + (int)sh.between[31 - __clz(w2)].lane2 - 1 : 0;
             m = w2 ? (int)sh.between[31 - __clz(w2)].upto : SMP_LIST + 1;
             step1 = min(step1, step2);
-            listed = m <= SMP_LIST;
+            listed = m <= SMP_FEW_BY_WEIGHT;
             edge = step1 == 0 ? peak : peak - (step1 - 0.5f) / scale;
             scale2 = scale * SMP_BINS / (step2 - step1 + 1);
             // the smallest value of the steps up to step2: a warp looks at 32 at once
@@ -401,8 +414,6 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
                 if (f) from += (f - 1) * apart + 1;
             }
             const float lowest = value_of(to);
-            cluster_sync();                            // the others have read this CTA's histogram
-            clear();
             // every token is weighed, once: what lies below the steps, and all
             uint64_t all = 0, below = 0;
             if (last == -INFINITY) {
@@ -456,10 +467,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
                 });
                 cluster_sync();
             }
-            const uint32_t cnt = joined(0);
+            const uint32_t cnt = joined(sh.hist[0]);
             uint64_t total;
             uint32_t upto;
-            const uint64_t sum = by_weight ? joined(1) + ((uint64_t)joined(2) << 16) + ((uint64_t)joined(3) << 32) : cnt;
+            const uint64_t sum = by_weight ? joined(sh.hist[1]) + ((uint64_t)joined(sh.hist[2]) << 16) + ((uint64_t)joined(sh.hist[3]) << 32) : cnt;
             uint64_t before = block_scan(sum, cnt, total, upto);
             if (by_weight && !again) above -= total;
             before += above;
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             above = sh.border[w].above;
             step = w * 32 + sh.border[w].lane1 - 1;
             m = sh.border[w].count;
-            if (!by_weight && !again && sh.border[w].upto <= SMP_LIST) { m = sh.border[w].upto; listed = true; }
+            if (!by_weight && !again && (int)sh.border[w].upto <= (top_p < 1.f ? SMP_LIST : SMP_FEW_BY_COUNT)) { m = sh.border[w].upto; listed = true; }
             if (m <= SMP_LIST) break;
             // too many to be ranked: the step's range of keys, to be divided
             if (shift < 0) {
@@ -527,18 +538,28 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             if (tid < m) sh.all_key[tid] = ld_cluster_u64(in_rank(smem_u32(&sh.list_key[at]), c));
         }
         __syncthreads();
-        // how many of m keys are larger than the thread's: all threads share the comparisons
+        // How many of m keys are larger than the thread's.  All warps share the comparisons: a lane has four keys to count for, so that what
+        // it reads of shared memory is compared four times.
         auto rank_among = [&](const auto* keys, int m) -> int {
             sh.rank[tid] = 0;
             __syncthreads();
-            const int wide = (m + 31) / 32 * 32, shares = SMP_THREADS / wide, share = tid / wide, t = tid % wide;
-            if (share < shares && t < m) {
+            const int groups = (m + 127) / 128, shares = SMP_WARPS / groups, share = warp / groups, t = warp % groups * 128 + lane;
+            if (share < shares) {
                 const int end = m * (share + 1) / shares;
-                const auto mine = keys[t];
-                uint32_t larger = 0;
+                const auto a = keys[min(t, m - 1)], b = keys[min(t + 32, m - 1)], c = keys[min(t + 64, m - 1)], d = keys[min(t + 96, m - 1)];
+                uint32_t la = 0, lb = 0, lc = 0, ld = 0;
 #pragma unroll 4
-                for (int i = m * share / shares; i < end; ++i) larger += keys[i] > mine;
-                atomicAdd(&sh.rank[t], larger);
+                for (int i = m * share / shares; i < end; ++i) {
+                    const auto k = keys[i];
+                    la += k > a;
+                    lb += k > b;
+                    lc += k > c;
+                    ld += k > d;
+                }
+                if (t < m) atomicAdd(&sh.rank[t], la);
+                if (t + 32 < m) atomicAdd(&sh.rank[t + 32], lb);
+                if (t + 64 < m) atomicAdd(&sh.rank[t + 64], lc);
+                if (t + 96 < m) atomicAdd(&sh.rank[t + 96], ld);
             }
             __syncthreads();
             return (int)sh.rank[tid];
@@ -658,9 +679,15 @@ extern "C" int bn_sample_rows(const void* logits, int64_t row_stride, int dtype,
     p.out = out; p.cols = cols;
     p.unit_bits = 50;
     while ((1ll << (62 - p.unit_bits)) < cols) --p.unit_bits;
-    // as many CTAs for a row as there are SMs for, but no fewer than its tokens need, and parts of 1024 tokens at least
+    // As many CTAs for a row as there are SMs for, but no fewer than its tokens need: of more than 1024 tokens
+    // while half of the SMs are left over, of more than 6144 up to all SMs (us with top-k 50 by 1, 2, 4, 8 CTAs: 1 x 10007 11.4, 9.4, 9.0, 8.5; 32 x 10007 12.6, 10.1, 10.5, 12.5;
+    // 32 x 32000 21.7, 14.8, 12.6, 13.9; 64 x 32000 21.7, 14.8, 14.6, 26.8)
     int c = 1;
-    while (c < SMP_CLUSTER && (cols > c * SMP_MOST || (rows > 8 && cols > c * SMP_TWO) || ((int64_t)rows * 2 * c <= sm_count() && cols > c * 1024))) c *= 2;
+    while (c < SMP_CLUSTER) {
+        const int64_t ctas = (int64_t)rows * 2 * c;
+        if (!(cols > c * SMP_MOST || (rows > 8 && cols > c * SMP_TWO) || (ctas <= sm_count() && cols > c * (2 * ctas <= sm_count() ? 1024 : 6144)))) break;
+        c *= 2;
+    }
     p.slice = ((cols + c - 1) / c + 3) / 4 * 4;
     const size_t smem = (size_t)p.slice * 5;
     p.bf16 = dtype;
