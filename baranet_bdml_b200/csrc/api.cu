@@ -81,6 +81,16 @@ int bn_workspace_status(const void* workspace, bn_stream_t stream) {
     return BN_OK;
 }
 
+int bn_stream_capture_id(bn_stream_t stream, unsigned long long* id) {
+    if (!id) return bn::fail(BN_ERR_INVALID_ARG, "bn_stream_capture_id: null pointer");
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    *id = 0;
+    if (cudaError_t e = cudaStreamGetCaptureInfo(bn::as_stream(stream), &status, id))
+        return bn::fail(BN_ERR_CUDA, "bn_stream_capture_id: %s", cudaGetErrorString(e));
+    if (status != cudaStreamCaptureStatusActive) *id = 0;
+    return BN_OK;
+}
+
 int bn_selftest_wait_timeout(void* workspace, unsigned limit_us, bn_stream_t stream) {
     if (!workspace) return bn::fail(BN_ERR_INVALID_ARG, "bn_selftest_wait_timeout: null workspace");
     if (limit_us == 0 || limit_us > 100000) return bn::fail(BN_ERR_INVALID_ARG, "bn_selftest_wait_timeout: limit of 1..100000 us");

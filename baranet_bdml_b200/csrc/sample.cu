@@ -194,8 +194,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
     uint32_t top_order = order_of(top), low_order = order_of(low);
     join(top_order, low_order);
     tell_and_go_on((uint64_t)top_order << 32 | top_at, low_order);
-    // (what the row's numbers alone say is worked out while the barrier is waited for)
-    const float temp_given = p.temperature ? p.temperature[r] : p.temperature1, temp = temp_given > 3e38f ? 3e38f : temp_given;
+    // (what the row's numbers alone say is worked out while the barrier is waited for; a temperature above 0 is one from 1e-30 to 3e38, for
+    // which the steps of the value are finite: beyond, the weights are those at the end, but for logits less than 1e-27 apart)
+    const float temp_given = p.temperature ? p.temperature[r] : p.temperature1, temp = temp_given > 0.f ? fminf(fmaxf(temp_given, 1e-30f), 3e38f) : 0.f;
     const int top_k = p.top_k ? p.top_k[r] : p.top_k1;
     const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
     const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);

@@ -12,6 +12,7 @@ not be contiguous.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional
 
 import torch
@@ -150,6 +151,7 @@ class QuantizedKVCache(PagedKVCache):
                 raise RuntimeError(f"QuantizedKVCache: storage must be a contiguous {dtype} tensor of {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
         super().__init__(num_pages, num_seqs, max_pages_per_seq, num_kv_heads, head_dim, theta, device, storage)
         self.values = values
+        self._spare = None     # scratch for the next capture
 
     def _here(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
         dev = self.pool.get_device()
@@ -219,15 +221,25 @@ class QuantizedKVCache(PagedKVCache):
                 raise
 
     def workspace(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int = 0) -> Workspace:
-        """The current stream's decode scratch, for all shapes, kept while the cache lives (a captured graph may hold its address:
-        graphs of one cache, which are captured on one stream, run one after the other)."""
+        """The current stream's decode scratch, for all shapes, kept while the cache lives.  A capture has one of its own on each of its
+        streams, so that graphs run beside each other and beside other calls: laid out and zeroed by an earlier call, where there
+        was one, else by the graph itself at each replay."""
         n = _lib.load().bn_attn_decode_kv8_workspace_bytes(B, Hq, self.num_kv_heads, self.head_dim, max_seq_len, chunk_tokens)
         if n == 0:
             raise RuntimeError("bn_attn_decode_kv8: unsupported shape")
-        key = _stream()
-        if key not in self._ws:
-            self._ws[key] = Workspace(n, self.pool.device)
-        return self._ws[key]
+        key, capture = _stream(), torch.cuda.is_current_stream_capturing()
+        if capture:
+            number = ctypes.c_ulonglong()
+            _lib.check(_lib.load().bn_stream_capture_id(key, ctypes.byref(number)))
+            key = key, number.value
+        ws = self._ws.get(key)
+        if ws is None:
+            ws = self._ws[key] = (self._spare if capture else None) or Workspace(n, self.pool.device)
+            if capture:
+                self._spare = None
+        if not capture and self._spare is None:
+            self._spare = Workspace(n, self.pool.device)
+        return ws
 
     def decode(self, q: torch.Tensor, *, num_heads: int, scale: Optional[float] = None, rope_q: bool = True,
                q_positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -266,7 +278,8 @@ class QuantizedKVCache(PagedKVCache):
             scale = 1.0 / (D ** 0.5)
         if B:
             stream = _stream()
-            ws = self._ws.get(stream) or self.workspace(B, Hq, max_seq_len, chunk_tokens)
+            ws = self._ws.get(stream) if self._spare is not None and not torch.cuda.is_current_stream_capturing() else None
+            ws = ws or self.workspace(B, Hq, max_seq_len, chunk_tokens)
             _lib.check(_lib.load().bn_attn_decode_kv8(
                 q.data_ptr(), self.pool.data_ptr(), self.num_pages, page_table.data_ptr(), width, seq_lens.data_ptr(),
                 q_positions.data_ptr() if q_positions is not None else None, out.data_ptr() if out is not None else None,

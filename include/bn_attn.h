@@ -87,6 +87,10 @@ BN_API int bn_version(void);
  * zero-filled again before reuse. */
 BN_API int bn_workspace_status(const void* workspace, bn_stream_t stream);
 
+/* The number of the capture into a CUDA graph that `stream` takes part in, 0 for none (no counterpart in the reference): for a scratch
+ * buffer that belongs to one graph. */
+BN_API int bn_stream_capture_id(bn_stream_t stream, unsigned long long* id);
+
 /* Self-test of that mechanism (no counterpart in the reference): launches a small kernel whose only wait is for a
  * barrier that nothing arrives at, with a limit of limit_us microseconds (1..100000).  The wait gives up, the kernel
  * stores BN_ERR_TIMEOUT in the error word at the head of `workspace` (any scratch buffer of this library, or 4

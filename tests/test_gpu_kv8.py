@@ -440,6 +440,39 @@ def test_one_cache_on_two_streams(lib, values):
     assert all(torch.equal(g, w) for w, rows in zip(want, got) for g in rows)
 
 
+def test_graphs_of_one_cache_side_by_side(lib):
+    """Captured before any call, behind calls, and behind another capture; replayed last one first, on two streams at once"""
+    lens = [9000, 5000, 7]
+    cache, table, rng = make(lens, 4, "e4m3", 41)
+    k, v = fill(cache, "e4m3", rng)
+    qs = [queries(rng, 3, 32) for _ in range(4)]
+    on_gpu, got = [q.cuda() for q in qs], [torch.empty((3, 32, 64), device="cuda") for _ in qs]
+    graphs = [torch.cuda.CUDAGraph() for _ in qs]
+
+    def capture(i):
+        with torch.cuda.graph(graphs[i]):
+            cache.decode(on_gpu[i], num_heads=32, out_f32=got[i])
+
+    capture(0)
+    capture(1)
+    want = [check_decode(cache, k, v, table, lens, q)[1].clone() for q in qs]
+    capture(2)
+    capture(3)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for first, second in ((1, 0), (3, 2), (0, 3), (2, 1)):
+        for _ in range(10):
+            for s, i in zip(streams, (first, second)):
+                with torch.cuda.stream(s):
+                    graphs[i].replay()
+        torch.cuda.synchronize()
+        cache.status()
+        for i in (first, second):
+            assert torch.equal(got[i], want[i])
+            got[i].zero_()
+        torch.cuda.synchronize()
+
+
 def test_refusals_on_the_gpu(lib):
     cache, table, rng = make([100], 2, "e4m3", 13)
     i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")      # noqa: E731

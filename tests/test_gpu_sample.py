@@ -111,6 +111,27 @@ def test_masked_rows(lib):
     check(x, u, top_k=2999)
 
 
+@pytest.mark.parametrize("kept", [31, 127, 128, 129, 200, 255, 256, 257, 300, 384, 385, 511, 512, 513])
+def test_as_many_as_a_list_holds(lib, kept):
+    """Where the choice is made from a list and where not, and how the list is ranked"""
+    x, u = logits(6, 4000, kept)
+    check(x, u, top_k=kept, temperature=3.0)
+    check(x, u, top_k=kept, top_p=0.95, temperature=3.0)
+    x[:, kept:] -= 1000.0                                     # top-p: of kept ids, and of some more equals
+    check(x, u, top_p=0.999, temperature=3.0)
+    x[:, kept:2 * kept] = x[:, :1]
+    check(x, u, top_p=0.6)
+
+
+@pytest.mark.parametrize("temperature", [1e-45, 1e-38, 1e-30, 1e-20])
+def test_the_smallest_temperatures(lib, temperature):
+    x, u = logits(5, 3000, 12)
+    x[1] *= 1e-18
+    x[2] = x[2].round()
+    for knobs in ({}, {"top_k": 30}, {"top_p": 0.9}, {"top_k": 300, "top_p": 0.5, "min_p": 0.1}):
+        check(x, u, temperature=temperature, **knobs)
+
+
 @pytest.mark.parametrize("knobs", KNOBS[3:8] + KNOBS[11:13], ids=str)
 def test_bf16_and_strided_rows(lib, knobs):
     x, u = logits(9, 5005, 6, dtype=torch.bfloat16)
