@@ -8,7 +8,7 @@
 // What is kept is always a prefix of the order, so that it is named by its last element.
 //
 // Sums decide which side of a border a token falls on, so they have to come out the same however the row is divided: weights are
-// computed in fp64 (2^f for |f| <= 1/2 by twelve terms of the exponential series, whose rest is below 2e-16) and summed as 64-bit whole
+// computed in fp64 (2^(i / 32) from a table, and 2^f for |f| <= 1/64 by seven terms of the exponential series, whose rest is below 4e-18) and summed as 64-bit whole
 // numbers of 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight above 0 counts at least
 // one such unit.
 //
@@ -21,10 +21,10 @@
 // Where no more than 512 tokens lie in the steps down to the border, all that is left is done with a list of them, in every CTA alike:
 // ranks, sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and what is kept is passed over once
 // more for the choice.  A step with too many (equal logits, far outliers) is divided again by (value, index) until it has not.
-// A batch pays for the instructions per token: 256 rows of 32000 with top-p of 0.9 take 83 us, 0.39 TB/s, at 62% of the instructions that
-// the SMs can issue (107 with every weight through the histogram, 155 with the tokens that cannot matter left out by a bound on their number
-// alone; the exponential series is 18 of the 83).  Few rows pay for barriers of the cluster, about 1 us each, three with a short list and six
-// without: a row of 32000 with top-k 50 takes 10.2 us, without any limit 6.1.
+// A batch pays for the instructions per token: 256 rows of 32000 with top-p of 0.9 take 74 us, 0.44 TB/s: 115 instructions per token and
+// 2300 per warp, at 62% of what the SMs can issue, in 1.7 waves (107 with every weight through the histogram, 155 with the tokens that cannot
+// matter left out by a bound on their number alone, 83 with twelve terms of the series and no table).  Few rows pay for barriers of the
+// cluster, about 1 us each, three with a short list and six without: a row of 32000 with top-k 50 takes 10.1 us, without any limit 5.7.
 #include <math.h>
 
 #include "hybrid.cuh"
@@ -38,10 +38,11 @@ constexpr int SMP_WARPS = SMP_THREADS / 32;
 constexpr int SMP_BINS = SMP_THREADS;                 // a thread has one
 constexpr int SMP_LIST = SMP_THREADS;                 // elements that are ranked among each other, a thread each
 // Up to so many elements the row's choice is made with them alone: ranking m costs m^2 / 512 comparisons a thread, and saves other passes
-// and barriers.  By top-k alone (16 x 4000, us with the list and without, k of 100: 9.1, 9.2; 150: 10.2, 9.4; 300: 13.7, 9.4), by top-p
-// alone (what is kept up to 99: 11.9, 14.3; 291: 15.0, 14.3), and by top-k before top-p, which the list then does as well (k of 200: 10.2,
-// 16.9; 300: 12.0, 17.5; 480: 15.9, 19.2).
+// and barriers.  By top-k alone (16 x 4000, us with the list and without, k of 100: 8.8, 9.2; 150: 10.3, 9.2; 300: 14.3, 9.3), by top-p
+// alone (what is kept up to 99: 11.4, 14.3; 291: 17.2, 14.2), and by top-k before top-p, which the list then does as well (k of 200: 10.3,
+// 19.0; 300: 12.6, 19.1; 480: 17.3, 19.2).
 constexpr int SMP_FEW_BY_COUNT = 128, SMP_FEW_BY_WEIGHT = 256;
+constexpr int SMP_LOG_STEPS = 5, SMP_STEPS = 1 << SMP_LOG_STEPS;      // of a power of two, in a table
 constexpr int SMP_CLUSTER = 8;                        // CTAs per row at most
 constexpr int SMP_MOST = 32768;                       // tokens per CTA: 5 bytes of shared memory each
 constexpr int SMP_TWO = 16384;                        // tokens per CTA of which an SM takes two
@@ -80,6 +81,7 @@ struct SampleShared {
     struct { uint32_t lane1, lane2, upto; } between[SMP_WARPS];
     uint64_t sums[SMP_WARPS][2];
     uint64_t kept_sum;
+    double exp2[SMP_STEPS];                            // 2^(i / SMP_STEPS)
     uint32_t rank[SMP_LIST];
     int list_n;
 };
@@ -125,6 +127,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
     // a warp has a run of the part, so that its sum is one of neighbours; in pieces of four
     const int run = (n4 + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n4, begin + run);
     uint16_t* places = reinterpret_cast<uint16_t*>(sx + p.slice) + 2 * begin;      // of the warp's run, from its start
+    if (tid < SMP_STEPS) sh.exp2[tid] = exp2((double)tid / SMP_STEPS);
     grid_dependency_wait();
     grid_launch_dependents();
 
@@ -201,8 +204,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
     const float top_p = p.top_p ? p.top_p[r] : p.top_p1, min_p = p.min_p ? p.min_p[r] : p.min_p1;
     const double u = fmin(fmax((double)p.u[r], 0.0), 1.0);
     const double per = 1.4426950408889634 / (double)temp;
+    const double per_step = per * SMP_STEPS;
     const int unit = p.unit_bits;
-    const double floor_w = (min_p > 1.f ? 1.0 : (double)min_p) * (double)(1ull << unit);
+    const uint64_t floor_w = min_p > 0.f ? (uint64_t)ceil((double)fminf(min_p, 1.f) * (double)(1ull << unit)) : 0;      // least weight that min-p keeps
     cluster_wait();
     top_order = order_of(-INFINITY);
     for (int i = lane; i < C * SMP_WARPS; i += 32) {
@@ -228,25 +232,21 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
     // warp weighs different values.  The smallest values above one unit and above nothing are rounded up, so that they part exactly.
     const float one_unit = __double2float_ru((double)peak - unit / per), nothing = __double2float_ru((double)peak - 1074.5 / per);
     auto weigh = [&](float v) -> uint64_t {
-        const double t = ((double)v - (double)peak) * per;
-        const double rounded = t + (0x1.8p52 + unit);  // to a whole number, which, with unit, is the low word
-        const double f = t - (rounded - (0x1.8p52 + unit));
-        // (ln 2)^i / i!
-        double w = 2.5678435993488196e-11;
-        w = fma(w, f, 4.4455382718708101e-10);
-        w = fma(w, f, 7.0549116208011209e-09);
-        w = fma(w, f, 1.0178086009239696e-07);
-        w = fma(w, f, 1.3215486790144305e-06);
-        w = fma(w, f, 1.5252733804059838e-05);
-        w = fma(w, f, 1.5403530393381606e-04);
-        w = fma(w, f, 1.3333558146428441e-03);
-        w = fma(w, f, 9.6181291076284769e-03);
-        w = fma(w, f, 5.5504108664821576e-02);
-        w = fma(w, f, 2.4022650695910069e-01);
-        w = fma(w, f, 6.9314718055994529e-01);
+        const double d = (double)v - (double)peak;
+        const double rounded = fma(d, per_step, 0x1.8p52 + SMP_STEPS * unit);      // to a whole number of steps: with the unit's, the low word
+        const double f = fma(d, per_step, (0x1.8p52 + SMP_STEPS * unit) - rounded);
+        const int steps = __double2loint(rounded);
+        const double power = sh.exp2[steps & (SMP_STEPS - 1)];
+        // (ln 2 / 32)^i / i!
+        double w = 1.4345655584131934e-13;
+        w = fma(w, f, 3.973709984549416e-11);
+        w = fma(w, f, 9.172562701824643e-09);
+        w = fma(w, f, 1.693850972437182e-06);
+        w = fma(w, f, 0.0002345961982022468);
+        w = fma(w, f, 0.02166084939249829);
         w = fma(w, f, 1.0);
-        w = __hiloint2double(__double2hiint(w) + (__double2loint(rounded) << 20), __double2loint(w));
-        w += 0x1p52;                                   // (what is left are the low bits)
+        // (what is left behind 2^52 are the low bits)
+        w = fma(w, __hiloint2double(__double2hiint(power) + (steps >> SMP_LOG_STEPS << 20), __double2loint(power)), 0x1p52);
         const uint32_t hi = v >= one_unit ? (uint32_t)__double2hiint(w) - 0x43300000u : 0u;
         const uint32_t lo = v >= one_unit ? (uint32_t)__double2loint(w) : v >= nothing ? 1u : 0u;
         return (uint64_t)hi << 32 | lo;
@@ -270,8 +270,9 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             bool in[4];
             int before = at, own = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                in[e] = which(v[e], 4 * q + e);
+            for (int e = 0; e < 4; ++e) in[e] = which(v[e], 4 * q + e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {              // (not in turn with the weights: their chains overlap)
                 const uint32_t who = __ballot_sync(0xffffffffu, in[e]);
                 before += __popc(who & lower);
                 at += __popc(who);
@@ -302,6 +303,19 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
                 f(four.z, 4 * q + 2);
                 f(four.w, 4 * q + 3);
             }
+        }
+    };
+
+    // the same, and may leave out what is below `near`
+    auto each_from = [&](float near, auto f) {
+        if (held >= 0 || near == -INFINITY) return each(f);
+        for (int q = begin + lane; q < end; q += 32) {
+            const float4 four = *reinterpret_cast<const float4*>(sx + 4 * q);
+            if (fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)) < near) continue;
+            f(four.x, 4 * q);
+            f(four.y, 4 * q + 1);
+            f(four.z, 4 * q + 2);
+            f(four.w, 4 * q + 3);
         }
     };
 
@@ -380,13 +394,19 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             }
             if (lane == 31) { sh.sums[warp][0] = (uint64_t)__float_as_uint(a) << 32 | __float_as_uint(b); sh.sums[warp][1] = upto; }
             __syncthreads();
-            float all_a = 0.f, all_b = 0.f, low_a = 0.f, low_b = 0.f;
-            for (int w = 0; w < SMP_WARPS; ++w) {
-                if (w == warp) { low_a = all_a; low_b = all_b; }
-                if (w < warp) upto += (uint32_t)sh.sums[w][1];
-                all_a += __uint_as_float((uint32_t)(sh.sums[w][0] >> 32));
-                all_b += __uint_as_float((uint32_t)sh.sums[w][0]);
+            const uint64_t ab = sh.sums[lane % SMP_WARPS][0];
+            float all_a = __uint_as_float((uint32_t)(ab >> 32)), all_b = __uint_as_float((uint32_t)ab);
+            uint32_t all_c = (uint32_t)sh.sums[lane % SMP_WARPS][1];
+#pragma unroll
+            for (int o = 1; o < SMP_WARPS; o <<= 1) {
+                const float ta = __shfl_up_sync(0xffffffffu, all_a, o), tb = __shfl_up_sync(0xffffffffu, all_b, o);
+                const uint32_t tc = __shfl_up_sync(0xffffffffu, all_c, o);
+                if (lane >= o) { all_a += ta; all_b += tb; all_c += tc; }
             }
+            const float low_a = warp ? __shfl_sync(0xffffffffu, all_a, warp - 1) : 0.f, low_b = warp ? __shfl_sync(0xffffffffu, all_b, warp - 1) : 0.f;
+            upto += warp ? __shfl_sync(0xffffffffu, all_c, warp - 1) : 0;
+            all_a = __shfl_sync(0xffffffffu, all_a, SMP_WARPS - 1);
+            all_b = __shfl_sync(0xffffffffu, all_b, SMP_WARPS - 1);
             const uint32_t first_ok = __ballot_sync(0xffffffffu, cnt && (a - own_a + low_a) * 1.0001f < top_p * all_b * 0.9999f);
             const uint32_t last_ok = __ballot_sync(0xffffffffu, cnt && (b - own_b + low_b) * 0.9999f <= top_p * all_a * 1.0001f);
             if (lane == (last_ok ? 31 - __clz(last_ok) : 0)) {
@@ -406,6 +426,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             scale2 = scale * SMP_BINS / (step2 - step1 + 1);
             // the smallest value of the steps up to step2: a warp looks at 32 at once
             uint32_t from = order_of(-INFINITY) + 1, to = order_of(peak);
+            if (step2 < SMP_BINS - 1 && scale > 0.f) { // (whatever is rounded: a whole step lower none is in step2, half a step higher all)
+                from = max(from, order_of(__fsub_rd(peak, __fdiv_ru(step2 + 1.f, scale))));
+                to = min(to, order_of(__fsub_ru(peak, __fdiv_rd((float)step2, scale))));
+            }
             while (from < to) {
                 const uint32_t apart = (to - from) / 32 + 1, at = from + lane * apart;
                 const uint32_t who = __ballot_sync(0xffffffffu, at >= to || coarse(value_of(at)) <= step2);
@@ -453,9 +477,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             limit = fmax((double)top_p * (double)all, 0.5);
             above = all - warp_total(below);           // (and less by what the steps hold)
         } else {
-            each([&](float v, int i) {
-                const int b = in_step(v, i);
-                if (b >= 0) add(b, 0);
+            each([&](float v, int) {
+                if (v > -INFINITY) add(coarse(v), 0);
             });
             cluster_sync();
         }
@@ -521,14 +544,15 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
         if (by_weight && listed) {
             above = 0;
         } else {
-            // the list: the step's elements, or all down to it
-            each([&](float v, int i) {
+            // the list: the step's elements, or all down to it.  (What is smaller than this lies in a later step, whatever was rounded.)
+            const float near = !by_weight && shift < 0 && step < SMP_BINS - 1 ? __fsub_rd(peak, __fdiv_ru(step + 1.f, scale)) : -INFINITY;
+            each_from(near, [&](float v, int i) {
                 const int b = in_step(v, i);
                 if (b >= 0 && b <= step && (b == step || listed)) put(v, i);
             });
             cluster_sync();
         }
-        {
+        if (!listed || rank == 0) {
             // the thread's element of the cluster's list: which CTA's, and which there
             uint32_t here = lane < C ? ld_cluster_u32(in_rank(smem_u32(&sh.list_n), min(lane, C - 1))) : 0;
             int c = 0, at = tid;
@@ -538,19 +562,29 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             }
             if (tid < m) sh.all_key[tid] = ld_cluster_u64(in_rank(smem_u32(&sh.list_key[at]), c));
         }
+        if (listed) {                                  // the first CTA goes on alone; the others stay until it has read their lists
+            cluster_arrive();
+            if (rank) {
+                cluster_wait();
+                return true;
+            }
+        }
         __syncthreads();
         // How many of m keys are larger than the thread's.  All warps share the comparisons: a lane has four keys to count for, so that what
         // it reads of shared memory is compared four times.
         auto rank_among = [&](const auto* keys, int m) -> int {
             sh.rank[tid] = 0;
             __syncthreads();
-            const int groups = (m + 127) / 128, shares = SMP_WARPS / groups, share = warp / groups, t = warp % groups * 128 + lane;
+            // 1 to 4 groups of 128 keys, 16, 8, 5 or 4 parts of what they are compared to; the quotients by multiplication
+            const int groups = (m + 127) / 128, shares = groups == 1 ? 16 : groups == 2 ? 8 : groups == 3 ? 5 : 4;
+            const int share = warp * (groups == 3 ? 11 : groups == 1 ? 32 : groups == 2 ? 16 : 8) >> 5, t = (warp - share * groups) * 128 + lane;
+            const int part = m * (groups == 3 ? 13108 : groups == 1 ? 4096 : groups == 2 ? 8192 : 16384);
             if (share < shares) {
-                const int end = m * (share + 1) / shares;
+                const int end = part * (share + 1) >> 16;
                 const auto a = keys[min(t, m - 1)], b = keys[min(t + 32, m - 1)], c = keys[min(t + 64, m - 1)], d = keys[min(t + 96, m - 1)];
                 uint32_t la = 0, lb = 0, lc = 0, ld = 0;
 #pragma unroll 4
-                for (int i = m * share / shares; i < end; ++i) {
+                for (int i = part * share >> 16; i < end; ++i) {
                     const auto k = keys[i];
                     la += k > a;
                     lb += k > b;
@@ -588,7 +622,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
         const int few = !by_weight && top_k < m ? top_k : m;
         const uint64_t before = block_scan(tid < few ? w : 0, 0, total, unused);
         if (!by_weight) limit = fmax((double)top_p * (double)total, 0.5);
-        const int stay = __syncthreads_count(tid < few && (tid == 0 || ((!(top_p < 1.f) || (double)before < limit) && !((double)w < floor_w))));
+        const int stay = __syncthreads_count(tid < few && (tid == 0 || ((!(top_p < 1.f) || (double)before < limit) && w >= floor_w)));
         if (tid == stay - 1) sh.kept_sum = before + w;
         __syncthreads();
         const uint64_t all = sh.kept_sum, reach = min((uint64_t)(u * (double)all), all - 1);
@@ -605,23 +639,21 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
         }
         __syncthreads();
         const uint64_t w2 = tid < stay ? by_index[tid] : 0, earlier = block_scan(w2, 0, total, unused);
-        if (rank == 0 && tid < stay && earlier <= reach && reach < earlier + w2) p.out[r] = (int)~index[tid];
+        if (tid < stay && earlier <= reach && reach < earlier + w2) p.out[r] = (int)~index[tid];
+        cluster_wait();
         return true;
     };
 
     bool chosen = false;
     if (top_k > 0 && top_k < p.cols) chosen = cut(false, fminf(depth, 128.f));
     if (!chosen && top_p < 1.f) chosen = cut(true, fminf(fminf(depth, 64.f * temp), 3e38f));
-    if (chosen) {
-        cluster_sync();                                // the others have read this CTA's list
-        return;
-    }
+    if (chosen) return;
     if (held < 0 && last > -INFINITY) compact(kept);
 
     // ---------------------------------------------------------------------------------------- the choice from all that is kept
     auto counted = [&](float v, int i) -> uint64_t {
         const uint64_t w = kept(v, i) ? weigh(v) : 0;
-        return (double)w < floor_w && (uint32_t)(first + i) != top_at ? 0 : w;
+        return w < floor_w && (uint32_t)(first + i) != top_at ? 0 : w;
     };
     uint64_t mine = 0;
     each([&](float v, int i) { mine += counted(v, i); });
