@@ -669,18 +669,42 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
     below = warp_total(below);
     const uint64_t reach = min((uint64_t)(u * (double)all), all - 1);
     if (reach < below || reach >= below + mine) return;
-    const int looked = held >= 0 ? held : 4 * (end - begin);
-    for (int j = lane; j - lane < looked; j += 32) {
-        const int i = 4 * begin + (held < 0 || j >= looked ? j : places[j]);
-        uint64_t sum = j < looked ? counted(sx[i], i) : 0;
+    // one warp finds it in its run: of many tokens the lane whose share of them it is in first, then 32 at a time
+    auto value_at = [&](int j, uint64_t& w) -> int {
+        const int i = 4 * begin + (held < 0 ? j : places[j]);
+        w = counted(sx[i], i);
+        return first + i;
+    };
+    auto scan = [&](uint64_t sum) -> uint64_t {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint64_t t = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += t;
         }
+        return sum;
+    };
+    int from = 0, to = held >= 0 ? held : 4 * (end - begin);
+    if (to > 4 * 32) {
+        const int share = (to + 31) / 32, stop = min(to, share * (lane + 1));
+        uint64_t own = 0, w;
+#pragma unroll 4
+        for (int j = share * lane; j < stop; ++j) {
+            value_at(j, w);
+            own += w;
+        }
+        const uint64_t sum = scan(own);
+        const int lane_of = __ffs(__ballot_sync(0xffffffffu, below + sum > reach)) - 1;
+        below += __shfl_sync(0xffffffffu, sum - own, lane_of);
+        from = share * lane_of;
+        to = min(to, from + share);
+    }
+    for (int j = from + lane; j - lane < to; j += 32) {
+        uint64_t w = 0;
+        const int id = j < to ? value_at(j, w) : 0;
+        const uint64_t sum = scan(w);
         const uint32_t over = __ballot_sync(0xffffffffu, below + sum > reach);
         if (over) {
-            if (lane == __ffs(over) - 1) p.out[r] = first + i;
+            if (lane == __ffs(over) - 1) p.out[r] = id;
             return;
         }
         below += __shfl_sync(0xffffffffu, sum, 31);
