@@ -484,7 +484,7 @@ extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_
     if (Hq % Hkv != 0 || Hq / Hkv > DEC_G) return fail(BN_ERR_UNSUPPORTED, "%s: Hq/Hkv=%d/%d (group of 1..8 supported)", what, Hq, Hkv);
     if (B > DEC_MAX_SEQS) return fail(BN_ERR_UNSUPPORTED, "%s: %d sequences in one launch (<= %d supported)", what, B, DEC_MAX_SEQS);
     if ((long long)B * Hkv * (max_seq_len / DEC8_STAGE_TOKENS + 1) > 0x3fffffffLL || max_seq_len > 0x7fffffff - DEC8_STAGE_TOKENS ||
-        chunk_tokens > 0x7fffffff - DEC8_STAGE_TOKENS)
+        (long long)B * Hkv > 0x7fffffffLL / DEC8_MAX_CTAS || chunk_tokens > 0x7fffffff - DEC8_STAGE_TOKENS)
         return fail(BN_ERR_UNSUPPORTED, "%s: B * Hkv * max_seq_len is too large for one launch", what);
     if (chunk_tokens < 0 || chunk_tokens % 128) return fail(BN_ERR_INVALID_ARG, "%s: chunk_tokens=%d must be 0 or a multiple of 128", what, chunk_tokens);
     if ((int64_t)max_pages * BN_PAGE_TOKENS < max_seq_len)

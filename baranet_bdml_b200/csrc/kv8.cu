@@ -198,7 +198,7 @@ extern "C" int bn_kv8_gather(const void* pool, int64_t pool_pages, const int32_t
     if (int rc = kv8_shape(what, pool, pool_pages, page_table, num_seqs, max_pages, Hkv, D, values)) return rc;
     if (!seq_lens || !seq_ids || !starts || !k_out || !v_out) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
     const int64_t units = (int64_t)n_seqs * n_tokens * Hkv;
-    if (n_seqs < 0 || n_tokens < 0 || units > 0x7fffffffLL * 16) return fail(BN_ERR_INVALID_ARG, "%s: bad sizes n_seqs=%d n_tokens=%d", what, n_seqs, n_tokens);
+    if (n_seqs < 0 || n_tokens < 0 || (int64_t)n_seqs * n_tokens > 0x7fffffffLL * 16 / Hkv) return fail(BN_ERR_INVALID_ARG, "%s: bad sizes n_seqs=%d n_tokens=%d", what, n_seqs, n_tokens);
     if (out_dtype != 0 && out_dtype != 1) return fail(BN_ERR_INVALID_ARG, "%s: out_dtype=%d (0 = fp32, 1 = bf16)", what, out_dtype);
     if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15)
         return fail(BN_ERR_INVALID_ARG, "%s: the outputs must be 16-byte aligned", what);

@@ -57,6 +57,15 @@ def test_status_codes(lib):
     assert lib.bn_attn_decode_kv8_workspace_bytes(1, 8, 2, 32, 100, 0) == 0 and lib.bn_attn_decode_kv8_workspace_bytes(64, 32, 4, 64, 4096, 0) > 0
 
 
+def test_sizes_whose_products_overflow(lib):
+    from baranet_bdml_b200 import _lib
+    p, most = 4096, 2 ** 31 - 1
+    assert lib.bn_kv8_gather(p, 4, p, 2, 2, p, p, p, most, most, p, p, 1, 0, 4, 64, None) == _lib.BN_ERR_INVALID_ARG
+    assert lib.bn_kv8_append(p, 4, p, 2, 2, p, p, most, p, 128, p, 128, 1, 0, 1, 64, 64, 1e4, None) == _lib.BN_ERR_INVALID_ARG
+    for B, hkv, longest in ((1024, 1 << 16, 16), (1024, 4, 1 << 30), (1, 1, most)):
+        assert lib.bn_attn_decode_kv8(p, p, 4, p, most, p, None, p, None, None, 0, B, hkv, hkv, 64, 0.125, 1e4, 1, longest, 0, p, 1 << 30, None) == _lib.BN_ERR_UNSUPPORTED
+
+
 def test_choice_by_hand():
     """The plain form of the choice itself"""
     x = [2.0, 1.0, 2.0, 0.0]
