@@ -176,14 +176,23 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     if (warp == DEC8_QUERY_WARP) {
         // ---------------------------------------------------------- query warp: lane -> dims 2 * lane, + 1, of all heads
         const double freq = p.freqs.f[lane];           // (of 32 different parameters a warp reads one at a time: not in every segment)
-        for (int n = 0; iter.next<true>(sc, sg, false); ++n) {
-            const int buf = n % 2;
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + ((size_t)sg.b * p.Hq + (size_t)sg.g * p.n_rep) * (DEC_D / 2) + lane;
-            uint32_t raw[DEC_G];
+        auto load = [&](const Segment& of, uint32_t (&raw)[DEC_G]) {
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + ((size_t)of.b * p.Hq + (size_t)of.g * p.n_rep) * (DEC_D / 2) + lane;
 #pragma unroll
             for (int h = 0; h < DEC_G; ++h) raw[h] = h < p.n_rep ? src[h * (DEC_D / 2)] : 0u;
-            float c = 1.f, s = 0.f;
-            if (p.rope_q) kv8_rotation(p.q_positions ? p.q_positions[sg.b] : sg.L - 1, freq, &c, &s);
+            return p.rope_q && p.q_positions ? p.q_positions[of.b] : of.L - 1;
+        };
+        uint32_t raw[DEC_G], raw_next[DEC_G];
+        int pos = 0, pos_next = 0, known = -1;
+        float c = 1.f, s = 0.f;
+        bool have = iter.next<true>(sc, sg, false);
+        if (have) pos = load(sg, raw);
+        for (int n = 0; have; ++n) {
+            const int buf = n % 2, b = sg.b;
+            have = iter.next<true>(sc, sg, false);
+            if (have) pos_next = load(sg, raw_next);                   // under way while this one is rotated
+            if (p.rope_q && b != known) kv8_rotation(pos, freq, &c, &s);
+            known = b;
             if (!mbar_wait_warp(smem_u32(&q_free[buf]), (n / 2 & 1) ^ 1u, &s_abort)) break;
 #pragma unroll
             for (int h = 0; h < DEC_G; ++h) {
@@ -197,6 +206,9 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&q_full[buf]));
+            pos = pos_next;
+#pragma unroll
+            for (int h = 0; h < DEC_G; ++h) raw[h] = raw_next[h];
         }
         if (lane == 0 && s_abort) atomicExch(&p.hdr->error, BN_ERR_TIMEOUT);
         return;
