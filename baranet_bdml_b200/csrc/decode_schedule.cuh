@@ -139,32 +139,44 @@ struct SegmentIter {
     }
 };
 
-// Lengths and stages of all sequences into shared memory, by the whole block: an exclusive prefix sum (warp 0)
+// Lengths and stages of all sequences into shared memory, by the whole block: an exclusive prefix sum, of 32 sequences a warp and then
+// of the warps' sums.  (One warp alone, 32 after 32: 0.5 us more for 256 sequences, 2 us for 1000.)
 template <int THREADS, int STAGE_TOKENS>
 __device__ __forceinline__ void decode_prefix(const int32_t* seq_lens, int B, int max_seq_len, int* s_len, int* s_prefix, int* s_nmax) {
-    for (int b = threadIdx.x; b < B; b += THREADS) {
-        const int L = max(0, min(seq_lens[b], max_seq_len));
-        s_len[b] = L;
-        s_prefix[b + 1] = (L + STAGE_TOKENS - 1) / STAGE_TOKENS;
+    __shared__ int s_sum[DEC_MAX_SEQS / 32], s_most[DEC_MAX_SEQS / 32];
+    constexpr int TURNS = (DEC_MAX_SEQS + THREADS - 1) / THREADS;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, blocks = (B + 31) / 32;
+    auto scan = [&](int v) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += t;
+        }
+        return v;
+    };
+    int upto[TURNS];
+#pragma unroll
+    for (int i = 0; i < TURNS; ++i) {
+        const int k = warp + i * (THREADS / 32), b = k * 32 + lane;
+        if (k >= blocks) break;
+        const int L = b < B ? max(0, min(seq_lens[b], max_seq_len)) : 0, v = (L + STAGE_TOKENS - 1) / STAGE_TOKENS;
+        if (b < B) s_len[b] = L;
+        upto[i] = scan(v);
+        const int most = __reduce_max_sync(0xffffffffu, v);
+        if (lane == 31) { s_sum[k] = upto[i]; s_most[k] = most; }
     }
     __syncthreads();
-    const int lane = threadIdx.x % 32;
-    if (threadIdx.x < 32) {
-        int carry = 0, nmax = 0;
-        for (int b0 = 0; b0 < B; b0 += 32) {
-            const int b = b0 + lane;
-            int v = b < B ? s_prefix[b + 1] : 0;
-            nmax = max(nmax, v);
+    const int sums = scan(lane < blocks ? s_sum[lane] : 0);
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += t;
-            }
-            if (b < B) s_prefix[b + 1] = carry + v;
-            carry += __shfl_sync(0xffffffffu, v, 31);
-        }
-        nmax = __reduce_max_sync(0xffffffffu, nmax);
-        if (lane == 0) { s_prefix[0] = 0; *s_nmax = nmax; }
+    for (int i = 0; i < TURNS; ++i) {
+        const int k = warp + i * (THREADS / 32), b = k * 32 + lane;
+        if (k >= blocks) break;
+        const int before = __shfl_sync(0xffffffffu, sums, max(k - 1, 0));
+        if (b < B) s_prefix[b + 1] = upto[i] + (k ? before : 0);
+    }
+    if (warp == 0) {
+        const int most = __reduce_max_sync(0xffffffffu, lane < blocks ? s_most[lane] : 0);
+        if (lane == 0) { s_prefix[0] = 0; *s_nmax = most; }
     }
     __syncthreads();
 }
