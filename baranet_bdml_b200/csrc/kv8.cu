@@ -100,7 +100,8 @@ struct Kv8GatherParams {
     int num_seqs, max_pages, n_tokens, Hkv;
 };
 
-// Four lanes per (row of the result, key head), 16 bytes of K and of V each
+// Four lanes per (row of the result, key head), bytes 8 part .. and 32 + 8 part .. of K and of V each: what the four read or store at once lies
+// side by side
 constexpr int KV8_GLANES = 4;
 template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8GatherParams p) {
     ptx::grid_dependency_wait();
@@ -121,12 +122,15 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_gat
     uint32_t scales = 0u;
     if (there) {
         const uint8_t* block = p.pool + ((int64_t)page * p.Hkv + g) * BN_KV8_BLOCK;
-        kb = *reinterpret_cast<const uint4*>(block + slot * KV8_D + part * 16);
-        vb = *reinterpret_cast<const uint4*>(block + KV8_V + slot * KV8_D + kv8_v_place(slot, part * 16));
+        const uint2 k0 = *reinterpret_cast<const uint2*>(block + slot * KV8_D + part * 8), k1 = *reinterpret_cast<const uint2*>(block + slot * KV8_D + 32 + part * 8);
+        const uint8_t* v = block + KV8_V + slot * KV8_D;
+        const uint2 v0 = *reinterpret_cast<const uint2*>(v + kv8_v_place(slot, part * 8)), v1 = *reinterpret_cast<const uint2*>(v + kv8_v_place(slot, 32 + part * 8));
+        kb = make_uint4(k0.x, k0.y, k1.x, k1.y);
+        vb = make_uint4(v0.x, v0.y, v1.x, v1.y);
         scales = *reinterpret_cast<const uint32_t*>(block + KV8_SCALES + slot * 4);
     }
     auto put = [&](void* out, uint4 b, float scale) {
-        T* dst = static_cast<T*>(out) + unit * KV8_D + part * 16;
+        T* dst = static_cast<T*>(out) + unit * KV8_D + part * 8;
         const uint32_t words[4] = {b.x, b.y, b.z, b.w};
         float o[16];
 #pragma unroll
@@ -139,11 +143,11 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_gat
         if (sizeof(T) == 2) {
 #pragma unroll
             for (int w = 0; w < 2; ++w)
-                reinterpret_cast<uint4*>(dst)[w] = make_uint4(ptx::pack_bf16(o[8 * w], o[8 * w + 1]), ptx::pack_bf16(o[8 * w + 2], o[8 * w + 3]),
+                *reinterpret_cast<uint4*>(dst + 32 * w) = make_uint4(ptx::pack_bf16(o[8 * w], o[8 * w + 1]), ptx::pack_bf16(o[8 * w + 2], o[8 * w + 3]),
                                                               ptx::pack_bf16(o[8 * w + 4], o[8 * w + 5]), ptx::pack_bf16(o[8 * w + 6], o[8 * w + 7]));
         } else {
 #pragma unroll
-            for (int w = 0; w < 4; ++w) reinterpret_cast<float4*>(dst)[w] = make_float4(o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]);
+            for (int w = 0; w < 4; ++w) *reinterpret_cast<float4*>(dst + 32 * (w / 2) + 4 * (w % 2)) = make_float4(o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]);
         }
     };
     put(p.k, kb, ptx::bf16_lo(scales));
