@@ -20,14 +20,30 @@ template <typename T> __device__ __forceinline__ void load8(const T* p, bool wid
     }
 }
 
+// n / d of whole numbers by a multiplication: 2^(31 + s) / d rounded up, 2^s >= d, is exact for n < 2^31 (an instruction or two where a
+// division takes 20, and one of 64 bits 100)
+struct Divisor {
+    uint32_t d, mul, shift;
+    explicit Divisor(int by = 1) : d((uint32_t)by), mul(0), shift(31) {
+        while ((1ull << (shift - 31)) < d) ++shift;
+        mul = (uint32_t)(((1ull << shift) + d - 1) / d);
+    }
+    __device__ __forceinline__ uint32_t of(uint32_t n) const { return (uint32_t)((uint64_t)n * mul >> shift); }
+};
+
 // the largest magnitude of the lanes of a group, as bits (so that a NaN is larger than all numbers)
 __device__ __forceinline__ uint32_t group_most(const float (&x)[8]) {
-    uint32_t m = 0;
+    auto larger = [](float a, float b) {
+        float m;
+        asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
+        return m;
+    };
+    float m = x[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int i = 1; i < 8; ++i) m = larger(m, x[i]);
 #pragma unroll
-    for (int o = 1; o < KV8_LANES; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    return m;
+    for (int o = 1; o < KV8_LANES; o <<= 1) m = larger(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return __float_as_uint(m);
 }
 
 struct Kv8AppendParams {
@@ -37,6 +53,7 @@ struct Kv8AppendParams {
     const void *k, *v;
     int64_t k_stride, v_stride;
     int num_seqs, max_pages, T, Hkv, rotate, wide;
+    Divisor heads;
     RotationFreqs freqs;
 };
 
@@ -48,10 +65,10 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_app
     __syncthreads();
     ptx::grid_dependency_wait();
     ptx::grid_launch_dependents();
-    const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / KV8_LANES;
+    const uint32_t unit = blockIdx.x * (blockDim.x / KV8_LANES) + threadIdx.x / KV8_LANES;
     const int part = threadIdx.x % KV8_LANES, group = threadIdx.x % 32 / KV8_LANES;
-    const bool there = unit < (int64_t)p.T * p.Hkv;
-    const int t = there ? (int)(unit / p.Hkv) : 0, g = there ? (int)(unit % p.Hkv) : 0;
+    const bool there = unit < (uint32_t)p.T * (uint32_t)p.Hkv;
+    const int t = there ? (int)p.heads.of(unit) : 0, g = there ? (int)(unit - (uint32_t)t * (uint32_t)p.Hkv) : 0;
     const int pos = p.positions[t], seq = p.seq_ids[t], slot = pos % BN_PAGE_TOKENS;
     int page = -1;
     if (there && pos >= 0 && pos / BN_PAGE_TOKENS < p.max_pages && seq >= 0 && seq < p.num_seqs)
@@ -98,6 +115,7 @@ struct Kv8GatherParams {
     void *k, *v;
     int64_t units;
     int num_seqs, max_pages, n_tokens, Hkv;
+    Divisor heads, tokens;
 };
 
 // Four lanes per (row of the result, key head), bytes 8 part .. and 32 + 8 part .. of K and of V each: what the four read or store at once lies
@@ -109,9 +127,19 @@ template <typename T, int VALUES> __global__ void __launch_bounds__(256) kv8_gat
     const int64_t unit = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / KV8_GLANES;
     const int part = threadIdx.x % KV8_GLANES;
     if (unit >= p.units) return;
-    const int64_t row = unit / p.Hkv;
-    const int g = (int)(unit % p.Hkv), i = (int)(row / p.n_tokens);
-    const int64_t pos = (int64_t)p.starts[i] + row % p.n_tokens;
+    int64_t row;
+    int i, j;
+    if (p.units < 0x7fffffffLL) {
+        row = p.heads.of((uint32_t)unit);
+        i = (int)p.tokens.of((uint32_t)row);
+        j = (int)row - i * p.n_tokens;
+    } else {
+        row = unit / p.Hkv;
+        i = (int)(row / p.n_tokens);
+        j = (int)(row % p.n_tokens);
+    }
+    const int g = (int)(unit - row * p.Hkv);
+    const int64_t pos = (int64_t)p.starts[i] + j;
     const int seq = p.seq_ids[i];
     int page = -1;
     if (seq >= 0 && seq < p.num_seqs && pos >= 0 && pos < p.seq_lens[seq] && pos / BN_PAGE_TOKENS < p.max_pages)
@@ -176,7 +204,7 @@ extern "C" int bn_kv8_append(void* pool, int64_t pool_pages, const int32_t* page
     const char* what = "bn_kv8_append";
     if (int rc = kv8_shape(what, pool, pool_pages, page_table, num_seqs, max_pages, Hkv, D, values)) return rc;
     if (!seq_ids || !positions || !k_new || !v_new) return fail(BN_ERR_INVALID_ARG, "%s: null pointer", what);
-    if (T < 0 || (int64_t)T * Hkv > 0x7fffffffLL * 16) return fail(BN_ERR_INVALID_ARG, "%s: T=%d tokens of %d heads", what, T, Hkv);
+    if (T < 0 || (int64_t)T * Hkv >= 0x7fffffffLL) return fail(BN_ERR_INVALID_ARG, "%s: T=%d tokens of %d heads", what, T, Hkv);
     if (dtype != 0 && dtype != 1) return fail(BN_ERR_INVALID_ARG, "%s: dtype=%d (0 = fp32, 1 = bf16)", what, dtype);
     if (rotate && !(theta > 0.f)) return fail(BN_ERR_INVALID_ARG, "%s: theta=%g", what, theta);
     if (int rc = require_sm100()) return rc;
@@ -188,6 +216,7 @@ extern "C" int bn_kv8_append(void* pool, int64_t pool_pages, const int32_t* page
     p.k = k_new; p.v = v_new; p.k_stride = k_row_stride; p.v_stride = v_row_stride;
     p.num_seqs = num_seqs; p.max_pages = max_pages; p.T = T; p.Hkv = Hkv; p.rotate = rotate;
     p.wide = ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 15) == 0 && ((k_row_stride | v_row_stride) % 8) == 0;
+    p.heads = Divisor(Hkv);
     if (rotate) p.freqs = rotation_freqs(theta);
     auto* kernel = dtype == 0 ? (values == BN_KV8_E4M3 ? kv8_append_kernel<float, BN_KV8_E4M3> : kv8_append_kernel<float, BN_KV8_INT8>)
                               : (values == BN_KV8_E4M3 ? kv8_append_kernel<__nv_bfloat16, BN_KV8_E4M3> : kv8_append_kernel<__nv_bfloat16, BN_KV8_INT8>);
@@ -214,6 +243,7 @@ extern "C" int bn_kv8_gather(const void* pool, int64_t pool_pages, const int32_t
     p.page_table = page_table; p.seq_lens = seq_lens; p.seq_ids = seq_ids; p.starts = starts;
     p.k = k_out; p.v = v_out; p.units = units;
     p.num_seqs = num_seqs; p.max_pages = max_pages; p.n_tokens = n_tokens; p.Hkv = Hkv;
+    p.heads = Divisor(Hkv); p.tokens = Divisor(n_tokens);
     auto* kernel = out_dtype == 0 ? (values == BN_KV8_E4M3 ? kv8_gather_kernel<float, BN_KV8_E4M3> : kv8_gather_kernel<float, BN_KV8_INT8>)
                                   : (values == BN_KV8_E4M3 ? kv8_gather_kernel<__nv_bfloat16, BN_KV8_E4M3> : kv8_gather_kernel<__nv_bfloat16, BN_KV8_INT8>);
     launch_dependent(kernel, (unsigned)((units * KV8_GLANES + 255) / 256), 256, 0, as_stream(stream), p);
