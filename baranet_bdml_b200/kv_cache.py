@@ -180,8 +180,8 @@ class QuantizedKVCache(PagedKVCache):
         if not (f32 or k_new.dtype == torch.bfloat16) or v_new.dtype != k_new.dtype:
             raise RuntimeError(f"{what}: k/v must both be fp32 or both bf16")
         self._here(what, seq_ids, positions, k_new, v_new)
-        shape, width = k_new.shape, self.num_kv_heads * self.head_dim
-        if len(shape) != 2 or shape[1] != width or v_new.shape != shape or k_new.stride(1) != 1 or v_new.stride(1) != 1:
+        shape, width, k_stride, v_stride = k_new.shape, self.num_kv_heads * self.head_dim, k_new.stride(), v_new.stride()
+        if len(shape) != 2 or shape[1] != width or v_new.shape != shape or k_stride[1] != 1 or v_stride[1] != 1:
             raise RuntimeError(f"{what}: k/v must be rows of {width} contiguous elements, as many of each")
         T = shape[0]
         self._ids(what, T, seq_ids, positions)
@@ -189,7 +189,7 @@ class QuantizedKVCache(PagedKVCache):
             return
         _lib.check(_lib.load().bn_kv8_append(
             self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, seq_ids.data_ptr(), positions.data_ptr(), T,
-            k_new.data_ptr(), k_new.stride(0), v_new.data_ptr(), v_new.stride(0), 0 if f32 else 1, KV8_VALUES[self.values], int(not rotated),
+            k_new.data_ptr(), k_stride[0], v_new.data_ptr(), v_stride[0], 0 if f32 else 1, KV8_VALUES[self.values], int(not rotated),
             self.num_kv_heads, self.head_dim, self.theta, _stream()))
 
     def gather(self, seq_ids: torch.Tensor, starts: torch.Tensor, n_tokens: int, *, dtype=torch.bfloat16):
@@ -203,7 +203,8 @@ class QuantizedKVCache(PagedKVCache):
         self._here(what, seq_ids, starts)
         n = seq_ids.numel()
         self._ids(what, n, seq_ids, starts)
-        k, v = torch.empty((2, n, n_tokens, self.num_kv_heads, self.head_dim), dtype=dtype, device=self.pool.device).unbind(0)
+        k = self.pool.new_empty((n, n_tokens, self.num_kv_heads, self.head_dim), dtype=dtype)
+        v = torch.empty_like(k)
         if n and n_tokens:
             _lib.check(_lib.load().bn_kv8_gather(
                 self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, self.seq_lens.data_ptr(),

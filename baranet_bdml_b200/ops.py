@@ -782,8 +782,10 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0,
             raise RuntimeError(f"{what}: {name}={v} (from {lo} to {hi})")
     u = per_row(uniform, torch.float32)
     if out is None:
-        out = torch.empty((rows,), dtype=torch.int32, device=logits.device)
-    o = per_row(out, torch.int32)
+        out = logits.new_empty(rows, dtype=torch.int32)
+        o = out.data_ptr()
+    else:
+        o = per_row(out, torch.int32)
     if rows:
         _lib.check(_lib.load().bn_sample_rows(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, 0 if f32 else 1, u, *args, o, rows, vocab, _stream()))
     return out
