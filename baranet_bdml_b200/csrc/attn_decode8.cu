@@ -122,7 +122,8 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     sc.G = sc.whole ? min(grid, p.B * p.Hkv) : max(1, min(grid, p.min_stages == 1 ? sc.T : sc.T / p.min_stages));
     const bool active = sc.T > 0 && (int)blockIdx.x < sc.G;
     SegmentIter iter;
-    iter.init(active ? sc.range_begin(blockIdx.x) : 0, active ? sc.range_begin(blockIdx.x + 1) : 0);
+    const int edge = active ? sc.range_begin(blockIdx.x + lane % 2) : 0;       // both ends by one run through the divisions
+    iter.init(__shfl_sync(0xffffffffu, edge, 0), __shfl_sync(0xffffffffu, edge, 1));
     Segment sg;
 
     if (warp >= DEC8_CWARPS && warp < DEC8_QUERY_WARP) {
