@@ -153,7 +153,8 @@ class QuantizedKVCache(PagedKVCache):
         self.values = values
         self._spare = None     # scratch for the next capture
 
-    def _here(self, what: str, *tensors: Optional[torch.Tensor]) -> None:
+    def _here(self, what: str, *tensors: Optional[torch.Tensor]) -> int:
+        """The current stream, where all tensors lie on the cache's device, which is the current one"""
         dev = self.pool.get_device()
         if dev < 0:
             raise RuntimeError(f"{what}: only GPU implementation available")
@@ -162,6 +163,7 @@ class QuantizedKVCache(PagedKVCache):
         for t in tensors:
             if t is not None and t.get_device() != dev:
                 raise RuntimeError(f"{what}: all tensors must lie on the cache's device")
+        return torch._C._cuda_getCurrentRawStream(dev)
 
     @staticmethod
     def _ids(what: str, n: int, *tensors: torch.Tensor) -> None:
@@ -179,7 +181,7 @@ class QuantizedKVCache(PagedKVCache):
         f32 = k_new.dtype == torch.float32
         if not (f32 or k_new.dtype == torch.bfloat16) or v_new.dtype != k_new.dtype:
             raise RuntimeError(f"{what}: k/v must both be fp32 or both bf16")
-        self._here(what, seq_ids, positions, k_new, v_new)
+        stream = self._here(what, seq_ids, positions, k_new, v_new)
         shape, width, k_stride, v_stride = k_new.shape, self.num_kv_heads * self.head_dim, k_new.stride(), v_new.stride()
         if len(shape) != 2 or shape[1] != width or v_new.shape != shape or k_stride[1] != 1 or v_stride[1] != 1:
             raise RuntimeError(f"{what}: k/v must be rows of {width} contiguous elements, as many of each")
@@ -190,7 +192,7 @@ class QuantizedKVCache(PagedKVCache):
         _lib.check(_lib.load().bn_kv8_append(
             self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, seq_ids.data_ptr(), positions.data_ptr(), T,
             k_new.data_ptr(), k_stride[0], v_new.data_ptr(), v_stride[0], 0 if f32 else 1, KV8_VALUES[self.values], int(not rotated),
-            self.num_kv_heads, self.head_dim, self.theta, _stream()))
+            self.num_kv_heads, self.head_dim, self.theta, stream))
 
     def gather(self, seq_ids: torch.Tensor, starts: torch.Tensor, n_tokens: int, *, dtype=torch.bfloat16):
         """What the cache holds of sequence seq_ids[i] from position starts[i] on: K (rotated, as it is stored) and V, each
@@ -200,7 +202,7 @@ class QuantizedKVCache(PagedKVCache):
             raise RuntimeError(f"{what}: {dtype} (float32 or bfloat16)")
         if n_tokens < 0:
             raise RuntimeError(f"{what}: {n_tokens} tokens")
-        self._here(what, seq_ids, starts)
+        stream = self._here(what, seq_ids, starts)
         n = seq_ids.numel()
         self._ids(what, n, seq_ids, starts)
         k = self.pool.new_empty((n, n_tokens, self.num_kv_heads, self.head_dim), dtype=dtype)
@@ -209,7 +211,7 @@ class QuantizedKVCache(PagedKVCache):
             _lib.check(_lib.load().bn_kv8_gather(
                 self.pool.data_ptr(), self.num_pages, self.page_table.data_ptr(), self.num_seqs, self.max_pages, self.seq_lens.data_ptr(),
                 seq_ids.data_ptr(), starts.data_ptr(), n, n_tokens, k.data_ptr(), v.data_ptr(), 0 if dtype == torch.float32 else 1,
-                KV8_VALUES[self.values], self.num_kv_heads, self.head_dim, _stream()))
+                KV8_VALUES[self.values], self.num_kv_heads, self.head_dim, stream))
         return k, v
 
     def status(self) -> None:
@@ -255,7 +257,7 @@ class QuantizedKVCache(PagedKVCache):
             seq_lens = self.seq_lens
         if page_table is None:
             page_table = self.page_table
-        self._here(what, q, seq_lens, page_table, q_positions, out, out_f32, lse)
+        stream = self._here(what, q, seq_lens, page_table, q_positions, out, out_f32, lse)
         shape = q.shape
         if len(shape) != 3 or shape[1] != num_heads or shape[2] != self.head_dim:
             raise RuntimeError(f"{what}: q must be (B, {num_heads}, {self.head_dim}), got {tuple(shape)}")
@@ -268,9 +270,10 @@ class QuantizedKVCache(PagedKVCache):
         rows, width = page_table.shape if page_table.dim() == 2 else (-1, 0)
         if rows < B:
             raise RuntimeError(f"{what}: a page table of {tuple(page_table.shape)} for {B} sequences")
-        for t, dtype, n in ((out, torch.bfloat16, B * Hq * D), (out_f32, torch.float32, B * Hq * D), (lse, torch.float32, B * Hq)):
-            if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.numel() != n):
-                raise RuntimeError(f"{what}: an output must be a contiguous {dtype} tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
+        if not (out is None and out_f32 is None and lse is None):
+            for t, dtype, n in ((out, torch.bfloat16, B * Hq * D), (out_f32, torch.float32, B * Hq * D), (lse, torch.float32, B * Hq)):
+                if t is not None and (t.dtype != dtype or not t.is_contiguous() or t.numel() != n):
+                    raise RuntimeError(f"{what}: an output must be a contiguous {dtype} tensor of {n} elements, got {t.dtype} {tuple(t.shape)}")
         if out is None and out_f32 is None:
             out = torch.empty_like(q)
         if max_seq_len is None:
@@ -278,7 +281,6 @@ class QuantizedKVCache(PagedKVCache):
         if scale is None:
             scale = 1.0 / (D ** 0.5)
         if B:
-            stream = _stream()
             ws = self._ws.get(stream) if self._spare is not None and not torch.cuda.is_current_stream_capturing() else None
             ws = ws or self.workspace(B, Hq, max_seq_len, chunk_tokens)
             _lib.check(_lib.load().bn_attn_decode_kv8(

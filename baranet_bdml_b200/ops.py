@@ -772,14 +772,14 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0,
         return t.data_ptr()
 
     args = []
-    for v, dtype, lo, hi, name in ((temperature, torch.float32, 0.0, 3.0e38, "temperature"), (top_k, torch.int32, 0, 2 ** 31 - 1, "top_k"),
-                                   (top_p, torch.float32, 0.0, 1.0, "top_p"), (min_p, torch.float32, 0.0, 1.0, "min_p")):
-        if isinstance(v, torch.Tensor):
-            args += (per_row(v, dtype), type(lo)(0))
-        elif lo <= v <= hi:
-            args += (None, type(lo)(v))
+    for v, dtype, kind, hi, name in ((temperature, torch.float32, float, 3.0e38, "temperature"), (top_k, torch.int32, int, 2 ** 31 - 1, "top_k"),
+                                     (top_p, torch.float32, float, 1.0, "top_p"), (min_p, torch.float32, float, 1.0, "min_p")):
+        if type(v) is not kind and isinstance(v, torch.Tensor):
+            args += (per_row(v, dtype), 0)
+        elif 0 <= v <= hi:
+            args += (None, kind(v))
         else:
-            raise RuntimeError(f"{what}: {name}={v} (from {lo} to {hi})")
+            raise RuntimeError(f"{what}: {name}={v} (from 0 to {hi})")
     u = per_row(uniform, torch.float32)
     if out is None:
         out = logits.new_empty(rows, dtype=torch.int32)
@@ -787,7 +787,7 @@ def sample_rows(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0,
     else:
         o = per_row(out, torch.int32)
     if rows:
-        _lib.check(_lib.load().bn_sample_rows(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, 0 if f32 else 1, u, *args, o, rows, vocab, _stream()))
+        _lib.check(_lib.load().bn_sample_rows(logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, 0 if f32 else 1, u, *args, o, rows, vocab, torch._C._cuda_getCurrentRawStream(dev)))
     return out
 
 
