@@ -93,6 +93,11 @@ def rotated_k(workspace: Workspace, B: int, S: int, Hkv: int, D: int = 64) -> to
     return workspace.buf[at:at + B * S * Hkv * D * 2].view(torch.bfloat16).view(B * S, Hkv * D)
 
 
+def _bf16_cache(cache, what: str) -> None:
+    if cache is not None and cache.pool.dtype != torch.bfloat16:
+        raise RuntimeError(f"{what}: appends to a bf16 cache, not to one of {cache.pool.dtype}")
+
+
 def gemm_qkv_rope_bf16(x: torch.Tensor, wqkv_t: torch.Tensor, B: int, S: int, Hq: int, Hkv: int, D: int,
                        workspace: Workspace, *, position_offset: int = 0, cache=None,
                        error_word: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -101,6 +106,7 @@ def gemm_qkv_rope_bf16(x: torch.Tensor, wqkv_t: torch.Tensor, B: int, S: int, Hq
     norms are left in `workspace` (whose table must be current: prefill_table) for
     attn_prefill_bf16(q, None, v, workspace=workspace, reuse_rotated_k=True); with `cache` (a PagedKVCache whose
     sequences are the B rows) rotated K and V are also appended at positions position_offset .. + S - 1."""
+    _bf16_cache(cache, "gemm_qkv_rope_bf16")
     _need(x, torch.bfloat16, "gemm_qkv_rope_bf16(x)")
     _need(wqkv_t, torch.bfloat16, "gemm_qkv_rope_bf16(wqkv_t)")
     hidden = x.shape[1]
@@ -250,6 +256,7 @@ def gemm_qkv_append_bf16_skinny(x: torch.Tensor, wqkv_t: torch.Tensor, cache, se
     """The q, k and v projections of one new token per row (rows <= 16) over the concatenated weight, with RoPE(K) and
     the append to `cache` (a PagedKVCache) in the same launch; returns q (rows, num_heads * D).  Leaves in the cache
     the bits of `gemm_bf16_nt_skinny` + `cache.append`."""
+    _bf16_cache(cache, "gemm_qkv_append_bf16_skinny")
     _need(x, torch.bfloat16, "gemm_qkv_append_bf16_skinny(x)")
     _need(wqkv_t, torch.bfloat16, "gemm_qkv_append_bf16_skinny(wqkv_t)")
     _need(seq_ids, torch.int32, "gemm_qkv_append_bf16_skinny(seq_ids)")

@@ -34,6 +34,16 @@ def test_cache_refuses(lib):
             call()
 
 
+def test_products_that_append_refuse_it(lib):
+    """They write the bf16 cache's blocks, which are larger"""
+    from baranet_bdml_b200 import ops
+    from baranet_bdml_b200.kv_cache import QuantizedKVCache
+    cache, i, x, w = QuantizedKVCache(4, 1, 2, 2, device="cpu"), torch.zeros(1, dtype=torch.int32), torch.zeros(1, 256).bfloat16(), torch.zeros(768, 256).bfloat16()
+    for call in (lambda: ops.gemm_qkv_append_bf16_skinny(x, w, cache, i, i, 8), lambda: ops.gemm_qkv_rope_bf16(x, w, 1, 1, 8, 2, 64, None, cache=cache)):
+        with pytest.raises(RuntimeError, match="bf16 cache"):
+            call()
+
+
 def test_status_codes(lib):
     """The C entries check their arguments before they look for a device"""
     from baranet_bdml_b200 import _lib
