@@ -12,6 +12,7 @@
 //     instruction chains are as long, 95 us instead of 91;
 //   * four merger warps, two heads each, join the consumers' (m, l, O) of a segment, write the result or a partial, and, where they hold
 //     the last of a (sequence, head)'s partials, join those; buffers are double, so that nobody waits for them.
+//     Partials are joined sixteen at a time, a lane having one's (m, l): one round of loads (1 x 16000 tokens 10.8 us; eight at a time 12.3).
 //     (Two mergers of four heads: 24.1 -> 24.9 us for 64 sequences of 1024 to 4096 tokens.  Taking the segment that a range's end cuts first, so
 //     that its partials are joined before the CTAs end, costs more at the start than it saves at the end: 22.9 -> 24.1 us.)
 // Both products are m16n8k16 MMAs of fp16, which holds every e4m3 and int8 number exactly:
@@ -76,6 +77,13 @@ __device__ __forceinline__ void decode8_store(const Decode8Params& p, size_t row
     if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
 }
 
+// the queries of a key head: lane -> dims 2 * lane, + 1, of each
+__device__ __forceinline__ void decode8_query(const Decode8Params& p, int b, int g, int lane, uint32_t (&raw)[DEC_G]) {
+    const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + ((size_t)b * p.Hq + (size_t)g * p.n_rep) * (DEC_D / 2) + lane;
+#pragma unroll
+    for (int h = 0; h < DEC_G; ++h) raw[h] = h < p.n_rep ? src[h * (DEC_D / 2)] : 0u;
+}
+
 template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8_kernel(const __grid_constant__ Decode8Params p) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t full_bar[DEC8_NSTAGES], empty_bar[DEC8_NSTAGES];
@@ -106,8 +114,17 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         s_abort = 0;
         fence_mbar_init();
     }
+    // Where this CTA begins (lane 1: and ends) if it takes whole (sequence, key head)s.  Its page numbers and queries are asked for before the
+    // lengths that tell whether it does, and then neither divisions nor a search lie between them and the first copies.
+    const int grid = gridDim.x, heads = p.B * p.Hkv, edge_of = (int)((blockIdx.x + lane % 2) * (unsigned)heads / (unsigned)min(grid, heads));
+    const int edge_b = edge_of / p.Hkv, edge_g = edge_of - edge_b * p.Hkv, guess = min(__shfl_sync(0xffffffffu, edge_of, 0), heads - 1);
+    const int guess_b = guess / p.Hkv, guess_g = guess - guess_b * p.Hkv;
+    int guess_ids = 0;
+    uint32_t guess_raw[DEC_G];
     grid_dependency_wait();
     grid_launch_dependents();
+    if (warp >= DEC8_CWARPS && warp < DEC8_QUERY_WARP && lane < p.max_pages) guess_ids = p.page_table[(size_t)guess_b * p.max_pages + lane];
+    if (warp == DEC8_QUERY_WARP) decode8_query(p, guess_b, guess_g, lane, guess_raw);
     decode_prefix<DEC8_THREADS, DEC8_STAGE_TOKENS>(p.seq_lens, p.B, p.max_seq_len, s_len, s_prefix, &s_nmax);
 
     Schedule sc;
@@ -117,13 +134,16 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     sc.B = p.B;
     sc.T = p.Hkv * s_prefix[p.B];
     // whole (sequence, key head)s for every CTA where equal shares would save less than their cuts cost
-    const int grid = gridDim.x;
     sc.whole = (int64_t)p.most_heads * s_nmax * grid <= sc.T + DEC8_CUT_STAGES * grid;
     sc.G = sc.whole ? min(grid, p.B * p.Hkv) : max(1, min(grid, p.min_stages == 1 ? sc.T : sc.T / p.min_stages));
     const bool active = sc.T > 0 && (int)blockIdx.x < sc.G;
     SegmentIter iter;
-    const int edge = active ? sc.range_begin(blockIdx.x + lane % 2) : 0;       // both ends by one run through the divisions
+    int edge = 0;                                      // both ends by one run through the divisions
+    if (active && sc.whole) edge = edge_of < heads ? p.Hkv * s_prefix[edge_b] + edge_g * sc.nst(edge_b) : sc.T;
+    else if (active) edge = sc.range_begin(blockIdx.x + lane % 2);
     iter.init(__shfl_sync(0xffffffffu, edge, 0), __shfl_sync(0xffffffffu, edge, 1));
+    if (sc.whole && sc.nst(guess_b) > 0) iter.start_at(guess_b, guess_g);
+    else iter.search_warp(sc);
     Segment sg;
 
     if (warp >= DEC8_CWARPS && warp < DEC8_QUERY_WARP) {
@@ -135,16 +155,18 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
         uint32_t phase = 0;
         bool ok = true, bad = false;
         Segment sg_next;
-        bool have = iter.next<true>(sc, sg, false);
+        bool have = iter.next(sc, sg, false);
         auto load_group = [&](const Segment& sgm, int grp) {
             const int e = grp * 32 + lane;
             const int n_pages_seq = (sgm.L + BN_PAGE_TOKENS - 1) / BN_PAGE_TOKENS;
             return e < n_pages_seq ? p.page_table[(size_t)sgm.b * p.max_pages + e] : 0;
         };
         const uint64_t stream_policy = l2_policy_evict_first();     // every cache byte is read once per launch
-        int ids = have ? load_group(sg, sg.s0 / GRP) : 0, ids_pref = 0;
+        int ids = 0, ids_pref = 0;
+        if (have && sg.b == guess_b && sg.s0 < GRP) ids = lane < (sg.L + BN_PAGE_TOKENS - 1) / BN_PAGE_TOKENS ? guess_ids : 0;
+        else if (have) ids = load_group(sg, sg.s0 / GRP);
         while (ok && have) {
-            const bool have_next = iter.next<true>(sc, sg_next, false);
+            const bool have_next = iter.next(sc, sg_next, false);
             const int n_pages_seq = (sg.L + BN_PAGE_TOKENS - 1) / BN_PAGE_TOKENS;
             for (int s = sg.s0; s < sg.s1; ++s) {
                 if (s == sg.s0 || s % GRP == 0) {
@@ -177,21 +199,24 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     if (warp == DEC8_QUERY_WARP) {
         // ---------------------------------------------------------- query warp: lane -> dims 2 * lane, + 1, of all heads
         const double freq = p.freqs.f[lane];           // (of 32 different parameters a warp reads one at a time: not in every segment)
-        auto load = [&](const Segment& of, uint32_t (&raw)[DEC_G]) {
-            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q) + ((size_t)of.b * p.Hq + (size_t)of.g * p.n_rep) * (DEC_D / 2) + lane;
-#pragma unroll
-            for (int h = 0; h < DEC_G; ++h) raw[h] = h < p.n_rep ? src[h * (DEC_D / 2)] : 0u;
-            return p.rope_q && p.q_positions ? p.q_positions[of.b] : of.L - 1;
-        };
+        auto position = [&](const Segment& of) { return p.rope_q && p.q_positions ? p.q_positions[of.b] : of.L - 1; };
         uint32_t raw[DEC_G], raw_next[DEC_G];
         int pos = 0, pos_next = 0, known = -1;
         float c = 1.f, s = 0.f;
-        bool have = iter.next<true>(sc, sg, false);
-        if (have) pos = load(sg, raw);
+        bool have = iter.next(sc, sg, false);
+        if (have) {
+            pos = position(sg);
+#pragma unroll
+            for (int h = 0; h < DEC_G; ++h) raw[h] = guess_raw[h];
+            if (sg.b != guess_b || sg.g != guess_g) decode8_query(p, sg.b, sg.g, lane, raw);
+        }
         for (int n = 0; have; ++n) {
             const int buf = n % 2, b = sg.b;
-            have = iter.next<true>(sc, sg, false);
-            if (have) pos_next = load(sg, raw_next);                   // under way while this one is rotated
+            have = iter.next(sc, sg, false);
+            if (have) {                                                // under way while this one is rotated
+                pos_next = position(sg);
+                decode8_query(p, sg.b, sg.g, lane, raw_next);
+            }
             if (p.rope_q && b != known) kv8_rotation(pos, freq, &c, &s);
             known = b;
             if (!mbar_wait_warp(smem_u32(&q_free[buf]), (n / 2 & 1) ^ 1u, &s_abort)) break;
@@ -226,7 +251,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
             for (int h = h0; h < h0 + DEC8_HPM; ++h)
                 if (h < p.n_rep) decode8_store(p, (size_t)b * p.Hq + (size_t)g * p.n_rep + h, lane, 0.f, 0.f, 0.f, 0.f);
         }
-        for (int n = 0; iter.next<true>(sc, sg, true); ++n) {
+        for (int n = 0; iter.next(sc, sg, true); ++n) {
             const int buf = n % 2;
             if (!mbar_wait_warp(smem_u32(&mrg_full[buf]), n / 2 & 1, &s_abort)) break;
             float m[DEC8_HPM], l[DEC8_HPM], a[DEC8_HPM], b[DEC8_HPM];
@@ -268,34 +293,44 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 // this CTA stored the last part: joined in the order of the parts, whoever is last
 #pragma unroll
                 for (int i = 0; i < DEC8_HPM; ++i) { m[i] = -INFINITY; l[i] = a[i] = b[i] = 0.f; }
-                constexpr int AHEAD = 8;               // parts whose loads are under way together
+                constexpr int AHEAD = 16;              // parts whose loads are under way together; a lane has a part's m and l
                 for (int c0 = 0; c0 < sg.n_parts; c0 += AHEAD) {
-                    float pm[AHEAD][DEC8_HPM], pl[AHEAD][DEC8_HPM];
+                    float pm[DEC8_HPM], pl[DEC8_HPM];
                     float2 po[AHEAD][DEC8_HPM];
+                    const int own = c0 + lane;
+                    const bool has = lane < AHEAD && own < sg.n_parts;
+                    const int at = ((sg.c_first + (has ? own : 0)) * 2 + (!has || own == 0)) * DEC_G + h0;
+#pragma unroll
+                    for (int i = 0; i < DEC8_HPM; ++i) {
+                        pm[i] = has ? __ldcg(p.part_m + at + i) : -INFINITY;
+                        pl[i] = has ? __ldcg(p.part_l + at + i) : 0.f;
+                    }
 #pragma unroll
                     for (int c = 0; c < AHEAD; ++c)
 #pragma unroll
                         for (int i = 0; i < DEC8_HPM; ++i) {
                             const bool on = c0 + c < sg.n_parts;
                             const int e = ((sg.c_first + (on ? c0 + c : 0)) * 2 + (!on || c0 + c == 0)) * DEC_G + h0 + i;
-                            pm[c][i] = on ? __ldcg(p.part_m + e) : -INFINITY;
-                            pl[c][i] = on ? __ldcg(p.part_l + e) : 0.f;
                             po[c][i] = on ? __ldcg(reinterpret_cast<const float2*>(p.part_o + e * DEC_D + 2 * lane)) : make_float2(0.f, 0.f);
                         }
 #pragma unroll
                     for (int i = 0; i < DEC8_HPM; ++i) {
-                        float top = m[i];
+                        float top = pm[i];
 #pragma unroll
-                        for (int c = 0; c < AHEAD; ++c) top = fmaxf(top, pm[c][i]);
-                        const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[i] - base);
+                        for (int o = 1; o < AHEAD; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                        top = fmaxf(m[i], __shfl_sync(0xffffffffu, top, 0));
+                        const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[i] - base), scl = ex2(pm[i] - base);
+                        float sum = pl[i] * scl;
+#pragma unroll
+                        for (int o = 1; o < AHEAD; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                         m[i] = top;
-                        l[i] *= keep; a[i] *= keep; b[i] *= keep;
+                        l[i] = l[i] * keep + __shfl_sync(0xffffffffu, sum, 0);
+                        a[i] *= keep; b[i] *= keep;
 #pragma unroll
                         for (int c = 0; c < AHEAD; ++c) {
-                            const float scl = ex2(pm[c][i] - base);
-                            l[i] += pl[c][i] * scl;
-                            a[i] += po[c][i].x * scl;
-                            b[i] += po[c][i].y * scl;
+                            const float f = __shfl_sync(0xffffffffu, scl, c);
+                            a[i] += po[c][i].x * f;
+                            b[i] += po[c][i].y * f;
                         }
                     }
                 }
@@ -313,7 +348,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     const int hA = 2 * (lane % 4);       // the two heads whose softmax state this thread carries
     int before = 0;                      // stages of the range that lie before the segment
     bool ok = true;
-    for (int n = 0; ok && iter.next<true>(sc, sg, false); ++n) {
+    for (int n = 0; ok && iter.next(sc, sg, false); ++n) {
         const int buf = n % 2;
         if (!mbar_wait_warp(smem_u32(&q_full[buf]), n / 2 & 1, &s_abort)) break;
         // Q^T fragments: dims 16 c .. 16 c + 15 of head lane / 4, c = lane % 4

@@ -103,17 +103,25 @@ struct SegmentIter {
     int pos, end, b, g;
     bool started;
     __device__ __forceinline__ void init(int lo, int hi) { pos = lo; end = hi; b = 0; g = 0; started = false; }
+    // the range's first segment: known, or found by a whole warp, which has the same range in all lanes
+    __device__ __forceinline__ void start_at(int first_b, int first_g) { b = first_b; g = first_g - 1; started = true; }
+    __device__ __forceinline__ void search_warp(const Schedule& sc) {
+        int first_b = 0, first_g = 0;
+        if (pos < end) {
+            first_b = sc.seq_of_warp(pos);
+            const int n = sc.nst(first_b), at = pos - sc.Hkv * sc.prefix[first_b];
+            first_g = sc.Hkv <= 32 ? __ffs(__ballot_sync(0xffffffffu, ((int)(threadIdx.x % 32) + 1) * n > at)) - 1 : at / n;
+        }
+        start_at(first_b, first_g);
+    }
     // `want_parts` = false skips c_first / n_parts (two divisions), which the producer never reads
-    // WARP: called by whole warps, with the same range in all lanes
-    template <bool WARP = false> __device__ __forceinline__ bool next(const Schedule& sc, Segment& sg, bool want_parts = true) {
+    __device__ __forceinline__ bool next(const Schedule& sc, Segment& sg, bool want_parts = true) {
         if (pos >= end) return false;
         int n;
         if (!started) {
-            b = WARP ? sc.seq_of_warp(pos) : sc.seq_of(pos);
+            b = sc.seq_of(pos);
             n = sc.nst(b);
-            const int at = pos - sc.Hkv * sc.prefix[b];
-            if (WARP && sc.Hkv <= 32) g = __ffs(__ballot_sync(0xffffffffu, ((int)(threadIdx.x % 32) + 1) * n > at)) - 1;
-            else g = at / n;
+            g = (pos - sc.Hkv * sc.prefix[b]) / n;
             started = true;
         } else {
             if (++g == sc.Hkv) {
