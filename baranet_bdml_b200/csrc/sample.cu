@@ -8,18 +8,18 @@
 // What is kept is always a prefix of the order, so that it is named by its last element.
 //
 // Sums decide which side of a border a token falls on, so they have to come out the same however the row is divided: weights are
-// computed in fp64 (2^(i / 32) from a table, and 2^f for |f| <= 1/64 by seven terms of the exponential series, whose rest is below 4e-18) and summed as 64-bit whole
-// numbers of 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight above 0 counts at least
-// one such unit.
+// computed in fp64 (2^(i / 32) from a table, and 2^f for |f| <= 1/64 by seven terms of the exponential series, whose rest is below 4e-18)
+// and summed as 64-bit whole numbers of 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight
+// above 0 counts at least one such unit.
 //
 // A cluster of CTAs per row, each with a part of the row in shared memory: read once.  The border of top-k is found by a histogram of
 // counts over 512 steps of the value below the maximum, which every CTA joins for itself through distributed shared memory.  For top-p the
 // same counts, with the largest and the smallest weight of each step, tell between which two steps the border must lie.  Every token is
-// then weighed once: those above and below only go into sums, those between into a second
-// histogram, of weights as three 16-bit limbs (whose sums fit the 32-bit atomics that shared memory has; 64-bit ones take 50 times as
-// long), and the places of all that may be kept are put side by side for the choice.
-// Where no more than 512 tokens lie in the steps down to the border, all that is left is done with a list of them, in every CTA alike:
-// ranks, sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and what is kept is passed over once
+// then weighed once: those above and below only go into sums, those between into a second histogram, of weights as three 16-bit limbs
+// (whose sums fit the 32-bit atomics that shared memory has; 64-bit ones take 50 times as long), and the places of all that may be kept
+// are put side by side for the choice.
+// Where few tokens lie in the steps down to the border, all that is left is done with a list of them, by the cluster's first CTA: ranks,
+// sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and what is kept is passed over once
 // more for the choice.  A step with too many (equal logits, far outliers) is divided again by (value, index) until it has not.
 // A batch pays for the instructions per token: 256 rows of 32000 with top-p of 0.9 take 74 us, 0.44 TB/s: 115 instructions per token and
 // 2300 per warp, at 62% of what the SMs can issue, in 1.7 waves (107 with every weight through the histogram, 155 with the tokens that cannot
@@ -73,7 +73,8 @@ struct SampleShared {
     uint32_t hist[4][SMP_BINS];                        // counts, and the limbs of weights
     uint32_t coarse[SMP_BINS];                         // counts that say where to look
     uint64_t list_key[SMP_LIST];                       // this CTA's elements
-    uint64_t all_key[SMP_LIST], all_w[SMP_LIST];       // the cluster's
+    uint64_t all_key[SMP_LIST];                        // the cluster's
+    uint32_t index[SMP_LIST];                          // of what is kept of it
     uint64_t from[2][SMP_CLUSTER * SMP_WARPS][2];      // what all warps of the cluster tell each other
     uint64_t warp_sum[2][SMP_WARPS];
     uint32_t warp_cnt[2][SMP_WARPS];
@@ -627,7 +628,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
         __syncthreads();
         const uint64_t all = sh.kept_sum, reach = min((uint64_t)(u * (double)all), all - 1);
         // in the order of the index (whose complement the key has), for the sums up to each
-        uint32_t* index = reinterpret_cast<uint32_t*>(sh.all_w);
+        uint32_t* index = sh.index;
         uint64_t* by_index = sh.all_key;
         if (tid < stay) index[tid] = (uint32_t)in_key[tid];
         const int place = rank_among(index, stay);
