@@ -16,8 +16,8 @@
 // counts over 512 steps of the value below the maximum, which every CTA joins for itself through distributed shared memory.  For top-p the
 // same counts, with the largest and the smallest weight of each step, tell between which two steps the border must lie.  Every token is
 // then weighed once: those above and below only go into sums, those between into a second histogram, of weights as three 16-bit limbs
-// (whose sums fit the 32-bit atomics that shared memory has; 64-bit ones take 50 times as long), and the places of all that may be kept
-// are put side by side for the choice.
+// (whose sums over a CTA's part, 32768 tokens at most, fit the 32-bit atomics that shared memory has, where 64-bit ones take 50 times as
+// long; over the cluster they are added in 64 bits), and the places of all that may be kept are put side by side for the choice.
 // Where few tokens lie in the steps down to the border, all that is left is done with a list of them, by the cluster's first CTA: ranks,
 // sums, choice.  Otherwise the few elements of the border's step are ranked among each other, and what is kept is passed over once
 // more for the choice.  A step with too many (equal logits, far outliers) is divided again by (value, index) until it has not.
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             const int at = min(atomicAdd(&sh.list_n, 1), SMP_LIST - 1);      // (m of them in the whole cluster)
             sh.list_key[at] = key_of(v, i);
         };
-        auto joined = [&](const uint32_t* row) -> uint32_t {       // the cluster's histogram at the thread's step
-            uint32_t sum = 0;
+        auto joined = [&](const uint32_t* row) -> uint64_t {       // the cluster's histogram at the thread's step
+            uint64_t sum = 0;                          // (eight CTAs' sums of limbs have up to 34 bits)
 #pragma unroll
             for (int c = 0; c < SMP_CLUSTER; ++c)
                 if (c < C) sum += ld_cluster_u32(in_rank(smem_u32(row + tid), c));
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
                 });
             }
             cluster_sync();
-            const uint32_t cnt = joined(sh.coarse);
+            const uint32_t cnt = (uint32_t)joined(sh.coarse);
             // the step's weights lie between these, its sums between theirs (a thousandth of a step and 1e-4 for the roundings)
             const float wide = range / SMP_BINS / temp, most = tid == 0 ? 1.f : __expf(-(tid - 0.501f) * wide), least = tid == SMP_BINS - 1 ? 0.f : __expf(-(tid + 0.501f) * wide);
             float a = cnt * most, b = cnt ? cnt * least : 0.f;
@@ -492,10 +492,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
                 });
                 cluster_sync();
             }
-            const uint32_t cnt = joined(sh.hist[0]);
+            const uint32_t cnt = (uint32_t)joined(sh.hist[0]);
             uint64_t total;
             uint32_t upto;
-            const uint64_t sum = by_weight ? joined(sh.hist[1]) + ((uint64_t)joined(sh.hist[2]) << 16) + ((uint64_t)joined(sh.hist[3]) << 32) : cnt;
+            const uint64_t sum = by_weight ? joined(sh.hist[1]) + (joined(sh.hist[2]) << 16) + (joined(sh.hist[3]) << 32) : cnt;
             uint64_t before = block_scan(sum, cnt, total, upto);
             if (by_weight && !again) above -= total;
             before += above;
