@@ -386,7 +386,6 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             const float wide = range / SMP_BINS / temp, most = tid == 0 ? 1.f : __expf(-(tid - 0.501f) * wide), least = tid == SMP_BINS - 1 ? 0.f : __expf(-(tid + 0.501f) * wide);
             float a = cnt * most, b = cnt ? cnt * least : 0.f;
             uint32_t upto = cnt;
-            const float own_a = a, own_b = b;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const float ta = __shfl_up_sync(0xffffffffu, a, o), tb = __shfl_up_sync(0xffffffffu, b, o);
@@ -405,11 +404,14 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
                 if (lane >= o) { all_a += ta; all_b += tb; all_c += tc; }
             }
             const float low_a = warp ? __shfl_sync(0xffffffffu, all_a, warp - 1) : 0.f, low_b = warp ? __shfl_sync(0xffffffffu, all_b, warp - 1) : 0.f;
+            // of the steps before this one.  (Not the sum less the step's own part: of 1e5 tokens in a step nothing would be left of 1e-4.)
+            const float ta = __shfl_up_sync(0xffffffffu, a, 1), tb = __shfl_up_sync(0xffffffffu, b, 1);
+            const float before_a = low_a + (lane ? ta : 0.f), before_b = low_b + (lane ? tb : 0.f);
             upto += warp ? __shfl_sync(0xffffffffu, all_c, warp - 1) : 0;
             all_a = __shfl_sync(0xffffffffu, all_a, SMP_WARPS - 1);
             all_b = __shfl_sync(0xffffffffu, all_b, SMP_WARPS - 1);
-            const uint32_t first_ok = __ballot_sync(0xffffffffu, cnt && (a - own_a + low_a) * 1.0001f < top_p * all_b * 0.9999f);
-            const uint32_t last_ok = __ballot_sync(0xffffffffu, cnt && (b - own_b + low_b) * 0.9999f <= top_p * all_a * 1.0001f);
+            const uint32_t first_ok = __ballot_sync(0xffffffffu, cnt && before_a * 1.0001f < top_p * all_b * 0.9999f);
+            const uint32_t last_ok = __ballot_sync(0xffffffffu, cnt && before_b * 0.9999f <= top_p * all_a * 1.0001f);
             if (lane == (last_ok ? 31 - __clz(last_ok) : 0)) {
                 sh.between[warp].lane1 = first_ok ? 32 - __clz(first_ok) : 0;
                 sh.between[warp].lane2 = last_ok ? 32 - __clz(last_ok) : 0;
@@ -496,11 +498,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
             uint64_t total;
             uint32_t upto;
             const uint64_t sum = by_weight ? joined(sh.hist[1]) + (joined(sh.hist[2]) << 16) + (joined(sh.hist[3]) << 32) : cnt;
-            uint64_t before = block_scan(sum, cnt, total, upto);
+            const uint64_t earlier = block_scan(sum, cnt, total, upto);
             if (by_weight && !again) above -= total;
-            before += above;
-            // the last step that has elements and less than the limit above it
-            const uint32_t here = __ballot_sync(0xffffffffu, cnt > 0 && (double)before < limit);
+            const uint64_t before = earlier + above;
+            // the last step that has elements and less than the limit above it; the first that has any qualifies, whatever was rounded
+            const uint32_t here = __ballot_sync(0xffffffffu, cnt > 0 && (earlier == 0 || (double)before < limit));
             if (lane == (here ? 31 - __clz(here) : 0)) {
                 sh.border[warp].above = before;
                 sh.border[warp].lane1 = here ? lane + 1 : 0;
@@ -613,7 +615,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
         uint32_t unused;
         if (!listed) {
             const uint64_t before = block_scan(w, 0, total, unused) + above;
-            const int stay = __syncthreads_count(tid < m && (double)before < limit);
+            const int stay = __syncthreads_count(tid < m && (tid == 0 || (double)before < limit));
             const uint64_t k = in_key[stay - 1];
             last = value_of((uint32_t)(k >> 32));
             last_at = (int)~(uint32_t)k;

@@ -50,3 +50,14 @@ def test_few_values(lib, cols, knobs):
     value = torch.tensor([0.0, -0.7, -1.9, -2.0, -2.1, -4.0, -7.3])
     which = torch.multinomial(torch.tensor([0.001, 0.01, 0.04, 0.8, 0.1, 0.04, 0.009]), cols, replacement=True, generator=g)
     check(value[which], **knobs)
+
+
+@pytest.mark.parametrize("share", [0.999, 0.9995, 0.9999999, 1.0005, 1.001])
+@pytest.mark.parametrize("cols,depth,run,second", [(187324, 0.25, 26, 22), (251913, 0.5, 11, 10), (167815, 1.0, 4, 3), (229292, 0.25, 16, 11), (187712, 0.5, 13, 7)])
+def test_a_border_before_a_long_run(lib, cols, depth, run, second, share):
+    """Two ids, then all others (`second` and `run` steps of the histogram below, and one at its end), and a top-p whose share of the sum is about
+    what the two weigh: fp32 sums that take in the run have lost what tells on which side of it the border lies"""
+    row = torch.full((cols,), float(np.float32(-run * depth / 512)))
+    row[5], row[100], row[200] = -depth, 0.0, float(np.float32(-second * depth / 512))
+    w = np.exp(row.double().numpy())
+    check(row, top_p=float(np.float32((w[100] + w[200]) / w.sum() * share)))
