@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
     // a warp has a run of the part, so that its sum is one of neighbours; in pieces of four
     const int run = (n4 + SMP_WARPS * 32 - 1) / (SMP_WARPS * 32) * 32, begin = warp * run, end = min(n4, begin + run);
     uint16_t* places = reinterpret_cast<uint16_t*>(sx + p.slice) + 2 * begin;      // of the warp's run, from its start
+    cluster_arrive();                                  // waited for before the first number that goes to another CTA: all have started then
     if (tid < SMP_STEPS) sh.exp2[tid] = exp2((double)tid / SMP_STEPS);
     grid_dependency_wait();
     grid_launch_dependents();
@@ -197,6 +198,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const Sampl
     };
     uint32_t top_order = order_of(top), low_order = order_of(low);
     join(top_order, low_order);
+    cluster_wait();
     tell_and_go_on((uint64_t)top_order << 32 | top_at, low_order);
     // (what the row's numbers alone say is worked out while the barrier is waited for; a temperature above 0 is one from 1e-30 to 3e38, for
     // which the steps of the value are finite: beyond, the weights are those at the end, but for logits less than 1e-27 apart)
