@@ -27,6 +27,11 @@
 //     tokens that count most in the result have the most bits of fp16, however far scales and weights are apart.  m is only renewed
 //     when a weight would pass 2^14 (a vote instead of a reduction in every stage).  The sum of weights l runs in fp32 without vs: log2 vs
 //     counts as -90 at least there and a weight without vs renews m beyond 2^100, so l has room for 2^27 tokens.
+//   * Scales lie anywhere in 2^-100 .. 2^122 (zeros have the least), so m may be 98 below the largest score or 114 above it, and rise by far more than
+//     126 over weights that still count: l is between 2^-114 and 2^127, but 2^-126 is the least single factor.  Whatever l is multiplied by
+//     where m rises or sums are joined is therefore the square of a half power, one factor after the other, and so are the weights themselves
+//     where m is renewed, and in every stage from a vs above 2^60 on: below that, a weight that is flushed to 0 is less than 2^-74 of l.  (A second
+//     maximum for l alone took 2 to 8 % longer where sequences are short: code, which each launch fetches anew.)  The code has s and m in halves.
 #include "decode_schedule.cuh"
 #include "kv8.cuh"
 
@@ -65,16 +70,16 @@ struct Decode8Params {
     float *part_m, *part_l, *part_o;            // [CTA][0: the segment began before its range, 1: it ends behind it][head] ([dim])
     int B, Hq, Hkv, n_rep, max_pages, max_seq_len, min_stages, rope_q;
     int most_heads;                             // (sequence, key head)s of a CTA that takes whole ones
-    float scale_log2;
+    float half_scale_log2;
     RotationFreqs freqs;
 };
 
-// results of one head: lane -> dims 2 * lane, + 1
+// results of one head (m in halves): lane -> dims 2 * lane, + 1
 __device__ __forceinline__ void decode8_store(const Decode8Params& p, size_t row, int lane, float m, float l, float a, float b) {
     const float inv = l > 0.f ? 1.f / l : 0.f;
     if (p.out) *reinterpret_cast<uint32_t*>(p.out + row * DEC_D + 2 * lane) = pack_bf16(a * inv, b * inv);
     if (p.out_f32) *reinterpret_cast<float2*>(p.out_f32 + row * DEC_D + 2 * lane) = make_float2(a * inv, b * inv);
-    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * LN2;
+    if (p.lse && lane == 0) p.lse[row] = l == 0.f ? -INFINITY : (2.f * m + log2f(l)) * LN2;
 }
 
 // the queries of a key head: lane -> dims 2 * lane, + 1, of each
@@ -94,7 +99,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
     __shared__ float mrg_m[2][DEC8_CWARPS][DEC_G], mrg_l[2][DEC8_CWARPS][DEC_G];
     __shared__ __align__(16) float mrg_o[2][DEC8_CWARPS][DEC_G][DEC_D + 2];   // written and read as float2
     __shared__ __align__(16) uint32_t s_q[2][DEC_G][DEC_D / 2]; // rotated query heads of a segment, pairs of fp16
-    __shared__ float s_factor[2][DEC_G];                        // scale * log2(e) * what q was divided by
+    __shared__ float s_factor[2][DEC_G];                        // half of scale * log2(e) * what q was divided by
     __shared__ int s_abort;
 
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -228,7 +233,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 const uint32_t e = max(most >> 23, 30u);
                 const float up = __uint_as_float((254u + 14u - e) << 23);              // the largest magnitude to 2^14 and above
                 s_q[buf][h][lane] = pack_f16(y0 * up, y1 * up);
-                if (lane == 0) s_factor[buf][h] = p.scale_log2 * __uint_as_float((e - 14u) << 23);
+                if (lane == 0) s_factor[buf][h] = p.half_scale_log2 * __uint_as_float((e - 14u) << 23);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(smem_u32(&q_full[buf]));
@@ -265,9 +270,9 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 l[i] = a[i] = b[i] = 0.f;
 #pragma unroll
                 for (int w = 0; w < DEC8_CWARPS; ++w) {
-                    const float scl = ex2(mrg_m[buf][w][h] - base);
+                    const float half = ex2(mrg_m[buf][w][h] - base), scl = half * half;
                     const float2 o = *reinterpret_cast<const float2*>(&mrg_o[buf][w][h][2 * lane]);
-                    l[i] += mrg_l[buf][w][h] * scl;
+                    l[i] += mrg_l[buf][w][h] * half * half;
                     a[i] += o.x * scl;
                     b[i] += o.y * scl;
                 }
@@ -319,13 +324,13 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 #pragma unroll
                         for (int o = 1; o < AHEAD; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                         top = fmaxf(m[i], __shfl_sync(0xffffffffu, top, 0));
-                        const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[i] - base), scl = ex2(pm[i] - base);
-                        float sum = pl[i] * scl;
+                        const float base = top == -INFINITY ? 0.f : top, keep = ex2(m[i] - base), half = ex2(pm[i] - base), scl = half * half;
+                        float sum = pl[i] * half * half;
 #pragma unroll
                         for (int o = 1; o < AHEAD; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
                         m[i] = top;
-                        l[i] = l[i] * keep + __shfl_sync(0xffffffffu, sum, 0);
-                        a[i] *= keep; b[i] *= keep;
+                        l[i] = l[i] * keep * keep + __shfl_sync(0xffffffffu, sum, 0);
+                        a[i] *= keep * keep; b[i] *= keep * keep;
 #pragma unroll
                         for (int c = 0; c < AHEAD; ++c) {
                             const float f = __shfl_sync(0xffffffffu, scl, c);
@@ -364,6 +369,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
 
         float m_run[2] = {-INFINITY, -INFINITY}, less[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f};
         float o[4][4];
+        bool high = false;                             // a vs above 2^60 has been
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -378,7 +384,7 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 const uint32_t sbase = ring + stage * DEC8_STAGE_BYTES + gwarp * DEC8_PPW * BN_KV8_BLOCK;
                 // thread owns heads hA, hA + 1 and tokens lane / 4 (+ 8) of each page
                 float sv[DEC8_PPW][4], pr[DEC8_PPW][4], vs[DEC8_PPW][2];
-                bool renew = m_run[0] == -INFINITY || m_run[1] == -INFINITY;
+                bool renew = high || m_run[0] == -INFINITY || m_run[1] == -INFINITY;
                 const bool ragged = mine < DEC8_PPW * BN_PAGE_TOKENS;
                 if (VALUES == BN_KV8_E4M3 && ragged) {
                     // what lies behind the last token may be a NaN, and 0 * NaN must not reach O (whole pages may not have been loaded)
@@ -415,10 +421,10 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 }
 #pragma unroll
                 for (int pi = 0; pi < DEC8_PPW; ++pi) {
-                    float most = 0.f;
+                    float most = 1.4210855e-14f;       // 2^-46: a vs above 2^60 renews
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        pr[pi][j] = ex2(sv[pi][j] - less[j & 1]);
+                        pr[pi][j] = ex2(fmaf(2.f, sv[pi][j], -2.f * less[j & 1]));
                         most = fmaxf(most, pr[pi][j]);
                     }
                     // (2^-86: the sum of weights does without vs, and has to stay a number where vs is very small)
@@ -427,27 +433,32 @@ template <int VALUES> __global__ void __launch_bounds__(DEC8_THREADS, 1) decode8
                 if (__any_sync(0xffffffffu, renew)) {
                     float tmax[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int pi = 0; pi < DEC8_PPW; ++pi)
+                    for (int pi = 0; pi < DEC8_PPW; ++pi) {
+                        high |= fmaxf(vs[pi][0], vs[pi][1]) > 1.1529215e18f;
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            tmax[j & 1] = fmaxf(tmax[j & 1], sv[pi][j] + lg2(fmaxf(vs[pi][j >> 1], 8.0779357e-28f)));      // 2^-90
+                            tmax[j & 1] = fmaxf(tmax[j & 1], fmaf(0.5f, lg2(fmaxf(vs[pi][j >> 1], 8.0779357e-28f)), sv[pi][j]));      // 2^-90
+                    }
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh) {
                         tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 4));
                         tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 8));
                         tmax[hh] = fmaxf(tmax[hh], __shfl_xor_sync(0xffffffffu, tmax[hh], 16));
-                        const float m_new = fmaxf(m_run[hh], tmax[hh] - 8.f);
+                        const float m_new = fmaxf(m_run[hh], tmax[hh] - 4.f);
                         less[hh] = m_new == -INFINITY ? 0.f : m_new;
-                        const float alpha = ex2(m_run[hh] - less[hh]);
+                        const float half = ex2(m_run[hh] - less[hh]), alpha = half * half;
                         m_run[hh] = m_new;
-                        l_run[hh] *= alpha;
+                        l_run[hh] = l_run[hh] * half * half;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) { o[i][hh] *= alpha; o[i][hh + 2] *= alpha; }
                     }
 #pragma unroll
                     for (int pi = 0; pi < DEC8_PPW; ++pi)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) pr[pi][j] = ex2(sv[pi][j] - less[j & 1]);
+                        for (int j = 0; j < 4; ++j) {
+                            const float half = ex2(sv[pi][j] - less[j & 1]);
+                            pr[pi][j] = half * half;
+                        }
                 }
 #pragma unroll
                 for (int pi = 0; pi < DEC8_PPW; ++pi) {
@@ -562,7 +573,7 @@ extern "C" int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_
     p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.n_rep = Hq / Hkv; p.max_pages = max_pages; p.max_seq_len = max_seq_len;
     p.min_stages = chunk_tokens > DEC8_STAGE_TOKENS ? (chunk_tokens + DEC8_STAGE_TOKENS - 1) / DEC8_STAGE_TOKENS : 1;
     p.rope_q = rope_q;
-    p.scale_log2 = scale * LOG2E;
+    p.half_scale_log2 = 0.5f * scale * LOG2E;
     if (rope_q) p.freqs = rotation_freqs(theta);
 
     static thread_local int configured_dev = -1;
