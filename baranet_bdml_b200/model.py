@@ -96,6 +96,7 @@ class CausalLM:
             return logits, nxt
 
         step.graph = graph
+        step.how = how                                     # (the graph reads its tensors where they are)
         return step
 
     def generate(self, input_ids, max_new_tokens: int = 50, *, temperature: float = 0.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
