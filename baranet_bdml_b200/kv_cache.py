@@ -215,13 +215,22 @@ class QuantizedKVCache(PagedKVCache):
         return k, v
 
     def status(self) -> None:
-        """Raises if a decode launch gave up on a bounded wait, or met a page outside the pool; the scratch buffer starts afresh then."""
-        for ws in self._ws.values():
-            try:
-                ws.status()
-            except RuntimeError:
-                ws.buf.zero_()
-                raise
+        """Raises if a decode launch gave up on a bounded wait, or met a page outside the pool, on any stream: waits for all that the
+        device has been given.  The scratch buffers concerned start afresh then."""
+        if not self._ws:
+            return
+        with torch.cuda.device(self.pool.device):
+            torch.cuda.synchronize()
+            failed = None
+            for ws in self._ws.values():
+                try:
+                    ws.status()
+                except RuntimeError as e:
+                    ws.buf.zero_()
+                    failed = failed or e
+            if failed is not None:
+                torch.cuda.synchronize()                       # (a buffer's next call may come from another stream)
+                raise failed
 
     def workspace(self, B: int, Hq: int, max_seq_len: int, chunk_tokens: int = 0) -> Workspace:
         """The current stream's decode scratch, for all shapes, kept while the cache lives.  A capture has one of its own on each of its
