@@ -9,7 +9,7 @@
 //
 // Sums decide which side of a border a token falls on, so they have to come out the same however the row is divided: weights are
 // computed in fp64 (2^(i / 32) from a table, and 2^f for |f| <= 1/64 by seven terms of the exponential series, whose rest is below 4e-18)
-// and summed as 64-bit whole numbers of 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens).  A weight
+// and summed as 64-bit whole numbers of 2^-s, s the largest up to 50 for which a row's sum fits in 62 bits (47 for 32000 tokens, 44 for 262144).  A weight
 // above 0 counts at least one such unit.
 //
 // A cluster of CTAs per row, each with a part of the row in shared memory: read once.  The border of top-k is found by a histogram of

@@ -131,8 +131,8 @@ class PagedKVCache:
 
 class QuantizedKVCache(PagedKVCache):
     """The paged cache in 8 bits, `values` "e4m3" or "int8", a scale for each token and key head: about half the bytes of the bf16
-    cache, for each of which attention takes as long.  e4m3 numbers are off by up to 2^-4 of themselves, int8 numbers by up to
-    1 / 254 of the largest of their token and head.  Pool: [page][kv_head][2112 bytes], laid out as bn_kv8_append has it.
+    cache, for each of which attention takes as long.  e4m3 numbers are off by up to 2^-4 of themselves or 2^-10 of their scale, whichever is
+    more, int8 numbers by up to 1 / 252 of the largest of their token and head (half a scale, which is rounded up to bf16).  Pool: [page][kv_head][2112 bytes], laid out as bn_kv8_append has it.
 
     All tensors of a call lie on the cache's device, which is the current one."""
 

@@ -233,7 +233,7 @@ class GroupedQueryAttentionBF16:
         rotation (and, with `cache`, the append of K and V at positions position_offset ..) in its epilogue, then the
         fused attention kernel on the rotated K it left in the scratch buffer.  head_dim 64.  A caller that passes
         its own `workspace` keeps its cos/sin table current itself (ops.prefill_table).  A cache in 8 bits takes the rotated
-        K and V in a launch of its own; `cache_rows`: (sequence, position) of the B*S rows, where the caller has them."""
+        K and V, which are bf16 by then (a step's K is rotated in fp32 and rounded once), in a launch of its own; `cache_rows`: (sequence, position) of the B*S rows, where the caller has them."""
         from . import ops
         from .kv_cache import QuantizedKVCache, token_rows
         eight = isinstance(cache, QuantizedKVCache)

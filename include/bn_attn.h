@@ -446,7 +446,7 @@ BN_API int bn_attn_decode_kv8(const void* q, const void* pool, int64_t pool_page
  *   The first always stays.
  *   out[r] = the lowest index for which the sum of what is kept, up to and with it, exceeds uniform[r] times all that is kept.
  * Weights are fp64 and summed as whole numbers, so that a result does not depend on how the work is divided.  temperature 0: the
- * first maximum.  NaN counts as -inf; a row with nothing above -inf gives 0; +inf entries share the weight.
+ * first maximum, one below 1e-30 counts as 1e-30.  NaN counts as -inf; a row with nothing above -inf gives 0; +inf entries share the weight.
  * temperature, top_k, top_p, min_p: one value a row (device), or NULL for the value beside it.  cols <= 262144. */
 BN_API int bn_sample_rows(const void* logits, int64_t row_stride, int dtype, const float* uniform, const float* temperature,
                           float temperature_all, const int32_t* top_k, int top_k_all, const float* top_p, float top_p_all,
