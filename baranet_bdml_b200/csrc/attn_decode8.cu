@@ -27,6 +27,8 @@
 //     tokens that count most in the result have the most bits of fp16, however far scales and weights are apart.  m is only renewed
 //     when a weight would pass 2^14 (a vote instead of a reduction in every stage).  The sum of weights l runs in fp32 without vs: log2 vs
 //     counts as -90 at least there and a weight without vs renews m beyond 2^100, so l has room for 2^27 tokens.
+//     fp16 ends at 2^-24: a share 2^-33 below the largest p' (zeros count with 2^-90 there) is lost, which shows only in elements to which
+//     all larger tokens add a zero.
 //   * Scales lie anywhere in 2^-100 .. 2^122 (zeros have the least), so m may be 98 below the largest score or 114 above it, and rise by far more than
 //     126 over weights that still count: l is between 2^-114 and 2^127, but 2^-126 is the least single factor.  Whatever l is multiplied by
 //     where m rises or sums are joined is therefore the square of a half power, one factor after the other, and so are the weights themselves
